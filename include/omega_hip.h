@@ -300,6 +300,71 @@ int omega_moe_get_profile(omega_moe *moe, float stage_ms_sum[5], int *n_calls);
  * tiles[2] = edge of a tile of dW2 and of dW1 | dW3 (64 or 128).  For tests, which have to know which kernel they check. */
 int omega_moe_get_f32_tiles(omega_moe *moe, int T, int32_t tiles[3]);
 
+/* ---- Operators of the model around the layer, on caller-owned device buffers (row-major, contiguous) ----
+ * Asynchronous on the context's stream like omega_moe_forward: buffers that another stream writes or reads are the
+ * caller's to synchronise.  Temporary memory is one workspace of the context that grows on demand (a call that needs more than
+ * any call before waits for the stream and allocates); it is given back with the context.  An output may not overlap an input
+ * or another output (refused) unless a call says otherwise; buffers need the alignment of their element type only, 16-byte
+ * aligned buffers and widths that are multiples of 8 elements are faster.  No operation uses atomics on floating values: the
+ * same inputs give the same bits.  Sizes of zero rows are valid calls. */
+
+/* Token embedding: out[t,:] = scale * table[ids[t],:], table [V,d] and out [T,d] of one dtype, ids [T]; one rounding per
+ * element.  An id outside 0..V-1 (padding) gives a row of zeros.  EmbeddingFW, J/engine/nn/layer/gpu/EmbeddingKernel.cu:13-34
+ * (float-encoded ids there). */
+int omega_hip_embedding_forward(omega_ctx *ctx, const void *table, int dtype, int V, int d, const int32_t *ids, int T,
+                                float scale, void *out);
+/* Its gradient: dtable[v,:] = scale * sum of dout[t,:] over the tokens t with ids[t] = v, in ascending t, summed in fp32
+ * (EmbeddingGrad adds with atomicAdd, J/engine/nn/layer/gpu/EmbeddingKernel.cu:36-56).  dout [T,d] is of `dtype`, dtable [V,d] of
+ * `grad_dtype` (rounded once).  accumulate = 0: every row of dtable is written, rows without tokens with zeros; 1: the sums are
+ * added to what dtable holds (a table tied to the head: after omega_hip_head_loss_backward), rows without tokens are not touched. */
+int omega_hip_embedding_backward(omega_ctx *ctx, const int32_t *ids, int T, const void *dout, int dtype, int V, int d,
+                                 float scale, int accumulate, void *dtable, int grad_dtype);
+
+/* Layer norm: out = (x - mean) * rstd * gamma + beta over each row of x [T,d], mean and 1/sqrt(variance + eps) of a row in
+ * fp32; gamma and beta [d] always fp32.  mean and rstd [T] may be NULL where no backward pass follows.  Of the norm layers of
+ * J/engine/nn/layer/normalization. */
+int omega_hip_layernorm_forward(omega_ctx *ctx, const void *x, int dtype, int T, int d, const float *gamma, const float *beta,
+                                float eps, void *out, float *mean, float *rstd);
+/* Backward, with the mean and rstd of the forward pass: dx [T,d] (dtype), dgamma and dbeta [d] (fp32, overwritten, summed in a
+ * fixed order). */
+int omega_hip_layernorm_backward(omega_ctx *ctx, const void *x, const void *dout, int dtype, int T, int d, const float *gamma,
+                                 const float *mean, const float *rstd, void *dx, float *dgamma, float *dbeta);
+
+/* The head and its loss: softmax cross entropy of logits = x W^T (x [T,d], w [V,d], FullyLayer layout) against targets [T],
+ * in pieces of the vocabulary: the [T,V] logits are never kept.
+ *   loss[t] = log(sum_v exp(logit[t,v])) - logit[t,targets[t]], 0 for a token whose target is outside 0..V-1 (padding);
+ *   mean[0] = sum of loss / n, mean[1] = n = tokens with a target (n = 0: mean[0] = 0);
+ *   row_stats [2,T] = maximum of a row's logits, then the sum of exp(logit - maximum): what the backward pass needs.
+ * loss and mean are required, row_stats may be NULL where no backward pass follows.  All fp32.  Products of bf16 operands are
+ * summed in fp32; products of fp32 operands are formed from three bf16 parts of each factor (24 bits).
+ * FullyLayer.output + the softmax and log of J/engine/gpu/SoftmaxKernel.cu:4-24. */
+int omega_hip_head_loss_forward(omega_ctx *ctx, const void *x, const void *w, int dtype, int T, int V, int d,
+                                const int32_t *targets, float *loss, float *row_stats, float *mean);
+/* Gradients of dloss * mean[0] (dloss: one float on the device, NULL = 1), with the same x, w and targets and what the forward
+ * call returned: dx [T,d] and dw [V,d], of dtype, overwritten; either may be NULL (not computed).  Tokens without a target have
+ * zero rows in dx and no part in dw, whatever their rows of x hold.  The logits are computed again; in bf16 the gradient of the
+ * logits is rounded to bf16 before its two products, whose sums are fp32, and dx and dw are rounded once. */
+int omega_hip_head_loss_backward(omega_ctx *ctx, const void *x, const void *w, int dtype, int T, int V, int d,
+                                 const int32_t *targets, const float *row_stats, const float *mean, const float *dloss, void *dx,
+                                 void *dw);
+
+/* Clipping by the global norm over many tensors (Network.clipGradNorm, J/engine/nn/network/Network.java:379-432) without a copy
+ * to the host: norm = sqrt(sum of squares of all elements) (sums in double), coef = min(1, max_norm / (norm + 1e-6)), and every
+ * tensor times coef, rounded once per element.  Tensor i: n elements of dtype from src to dst; dst = src (in place) or a buffer
+ * that overlaps no other tensor.  The gradients of `layers` (the accumulators where accGrad has run, as omega_moe_scale_grad)
+ * are clipped with them, in place; the layers must belong to ctx.  norm_out: two floats on the device, norm and coef; may
+ * be NULL.  max_norm >= 0; infinity computes the norm and leaves in-place tensors as they are.  A norm that is infinite or no number
+ * gives what that arithmetic gives (coef 0 or NaN). */
+typedef struct {
+    const void *src;
+    void *dst;
+    uint64_t n;
+    int32_t dtype;
+    int32_t reserved; /* 0 */
+} omega_grad_tensor;
+int omega_hip_clip_grad_norm(omega_ctx *ctx, const omega_grad_tensor *tensors, int n_tensors, omega_moe *const *layers,
+                             int n_layers, float max_norm, float *norm_out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,10 @@ class MoEConfigStruct(C.Structure):
                 ("T_max", "d", "E", "K", "H", "Es", "renorm", "has_gate_bias", "dtype", "router_mode")]
 
 
+class GradTensorStruct(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("n", C.c_uint64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/omega_hip.h declares
 SIGNATURES = {
     "omega_hip_version": (C.c_int, []),
@@ -77,6 +81,15 @@ SIGNATURES = {
     "omega_moe_set_profiling": (C.c_int, [C.c_void_p, C.c_int]),
     "omega_moe_get_profile": (C.c_int, [C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)]),
     "omega_moe_get_f32_tiles": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_int32)]),
+    "omega_hip_embedding_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_float, C.c_void_p]),
+    "omega_hip_embedding_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_void_p,
+                                               C.c_int]),
+    "omega_hip_layernorm_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
+                                              C.c_void_p]),
+    "omega_hip_layernorm_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 6),
+    "omega_hip_head_loss_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 4),
+    "omega_hip_head_loss_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 6),
+    "omega_hip_clip_grad_norm": (C.c_int, [C.c_void_p, C.POINTER(GradTensorStruct), C.c_int, C.POINTER(C.c_void_p), C.c_int, C.c_float, C.c_void_p]),
 }
 
 _lib = None

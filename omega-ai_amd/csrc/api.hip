@@ -87,15 +87,11 @@ int omega_hip_ctx_destroy(omega_ctx *ctx)
     if (!ctx) return OMEGA_OK;
     hipSetDevice(ctx->device);
     hipStreamSynchronize(ctx->stream);
+    if (ctx->op_ws) hipFree(ctx->op_ws);
     hipStreamDestroy(ctx->stream);
     delete ctx;
     return OMEGA_OK;
 }
-
-#define CTX_ENTER(ctx)                                                                      \
-    if (!(ctx)) OMEGA_FAIL(nullptr, OMEGA_ERR_INVALID_ARG, "NULL context");                \
-    std::lock_guard<std::mutex> _lk((ctx)->mu);                                             \
-    OMEGA_HIP_CHECK((ctx), hipSetDevice((ctx)->device))
 
 int omega_hip_malloc(omega_ctx *ctx, size_t bytes, void **dptr)
 {
@@ -1409,3 +1405,13 @@ int omega_moe_time_stage(omega_moe *m, int stage, const void *x, int T, void *ou
 }
 
 }  // extern "C"
+
+// (what is scaled on the device may become no number: no block of the gradients is known to be zero any longer)
+bool moe_grad_view(omega_moe *m, float **g, size_t *n)
+{
+    if (!has_grads(m)) return false;
+    *g = m->acc_valid ? m->acc_grad : m->grads;
+    *n = grad_block_floats(m);
+    if (!m->acc_valid) m->bw_zero_valid = false;
+    return true;
+}

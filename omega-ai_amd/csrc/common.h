@@ -18,6 +18,11 @@ struct omega_ctx {
     std::string last_error;
     int num_cus = 256;
     float *noalloc_scratch = nullptr;  // this device's copy of the static scratch array of the allocation-free entry point
+    // workspace of the operators on caller-owned buffers (embedding gradient, layer norm, head, clipping): one block, grown on
+    // demand; calls on a context are serialised and run on one stream, so each finds it free
+    void *op_ws = nullptr;
+    size_t op_ws_bytes = 0;
+    bool head_ready = false;  // the head's kernels may take a compute unit's whole LDS (head_init has run)
 };
 
 // One entry per row tile of the grouped products: written on the device by the scan kernel.
@@ -238,6 +243,11 @@ static inline bool f32_wgrad_wide(const omega_moe *m, int T, int mats)
     return (long long)T * c.K >= 128LL * c.E && 4 * tiles * mats >= 5LL * m->ctx->num_cus && (c.Es == 0 || tiles * (mats / m->G) * (c.K + c.Es) >= m->ctx->num_cus);
 }
 
+#define CTX_ENTER(ctx)                                                                      \
+    if (!(ctx)) OMEGA_FAIL(nullptr, OMEGA_ERR_INVALID_ARG, "NULL context");                \
+    std::lock_guard<std::mutex> _lk((ctx)->mu);                                             \
+    OMEGA_HIP_CHECK((ctx), hipSetDevice((ctx)->device))
+
 #define OMEGA_FAIL(ctx, status, what) return omega_set_error((ctx), (status), (what), hipSuccess, __FILE__, __LINE__)
 #define OMEGA_HIP_CHECK(ctx, expr)                                                             \
     do {                                                                                       \
@@ -344,6 +354,34 @@ __host__ __device__ static inline int wgrad_tile(const wgrad_deal &w, int x, int
     *mat += g * w.together;
     return x * q + (x < e ? x : e) - (x < s ? x : s) + (x < e - 8 ? x : e > 8 ? e - 8 : 0) + j - before(g);
 }
+// ---- operators on caller-owned buffers (ops_api.hip checks their arguments) ----
+// gradients an update of the layer would use (api.hip): the accumulators or the gradients, *n floats; false: no backward has run
+bool moe_grad_view(omega_moe *m, float **g, size_t *n);
+hipError_t launch_embedding_forward(const void *table, int dtype, int V, int d, const int32_t *ids, int T, float scale, void *out,
+                                    hipStream_t s);
+size_t embedding_backward_workspace(int V, int d, int T);
+hipError_t launch_embedding_backward(const int32_t *ids, int T, const void *dout, int dtype, int V, int d, float scale, bool accumulate,
+                                     void *dtable, int grad_dtype, void *ws, hipStream_t s);
+hipError_t launch_layernorm_forward(const void *x, int dtype, int T, int d, const float *gamma, const float *beta, float eps, void *out,
+                                    float *mean, float *rstd, hipStream_t s);
+size_t layernorm_backward_workspace(const omega_ctx *ctx, int T, int d);
+hipError_t launch_layernorm_backward(const omega_ctx *ctx, const void *x, const void *dout, int dtype, int T, int d, const float *gamma,
+                                     const float *mean, const float *rstd, void *dx, float *dgamma, float *dbeta, void *ws, hipStream_t s);
+size_t clip_workspace(const omega_grad_tensor *t, int n);
+hipError_t launch_clip(const omega_grad_tensor *t, int n, float max_norm, float *norm_out, void *ws, hipStream_t s);
+struct head_args {
+    const void *x, *w;
+    int dtype, T, V, d;
+    const int32_t *targets;
+    float *loss, *row_stats, *mean;  // forward: out; backward: row_stats and mean in
+    const float *dloss;
+    void *dx, *dw;
+};
+size_t head_workspace(const omega_ctx *ctx, const head_args &a, bool backward);
+hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s);
+hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s);
+hipError_t head_init(void);  // kernel attributes (LDS beyond 64 KiB), once per device
+
 #define F32_TILE_M 128       // row-tile heights of fp32 layers: experts_f32_tile_m chooses one per batch
 #define F32_TILE_M_MID 64
 #define F32_TILE_M_SMALL 32

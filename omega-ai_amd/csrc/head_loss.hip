@@ -1,0 +1,1061 @@
+// The head of a language model with its loss: softmax cross entropy of logits = x W^T (x [T,d], W [V,d]) against targets, and its
+// gradients, in pieces of the vocabulary.  The [T,V] logits are never in memory: the forward product's epilogue keeps, for every
+// token and 128 columns, the maximum and the sum of exp(logit - maximum); a second launch joins these; the backward pass computes the
+// logits of a piece of the vocabulary again and turns them, in registers, into their gradient P, of which one piece at a time exists:
+//   loss_t = m_t + log s_t - l[t,y_t],   P[t,v] = (exp(l[t,v] - m_t) / s_t - [v = y_t]) * dloss / n,   dx = P W,   dW = P^T x
+// (m_t, s_t: a row's maximum and sum.  The pair is kept instead of m + log s, whose rounding would stand in every exp.)
+//
+// All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], both operands contiguous in k, bf16 on
+// v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
+// to LDS in a ring of five steps of 32 k; persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that
+// head_images_kernel writes, transposed where the product sums over rows, zero where k goes beyond the matrix; W itself is read in
+// place where its rows are whole and aligned.
+// fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
+// six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first); what is left out is below 2^-24 of a term.
+// Batches of up to 16 tokens stream W once through registers (head_few_kernel).
+// Bound: the matrix cores (2 T V d for the loss, 8 T V d with gradients, logits formed twice); few tokens: the bytes of W.
+#include <algorithm>
+
+#include "common.h"
+#include "pack.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
+#define HP_BK 32
+#define HP_TILE 256
+#define HP_TILE_BYTES (HP_TILE * HP_BK * 2)     // one operand's step: 16 KiB
+#define HP_STAGE_BYTES (2 * HP_TILE_BYTES)
+#define HP_STAGES 5
+#define HP_SMEM (HP_STAGES * HP_STAGE_BYTES)    // 160 KiB
+#define HEAD_FEW 16                             // tokens of the streaming kernel
+
+// What a product does with its tile:
+//   LSE  rows = tokens, columns = vocabulary: (max, sum) of every token and 128 columns, the target's logit
+//   P    the same product: gradient of the logits as tile images (1 or 3 parts)
+//   ACC  fp32 sums, ADD: added to what is there (dx over the pieces; a k slice has a slab of its own)
+//   OUT  the caller's rows (dW)
+enum { HEAD_LSE = 0, HEAD_P, HEAD_ACC, HEAD_ADD, HEAD_OUT };
+
+struct head_prod {
+    const unsigned char *A, *B;      // tile images, or B: rows of b_ld bytes
+    size_t planeA, planeB;           // bytes from one part to the next (fp32)
+    size_t b_ld;                     // 0: image
+    int kt;                          // k steps (even, 8 or more)
+    int M, N, mt, nt, slices;        // mt row tiles of `th` rows (64, 128, 192 or 256), nt column tiles of 256
+    int th;
+    // epilogues
+    const int32_t *targets;
+    const float *row_stats, *mean, *dloss;
+    int T, V, v0;                    // tokens, vocabulary, first column of the piece
+    float2 *part;                    // LSE
+    float *tlogit;
+    unsigned char *P;                // P
+    size_t planeP;
+    float *C;                        // ACC: slabs [slices][rows][ld]
+    size_t slab;
+    int ld;                          // (a multiple of 256)
+    void *out;                       // OUT: row-major, ld = N
+    int out_bf, out_vec;
+};
+
+template <int LDS_OFF>
+__device__ __forceinline__ void hp_dma16(const void *sbase, uint32_t voff, uint32_t lds_base)
+{
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(sbase), "v"(voff), "s"(lds_base), "n"(LDS_OFF)
+                 : "memory", "scc");
+}
+
+__device__ __forceinline__ const unsigned char *hp_uniform(const unsigned char *p)
+{
+    const uint64_t v = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (const unsigned char *)(((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ uint32_t hp_pack2(float lo, float hi)
+{
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const b2 r = __builtin_convertvector(f2{lo, hi}, b2);
+    return *(const uint32_t *)&r;
+}
+
+// part q (0 leading) of an fp32 number: 8 bits each, by truncation.  A number that is infinite or none has it all in the leading part.
+__device__ __forceinline__ void hp_split(float v, uint32_t (&h)[3])
+{
+    const uint32_t u = __float_as_uint(v);
+    h[0] = u >> 16;
+    h[1] = h[2] = 0;
+    if ((u & 0x7f800000u) == 0x7f800000u) {
+        if (u & 0xffffu) h[0] |= 0x40u;  // no number stays none
+        return;
+    }
+    const float r1 = v - __uint_as_float(u & 0xffff0000u);
+    const uint32_t u1 = __float_as_uint(r1);
+    h[1] = u1 >> 16;
+    h[2] = __float_as_uint(r1 - __uint_as_float(u1 & 0xffff0000u)) >> 16;
+}
+
+// One tile of a product, or a k slice of one
+struct hp_item {
+    const unsigned char *A, *B;   // first step of the tile's rows and columns
+    int row0, n0, slice;          // first row (-1: no item) and column
+    int kt;                       // steps (of a part)
+};
+
+__device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
+{
+    hp_item it = {};
+    it.row0 = -1;
+    const int per = p.mt * p.nt;
+    if (idx >= per * p.slices) return it;
+    // column tiles outside, up to 8 row tiles inside: the 32 neighbours that an XCD works on share operand tiles in its L2
+    const int sl = idx / per, rem = idx - sl * per, g = rem / (8 * p.nt), gm = min(8, p.mt - 8 * g), r2 = rem - g * 8 * p.nt, n = r2 / gm;
+    it.row0 = __builtin_amdgcn_readfirstlane((8 * g + (r2 - n * gm)) * p.th);
+    it.n0 = __builtin_amdgcn_readfirstlane(n * HP_TILE);
+    it.slice = __builtin_amdgcn_readfirstlane(sl);
+    const int first = ((it.slice * p.kt) / p.slices) & ~1;
+    it.kt = __builtin_amdgcn_readfirstlane((it.slice + 1 == p.slices ? p.kt : (((it.slice + 1) * p.kt) / p.slices) & ~1) - first);
+    const size_t rg = (size_t)p.kt * 8192;  // bytes of a row group of an image
+    it.A = hp_uniform(p.A + (size_t)(it.row0 >> 7) * rg + (size_t)first * 8192);
+    it.B = hp_uniform(p.b_ld == 0 ? p.B + (size_t)(it.n0 >> 7) * rg + (size_t)first * 8192 : p.B + (size_t)it.n0 * p.b_ld + (size_t)first * 64);
+    return it;
+}
+// what the lane adds for the wave's loads: blocks of 16 rows wave + 4 n of the item's rows and columns
+__device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_item &it, int wave, int lane, uint32_t (&va)[4], uint32_t (&vb)[4])
+{
+    const uint32_t rg = (uint32_t)p.kt * 8192u;
+    const int blk0 = (it.row0 & 127) >> 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int q = wave + 4 * k;
+        const bool valid = 16 * q < p.th && it.row0 + 16 * q < p.M;  // (a block without rows: every lane reads the first 16 bytes of the item's first block)
+        const int b = blk0 + (valid ? q : 0);
+        va[k] = (uint32_t)(b >> 3) * rg + (uint32_t)(b & 7) * 1024u + (valid ? (uint32_t)lane * 16u : 0u);
+        if (p.b_ld == 0) {
+            vb[k] = (uint32_t)(q >> 3) * rg + (uint32_t)(q & 7) * 1024u + (uint32_t)lane * 16u;
+        } else {
+            const int r = 16 * q + (lane >> 2);
+            vb[k] = (uint32_t)min(r, p.N - 1 - it.n0) * (uint32_t)p.b_ld + (uint32_t)(((lane & 3) ^ pk_swz(r)) << 4);
+        }
+    }
+}
+
+// pairs of parts in the order they are added: (A, B) = mm, lh, hl, mh, hm, hh
+#define HP_SEG_A 0x001021  // nibble s = part of segment s, from the right: 1, 2, 0, 1, 0, 0
+#define HP_SEG_B 0x010201  // 1, 0, 2, 0, 1, 0
+
+struct hp_state {
+    int cur;                             // ring position
+    bf16x8_t fa0[8], fb0[8], fa1[8], fb1[8];
+    const unsigned char *lA, *lB;        // where the loads have got to
+    uint32_t va[4], vb[4];
+};
+
+// Loads and fragments of the ring, the MFMAs of a step.  The first 8 groups of 4 MFMAs carry the 16 fragment reads of the
+// next step, every other group one of the 8 direct loads of the step five ahead.
+#define HP_READ(FA, FB, r)                                                                            \
+    do {                                                                                              \
+        if ((r) < 8) FB[(r) & 7] = *(const bf16x8_t *)(((r) & 1 ? rb1 : rb0) + (((r) & 7) >> 1) * 2048u); \
+        else FA[((r) - 8) & 7] = *(const bf16x8_t *)(ra + (((r) - 8) & 7) * 2048u);                   \
+    } while (0)
+#define HP_LOAD(l, sb)                                                                     \
+    do {                                                                                   \
+        if ((l) < 4) hp_dma16<((l) & 3) * 4096>(lA, st.va[(l) & 3], sb);                   \
+        else hp_dma16<HP_TILE_BYTES + ((l) & 3) * 4096>(lB, st.vb[(l) & 3], sb);           \
+    } while (0)
+#define HP_MFMA(PA, PB, Z, iu, c)                                                                                                    \
+    do {                                                                                                                             \
+        if ((iu) < NU)                                                                                                               \
+            acc[(iu) % NU][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(PB[c], PA[iu], (Z) ? zero4 : acc[(iu) % NU][c], 0, 0, 0);    \
+    } while (0)
+#define HP_GROUP(PA, PB, QA, QB, Z, g)                     \
+    do {                                                   \
+        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1));       \
+        if ((g) < 8) {                                     \
+            HP_READ(QA, QB, 2 * (g));                      \
+            HP_READ(QA, QB, 2 * (g) + 1);                  \
+        }                                                  \
+        __builtin_amdgcn_sched_barrier(0);                 \
+        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 1);   \
+        if ((g) & 1) HP_LOAD((g) >> 1, sb);                \
+        __builtin_amdgcn_sched_barrier(0);                 \
+        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 2);   \
+        __builtin_amdgcn_sched_barrier(0);                 \
+        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 3);   \
+        __builtin_amdgcn_sched_barrier(0);                 \
+    } while (0)
+#define HP_STEP(PA, PB, QA, QB, Z)                                                                          \
+    do {                                                                                                    \
+        HP_GROUP(PA, PB, QA, QB, Z, 0); HP_GROUP(PA, PB, QA, QB, Z, 1); HP_GROUP(PA, PB, QA, QB, Z, 2);     \
+        HP_GROUP(PA, PB, QA, QB, Z, 3); HP_GROUP(PA, PB, QA, QB, Z, 4); HP_GROUP(PA, PB, QA, QB, Z, 5);     \
+        HP_GROUP(PA, PB, QA, QB, Z, 6); HP_GROUP(PA, PB, QA, QB, Z, 7); HP_GROUP(PA, PB, QA, QB, Z, 8);     \
+        HP_GROUP(PA, PB, QA, QB, Z, 9); HP_GROUP(PA, PB, QA, QB, Z, 10); HP_GROUP(PA, PB, QA, QB, Z, 11);   \
+        HP_GROUP(PA, PB, QA, QB, Z, 12); HP_GROUP(PA, PB, QA, QB, Z, 13); HP_GROUP(PA, PB, QA, QB, Z, 14);  \
+        HP_MFMA(PA, PB, Z, 7, 4);                                                                           \
+        __builtin_amdgcn_sched_barrier(0);                                                                  \
+        HP_MFMA(PA, PB, Z, 7, 5);                                                                           \
+        HP_LOAD(7, sb);                                                                                     \
+        __builtin_amdgcn_sched_barrier(0);                                                                  \
+        HP_MFMA(PA, PB, Z, 7, 6);                                                                           \
+        cur = cur + 1 == HP_STAGES ? 0 : cur + 1;                                                           \
+        sb = lds_wave + cur * HP_STAGE_BYTES;                                                               \
+        lA += 8192;                                                                                         \
+        lB += stepB;                                                                                        \
+        __builtin_amdgcn_sched_barrier(0);                                                                  \
+        HP_MFMA(PA, PB, Z, 7, 7);                                                                           \
+        {                                                                                                   \
+            const unsigned char *sn = smem + (cur + 1 == HP_STAGES ? 0 : cur + 1) * HP_STAGE_BYTES;         \
+            ra = sn + pa;                                                                                   \
+            rb0 = sn + pb0;                                                                                 \
+            rb1 = sn + pb1;                                                                                 \
+        }                                                                                                   \
+        __builtin_amdgcn_sched_barrier(0);                                                                  \
+        asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)" ::: "memory");                                        \
+        __syncthreads();                                                                                    \
+    } while (0)
+
+// exp of a difference to the row's maximum.  bf16: v_exp_f32 of v log2(e), whose rounding weighs a few 2^-24 for the differences that
+// count; fp32: what the rounding of the product leaves is put back, exp2(t + e) = exp2(t) (1 + e ln 2).
+// (differences below -200 are 0 either way; a comparison, not a maximum, so that no number stays none)
+template <int NSEG>
+__device__ __forceinline__ float hp_exp(float v)
+{
+    if (NSEG == 1) return __expf(v);
+    v = v < -200.0f ? -200.0f : v;
+    const float t = v * 1.44269504088896341f;
+    const float e = fmaf(v, 1.92596299e-8f, fmaf(v, 1.44269504088896341f, -t));
+    const float r = __builtin_amdgcn_exp2f(t);
+    return fmaf(r, e * 0.693147181f, r);
+}
+
+// Stores into the caller's rows that fall away where `ok` is false, without a branch: a buffer store beyond its range does nothing.
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+#define HP_OUTSIDE 0xffffffffu
+
+// A tile of 32 NU rows by 256 columns.  acc[iu][c][r]: row 16 (2 iu + wm) + lane % 16, column 128 wn + 16 c + 4 (lane / 16) + r.
+template <int NU, int EPI, int NSEG>
+__device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane)
+{
+    const int wm = wave >> 1, wn = wave & 1, l16 = lane & 15, lq = lane >> 4;
+    const int kt = __builtin_amdgcn_readfirstlane(it.kt);
+    const size_t stepB = p.b_ld == 0 ? 8192 : 64;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
+    const uint32_t lds_wave = lds0 + wave * 1024;
+    const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
+    const uint32_t pb0 = HP_TILE_BYTES + (uint32_t)(wn * 128 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16)) << 4);
+    const uint32_t pb1 = HP_TILE_BYTES + (uint32_t)(wn * 128 + 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | 16)) << 4);
+    int cur = __builtin_amdgcn_readfirstlane(st.cur);
+    const unsigned char *lA = hp_uniform(st.lA), *lB = hp_uniform(st.lB);
+    nxt = hp_make_item(p, next_idx);
+    uint32_t sb = lds_wave + cur * HP_STAGE_BYTES;
+    const unsigned char *ra, *rb0, *rb1;
+    {
+        const unsigned char *sn = smem + (cur + 1 == HP_STAGES ? 0 : cur + 1) * HP_STAGE_BYTES;
+        ra = sn + pa;
+        rb0 = sn + pb0;
+        rb1 = sn + pb1;
+    }
+    f32x4_t acc[NU][8];
+    const f32x4_t zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    // The steps of a pair of parts two at a time (their number is even, at least 8).  The loads of the last five are the next pair's
+    // or the next item's first (behind the last item: this one's once more, which nobody reads).
+    if (NSEG > 1) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[i][c] = zero4;
+    }
+#pragma unroll 1
+    for (int seg = 0; seg < NSEG; ++seg) {
+        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, NSEG == 1);
+        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
+#pragma unroll 1
+        for (int k = 2; k < kt - 6; k += 2) {
+            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
+            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
+        }
+        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
+        {
+            const int ns = seg + 1 < NSEG ? seg + 1 : 0;
+            const bool more = ns == 0 && nxt.row0 >= 0;
+            const size_t a0 = NSEG > 1 ? (size_t)((HP_SEG_A >> (4 * ns)) & 3) * p.planeA : 0, b0 = NSEG > 1 ? (size_t)((HP_SEG_B >> (4 * ns)) & 3) * p.planeB : 0;
+            lA = hp_uniform((more ? nxt.A : it.A) + a0);
+            lB = hp_uniform((more ? nxt.B : it.B) + b0);
+            if (more) hp_lane_offsets(p, nxt, wave, lane, st.va, st.vb);
+        }
+        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
+            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
+        }
+    }
+    st.cur = cur;
+    st.lA = lA;
+    st.lB = lB;
+
+    const int col0 = it.n0 + wn * 128 + 4 * lq;  // column of acc[.][0][0]
+    if (EPI == HEAD_LSE) {
+        const bool whole = it.n0 + wn * 128 + 128 <= p.N;
+#pragma unroll
+        for (int iu = 0; iu < NU; ++iu) {
+            __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
+            const int t = it.row0 + 16 * (2 * iu + wm) + l16;
+            const bool held = t < p.M;
+            float m = -INFINITY, s = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (!whole && col0 + 16 * c + r >= p.N) acc[iu][c][r] = -INFINITY;
+                    m = fmaxf(m, acc[iu][c][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const float m0 = m == -INFINITY ? 0.0f : m;  // (no column, or every logit -inf: the sum is 0)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += hp_exp<NSEG>(acc[iu][c][r] - m0);
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (held && lq == 0) p.part[(size_t)((p.v0 + it.n0) / 128 + wn) * p.T + t] = make_float2(m, s);
+            const int y = held ? p.targets[t] - p.v0 - it.n0 - wn * 128 : -1;  // the target's column among the wave's 128
+            if (__ballot(y >= 0 && y < 128 && it.n0 + wn * 128 + y < p.N)) {
+                const int k = y - 4 * lq;
+                float v = 0.0f;
+                bool mine = false;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (k == 16 * c + r) v = acc[iu][c][r], mine = true;
+                if (mine && y >= 0 && it.n0 + wn * 128 + y < p.N) p.tlogit[t] = v;
+            }
+        }
+    } else if (EPI == HEAD_P) {
+        // (rows behind the last token are written with what the last one's statistics give: nothing reads them)
+        const bool whole = it.n0 + wn * 128 + 128 <= p.N;
+        const float gs = (p.dloss ? p.dloss[0] : 1.0f) / fmaxf(p.mean[1], 1.0f);
+        const int KTp = p.nt * (HP_TILE / HP_BK);
+        constexpr int NP = NSEG > 1 ? 3 : 1;
+        // (to the image's end: rows of the tile behind it fall away)
+        const int rgs = ((p.M + 127) >> 7) - (it.row0 >> 7), kb = (it.n0 >> 5) + 4 * wn;
+        __amdgpu_buffer_rsrc_t rs[NP];
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+            rs[q] = __builtin_amdgcn_make_buffer_rsrc((void *)hp_uniform(p.P + q * p.planeP + (size_t)(it.row0 >> 7) * KTp * 8192 + (size_t)kb * 8192), 0,
+                                                      (rgs * KTp - kb) * 8192, 0x00020000);
+#pragma unroll
+        for (int iu = 0; iu < NU; ++iu) {
+            __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
+            const int row = it.row0 + 16 * (2 * iu + wm) + l16, t = min(row, p.M - 1);
+            const int y = p.targets[t];
+            const bool held = y >= 0 && y < p.V;
+            const float m = p.row_stats[t], f = gs / p.row_stats[p.T + t];
+            const int k = y - p.v0 - col0, end = held ? (whole ? 0x7fffffff : p.N - col0) : 0;  // columns from `end` on are zero
+            const uint32_t rg0 = (uint32_t)((row >> 7) - (it.row0 >> 7)) * (uint32_t)KTp * 8192u + (uint32_t)(((row & 127) >> 4) * 1024 + (row & 15) * 64 + (lq & 1) * 8);
+            const uint32_t o0 = rg0 + (uint32_t)(((lq >> 1) ^ pk_swz(row)) << 4), o1 = rg0 + (uint32_t)(((2 + (lq >> 1)) ^ pk_swz(row)) << 4);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = hp_exp<NSEG>(acc[iu][c][r] - m) * f;
+                    v[r] -= k == 16 * c + r ? gs : 0.0f;
+                    v[r] = 16 * c + r < end ? v[r] : 0.0f;
+                }
+                const uint32_t at = (c & 1 ? o1 : o0) + (c >> 1) * 8192;
+                if (NSEG == 1) {
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{hp_pack2(v[0], v[1]), hp_pack2(v[2], v[3])}, rs[0], at, 0, 0);
+                } else {
+                    uint32_t h[4][3];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) hp_split(v[r], h[r]);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{h[0][q] | h[1][q] << 16, h[2][q] | h[3][q] << 16}, rs[q % NP], at, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+    } else if (EPI == HEAD_ACC || EPI == HEAD_ADD) {
+        // (a slab has room for whole tiles)
+        float *tile = p.C + (size_t)it.slice * p.slab + (size_t)it.row0 * p.ld + it.n0 + wn * 128;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)hp_uniform((const unsigned char *)tile), 0, 256 * p.ld * 4, 0x00020000);
+        uint32_t off = (uint32_t)(16 * wm + l16) * (uint32_t)p.ld * 4u + (uint32_t)lq * 16u;
+#pragma unroll
+        for (int iu = 0; iu < NU; ++iu) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (EPI == HEAD_ADD) {
+                f32x4_t old[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const u32x4_t u = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 64 * c, 0, 0);
+                    old[c] = *(const f32x4_t *)&u;
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) acc[iu][c] += old[c];
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t *)&acc[iu][c], rs, off + 64 * c, 0, 0);
+            off += 32u * (uint32_t)p.ld * 4u;
+        }
+    } else {
+        const int es = p.out_bf ? 2 : 4;
+        // from the tile's first row on: at most 256 rows of N values
+        const uint64_t tile = (uint64_t)p.out + (uint64_t)it.row0 * p.N * es;
+        const int rows = min(32 * NU, p.M - it.row0);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)hp_uniform((const unsigned char *)tile), 0, rows * p.N * es, 0x00020000);
+        const int step = 32 * p.N * es, row1 = 16 * wm + l16;
+        int off = (row1 * p.N + col0) * es;
+        const int cols = p.N - col0;  // columns from there on
+#pragma unroll
+        for (int iu = 0; iu < NU; ++iu) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (p.out_vec) {  // (N is a multiple of 4)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const f32x4_t v = acc[iu][c];
+                    const uint32_t at = 16 * c < cols ? (uint32_t)(off + 16 * c * es) : HP_OUTSIDE;  // (rows behind the last: beyond the range as well)
+                    if (p.out_bf) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{hp_pack2(v[0], v[1]), hp_pack2(v[2], v[3])}, rs, at, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t *)&v, rs, at, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = acc[iu][c][r];
+                        const uint32_t at = 16 * c + r < cols ? (uint32_t)(off + (16 * c + r) * es) : HP_OUTSIDE;
+                        if (p.out_bf) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)hp_pack2(v, 0.0f), rs, at, 0, 0);
+                        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, at, 0, 0);
+                    }
+            }
+            off += step;
+        }
+    }
+}
+
+// Persistent: workgroup w takes items w, w + n, ... in rounds of n = gridDim.x; within a round XCD x (w % 8) takes neighbouring items.
+template <int NU, int EPI, int NSEG>
+__global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
+{
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1, l16 = lane & 15, lq = lane >> 4;
+    const int n_wg = gridDim.x;
+    const int at = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    int idx = at;
+    hp_item it = hp_make_item(p, idx);
+    if (it.row0 < 0) return;
+    hp_state st;
+    const unsigned char *lA = hp_uniform(it.A + (NSEG > 1 ? (size_t)(HP_SEG_A & 3) * p.planeA : 0));
+    const unsigned char *lB = hp_uniform(it.B + (NSEG > 1 ? (size_t)(HP_SEG_B & 3) * p.planeB : 0));
+    hp_lane_offsets(p, it, wave, lane, st.va, st.vb);
+    const size_t stepB = p.b_ld == 0 ? 8192 : 64;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
+    for (int s5 = 0; s5 < HP_STAGES; ++s5) {  // the first item's steps 0 .. 4 (of 8 or more of its first part)
+        const uint32_t sb = lds0 + wave * 1024 + s5 * HP_STAGE_BYTES;
+        HP_LOAD(0, sb); HP_LOAD(1, sb); HP_LOAD(2, sb); HP_LOAD(3, sb);
+        HP_LOAD(4, sb); HP_LOAD(5, sb); HP_LOAD(6, sb); HP_LOAD(7, sb);
+        lA += 8192;
+        lB += stepB;
+    }
+    st.lA = lA;
+    st.lB = lB;
+    asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+    __syncthreads();
+    {
+        const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const uint32_t pb = HP_TILE_BYTES + (uint32_t)(wn * 128 + 16 * (r & 1) + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | ((r & 1) << 4))) << 4);
+            st.fb0[r] = *(const bf16x8_t *)(smem + pb + (r >> 1) * 2048u);
+            st.fa0[r] = *(const bf16x8_t *)(smem + pa + r * 2048u);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)" ::: "memory");  // step 1 has landed; every wave has taken step 0 out of its stage
+    __syncthreads();
+    st.cur = 0;
+#pragma unroll 1
+    for (;;) {
+        idx += n_wg;
+        hp_item nxt;
+        hp_run_item<NU, EPI, NSEG>(smem, st, p, it, nxt, idx, wave, lane);
+        if (nxt.row0 < 0) break;
+        it = nxt;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads behind the last item land in LDS that nobody reads)
+}
+
+// ---- tile images ----
+// Rows 64 bx .., columns 64 by .. of a row-major matrix [R,K] as parts of a tile image (`img`, KTi k steps a row group) and of the image
+// of its transpose (`tr`, KTt k steps); zero outside the matrix and in rows whose token has no target.
+template <bool BF>
+__global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict__ src, int R, int K, int vec, const int32_t *__restrict__ targets, int V,
+                                                          unsigned char *__restrict__ img, int KTi, size_t plane_i, unsigned char *__restrict__ tr, int KTt, size_t plane_t)
+{
+    constexpr int NP = BF ? 1 : 3;
+    __shared__ __attribute__((aligned(16))) uint16_t tile[NP][64][64];
+    const int tid = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int idx = tid + u * 256, rr = idx >> 3, ch = idx & 7, row = r0 + rr, c = c0 + ch * 8;
+        uint16_t e[NP][8];
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[q][k] = 0;
+        bool held = row < R && c < K;
+        if (held && targets) held = targets[row] >= 0 && targets[row] < V;
+        if (held) {
+            const size_t at = (size_t)row * K + c;
+            if (BF) {
+                const bf16_t *s = (const bf16_t *)src + at;
+                if (vec) {
+                    *(uint4 *)&e[0][0] = *(const uint4 *)s;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (c + k < K) e[0][k] = s[k];
+                }
+            } else {
+                const float *s = (const float *)src + at;
+                float v[8];
+                if (vec) {
+                    *(float4 *)&v[0] = *(const float4 *)s;
+                    *(float4 *)&v[4] = *(const float4 *)(s + 4);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = c + k < K ? s[k] : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    uint32_t h[3];
+                    hp_split(v[k], h);
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) e[q][k] = (uint16_t)h[q];
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if (img) *(uint4 *)(img + q * plane_i + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = *(const uint4 *)&e[q][0];
+            if (tr) *(uint4 *)&tile[q][rr][(ch ^ (2 * (rr >> 3) & 6)) * 8] = *(const uint4 *)&e[q][0];
+        }
+    }
+    if (!tr) return;
+    __syncthreads();
+    // (column chunks swapped by row group: the chunks that a wave reads for one destination row sit in different banks)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int blk = (tid >> 6) + 4 * u, l = tid & 63;
+        const int cc = (blk & 3) * 16 + (l >> 2), kc = (blk >> 2) * 4 + (l & 3);  // destination row c0 + cc, k places 8 kc .. of the 64
+        const int col = ((cc >> 3) ^ (2 * kc & 6)) * 8 + (cc & 7);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = tile[q][kc * 8 + 2 * k][col] | (uint32_t)tile[q][kc * 8 + 2 * k + 1][col] << 16;
+            *(uint4 *)(tr + q * plane_t + pk_chunk_off(c0 + cc, (r0 >> 5) + (kc >> 2), kc & 3, KTt)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
+}
+
+// Transposes a tile image: rows 64 bx .., columns 64 by .. of `src` (KTs k steps; rows from R on count as zero), part blockIdx.z
+__global__ __launch_bounds__(256) void head_transpose_kernel(const unsigned char *__restrict__ src, int R, int KTs, size_t plane_s, unsigned char *__restrict__ dst,
+                                                             int KTd, size_t plane_d)
+{
+    __shared__ __attribute__((aligned(16))) uint16_t tile[64][64];
+    const int tid = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    src += blockIdx.z * plane_s;
+    dst += blockIdx.z * plane_d;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int idx = tid + u * 256, rr = idx >> 3, ch = idx & 7, c = c0 + ch * 8;
+        uint4 v = {0u, 0u, 0u, 0u};
+        if (r0 + rr < R) v = *(const uint4 *)(src + pk_chunk_off(r0 + rr, c >> 5, (c & 31) >> 3, KTs));
+        *(uint4 *)&tile[rr][(ch ^ (2 * (rr >> 3) & 6)) * 8] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int blk = (tid >> 6) + 4 * u, l = tid & 63;
+        const int cc = (blk & 3) * 16 + (l >> 2), kc = (blk >> 2) * 4 + (l & 3);
+        const int col = ((cc >> 3) ^ (2 * kc & 6)) * 8 + (cc & 7);
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = tile[kc * 8 + 2 * k][col] | (uint32_t)tile[kc * 8 + 2 * k + 1][col] << 16;
+        *(uint4 *)(dst + pk_chunk_off(c0 + cc, (r0 >> 5) + (kc >> 2), kc & 3, KTd)) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// ---- a few tokens: W streams through registers ----
+// A workgroup takes 16 NF rows of W; its four waves share k.  Lane l holds 16 bytes (8 or 4 k) of row l % 16 and of token l % 16, k
+// chunk l / 16: a fragment of v_mfma_f32_16x16x32_bf16, or four of v_mfma_f32_16x16x4_f32 (any order of k serves, as long as both
+// operands have it).  The waves' sums are added in LDS in wave order; (max, sum) of each token over the rows go to `part`.
+template <bool BF, bool VEC>
+__device__ __forceinline__ void head_few_load(const unsigned char *p, int k, int K, f32x4_t &v)  // p: k = 0 of the row; zero from K on
+{
+    constexpr int W = BF ? 8 : 4;
+    v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if (VEC) {
+        if (k < K) v = *(const f32x4_t *)(p + (size_t)k * (BF ? 2 : 4));
+    } else {
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (k + j < K) {
+                if (BF) u[j >> 1] |= (uint32_t)((const bf16_t *)p)[k + j] << (16 * (j & 1));
+                else u[j & 3] = ((const uint32_t *)p)[k + j];
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(u[j]);
+    }
+}
+template <bool BF, bool VEC, int NF>
+__global__ __launch_bounds__(256) void head_few_kernel(const void *__restrict__ x, const void *__restrict__ w, int T, int V, int K, const int32_t *__restrict__ targets,
+                                                       float2 *__restrict__ part, float *__restrict__ tlogit)
+{
+    __shared__ f32x4_t sums[3][NF][64];
+    constexpr int KS = BF ? 32 : 16, ES = BF ? 2 : 4, UN = 8 / NF;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
+    const int v0 = blockIdx.x * 16 * NF;
+    const unsigned char *xr = (const unsigned char *)x + (size_t)min(l16, T - 1) * K * ES;
+    const unsigned char *wr[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) wr[f] = (const unsigned char *)w + (size_t)min(v0 + 16 * f + l16, V - 1) * K * ES;
+    f32x4_t acc[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const int steps = (K + KS - 1) / KS, first = wave * steps / 4, last = (wave + 1) * steps / 4;
+    for (int s = first; s < last; s += UN) {
+        f32x4_t xv[UN], wv[UN][NF];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int k = s + u < last ? (s + u) * KS + lq * (KS / 4) : K;  // (behind the wave's steps: zeros)
+            head_few_load<BF, VEC>(xr, k, K, xv[u]);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) head_few_load<BF, VEC>(wr[f], k, K, wv[u][f]);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                if (BF) {
+                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8_t *)&wv[u][f], *(const bf16x8_t *)&xv[u], acc[f], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u][f][j], xv[u][j], acc[f], 0, 0, 0);
+                }
+            }
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) sums[wave - 1][f][lane] = acc[f];
+    __syncthreads();
+    if (wave > 0) return;
+    const int t = l16;
+    float m = -INFINITY, s = 0.0f;
+    const int y = t < T ? targets[t] : -1;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        acc[f] = ((acc[f] + sums[0][f][lane]) + sums[1][f][lane]) + sums[2][f][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int v = v0 + 16 * f + 4 * lq + r;
+            if (v >= V) acc[f][r] = -INFINITY;
+            else if (v == y && t < T) tlogit[t] = acc[f][r];
+            m = fmaxf(m, acc[f][r]);
+        }
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += BF ? __expf(acc[f][r] - m0) : expf(acc[f][r] - m0);
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (t < T && lq == 0) part[(size_t)blockIdx.x * T + t] = make_float2(m, s);
+}
+
+// ---- joins ----
+__device__ __forceinline__ float2 head_join2(float2 a, float2 b)
+{
+    const float m = fmaxf(a.x, b.x), m0 = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, a.y * expf(a.x - m0) + b.y * expf(b.x - m0));
+}
+// mean[0] = sum of the losses / n, mean[1] = n, by one workgroup (sums in double: a large batch's do not lose the small losses)
+__device__ void head_mean(const float *loss, const int32_t *targets, int T, int V, float *mean)
+{
+    __shared__ double sd[16];
+    __shared__ int sn[16];
+    double a = 0.0;
+    int n = 0;
+    for (int t = threadIdx.x; t < T; t += blockDim.x) {
+        const bool held = targets[t] >= 0 && targets[t] < V;
+        n += held;
+        if (held) a += (double)loss[t];
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        a += __shfl_xor(a, m, 64);
+        n += __shfl_xor(n, m, 64);
+    }
+    if ((threadIdx.x & 63) == 0) sd[threadIdx.x >> 6] = a, sn[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) a += sd[w], n += sn[w];
+        mean[0] = n > 0 ? (float)(a / n) : 0.0f;
+        mean[1] = (float)n;
+    }
+}
+// (max, sum) of a token over nb column blocks: TL tokens (a power of two) a workgroup, 1024 / TL threads each, joined in a fixed order.
+// A launch of one workgroup forms the mean too.
+__global__ __launch_bounds__(1024) void head_join_kernel(const float2 *__restrict__ part, int nb, const float *__restrict__ tlogit, const int32_t *__restrict__ targets,
+                                                         int T, int V, int TL, float *__restrict__ loss, float *__restrict__ row_stats, float *__restrict__ mean)
+{
+    __shared__ float2 red[1024];
+    const int tid = threadIdx.x, sub = tid / TL, n_sub = 1024 / TL, t = blockIdx.x * TL + (tid & (TL - 1));
+    // the maximum first: one exp a block instead of two
+    float m = -INFINITY, s = 0.0f;
+    if (t < T) {
+#pragma unroll 8
+        for (int b = sub; b < nb; b += n_sub) m = fmaxf(m, part[(size_t)b * T + t].x);
+        const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll 8
+        for (int b = sub; b < nb; b += n_sub) {
+            const float2 v = part[(size_t)b * T + t];
+            s += v.y * expf(v.x - m0);
+        }
+    }
+    red[tid] = make_float2(m, s);
+    __syncthreads();
+    for (int h = 512; h >= TL; h >>= 1) {
+        if (tid < h) red[tid] = head_join2(red[tid], red[tid + h]);
+        __syncthreads();
+    }
+    if (tid < TL && t < T) {
+        const float2 v = red[tid];
+        const int y = targets[t];
+        loss[t] = y >= 0 && y < V ? (v.x - tlogit[t]) + logf(v.y) : 0.0f;
+        if (row_stats) {
+            row_stats[t] = v.x;
+            row_stats[T + t] = v.y;
+        }
+    }
+    if (gridDim.x == 1) {
+        __syncthreads();
+        head_mean(loss, targets, T, V, mean);
+    }
+}
+__global__ __launch_bounds__(1024) void head_mean_kernel(const float *loss, const int32_t *__restrict__ targets, int T, int V, float *__restrict__ mean)
+{
+    head_mean(loss, targets, T, V, mean);
+}
+
+// dx: the slabs added in slice order, rounded once; rows without a target are zero
+template <bool BF>
+__global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ targets, int T, int V,
+                                                      int d, void *__restrict__ dx)
+{
+    const int t = blockIdx.x, y = targets[t];
+    const bool held = y >= 0 && y < V;
+    for (int c = blockIdx.y * 256 + threadIdx.x; c < d; c += gridDim.y * 256) {
+        float s = 0.0f;
+        if (held)
+            for (int k = 0; k < slices; ++k) s += slabs[(size_t)k * slab + (size_t)t * ld + c];
+        if (BF) ((bf16_t *)dx)[(size_t)t * d + c] = f32_to_bf16(s);
+        else ((float *)dx)[(size_t)t * d + c] = s;
+    }
+}
+__global__ __launch_bounds__(256) void head_zero_kernel(void *p, size_t bytes)  // (memset nodes are not for captured graphs)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < bytes; i += (size_t)gridDim.x * 256) ((unsigned char *)p)[i] = 0;
+}
+
+// ---- host side ----
+static size_t up_to(size_t x, size_t m) { return (x + m - 1) / m * m; }
+static int k_pad(int n) { return std::max(256, (int)up_to(n, 64)); }  // k of a product: whole pairs of steps, eight steps or more
+
+// Sizes of a call and where its parts lie in the workspace
+struct head_plan {
+    int planes, dp, Tp, piece, pieces;  // k of d, k of T, columns of a piece (a multiple of 256)
+    int nb;                             // column blocks of the forward pass
+    int slices;                         // k slices of dx
+    bool direct, few;
+    size_t x_img, xT_img, w_img, wT_img, p_img, pT_img, slabs, part, tlogit, bytes;
+    size_t x_plane, xT_plane, w_plane, wT_plane, p_plane, pT_plane, slab;
+};
+
+static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool backward)
+{
+    head_plan h = {};
+    h.planes = a.dtype == OMEGA_DTYPE_BF16 ? 1 : 3;
+    h.few = !backward && a.T <= HEAD_FEW;
+    h.dp = k_pad(a.d);
+    h.Tp = k_pad(a.T);
+    // W in place: bf16 rows of whole pairs of k steps, 16-byte aligned (tile offsets within 32 bits)
+    h.direct = h.planes == 1 && a.d == h.dp && (uintptr_t)a.w % 16 == 0 && a.d <= (1 << 20);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at += up_to(bytes, 1024);
+        return o;
+    };
+    if (h.few) {
+        h.nb = a.V > 0 ? ceil_div(a.V, 16) : 0;  // (an upper bound: workgroups of 16 rows)
+        h.part = take((size_t)h.nb * a.T * sizeof(float2));
+        h.tlogit = take((size_t)a.T * 4);
+        h.bytes = at;
+        return h;
+    }
+    // what a column of the vocabulary needs while its piece is worked on
+    const size_t per = backward ? (size_t)h.planes * 2 * (2 * (size_t)h.Tp + 2 * (size_t)h.dp) : h.direct ? 0 : (size_t)h.planes * 2 * h.dp;
+    const size_t budget = (size_t)1 << 30;
+    const int all = (int)up_to(a.V, 256);
+    h.piece = per == 0 ? all : (int)std::min<size_t>(all, std::max<size_t>(256, budget / per / 256 * 256));
+    h.pieces = ceil_div(a.V, h.piece);
+    h.piece = (int)up_to(ceil_div(a.V, h.pieces), 256);
+    h.x_plane = up_to(backward ? h.Tp : a.T, 128) * (size_t)h.dp * 2;
+    h.x_img = take(h.x_plane * h.planes);
+    if (!h.direct) {
+        h.w_plane = (size_t)h.piece * h.dp * 2;
+        h.w_img = take(h.w_plane * h.planes);
+    }
+    if (backward) {
+        const size_t dr = up_to(h.dp, 256);
+        h.xT_plane = dr * h.Tp * 2;
+        h.xT_img = take(h.xT_plane * h.planes);
+        h.wT_plane = dr * h.piece * 2;
+        h.wT_img = take(h.wT_plane * h.planes);
+        h.p_plane = up_to(a.T, 128) * (size_t)h.piece * 2;
+        h.p_img = take(h.p_plane * h.planes);
+        h.pT_plane = (size_t)h.piece * h.Tp * 2;
+        h.pT_img = take(h.pT_plane * h.planes);
+        // few tiles of dx: the vocabulary is shared out to k slices, a slab of sums each
+        const int tiles = ceil_div(a.T, 256) * ceil_div(a.d, 256);
+        h.slices = tiles < ctx->num_cus ? std::max(1, std::min(ctx->num_cus / std::max(tiles, 1), h.piece / 32 / 16)) : 1;
+        h.slab = (up_to(a.T, 64) + 192) * up_to(h.dp, 256);  // whole tiles
+        h.slabs = take(h.slab * h.slices * 4);
+    } else {
+        h.nb = ceil_div(a.V, 256) * 2;
+        h.part = take((size_t)h.nb * a.T * sizeof(float2));
+        h.tlogit = take((size_t)a.T * 4);
+    }
+    h.bytes = at;
+    return h;
+}
+
+size_t head_workspace(const omega_ctx *ctx, const head_args &a, bool backward) { return a.T > 0 ? head_plan_of(ctx, a, backward).bytes : 0; }
+
+template <int EPI, int NSEG>
+static const void *head_kernel_of(int th)
+{
+    return th == 256   ? (const void *)head_product_kernel<8, EPI, NSEG>
+           : th == 192 ? (const void *)head_product_kernel<6, EPI, NSEG>
+           : th == 128 ? (const void *)head_product_kernel<4, EPI, NSEG>
+                       : (const void *)head_product_kernel<2, EPI, NSEG>;
+}
+template <int EPI>
+static hipError_t head_init_of()
+{
+    for (int th = 64; th <= 256; th += 64)
+        for (const void *f : {head_kernel_of<EPI, 1>(th), head_kernel_of<EPI, 6>(th)}) {
+            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, HP_SMEM);
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+hipError_t head_init(void)
+{
+    hipError_t e = head_init_of<HEAD_LSE>();
+    if (e == hipSuccess) e = head_init_of<HEAD_P>();
+    if (e == hipSuccess) e = head_init_of<HEAD_ACC>();
+    if (e == hipSuccess) e = head_init_of<HEAD_ADD>();
+    if (e == hipSuccess) e = head_init_of<HEAD_OUT>();
+    return e;
+}
+
+template <int EPI>
+static hipError_t head_product(const omega_ctx *ctx, head_prod p, int planes, hipStream_t s)
+{
+    // height of a row tile: the one whose tiles are the least work, a tile of n x 64 rows counted as n + 1/2 (its columns' loads)
+    int best = 0;
+    for (int n = 4; n >= 1; --n) {
+        const int mt = ceil_div(p.M, 64 * n), cost = mt * (2 * n + 1);
+        if (best == 0 || cost < best) {
+            best = cost;
+            p.th = 64 * n;
+            p.mt = mt;
+        }
+    }
+    p.nt = ceil_div(p.N, HP_TILE);
+    const long long items = (long long)p.mt * p.nt * p.slices;
+    if (items > 0x3fffffff) return hipErrorInvalidValue;
+    const int grid = (int)std::min<long long>(items, ctx->num_cus);
+    void *args[] = {&p};
+    return hipLaunchKernel(planes == 1 ? head_kernel_of<EPI, 1>(p.th) : head_kernel_of<EPI, 6>(p.th), dim3(grid), dim3(256), args, HP_SMEM, s);
+}
+#define HEAD_TRY(expr)                          \
+    do {                                        \
+        const hipError_t _e = (expr);           \
+        if (_e != hipSuccess) return _e;        \
+    } while (0)
+
+// Images of rows [R,K] at src: rows up to Rp (a multiple of 64), columns up to Kp
+static void head_images(const head_args &a, const void *src, int R, int K, int Rp, int Kp, const int32_t *targets, unsigned char *img, size_t plane_i,
+                        unsigned char *tr, int KTt, size_t plane_t, hipStream_t s)
+{
+    const bool bf = a.dtype == OMEGA_DTYPE_BF16;
+    const int vec = K % 8 == 0 && (uintptr_t)src % 16 == 0;
+    const dim3 grid(Rp / 64, Kp / 64);
+    if (bf) hipLaunchKernelGGL(head_images_kernel<true>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane_i, tr, KTt, plane_t);
+    else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane_i, tr, KTt, plane_t);
+}
+
+static void head_zero(void *p, size_t bytes, hipStream_t s)
+{
+    if (bytes > 0) hipLaunchKernelGGL(head_zero_kernel, dim3((unsigned)std::min<size_t>((bytes + 255) / 256, 4096)), dim3(256), 0, s, p, bytes);
+}
+
+hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s)
+{
+    if (a.T == 0) {
+        head_zero(a.mean, 8, s);
+        return hipGetLastError();
+    }
+    const head_plan h = head_plan_of(ctx, a, false);
+    unsigned char *base = (unsigned char *)ws;
+    float2 *part = (float2 *)(base + h.part);
+    float *tlogit = (float *)(base + h.tlogit);
+    const bool bf = a.dtype == OMEGA_DTYPE_BF16;
+    const size_t es = bf ? 2 : 4;
+    int nb = h.nb;
+    if (h.few) {
+        const bool vec = a.d % (bf ? 8 : 4) == 0 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
+        // 64 rows of W a workgroup read x a quarter as often as 16; vocabularies that would leave compute units idle take 16
+        const int nf = a.V >= 64 * 2 * ctx->num_cus ? 4 : 1;
+        nb = ceil_div(a.V, 16 * nf);
+#define HEAD_FEW_K(B, VV, F) hipLaunchKernelGGL((head_few_kernel<B, VV, F>), dim3(nb), dim3(256), 0, s, a.x, a.w, a.T, a.V, a.d, a.targets, part, tlogit)
+#define HEAD_FEW_F(B, VV) do { if (nf == 4) HEAD_FEW_K(B, VV, 4); else HEAD_FEW_K(B, VV, 1); } while (0)
+        if (bf) { if (vec) HEAD_FEW_F(true, true); else HEAD_FEW_F(true, false); }
+        else { if (vec) HEAD_FEW_F(false, true); else HEAD_FEW_F(false, false); }
+#undef HEAD_FEW_F
+#undef HEAD_FEW_K
+    } else {
+        head_images(a, a.x, a.T, a.d, (int)up_to(a.T, 64), h.dp, a.targets, base + h.x_img, h.x_plane, nullptr, 0, 0, s);
+        for (int v0 = 0; v0 < a.V; v0 += h.piece) {
+            const int vc = std::min(h.piece, a.V - v0);
+            const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
+            if (!h.direct) head_images(a, w, vc, a.d, (int)up_to(vc, 64), h.dp, nullptr, base + h.w_img, h.w_plane, nullptr, 0, 0, s);
+            head_prod p = {};
+            p.A = base + h.x_img;
+            p.planeA = h.x_plane;
+            p.B = h.direct ? w : base + h.w_img;
+            p.planeB = h.w_plane;
+            p.b_ld = h.direct ? (size_t)a.d * 2 : 0;
+            p.kt = h.dp / 32;
+            p.M = a.T;
+            p.N = vc;
+            p.slices = 1;
+            p.targets = a.targets;
+            p.T = a.T;
+            p.V = a.V;
+            p.v0 = v0;
+            p.part = part;
+            p.tlogit = tlogit;
+            HEAD_TRY(head_product<HEAD_LSE>(ctx, p, h.planes, s));
+        }
+    }
+    int TL = 1;
+    while (TL < 64 && TL < a.T) TL *= 2;
+    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(a.T, TL)), dim3(1024), 0, s, part, nb, tlogit, a.targets, a.T, a.V, TL, a.loss, a.row_stats, a.mean);
+    if (a.T > TL) hipLaunchKernelGGL(head_mean_kernel, dim3(1), dim3(1024), 0, s, a.loss, a.targets, a.T, a.V, a.mean);
+    return hipGetLastError();
+}
+
+hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s)
+{
+    const bool bf = a.dtype == OMEGA_DTYPE_BF16;
+    const size_t es = bf ? 2 : 4;
+    if (a.T == 0) {
+        if (a.dw) head_zero(a.dw, (size_t)a.V * a.d * es, s);
+        return hipGetLastError();
+    }
+    const head_plan h = head_plan_of(ctx, a, true);
+    unsigned char *base = (unsigned char *)ws;
+    head_images(a, a.x, a.T, a.d, h.Tp, h.dp, a.targets, base + h.x_img, h.x_plane, a.dw ? base + h.xT_img : nullptr, h.Tp / 32, h.xT_plane, s);
+    for (int v0 = 0; v0 < a.V; v0 += h.piece) {
+        const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256);
+        const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
+        if (!h.direct || a.dx)
+            head_images(a, w, vc, a.d, vp, h.dp, nullptr, h.direct ? nullptr : base + h.w_img, h.w_plane, a.dx ? base + h.wT_img : nullptr, vp / 32, h.wT_plane, s);
+        head_prod p = {};
+        p.A = base + h.x_img;
+        p.planeA = h.x_plane;
+        p.B = h.direct ? w : base + h.w_img;
+        p.planeB = h.w_plane;
+        p.b_ld = h.direct ? (size_t)a.d * 2 : 0;
+        p.kt = h.dp / 32;
+        p.M = a.T;
+        p.N = vc;
+        p.slices = 1;
+        p.targets = a.targets;
+        p.row_stats = a.row_stats;
+        p.mean = a.mean;
+        p.dloss = a.dloss;
+        p.T = a.T;
+        p.V = a.V;
+        p.v0 = v0;
+        p.P = base + h.p_img;
+        p.planeP = h.p_plane;
+        HEAD_TRY(head_product<HEAD_P>(ctx, p, h.planes, s));
+        if (a.dx) {
+            head_prod q = {};
+            q.A = base + h.p_img;
+            q.planeA = h.p_plane;
+            q.B = base + h.wT_img;
+            q.planeB = h.wT_plane;
+            q.kt = vp / 32;
+            q.M = a.T;
+            q.N = a.d;
+            q.slices = std::max(1, std::min(h.slices, q.kt / 8));
+            q.C = (float *)(base + h.slabs);
+            q.slab = h.slab;
+            q.ld = (int)up_to(h.dp, 256);
+            if (v0 == 0) HEAD_TRY(head_product<HEAD_ACC>(ctx, q, h.planes, s));
+            else HEAD_TRY(head_product<HEAD_ADD>(ctx, q, h.planes, s));
+        }
+        if (a.dw) {
+            hipLaunchKernelGGL(head_transpose_kernel, dim3(h.Tp / 64, vp / 64, h.planes), dim3(256), 0, s, base + h.p_img, a.T, vp / 32, h.p_plane, base + h.pT_img, h.Tp / 32,
+                               h.pT_plane);
+            head_prod q = {};
+            q.A = base + h.pT_img;
+            q.planeA = h.pT_plane;
+            q.B = base + h.xT_img;
+            q.planeB = h.xT_plane;
+            q.kt = h.Tp / 32;
+            q.M = vc;
+            q.N = a.d;
+            q.slices = 1;
+            q.out = (unsigned char *)a.dw + (size_t)v0 * a.d * es;
+            q.out_bf = bf;
+            q.out_vec = a.d % 4 == 0 && (uintptr_t)q.out % (bf ? 8 : 16) == 0;
+            HEAD_TRY(head_product<HEAD_OUT>(ctx, q, h.planes, s));
+        }
+    }
+    if (a.dx) {
+        const int vp0 = (int)up_to(std::min(h.piece, a.V), 256), slices = std::max(1, std::min(h.slices, vp0 / 32 / 8));
+        const dim3 grid(a.T, std::min(ceil_div(a.d, 256), 1024));
+        if (bf) hipLaunchKernelGGL(head_dx_kernel<true>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.dx);
+        else hipLaunchKernelGGL(head_dx_kernel<false>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.dx);
+    }
+    return hipGetLastError();
+}

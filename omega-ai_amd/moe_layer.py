@@ -16,6 +16,7 @@ argument meaning and error behaviour follow the reference's layers:
     LlamaTransformerBlock (norm2 -> mlp -> residual add and its backward, LlamaTransformerBlock.java:134-136,156-158)
 """
 import ctypes as C
+import math
 
 import numpy as np
 
@@ -65,28 +66,42 @@ class DeviceBuffer:
     """Caller-owned device memory (the role of Tensor.gpuData, J/engine/tensor/Tensor.java:23-47)."""
 
     def __init__(self, ctx, shape, dtype):
-        self.ctx, self.shape, self.dtype = ctx, tuple(shape), dtype
-        self.esize = 2 if dtype == "bf16" else 4
-        self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * self.esize
+        self._describe(ctx, shape, dtype)
+        self.owned = True
         p = C.c_void_p()
         ctx.check(ctx.lib.omega_hip_malloc(ctx.handle, max(self.nbytes, 16), C.byref(p)))
         self.ptr = p
 
+    def _describe(self, ctx, shape, dtype):
+        self.ctx, self.shape, self.dtype = ctx, tuple(shape), dtype   # dtype: "f32", "bf16" or "i32"
+        self.esize = 2 if dtype == "bf16" else 4
+        self.size = math.prod(self.shape)
+        self.nbytes = self.size * self.esize
+
+    @classmethod
+    def wrap(cls, ctx, address, shape, dtype):
+        """Device memory of another owner (a SerializablePointer's address, a tensor's data_ptr): used where it is, never freed here.
+        The owner's other streams are the caller's to synchronise with the context's."""
+        b = cls.__new__(cls)
+        b._describe(ctx, shape, dtype)
+        b.owned, b.ptr = False, C.c_void_p(address)
+        return b
+
     @classmethod
     def from_numpy(cls, ctx, a, dtype):
-        """a: fp32 values; stored as fp32 or as bf16 (round to nearest even)."""
+        """a: fp32 values, stored as fp32 or as bf16 (round to nearest even), or whole numbers stored as i32."""
         b = cls(ctx, a.shape, dtype)
         b.upload(a)
         return b
 
     def upload(self, a):
-        h = f32_to_bf16_bits(a) if self.dtype == "bf16" else np.ascontiguousarray(a, np.float32)
+        h = f32_to_bf16_bits(a) if self.dtype == "bf16" else np.ascontiguousarray(a, np.int32 if self.dtype == "i32" else np.float32)
         assert h.nbytes == self.nbytes
         self.ctx.check(self.ctx.lib.omega_hip_memcpy_h2d(self.ctx.handle, self.ptr, h.ctypes.data, h.nbytes))
 
     def to_numpy(self):
         """Blocking copy to host (Tensor.syncHost); bf16 buffers come back widened to fp32."""
-        h = np.empty(self.shape, np.uint16 if self.dtype == "bf16" else np.float32)
+        h = np.empty(self.shape, np.uint16 if self.dtype == "bf16" else np.int32 if self.dtype == "i32" else np.float32)
         self.ctx.check(self.ctx.lib.omega_hip_memcpy_d2h(self.ctx.handle, h.ctypes.data, self.ptr, h.nbytes))
         return bf16_bits_to_f32(h) if self.dtype == "bf16" else h
 
@@ -97,7 +112,8 @@ class DeviceBuffer:
 
     def free(self):
         if self.ptr:
-            self.ctx.lib.omega_hip_free(self.ctx.handle, self.ptr)
+            if self.owned:
+                self.ctx.lib.omega_hip_free(self.ctx.handle, self.ptr)
             self.ptr = None
 
 
