@@ -198,10 +198,21 @@ def _clip(case, s):
 _ctx = None
 
 
+class _Held:
+    """A layer, given back with the last tensor that looks at its buffers."""
+
+    def __init__(self, layer):
+        self.layer = layer
+
+    def __del__(self):
+        self.layer.close()
+
+
 class _Memory:
     """Device memory of a library buffer, for torch.as_tensor (no copy)."""
 
-    def __init__(self, buf):
+    def __init__(self, held, buf):
+        self.held = held
         self.__cuda_array_interface__ = {"version": 2, "shape": tuple(buf.shape), "data": (buf.ptr.value, False),
                                          "typestr": "<i2" if buf.dtype == "bf16" else "<f4", "strides": None}
 
@@ -229,8 +240,9 @@ class _Own:
         else:
             self.out = torch.empty_like(s["grads"])
             sizes = _sizes(case)
-            self.clip = P.GradClip(_ctx, [self.buffer(t) for t in s["grads"].split(sizes)],
-                                   out=[self.buffer(t) for t in self.out.split(sizes)])
+            self.layer = P.GradClip(_ctx, [self.buffer(t) for t in s["grads"].split(sizes)],
+                                    out=[self.buffer(t) for t in self.out.split(sizes)])
+        self.held = _Held(self.layer)
         if "dout" in s:
             self.dout = self.buffer(s["dout"])
 
@@ -241,7 +253,7 @@ class _Own:
     def tensor(self, buf):
         t = self.seen.get(buf.ptr.value)
         if t is None:
-            t = torch.as_tensor(_Memory(buf), device="cuda")
+            t = torch.as_tensor(_Memory(self.held, buf), device="cuda")
             t = self.seen[buf.ptr.value] = t.view(torch.bfloat16) if buf.dtype == "bf16" else t
         return t
 
@@ -262,7 +274,7 @@ class _Own:
                 got["dx"] = self.tensor(self.layer.back())
                 got["dw"] = self.tensor(self.layer.diffW)
             return got
-        return {"norm": self.tensor(self.clip.clip(case["limit"]))[0], "clipped": self.out}
+        return {"norm": self.tensor(self.layer.clip(case["limit"]))[0], "clipped": self.out}
 
 
 _PLAIN = {"embedding": _embedding, "layer_norm": _layer_norm, "head_loss": _head_loss, "clip": _clip}
