@@ -40,7 +40,7 @@ class _Layer:
             if buf is not None:
                 buf.free()
         self._owned = {}
-        self.diffW = self.diffGamma = self.diffBeta = None
+        self.input = self.diffW = self.diffGamma = self.diffBeta = None
 
 
 class EmbeddingLayer(_Layer):
