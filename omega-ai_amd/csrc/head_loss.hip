@@ -100,16 +100,14 @@ __device__ __forceinline__ void hp_split(float v, uint32_t (&h)[3])
 // One tile of a product, or a k slice of one
 struct hp_item {
     const unsigned char *A, *B;   // first step of the tile's rows and columns
-    int row0, n0, slice;          // first row (-1: no item) and column
+    int row0, n0, slice;          // first row and column
     int kt;                       // steps (of a part)
 };
 
 __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
 {
-    hp_item it = {};
-    it.row0 = -1;
+    hp_item it;
     const int per = p.mt * p.nt;
-    if (idx >= per * p.slices) return it;
     // column tiles outside, up to 8 row tiles inside: the 32 neighbours that an XCD works on share operand tiles in its L2
     const int sl = idx / per, rem = idx - sl * per, g = rem / (8 * p.nt), gm = min(8, p.mt - 8 * g), r2 = rem - g * 8 * p.nt, n = r2 / gm;
     it.row0 = __builtin_amdgcn_readfirstlane((8 * g + (r2 - n * gm)) * p.th);
@@ -121,6 +119,13 @@ __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
     it.A = hp_uniform(p.A + (size_t)(it.row0 >> 7) * rg + (size_t)first * 8192);
     it.B = hp_uniform(p.b_ld == 0 ? p.B + (size_t)(it.n0 >> 7) * rg + (size_t)first * 8192 : p.B + (size_t)it.n0 * p.b_ld + (size_t)first * 64);
     return it;
+}
+// The lane number as a value that the compiler cannot carry over: what follows from it is computed where it is used.  (Kept from item
+// to item it is spilled, and the wait for a reload in the middle of a k loop drains the ring: 49 % of the matrix rate instead of 80.)
+__device__ __forceinline__ int hp_fresh(int lane)
+{
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
 // what the lane adds for the wave's loads: blocks of 16 rows wave + 4 n of the item's rows and columns
 __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_item &it, int wave, int lane, uint32_t (&va)[4], uint32_t (&vb)[4])
@@ -165,46 +170,46 @@ struct hp_state {
         if ((l) < 4) hp_dma16<((l) & 3) * 4096>(lA, st.va[(l) & 3], sb);                   \
         else hp_dma16<HP_TILE_BYTES + ((l) & 3) * 4096>(lB, st.vb[(l) & 3], sb);           \
     } while (0)
-#define HP_MFMA(PA, PB, Z, iu, c)                                                                                                    \
+#define HP_MFMA(PA, PB, iu, c)                                                                                                    \
     do {                                                                                                                             \
         if ((iu) < NU)                                                                                                               \
-            acc[(iu) % NU][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(PB[c], PA[iu], (Z) ? zero4 : acc[(iu) % NU][c], 0, 0, 0);    \
+            acc[(iu) % NU][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(PB[c], PA[iu], acc[(iu) % NU][c], 0, 0, 0);    \
     } while (0)
-#define HP_GROUP(PA, PB, QA, QB, Z, g)                     \
+#define HP_GROUP(PA, PB, QA, QB, g)                     \
     do {                                                   \
-        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1));       \
+        HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1));       \
         if ((g) < 8) {                                     \
             HP_READ(QA, QB, 2 * (g));                      \
             HP_READ(QA, QB, 2 * (g) + 1);                  \
         }                                                  \
         __builtin_amdgcn_sched_barrier(0);                 \
-        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 1);   \
+        HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 1);   \
         if ((g) & 1) HP_LOAD((g) >> 1, sb);                \
         __builtin_amdgcn_sched_barrier(0);                 \
-        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 2);   \
+        HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 2);   \
         __builtin_amdgcn_sched_barrier(0);                 \
-        HP_MFMA(PA, PB, Z, (g) >> 1, 4 * ((g) & 1) + 3);   \
+        HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 3);   \
         __builtin_amdgcn_sched_barrier(0);                 \
     } while (0)
-#define HP_STEP(PA, PB, QA, QB, Z)                                                                          \
+#define HP_STEP(PA, PB, QA, QB)                                                                          \
     do {                                                                                                    \
-        HP_GROUP(PA, PB, QA, QB, Z, 0); HP_GROUP(PA, PB, QA, QB, Z, 1); HP_GROUP(PA, PB, QA, QB, Z, 2);     \
-        HP_GROUP(PA, PB, QA, QB, Z, 3); HP_GROUP(PA, PB, QA, QB, Z, 4); HP_GROUP(PA, PB, QA, QB, Z, 5);     \
-        HP_GROUP(PA, PB, QA, QB, Z, 6); HP_GROUP(PA, PB, QA, QB, Z, 7); HP_GROUP(PA, PB, QA, QB, Z, 8);     \
-        HP_GROUP(PA, PB, QA, QB, Z, 9); HP_GROUP(PA, PB, QA, QB, Z, 10); HP_GROUP(PA, PB, QA, QB, Z, 11);   \
-        HP_GROUP(PA, PB, QA, QB, Z, 12); HP_GROUP(PA, PB, QA, QB, Z, 13); HP_GROUP(PA, PB, QA, QB, Z, 14);  \
-        HP_MFMA(PA, PB, Z, 7, 4);                                                                           \
+        HP_GROUP(PA, PB, QA, QB, 0); HP_GROUP(PA, PB, QA, QB, 1); HP_GROUP(PA, PB, QA, QB, 2);     \
+        HP_GROUP(PA, PB, QA, QB, 3); HP_GROUP(PA, PB, QA, QB, 4); HP_GROUP(PA, PB, QA, QB, 5);     \
+        HP_GROUP(PA, PB, QA, QB, 6); HP_GROUP(PA, PB, QA, QB, 7); HP_GROUP(PA, PB, QA, QB, 8);     \
+        HP_GROUP(PA, PB, QA, QB, 9); HP_GROUP(PA, PB, QA, QB, 10); HP_GROUP(PA, PB, QA, QB, 11);   \
+        HP_GROUP(PA, PB, QA, QB, 12); HP_GROUP(PA, PB, QA, QB, 13); HP_GROUP(PA, PB, QA, QB, 14);  \
+        HP_MFMA(PA, PB, 7, 4);                                                                           \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
-        HP_MFMA(PA, PB, Z, 7, 5);                                                                           \
+        HP_MFMA(PA, PB, 7, 5);                                                                           \
         HP_LOAD(7, sb);                                                                                     \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
-        HP_MFMA(PA, PB, Z, 7, 6);                                                                           \
+        HP_MFMA(PA, PB, 7, 6);                                                                           \
         cur = cur + 1 == HP_STAGES ? 0 : cur + 1;                                                           \
         sb = lds_wave + cur * HP_STAGE_BYTES;                                                               \
         lA += 8192;                                                                                         \
         lB += stepB;                                                                                        \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
-        HP_MFMA(PA, PB, Z, 7, 7);                                                                           \
+        HP_MFMA(PA, PB, 7, 7);                                                                           \
         {                                                                                                   \
             const unsigned char *sn = smem + (cur + 1 == HP_STAGES ? 0 : cur + 1) * HP_STAGE_BYTES;         \
             ra = sn + pa;                                                                                   \
@@ -237,9 +242,10 @@ typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
 
 // A tile of 32 NU rows by 256 columns.  acc[iu][c][r]: row 16 (2 iu + wm) + lane % 16, column 128 wn + 16 c + 4 (lane / 16) + r.
 template <int NU, int EPI, int NSEG>
-__device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane)
+__device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane0)
 {
-    const int wm = wave >> 1, wn = wave & 1, l16 = lane & 15, lq = lane >> 4;
+    const int wm = wave >> 1, wn = wave & 1;
+    int lane = hp_fresh(lane0), l16 = lane & 15, lq = lane >> 4;
     const int kt = __builtin_amdgcn_readfirstlane(it.kt);
     const size_t stepB = p.b_ld == 0 ? 8192 : 64;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
@@ -262,41 +268,40 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     const f32x4_t zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
     // The steps of a pair of parts two at a time (their number is even, at least 8).  The loads of the last five are the next pair's
     // or the next item's first (behind the last item: this one's once more, which nobody reads).
-    if (NSEG > 1) {
+    // (zeros in the registers: a first step that starts from zero operands instead costs as many moves of registers)
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
+    for (int i = 0; i < NU; ++i)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) acc[i][c] = zero4;
-    }
+        for (int c = 0; c < 8; ++c) acc[i][c] = zero4;
 #pragma unroll 1
     for (int seg = 0; seg < NSEG; ++seg) {
-        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, NSEG == 1);
-        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
-#pragma unroll 1
-        for (int k = 2; k < kt - 6; k += 2) {
-            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
-            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
-        }
-        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
+        int k = kt - 6;
+        do {
+            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
+            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
+        } while ((k -= 2) > 0);
+        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
         {
             const int ns = seg + 1 < NSEG ? seg + 1 : 0;
-            const bool more = ns == 0 && nxt.row0 >= 0;
+            const hp_item &li = ns == 0 ? nxt : it;  // the item of the loads from here on
             const size_t a0 = NSEG > 1 ? (size_t)((HP_SEG_A >> (4 * ns)) & 3) * p.planeA : 0, b0 = NSEG > 1 ? (size_t)((HP_SEG_B >> (4 * ns)) & 3) * p.planeB : 0;
-            lA = hp_uniform((more ? nxt.A : it.A) + a0);
-            lB = hp_uniform((more ? nxt.B : it.B) + b0);
-            if (more) hp_lane_offsets(p, nxt, wave, lane, st.va, st.vb);
+            lA = hp_uniform(li.A + a0);
+            lB = hp_uniform(li.B + b0);
+            hp_lane_offsets(p, li, wave, hp_fresh(lane0), st.va, st.vb);
         }
-        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
-#pragma unroll 1
+        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         for (int k = 0; k < 2; ++k) {
-            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1, false);
-            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0, false);
+            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
+            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         }
     }
     st.cur = cur;
     st.lA = lA;
     st.lB = lB;
 
+    lane = hp_fresh(lane0);
+    l16 = lane & 15;
+    lq = lane >> 4;
     const int col0 = it.n0 + wn * 128 + 4 * lq;  // column of acc[.][0][0]
     if (EPI == HEAD_LSE) {
         const bool whole = it.n0 + wn * 128 + 128 <= p.N;
@@ -449,9 +454,10 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
     const int wm = wave >> 1, wn = wave & 1, l16 = lane & 15, lq = lane >> 4;
     const int n_wg = gridDim.x;
     const int at = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const int total = p.mt * p.nt * p.slices;
     int idx = at;
+    if (idx >= total) return;
     hp_item it = hp_make_item(p, idx);
-    if (it.row0 < 0) return;
     hp_state st;
     const unsigned char *lA = hp_uniform(it.A + (NSEG > 1 ? (size_t)(HP_SEG_A & 3) * p.planeA : 0));
     const unsigned char *lB = hp_uniform(it.B + (NSEG > 1 ? (size_t)(HP_SEG_B & 3) * p.planeB : 0));
@@ -481,12 +487,12 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
     asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)" ::: "memory");  // step 1 has landed; every wave has taken step 0 out of its stage
     __syncthreads();
     st.cur = 0;
-#pragma unroll 1
     for (;;) {
-        idx += n_wg;
-        hp_item nxt;
+        const bool more = idx + n_wg < total;
+        if (more) idx += n_wg;
+        hp_item nxt;  // (behind the last item: this one's loads once more, which nobody reads)
         hp_run_item<NU, EPI, NSEG>(smem, st, p, it, nxt, idx, wave, lane);
-        if (nxt.row0 < 0) break;
+        if (!more) break;
         it = nxt;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads behind the last item land in LDS that nobody reads)
