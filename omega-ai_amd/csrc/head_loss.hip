@@ -240,6 +240,138 @@ typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
 #define HP_OUTSIDE 0xffffffffu
 
+// Quarters of the wave (16 lanes) 1 and 3 of a change places with quarters 0 and 2 of b: [0] = a0 b0 a2 b2, [1] = a1 b1 a3 b3
+__device__ __forceinline__ u32x2_t hp_swap16(uint32_t a, uint32_t b)
+{
+    return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+}
+
+// Writers of the two products with the vocabulary.  WHOLE: every column of the wave is there.
+template <int NU, int NSEG, bool WHOLE>
+__device__ __forceinline__ void hp_write_lse(const head_prod &p, const hp_item &it, const f32x4_t (&acc)[NU][8], int wm, int wn, int l16, int lq)
+{
+    const int col0 = it.n0 + wn * 128 + 4 * lq;
+    // maximum and sum of a lane's 32 columns first, unit by unit; the four lanes of a row are joined for all units together, so that
+    // the latencies of the targets' loads and of the lane exchanges are paid once
+    float m[NU], s[NU];
+    int y[NU];
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) y[iu] = p.targets[min(it.row0 + 16 * (2 * iu + wm) + l16, p.M - 1)];
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) {
+        __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
+        float v[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = WHOLE || col0 + 16 * (k >> 2) + (k & 3) < p.N ? acc[iu][k >> 2][k & 3] : -INFINITY;  // (exp(-inf) is zero)
+        m[iu] = v[0];
+#pragma unroll
+        for (int k = 1; k < 32; ++k) m[iu] = fmaxf(m[iu], v[k]);
+        const float m0 = m[iu] == -INFINITY ? 0.0f : m[iu];  // (no column, or every logit -inf: the sum is 0)
+        s[iu] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s[iu] += hp_exp<NSEG>(v[k] - m0);
+        // the target's logit, where it is among the lane's columns
+        const int t = it.row0 + 16 * (2 * iu + wm) + l16, at = y[iu] - p.v0 - col0;
+        const bool mine = t < p.M && at >= 0 && at < 128 && (at & 12) == 0 && col0 + at < p.N;
+        if (__ballot(mine)) {
+            float l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) l = at == 16 * (k >> 2) + (k & 3) ? v[k] : l;
+            if (mine) p.tlogit[t] = l;
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) {
+        float all = fmaxf(m[iu], __shfl_xor(m[iu], 16, 64));
+        all = fmaxf(all, __shfl_xor(all, 32, 64));
+        s[iu] *= hp_exp<NSEG>(m[iu] - (all == -INFINITY ? 0.0f : all));
+        m[iu] = all;
+    }
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) s[iu] += __shfl_xor(s[iu], 16, 64);
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) s[iu] += __shfl_xor(s[iu], 32, 64);
+    float2 *part = p.part + (size_t)((p.v0 + it.n0) / 128 + wn) * p.T;
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) {
+        const int t = it.row0 + 16 * (2 * iu + wm) + l16;
+        if (lq == 0 && t < p.M) part[t] = make_float2(m[iu], s[iu]);
+    }
+}
+template <int NU, int NSEG, bool WHOLE>
+__device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it, const f32x4_t (&acc)[NU][8], int wm, int wn, int l16, int lq)
+{
+    const int col0 = it.n0 + wn * 128 + 4 * lq;
+    // (rows behind the last token are written with what the last one's statistics give: nothing reads them)
+    const float gs = (p.dloss ? p.dloss[0] : 1.0f) / fmaxf(p.mean[1], 1.0f);
+    const int KTp = p.nt * (HP_TILE / HP_BK);
+    constexpr int NP = NSEG > 1 ? 3 : 1;
+    // (to the image's end: rows of the tile behind it fall away)
+    const int rgs = ((p.M + 127) >> 7) - (it.row0 >> 7), kb = (it.n0 >> 5) + 4 * wn;
+    __amdgpu_buffer_rsrc_t rs[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+        rs[q] = __builtin_amdgcn_make_buffer_rsrc((void *)hp_uniform(p.P + q * p.planeP + (size_t)(it.row0 >> 7) * KTp * 8192 + (size_t)kb * 8192), 0,
+                                                  (rgs * KTp - kb) * 8192, 0x00020000);
+    int y[NU];
+    float m[NU], f[NU];
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) {
+        const int t = min(it.row0 + 16 * (2 * iu + wm) + l16, p.M - 1);
+        y[iu] = p.targets[t];
+        m[iu] = p.row_stats[t];
+        f[iu] = p.row_stats[p.T + t];
+    }
+#pragma unroll
+    for (int iu = 0; iu < NU; ++iu) {
+        __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
+        const int row = it.row0 + 16 * (2 * iu + wm) + l16;
+        const bool held = y[iu] >= 0 && y[iu] < p.V;
+        // (rows without a target: their logits here are zeros, the images' rows are; what their statistics say does not matter)
+        const float fu = held ? gs / f[iu] : 0.0f, mu = held ? m[iu] : 0.0f;
+        const int k = y[iu] - p.v0 - col0;
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            v[e] = hp_exp<NSEG>(acc[iu][e >> 2][e & 3] - mu) * fu;
+            if (!WHOLE) v[e] = col0 + 16 * (e >> 2) + (e & 3) < p.N ? v[e] : 0.0f;
+        }
+        if (__ballot(held && k >= 0 && k < 128 && (k & 12) == 0)) {
+            const float g1 = held ? gs : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] -= k == 16 * (e >> 2) + (e & 3) ? g1 : 0.0f;
+        }
+        // two fragments of 16 columns are a k step of the image: lanes of neighbouring quarters exchange halves, so that a lane has the 8
+        // columns of a 16-byte chunk and the wave stores a whole block of 16 rows x 32 columns at once
+        const uint32_t at = (uint32_t)((row >> 7) - (it.row0 >> 7)) * (uint32_t)KTp * 8192u +
+                            (uint32_t)(((row & 127) >> 4) * 1024 + (row & 15) * 64 + (((2 * (lq & 1) + (lq >> 1)) ^ pk_swz(row)) << 4));
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+            uint32_t h[NP][4];  // parts of fragment c (two words) and of fragment c + 1
+            if (NSEG == 1) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) h[0][w] = hp_pack2(v[4 * c + 2 * w], v[4 * c + 2 * w + 1]);
+            } else {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t lo[3], hi[3];
+                    hp_split(v[4 * c + 2 * w], lo);
+                    hp_split(v[4 * c + 2 * w + 1], hi);
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) h[q][w] = lo[q] | hi[q] << 16;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const u32x2_t a = hp_swap16(h[q][0], h[q][2]), b = hp_swap16(h[q][1], h[q][3]);
+                __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{a[0], b[0], a[1], b[1]}, rs[q], at + (c >> 1) * 8192, 0, 0);
+            }
+            if (NSEG > 1) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
 // A tile of 32 NU rows by 256 columns.  acc[iu][c][r]: row 16 (2 iu + wm) + lane % 16, column 128 wn + 16 c + 4 (lane / 16) + r.
 template <int NU, int EPI, int NSEG>
 __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane0)
@@ -273,6 +405,11 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     for (int i = 0; i < NU; ++i)
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[i][c] = zero4;
+    // (the sums stay in accumulation registers: with other uses in sight, the compiler keeps some elsewhere and moves them in the loop)
+#define HP_PIN()                          \
+    _Pragma("unroll") for (int i = 0; i < NU; ++i) \
+        _Pragma("unroll") for (int c = 0; c < 8; ++c) asm volatile("" : "+a"(acc[i][c]))
+    HP_PIN();
 #pragma unroll 1
     for (int seg = 0; seg < NSEG; ++seg) {
         int k = kt - 6;
@@ -295,6 +432,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         }
     }
+    HP_PIN();
     st.cur = cur;
     st.lA = lA;
     st.lB = lB;
@@ -303,90 +441,13 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     l16 = lane & 15;
     lq = lane >> 4;
     const int col0 = it.n0 + wn * 128 + 4 * lq;  // column of acc[.][0][0]
+    const bool whole = it.n0 + wn * 128 + 128 <= p.N;  // (the wave's columns are all there)
     if (EPI == HEAD_LSE) {
-        const bool whole = it.n0 + wn * 128 + 128 <= p.N;
-#pragma unroll
-        for (int iu = 0; iu < NU; ++iu) {
-            __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
-            const int t = it.row0 + 16 * (2 * iu + wm) + l16;
-            const bool held = t < p.M;
-            float m = -INFINITY, s = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (!whole && col0 + 16 * c + r >= p.N) acc[iu][c][r] = -INFINITY;
-                    m = fmaxf(m, acc[iu][c][r]);
-                }
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const float m0 = m == -INFINITY ? 0.0f : m;  // (no column, or every logit -inf: the sum is 0)
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s += hp_exp<NSEG>(acc[iu][c][r] - m0);
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if (held && lq == 0) p.part[(size_t)((p.v0 + it.n0) / 128 + wn) * p.T + t] = make_float2(m, s);
-            const int y = held ? p.targets[t] - p.v0 - it.n0 - wn * 128 : -1;  // the target's column among the wave's 128
-            if (__ballot(y >= 0 && y < 128 && it.n0 + wn * 128 + y < p.N)) {
-                const int k = y - 4 * lq;
-                float v = 0.0f;
-                bool mine = false;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (k == 16 * c + r) v = acc[iu][c][r], mine = true;
-                if (mine && y >= 0 && it.n0 + wn * 128 + y < p.N) p.tlogit[t] = v;
-            }
-        }
+        if (whole) hp_write_lse<NU, NSEG, true>(p, it, acc, wm, wn, l16, lq);
+        else hp_write_lse<NU, NSEG, false>(p, it, acc, wm, wn, l16, lq);
     } else if (EPI == HEAD_P) {
-        // (rows behind the last token are written with what the last one's statistics give: nothing reads them)
-        const bool whole = it.n0 + wn * 128 + 128 <= p.N;
-        const float gs = (p.dloss ? p.dloss[0] : 1.0f) / fmaxf(p.mean[1], 1.0f);
-        const int KTp = p.nt * (HP_TILE / HP_BK);
-        constexpr int NP = NSEG > 1 ? 3 : 1;
-        // (to the image's end: rows of the tile behind it fall away)
-        const int rgs = ((p.M + 127) >> 7) - (it.row0 >> 7), kb = (it.n0 >> 5) + 4 * wn;
-        __amdgpu_buffer_rsrc_t rs[NP];
-#pragma unroll
-        for (int q = 0; q < NP; ++q)
-            rs[q] = __builtin_amdgcn_make_buffer_rsrc((void *)hp_uniform(p.P + q * p.planeP + (size_t)(it.row0 >> 7) * KTp * 8192 + (size_t)kb * 8192), 0,
-                                                      (rgs * KTp - kb) * 8192, 0x00020000);
-#pragma unroll
-        for (int iu = 0; iu < NU; ++iu) {
-            __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
-            const int row = it.row0 + 16 * (2 * iu + wm) + l16, t = min(row, p.M - 1);
-            const int y = p.targets[t];
-            const bool held = y >= 0 && y < p.V;
-            const float m = p.row_stats[t], f = gs / p.row_stats[p.T + t];
-            const int k = y - p.v0 - col0, end = held ? (whole ? 0x7fffffff : p.N - col0) : 0;  // columns from `end` on are zero
-            const uint32_t rg0 = (uint32_t)((row >> 7) - (it.row0 >> 7)) * (uint32_t)KTp * 8192u + (uint32_t)(((row & 127) >> 4) * 1024 + (row & 15) * 64 + (lq & 1) * 8);
-            const uint32_t o0 = rg0 + (uint32_t)(((lq >> 1) ^ pk_swz(row)) << 4), o1 = rg0 + (uint32_t)(((2 + (lq >> 1)) ^ pk_swz(row)) << 4);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = hp_exp<NSEG>(acc[iu][c][r] - m) * f;
-                    v[r] -= k == 16 * c + r ? gs : 0.0f;
-                    v[r] = 16 * c + r < end ? v[r] : 0.0f;
-                }
-                const uint32_t at = (c & 1 ? o1 : o0) + (c >> 1) * 8192;
-                if (NSEG == 1) {
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{hp_pack2(v[0], v[1]), hp_pack2(v[2], v[3])}, rs[0], at, 0, 0);
-                } else {
-                    uint32_t h[4][3];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) hp_split(v[r], h[r]);
-#pragma unroll
-                    for (int q = 0; q < 3; ++q)
-                        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{h[0][q] | h[1][q] << 16, h[2][q] | h[3][q] << 16}, rs[q % NP], at, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-        }
+        if (whole) hp_write_p<NU, NSEG, true>(p, it, acc, wm, wn, l16, lq);
+        else hp_write_p<NU, NSEG, false>(p, it, acc, wm, wn, l16, lq);
     } else if (EPI == HEAD_ACC || EPI == HEAD_ADD) {
         // (a slab has room for whole tiles)
         float *tile = p.C + (size_t)it.slice * p.slab + (size_t)it.row0 * p.ld + it.n0 + wn * 128;
@@ -421,13 +482,19 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
 #pragma unroll
         for (int iu = 0; iu < NU; ++iu) {
             __builtin_amdgcn_sched_barrier(0);
-            if (p.out_vec) {  // (N is a multiple of 4)
+            if (p.out_vec && p.out_bf) {  // (rows of whole 16 bytes; halves exchanged as in the image of P)
+#pragma unroll
+                for (int c = 0; c < 8; c += 2) {
+                    const f32x4_t v = acc[iu][c], w = acc[iu][c + 1];
+                    const u32x2_t a = hp_swap16(hp_pack2(v[0], v[1]), hp_pack2(w[0], w[1])), b = hp_swap16(hp_pack2(v[2], v[3]), hp_pack2(w[2], w[3]));
+                    const int cc = 16 * (c + (lq & 1)) + 8 * (lq >> 1) - 4 * lq;  // from col0
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{a[0], b[0], a[1], b[1]}, rs, cc < cols ? (uint32_t)(off + cc * 2) : HP_OUTSIDE, 0, 0);
+                }
+            } else if (p.out_vec) {  // (fp32, a multiple of 4 columns)
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const f32x4_t v = acc[iu][c];
-                    const uint32_t at = 16 * c < cols ? (uint32_t)(off + 16 * c * es) : HP_OUTSIDE;  // (rows behind the last: beyond the range as well)
-                    if (p.out_bf) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{hp_pack2(v[0], v[1]), hp_pack2(v[2], v[3])}, rs, at, 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t *)&v, rs, at, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t *)&v, rs, 16 * c < cols ? (uint32_t)(off + 64 * c) : HP_OUTSIDE, 0, 0);
                 }
             } else {
 #pragma unroll
@@ -892,17 +959,19 @@ hipError_t head_init(void)
 template <int EPI>
 static hipError_t head_product(const omega_ctx *ctx, head_prod p, int planes, hipStream_t s)
 {
-    // height of a row tile: the one whose tiles are the least work, a tile of n x 64 rows counted as n + 1/2 (its columns' loads)
-    int best = 0;
+    // height of a row tile: the one that takes the least time by rounds of one tile per compute unit, a tile of n x 64 rows
+    // counted as n + 1/2 (its columns' loads)
+    p.nt = ceil_div(p.N, HP_TILE);
+    long long best = 0;
     for (int n = 4; n >= 1; --n) {
-        const int mt = ceil_div(p.M, 64 * n), cost = mt * (2 * n + 1);
+        const int mt = ceil_div(p.M, 64 * n);
+        const long long cost = ((long long)mt * p.nt * p.slices + ctx->num_cus - 1) / ctx->num_cus * (2 * n + 1);
         if (best == 0 || cost < best) {
             best = cost;
             p.th = 64 * n;
             p.mt = mt;
         }
     }
-    p.nt = ceil_div(p.N, HP_TILE);
     const long long items = (long long)p.mt * p.nt * p.slices;
     if (items > 0x3fffffff) return hipErrorInvalidValue;
     const int grid = (int)std::min<long long>(items, ctx->num_cus);
@@ -1053,7 +1122,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.slices = 1;
             q.out = (unsigned char *)a.dw + (size_t)v0 * a.d * es;
             q.out_bf = bf;
-            q.out_vec = a.d % 4 == 0 && (uintptr_t)q.out % (bf ? 8 : 16) == 0;
+            q.out_vec = a.d % (bf ? 8 : 4) == 0 && (uintptr_t)q.out % 16 == 0;
             HEAD_TRY(head_product<HEAD_OUT>(ctx, q, h.planes, s));
         }
     }
