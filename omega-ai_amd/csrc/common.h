@@ -362,7 +362,7 @@ hipError_t launch_embedding_forward(const void *table, int dtype, int V, int d, 
 size_t embedding_backward_workspace(int V, int d, int T);
 hipError_t launch_embedding_backward(const int32_t *ids, int T, const void *dout, int dtype, int V, int d, float scale, bool accumulate,
                                      void *dtable, int grad_dtype, void *ws, hipStream_t s);
-hipError_t launch_layernorm_forward(const void *x, int dtype, int T, int d, const float *gamma, const float *beta, float eps, void *out,
+hipError_t launch_layernorm_forward(const omega_ctx *ctx, const void *x, int dtype, int T, int d, const float *gamma, const float *beta, float eps, void *out,
                                     float *mean, float *rstd, hipStream_t s);
 size_t layernorm_backward_workspace(const omega_ctx *ctx, int T, int d);
 hipError_t launch_layernorm_backward(const omega_ctx *ctx, const void *x, const void *dout, int dtype, int T, int d, const float *gamma,

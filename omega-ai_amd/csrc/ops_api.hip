@@ -118,7 +118,7 @@ int omega_hip_layernorm_forward(omega_ctx *ctx, const void *x, int dtype, int T,
         OMEGA_FAIL(ctx, OMEGA_ERR_INVALID_ARG, "layernorm_forward: misaligned pointer");
     span s[] = {in_span(x, n), in_span(gamma, d4), in_span(beta, d4), out_span(out, n), out_span(mean, mean ? T4 : 0), out_span(rstd, rstd ? T4 : 0)};
     if (overlapping(s, 6)) OMEGA_FAIL(ctx, OMEGA_ERR_INVALID_ARG, "layernorm_forward: buffers overlap");
-    OMEGA_HIP_CHECK(ctx, launch_layernorm_forward(x, dtype, T, d, gamma, beta, eps, out, mean, rstd, ctx->stream));
+    OMEGA_HIP_CHECK(ctx, launch_layernorm_forward(ctx, x, dtype, T, d, gamma, beta, eps, out, mean, rstd, ctx->stream));
     return OMEGA_OK;
 }
 

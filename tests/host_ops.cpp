@@ -26,7 +26,7 @@ extern "C" hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int) {
 hipError_t launch_embedding_forward(const void *, int, int, int, const int32_t *, int, float, void *, hipStream_t) { return op("lookup", nullptr, 0); }
 size_t embedding_backward_workspace(int V, int d, int T) { return (size_t)V * 4 + (size_t)T * 8 + (size_t)d; }
 hipError_t launch_embedding_backward(const int32_t *, int, const void *, int, int, int, float, bool, void *, int, void *ws, hipStream_t) { return op("gradient", ws, 0); }
-hipError_t launch_layernorm_forward(const void *, int, int, int, const float *, const float *, float, void *, float *, float *, hipStream_t) { return op("norm", nullptr, 0); }
+hipError_t launch_layernorm_forward(const omega_ctx *, const void *, int, int, int, const float *, const float *, float, void *, float *, float *, hipStream_t) { return op("norm", nullptr, 0); }
 size_t layernorm_backward_workspace(const omega_ctx *, int, int d) { return (size_t)d * 8; }
 hipError_t launch_layernorm_backward(const omega_ctx *, const void *, const void *, int, int, int, const float *, const float *, const float *, void *, float *, float *, void *ws,
                                      hipStream_t)
