@@ -9,7 +9,8 @@
 
 #include "common.h"
 
-#define CLIP_CHUNK 16384   // elements
+#define CLIP_CHUNK 8192    // elements
+#define CLIP_FEW 1024      // chunks
 #define CLIP_TENSORS 96    // tensors of a launch (its table: 2.7 KiB of arguments)
 
 struct clip_table {
@@ -47,6 +48,15 @@ __device__ __forceinline__ clip_piece clip_find(const clip_table &t, uint32_t ch
     return p;
 }
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// NT: past the caches (what is written there fills them and more)
+template <bool NT, class V>
+__device__ __forceinline__ void clip_store(V *p, V v)
+{
+    if (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
 // W elements of a piece from element i on (aligned loads)
 template <bool BF>
 struct clip_io {
@@ -62,15 +72,16 @@ struct clip_io {
             *(float4 *)&v[0] = *(const float4 *)((const float *)p + i);
         }
     }
+    template <bool NT>
     static __device__ __forceinline__ void st(void *p, int i, const float (&v)[W])
     {
         if (BF) {
             uint32_t a[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) a[k] = (uint32_t)f32_to_bf16(v[(2 * k) % W]) | (uint32_t)f32_to_bf16(v[(2 * k + 1) % W]) << 16;
-            *(uint4 *)((bf16_t *)p + i) = make_uint4(a[0], a[1], a[2], a[3]);
+            clip_store<NT>((u4 *)((bf16_t *)p + i), u4{a[0], a[1], a[2], a[3]});
         } else {
-            *(float4 *)((float *)p + i) = *(const float4 *)&v[0];
+            clip_store<NT>((f4 *)((float *)p + i), f4{v[0], v[1 % W], v[2 % W], v[3 % W]});
         }
     }
     static __device__ __forceinline__ float ld1(const void *p, int i) { return BF ? bf16_to_f32(((const bf16_t *)p)[i]) : ((const float *)p)[i]; }
@@ -88,28 +99,60 @@ __device__ __forceinline__ int clip_head(const void *p, int n)
     return min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / es);
 }
 
+// A thread's share of a chunk: the whole 16-byte pieces threadIdx.x, + 256, ..., and one of the elements in front or behind.
+template <bool BF>
+struct clip_share {
+    int head, nv, one;  // first whole piece, pieces, the single element (-1: none)
+    __device__ __forceinline__ clip_share(const clip_piece &p)
+    {
+        constexpr int W = clip_io<BF>::W;
+        head = clip_head<BF>(p.src, p.n);
+        nv = (p.n - head) / W;
+        const int tail = head + nv * W;
+        one = (int)threadIdx.x < head ? (int)threadIdx.x : (int)threadIdx.x >= 64 && (int)threadIdx.x - 64 < p.n - tail ? tail + (int)threadIdx.x - 64 : -1;
+    }
+};
+// Its sum of squares: in fp32 (64 elements at most, four sums), or, where that is too large, or so small that squares were lost, again in
+// double.  (All in double: 325 us for 400 million elements, 290 so.)
 template <bool BF>
 __device__ __forceinline__ double clip_sumsq(const clip_piece &p)
 {
-    constexpr int W = clip_io<BF>::W;
-    double a[2] = {0.0, 0.0};
-    const int head = clip_head<BF>(p.src, p.n), nv = (p.n - head) / W, tail = head + nv * W;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < nv; i += 256) {
-        float v[W];
-        clip_io<BF>::ld(p.src, head + i * W, v);
+    constexpr int W = clip_io<BF>::W, U = 8;
+    const clip_share<BF> sh(p);
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = threadIdx.x; i0 < sh.nv; i0 += 256 * U) {
+        float v[U][W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) a[k & 1] = fma((double)v[k], (double)v[k], a[k & 1]);
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[u][k] = 0.0f;
+            if (i0 + 256 * u < sh.nv) clip_io<BF>::ld(p.src, sh.head + (i0 + 256 * u) * W, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < W; ++k) a[k & 3] = fmaf(v[u][k], v[u][k], a[k & 3]);
     }
-    // at most W - 1 elements in front and behind
-    int i = -1;
-    if ((int)threadIdx.x < head) i = threadIdx.x;
-    else if ((int)threadIdx.x >= 64 && (int)threadIdx.x - 64 < p.n - tail) i = tail + threadIdx.x - 64;
-    if (i >= 0) {
-        const double v = clip_io<BF>::ld1(p.src, i);
-        a[0] = fma(v, v, a[0]);
+    if (sh.one >= 0) {
+        const float v = clip_io<BF>::ld1(p.src, sh.one);
+        a[0] = fmaf(v, v, a[0]);
     }
-    return a[0] + a[1];
+    const float s = (a[0] + a[1]) + (a[2] + a[3]);
+    // squares below 2^-126 keep 2^-150 each: less than 2^-26 of a sum of 1e-35; no number stays none
+    if (s < 1e-35f || s > 3e38f) {
+        double d = 0.0;
+        for (int i = threadIdx.x; i < sh.nv; i += 256)
+            for (int k = 0; k < W; ++k) {
+                const double v = clip_io<BF>::ld1(p.src, sh.head + i * W + k);
+                d = fma(v, v, d);
+            }
+        if (sh.one >= 0) {
+            const double v = clip_io<BF>::ld1(p.src, sh.one);
+            d = fma(v, v, d);
+        }
+        return d;
+    }
+    return s;
 }
 
 __device__ __forceinline__ double block_sum(double s, double *red)  // 256 threads or fewer, whole waves; the result in every thread
@@ -132,57 +175,72 @@ __global__ __launch_bounds__(256) void clip_sumsq_kernel(clip_table t, double *_
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-// out[0] = norm, out[1] = coef, and the same at norm_out
-__global__ __launch_bounds__(1024) void clip_coef_kernel(const double *__restrict__ part, uint64_t n, float max_norm, float *__restrict__ out, float *__restrict__ norm_out)
+// Norm and coefficient from the chunks' sums, by a workgroup (x: norm, y: coefficient, in every thread)
+__device__ __forceinline__ float2 clip_coef(const double *part, uint64_t n, float max_norm)
 {
     __shared__ double red[16];
     double a = 0.0;
-#pragma unroll 8
-    for (uint64_t i = threadIdx.x; i < n; i += 1024) a += part[i];
-    const double norm = sqrt(block_sum(a, red));
-    if (threadIdx.x == 0) {
-        const double c = (double)max_norm / (norm + 1e-6);
-        const float coef = isinf(max_norm) || c > 1.0 ? 1.0f : (float)c;  // (a norm that is no number: neither, coef is none)
-        out[0] = (float)norm;
-        out[1] = coef;
-        if (norm_out) {
-            norm_out[0] = (float)norm;
-            norm_out[1] = coef;
-        }
+#pragma unroll 4
+    for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) a += part[i];
+    const double norm = sqrt(block_sum(a, red)), c = (double)max_norm / (norm + 1e-6);
+    return make_float2((float)norm, isinf(max_norm) || c > 1.0 ? 1.0f : (float)c);  // (a norm that is no number: neither, the coefficient is none)
+}
+__device__ __forceinline__ void clip_tell(float2 v, float *to)
+{
+    if (threadIdx.x == 0 && to) {
+        to[0] = v.x;
+        to[1] = v.y;
     }
 }
+__global__ __launch_bounds__(1024) void clip_coef_kernel(const double *__restrict__ part, uint64_t n, float max_norm, float *__restrict__ out, float *__restrict__ norm_out)
+{
+    const float2 v = clip_coef(part, n, max_norm);
+    clip_tell(v, out);
+    clip_tell(v, norm_out);
+}
 
-template <bool BF>
+template <bool BF, bool NT>
 __device__ __forceinline__ void clip_scale(const clip_piece &p, float coef)
 {
-    constexpr int W = clip_io<BF>::W;
-    const int head = clip_head<BF>(p.src, p.n);
-    if (clip_head<BF>(p.dst, p.n) != head) {  // source and destination are aligned differently
+    constexpr int W = clip_io<BF>::W, U = 4;
+    if (clip_head<BF>(p.dst, p.n) != clip_head<BF>(p.src, p.n)) {  // source and destination are aligned differently
         for (int i = threadIdx.x; i < p.n; i += 256) clip_io<BF>::st1(p.dst, i, clip_io<BF>::ld1(p.src, i) * coef);
         return;
     }
-    const int nv = (p.n - head) / W, tail = head + nv * W;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < nv; i += 256) {
-        float v[W];
-        clip_io<BF>::ld(p.src, head + i * W, v);
+    const clip_share<BF> sh(p);
+    for (int i0 = threadIdx.x; i0 < sh.nv; i0 += 256 * U) {
+        float v[U][W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) v[k] *= coef;
-        clip_io<BF>::st(p.dst, head + i * W, v);
+        for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < sh.nv) clip_io<BF>::ld(p.src, sh.head + (i0 + 256 * u) * W, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < sh.nv) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) v[u][k] *= coef;
+                clip_io<BF>::template st<NT>(p.dst, sh.head + (i0 + 256 * u) * W, v[u]);
+            }
     }
-    int i = -1;
-    if ((int)threadIdx.x < head) i = threadIdx.x;
-    else if ((int)threadIdx.x >= 64 && (int)threadIdx.x - 64 < p.n - tail) i = tail + threadIdx.x - 64;
-    if (i >= 0) clip_io<BF>::st1(p.dst, i, clip_io<BF>::ld1(p.src, i) * coef);
+    if (sh.one >= 0) clip_io<BF>::st1(p.dst, sh.one, clip_io<BF>::ld1(p.src, sh.one) * coef);
 }
 
-__global__ __launch_bounds__(256) void clip_scale_kernel(clip_table t, const float *__restrict__ norm)
+// FEW: the sums of all chunks, CLIP_FEW at most, are added by every workgroup for itself (a launch less: 200 000 elements 14.4 -> 10 us)
+template <bool FEW, bool NT>
+__global__ __launch_bounds__(256) void clip_scale_kernel(clip_table t, const float *__restrict__ norm, const double *__restrict__ part, uint64_t n, float max_norm,
+                                                         float *__restrict__ norm_out)
 {
-    const float coef = norm[1];
-    const clip_piece p = clip_find(t, gridDim.x - 1 - blockIdx.x);
+    float coef;
+    if (FEW) {
+        const float2 v = clip_coef(part, n, max_norm);
+        if (blockIdx.x == 0) clip_tell(v, norm_out);
+        coef = v.y;
+    } else {
+        coef = norm[1];
+    }
+    const clip_piece p = clip_find(t, gridDim.x - 1 - blockIdx.x);  // (from the end: what the first pass read last is in the caches)
     if (coef == 1.0f && p.src == p.dst) return;  // nothing to change
-    if (p.bf) clip_scale<true>(p, coef);
-    else clip_scale<false>(p, coef);
+    if (p.bf) clip_scale<true, NT>(p, coef);
+    else clip_scale<false, NT>(p, coef);
 }
 
 size_t clip_workspace(const omega_grad_tensor *t, int n)
@@ -226,13 +284,27 @@ hipError_t launch_clip(const omega_grad_tensor *t, int n, float max_norm, float 
 {
     float *norm = (float *)ws;
     double *part = (double *)((unsigned char *)ws + 256);
-    uint64_t chunks = 0;
+    uint64_t chunks = 0, bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += t[i].n * (t[i].dtype == OMEGA_DTYPE_BF16 ? 2 : 4);
     clip_table tab;
     for (clip_cursor c; clip_fill(t, n, c, tab);) {
         hipLaunchKernelGGL(clip_sumsq_kernel, dim3(tab.chunks), dim3(256), 0, s, tab, part + chunks);
         chunks += tab.chunks;
     }
+    if (n > 0 && chunks <= CLIP_FEW) {  // (one table: a chunk or more a tensor)
+        clip_cursor c;
+        clip_fill(t, n, c, tab);
+        if (c.i == n) {
+            hipLaunchKernelGGL((clip_scale_kernel<true, false>), dim3(tab.chunks), dim3(256), 0, s, tab, norm, part, chunks, max_norm, norm_out);
+            return hipGetLastError();
+        }
+    }
     hipLaunchKernelGGL(clip_coef_kernel, dim3(1), dim3(1024), 0, s, part, chunks, max_norm, norm, norm_out);
-    for (clip_cursor c; clip_fill(t, n, c, tab);) hipLaunchKernelGGL(clip_scale_kernel, dim3(tab.chunks), dim3(256), 0, s, tab, norm);
+    // (53 million bf16 elements, 105 MB: 75 us, past the caches 62)
+    const bool past = bytes >= OMEGA_LLC_BYTES / 8 * 3;
+    for (clip_cursor c; clip_fill(t, n, c, tab);) {
+        if (past) hipLaunchKernelGGL((clip_scale_kernel<false, true>), dim3(tab.chunks), dim3(256), 0, s, tab, norm, part, chunks, max_norm, norm_out);
+        else hipLaunchKernelGGL((clip_scale_kernel<false, false>), dim3(tab.chunks), dim3(256), 0, s, tab, norm, part, chunks, max_norm, norm_out);
+    }
     return hipGetLastError();
 }
