@@ -2,8 +2,9 @@
 // gradients, in pieces of the vocabulary.  The [T,V] logits are never in memory: the forward product's epilogue keeps, for every
 // token and 128 columns, the maximum and the sum of exp(logit - maximum); a second launch joins these; the backward pass computes the
 // logits of a piece of the vocabulary again and turns them, in registers, into their gradient P, of which one piece at a time exists:
-//   loss_t = m_t + log s_t - l[t,y_t],   P[t,v] = (exp(l[t,v] - m_t) / s_t - [v = y_t]) * dloss / n,   dx = P W,   dW = P^T x
-// (m_t, s_t: a row's maximum and sum.  The pair is kept instead of m + log s, whose rounding would stand in every exp.)
+//   loss_t = m_t + log s_t - l[t,y_t],   P[t,v] = exp(l[t,v] - m_t) / s_t - [v = y_t],   dx = g P W,   dW = g P^T x,   g = dloss / n
+// (m_t, s_t: a row's maximum and sum.  The pair is kept instead of m + log s, whose rounding would stand in every exp.  g multiplies the
+// products' fp32 sums: within P, whose elements are rounded to bf16, the rounding of a row's -g would be the same for all rows.)
 //
 // All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], both operands contiguous in k, bf16 on
 // v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
@@ -12,7 +13,7 @@
 // place where its rows are whole and aligned.
 // fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
 // six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first); what is left out is below 2^-24 of a term.
-// Batches of up to 16 tokens stream W once through registers (head_few_kernel).
+// Forward passes of up to 64 tokens (fp32: 128) stream W through a wave's LDS or registers (head_stream_kernel, head_few_kernel).
 // Bound: the matrix cores (2 T V d for the loss, 8 T V d with gradients, logits formed twice); few tokens: the bytes of W.
 #include <algorithm>
 
@@ -28,7 +29,9 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 #define HP_STAGE_BYTES (2 * HP_TILE_BYTES)
 #define HP_STAGES 5
 #define HP_SMEM (HP_STAGES * HP_STAGE_BYTES)    // 160 KiB
-#define HEAD_FEW 16                             // tokens of the streaming kernel
+// Tokens up to which the streaming kernels take a forward pass: W once for up to 64; fp32 twice for up to 128, whose other way is three
+// images of W
+#define HEAD_FEW(dtype) ((dtype) == OMEGA_DTYPE_BF16 ? 64 : 128)
 
 // What a product does with its tile:
 //   LSE  rows = tokens, columns = vocabulary: (max, sum) of every token and 128 columns, the target's logit
@@ -63,6 +66,14 @@ template <int LDS_OFF>
 __device__ __forceinline__ void hp_dma16(const void *sbase, uint32_t voff, uint32_t lds_base)
 {
     asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(sbase), "v"(voff), "s"(lds_base), "n"(LDS_OFF)
+                 : "memory", "scc");
+}
+
+// past the caches: what is read once
+template <int LDS_OFF>
+__device__ __forceinline__ void hp_dma16_nt(const void *sbase, uint32_t voff, uint32_t lds_base)
+{
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0 nt" ::"s"(sbase), "v"(voff), "s"(lds_base), "n"(LDS_OFF)
                  : "memory", "scc");
 }
 
@@ -246,6 +257,9 @@ __device__ __forceinline__ u32x2_t hp_swap16(uint32_t a, uint32_t b)
     return __builtin_amdgcn_permlane16_swap(a, b, false, false);
 }
 
+// what the gradients are multiplied by: dloss / tokens with a target
+__device__ __forceinline__ float head_scale(const float *mean, const float *dloss) { return (dloss ? dloss[0] : 1.0f) / fmaxf(mean[1], 1.0f); }
+
 // Writers of the two products with the vocabulary.  WHOLE: every column of the wave is there.
 template <int NU, int NSEG, bool WHOLE>
 __device__ __forceinline__ void hp_write_lse(const head_prod &p, const hp_item &it, const f32x4_t (&acc)[NU][8], int wm, int wn, int l16, int lq)
@@ -304,7 +318,6 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
 {
     const int col0 = it.n0 + wn * 128 + 4 * lq;
     // (rows behind the last token are written with what the last one's statistics give: nothing reads them)
-    const float gs = (p.dloss ? p.dloss[0] : 1.0f) / fmaxf(p.mean[1], 1.0f);
     const int KTp = p.nt * (HP_TILE / HP_BK);
     constexpr int NP = NSEG > 1 ? 3 : 1;
     // (to the image's end: rows of the tile behind it fall away)
@@ -329,7 +342,7 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
         const int row = it.row0 + 16 * (2 * iu + wm) + l16;
         const bool held = y[iu] >= 0 && y[iu] < p.V;
         // (rows without a target: their logits here are zeros, the images' rows are; what their statistics say does not matter)
-        const float fu = held ? gs / f[iu] : 0.0f, mu = held ? m[iu] : 0.0f;
+        const float fu = held ? 1.0f / f[iu] : 0.0f, mu = held ? m[iu] : 0.0f;
         const int k = y[iu] - p.v0 - col0;
         float v[32];
 #pragma unroll
@@ -338,7 +351,7 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
             if (!WHOLE) v[e] = col0 + 16 * (e >> 2) + (e & 3) < p.N ? v[e] : 0.0f;
         }
         if (__ballot(held && k >= 0 && k < 128 && (k & 12) == 0)) {
-            const float g1 = held ? gs : 0.0f;
+            const float g1 = held ? 1.0f : 0.0f;
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] -= k == 16 * (e >> 2) + (e & 3) ? g1 : 0.0f;
         }
@@ -472,6 +485,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
         }
     } else {
         const int es = p.out_bf ? 2 : 4;
+        const float g = head_scale(p.mean, p.dloss);
         // from the tile's first row on: at most 256 rows of N values
         const uint64_t tile = (uint64_t)p.out + (uint64_t)it.row0 * p.N * es;
         const int rows = min(32 * NU, p.M - it.row0);
@@ -485,7 +499,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             if (p.out_vec && p.out_bf) {  // (rows of whole 16 bytes; halves exchanged as in the image of P)
 #pragma unroll
                 for (int c = 0; c < 8; c += 2) {
-                    const f32x4_t v = acc[iu][c], w = acc[iu][c + 1];
+                    const f32x4_t v = acc[iu][c] * g, w = acc[iu][c + 1] * g;
                     const u32x2_t a = hp_swap16(hp_pack2(v[0], v[1]), hp_pack2(w[0], w[1])), b = hp_swap16(hp_pack2(v[2], v[3]), hp_pack2(w[2], w[3]));
                     const int cc = 16 * (c + (lq & 1)) + 8 * (lq >> 1) - 4 * lq;  // from col0
                     __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{a[0], b[0], a[1], b[1]}, rs, cc < cols ? (uint32_t)(off + cc * 2) : HP_OUTSIDE, 0, 0);
@@ -493,7 +507,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             } else if (p.out_vec) {  // (fp32, a multiple of 4 columns)
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const f32x4_t v = acc[iu][c];
+                    const f32x4_t v = acc[iu][c] * g;
                     __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t *)&v, rs, 16 * c < cols ? (uint32_t)(off + 64 * c) : HP_OUTSIDE, 0, 0);
                 }
             } else {
@@ -501,7 +515,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
                 for (int c = 0; c < 8; ++c)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float v = acc[iu][c][r];
+                        const float v = acc[iu][c][r] * g;
                         const uint32_t at = 16 * c + r < cols ? (uint32_t)(off + (16 * c + r) * es) : HP_OUTSIDE;
                         if (p.out_bf) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)hp_pack2(v, 0.0f), rs, at, 0, 0);
                         else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, at, 0, 0);
@@ -671,91 +685,216 @@ __global__ __launch_bounds__(256) void head_transpose_kernel(const unsigned char
 // A workgroup takes 16 NF rows of W; its four waves share k.  Lane l holds 16 bytes (8 or 4 k) of row l % 16 and of token l % 16, k
 // chunk l / 16: a fragment of v_mfma_f32_16x16x32_bf16, or four of v_mfma_f32_16x16x4_f32 (any order of k serves, as long as both
 // operands have it).  The waves' sums are added in LDS in wave order; (max, sum) of each token over the rows go to `part`.
-template <bool BF, bool VEC>
-__device__ __forceinline__ void head_few_load(const unsigned char *p, int k, int K, f32x4_t &v)  // p: k = 0 of the row; zero from K on
+// 16 bytes from element k of a row of K elements at p on (at the alignment of an element), zero from element K on
+typedef uint32_t u32x4_el __attribute__((ext_vector_type(4), aligned(2)));
+template <bool BF>
+__device__ __forceinline__ u32x4_t head_few_load(const unsigned char *p, int k, int K)
 {
-    constexpr int W = BF ? 8 : 4;
-    v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if (VEC) {
-        if (k < K) v = *(const f32x4_t *)(p + (size_t)k * (BF ? 2 : 4));
+    constexpr int W = BF ? 8 : 4, ES = BF ? 2 : 4;
+    u32x4_t v = {0u, 0u, 0u, 0u};
+    if (k + W <= K) {
+        const u32x4_el u = *(const u32x4_el *)(p + (size_t)k * ES);
+        v = u32x4_t{u[0], u[1], u[2], u[3]};
     } else {
-        uint32_t u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < W; ++j)
             if (k + j < K) {
-                if (BF) u[j >> 1] |= (uint32_t)((const bf16_t *)p)[k + j] << (16 * (j & 1));
-                else u[j & 3] = ((const uint32_t *)p)[k + j];
+                if (BF) v[j >> 1] |= (uint32_t)((const bf16_t *)p)[k + j] << (16 * (j & 1));
+                else v[j & 3] = ((const uint32_t *)p)[k + j];
             }
+    }
+    return v;
+}
+// 16 rows of W and 16 tokens, 16 bytes of k a lane
+template <bool BF>
+__device__ __forceinline__ void head_few_mfma(const u32x4_t &w, const u32x4_t &x, f32x4_t &acc)
+{
+    if (BF) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8_t *)&w, *(const bf16x8_t *)&x, acc, 0, 0, 0);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(u[j]);
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[j]), acc, 0, 0, 0);
     }
 }
-template <bool BF, bool VEC, int NF>
+// The end of both streaming kernels: the four waves' sums added in wave order, (max, sum) of each token over the workgroup's rows of W.
+template <bool BF, int NF, int TF>
+__device__ __forceinline__ void head_few_end(f32x4_t (&acc)[TF][NF], f32x4_t (*sums)[TF][NF][64], int t0, int T, int V, int v0, const int32_t *__restrict__ targets,
+                                             float2 *__restrict__ part, float *__restrict__ tlogit)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
+    if (wave > 0)
+#pragma unroll
+        for (int q = 0; q < TF; ++q)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) sums[wave - 1][q][f][lane] = acc[q][f];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int q = 0; q < TF; ++q) {
+        const int t = t0 + 16 * q + l16;
+        float m = -INFINITY, s = 0.0f;
+        const int y = t < T ? targets[t] : -1;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            f32x4_t &a = acc[q][f];
+            a = ((a + sums[0][q][f][lane]) + sums[1][q][f][lane]) + sums[2][q][f][lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int v = v0 + 16 * f + 4 * lq + r;
+                if (v >= V) a[r] = -INFINITY;
+                else if (v == y && t < T) tlogit[t] = a[r];
+                m = fmaxf(m, a[r]);
+            }
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += hp_exp<BF ? 1 : 6>(acc[q][f][r] - m0);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (t < T && lq == 0) part[(size_t)blockIdx.x * T + t] = make_float2(m, s);
+    }
+}
+
+template <bool BF, int NF, int TF>
 __global__ __launch_bounds__(256) void head_few_kernel(const void *__restrict__ x, const void *__restrict__ w, int T, int V, int K, const int32_t *__restrict__ targets,
                                                        float2 *__restrict__ part, float *__restrict__ tlogit)
 {
-    __shared__ f32x4_t sums[3][NF][64];
+    __shared__ f32x4_t sums[3][TF][NF][64];
     constexpr int KS = BF ? 32 : 16, ES = BF ? 2 : 4, UN = 8 / NF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
-    const int v0 = blockIdx.x * 16 * NF;
-    const unsigned char *xr = (const unsigned char *)x + (size_t)min(l16, T - 1) * K * ES;
-    const unsigned char *wr[NF];
+    const int v0 = blockIdx.x * 16 * NF, t0 = blockIdx.y * 16 * TF;
+    const unsigned char *xr[TF], *wr[NF];
+#pragma unroll
+    for (int q = 0; q < TF; ++q) xr[q] = (const unsigned char *)x + (size_t)min(t0 + 16 * q + l16, T - 1) * K * ES;
 #pragma unroll
     for (int f = 0; f < NF; ++f) wr[f] = (const unsigned char *)w + (size_t)min(v0 + 16 * f + l16, V - 1) * K * ES;
-    f32x4_t acc[NF];
+    f32x4_t acc[TF][NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < TF; ++q)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[q][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const int steps = (K + KS - 1) / KS, first = wave * steps / 4, last = (wave + 1) * steps / 4;
-    for (int s = first; s < last; s += UN) {
-        f32x4_t xv[UN], wv[UN][NF];
+    const int whole = min(last, K / KS);  // steps that are all there
+    int at = first;
+    for (; at + UN <= whole; at += UN) {
+        u32x4_t xv[UN][TF], wv[UN][NF];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int k = s + u < last ? (s + u) * KS + lq * (KS / 4) : K;  // (behind the wave's steps: zeros)
-            head_few_load<BF, VEC>(xr, k, K, xv[u]);
+            const size_t k = ((size_t)(at + u) * KS + lq * (KS / 4)) * ES;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) head_few_load<BF, VEC>(wr[f], k, K, wv[u][f]);
+            for (int q = 0; q < TF; ++q) {
+                const u32x4_el a = *(const u32x4_el *)(xr[q] + k);
+                xv[u][q] = u32x4_t{a[0], a[1], a[2], a[3]};
+            }
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const u32x4_el b = *(const u32x4_el *)(wr[f] + k);
+                wv[u][f] = u32x4_t{b[0], b[1], b[2], b[3]};
+            }
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u)
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                if (BF) {
-                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8_t *)&wv[u][f], *(const bf16x8_t *)&xv[u], acc[f], 0, 0, 0);
-                } else {
+            for (int q = 0; q < TF; ++q)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u][f][j], xv[u][j], acc[f], 0, 0, 0);
-                }
-            }
+                for (int f = 0; f < NF; ++f) head_few_mfma<BF>(wv[u][f], xv[u][q], acc[q][f]);
     }
-    if (wave > 0)
+    for (; at < last; ++at) {
+        const int k = at * KS + lq * (KS / 4);
+        u32x4_t wv[NF];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) sums[wave - 1][f][lane] = acc[f];
-    __syncthreads();
-    if (wave > 0) return;
-    const int t = l16;
-    float m = -INFINITY, s = 0.0f;
-    const int y = t < T ? targets[t] : -1;
+        for (int f = 0; f < NF; ++f) wv[f] = head_few_load<BF>(wr[f], k, K);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        acc[f] = ((acc[f] + sums[0][f][lane]) + sums[1][f][lane]) + sums[2][f][lane];
+        for (int q = 0; q < TF; ++q) {
+            const u32x4_t xv = head_few_load<BF>(xr[q], k, K);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int v = v0 + 16 * f + 4 * lq + r;
-            if (v >= V) acc[f][r] = -INFINITY;
-            else if (v == y && t < T) tlogit[t] = acc[f][r];
-            m = fmaxf(m, acc[f][r]);
+            for (int f = 0; f < NF; ++f) head_few_mfma<BF>(wv[f], xv, acc[q][f]);
         }
     }
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const float m0 = m == -INFINITY ? 0.0f : m;
+    head_few_end<BF, NF, TF>(acc, sums, t0, T, V, v0, targets, part, tlogit);
+}
+
+// The same for rows of whole 16-byte pieces: a wave brings 64 rows of W and the tokens' rows, 128 bytes of each, into a ring of LDS of
+// its own by direct loads, whole lines at a time (loads of 16 rows x 64 bytes straight into registers ask for every line twice: one
+// token x 4096, vocabulary 128000: 188 us, so 164, 6.4 TB/s).  A block of 8 rows is 1 KiB; chunk c of row r lies at slot c ^ r.
+#define HS_STAGES 2   // (80 KiB up to 16 tokens: two workgroups a compute unit; one with three or four stages: 164 -> 168 us)
+#define HS_LOADS(TF) (8 + 2 * (TF))  // 8 of W, 2 of 16 tokens each
+template <bool BF, int TF>
+__global__ __launch_bounds__(256) void head_stream_kernel(const unsigned char *__restrict__ x, const unsigned char *__restrict__ w, int T, int V, int row_bytes,
+                                                          const int32_t *__restrict__ targets, float2 *__restrict__ part, float *__restrict__ tlogit)
+{
+    constexpr int STAGE = HS_LOADS(TF) * 1024;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [4 waves][HS_STAGES][STAGE]; then the waves' sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, lq = lane >> 4;
+    const int v0 = blockIdx.x * 64, t0 = blockIdx.y * 16 * TF;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem + wave * (HS_STAGES * STAGE);
+    const unsigned char *mine = smem + wave * (HS_STAGES * STAGE);
+    const int steps = (row_bytes + 127) / 128, first = wave * steps / 4, n = (wave + 1) * steps / 4 - first;
+    const int last = wave == 3 ? row_bytes - (steps - 1) * 128 : 128;  // bytes of the wave's last step that are there
+    const uint32_t r8 = lane >> 3, ch = ((lane & 7) ^ r8) * 16;
+    const unsigned char *wb = hp_uniform(w + (size_t)v0 * row_bytes + (size_t)first * 128), *xb = hp_uniform(x + (size_t)t0 * row_bytes + (size_t)first * 128);
+    uint32_t vw[8], vx[2 * TF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
+    for (int i = 0; i < 8; ++i) vw[i] = (uint32_t)min(8 * i + (int)r8, V - 1 - v0) * (uint32_t)row_bytes + ch;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += BF ? __expf(acc[f][r] - m0) : expf(acc[f][r] - m0);
-    s += __shfl_xor(s, 16, 64);
-    s += __shfl_xor(s, 32, 64);
-    if (t < T && lq == 0) part[(size_t)blockIdx.x * T + t] = make_float2(m, s);
+    for (int i = 0; i < 2 * TF; ++i) vx[i] = (uint32_t)min(8 * i + (int)r8, T - 1 - t0) * (uint32_t)row_bytes + ch;
+    auto ask = [&](int step, int stage) {
+        const uint32_t sb = lds0 + stage * STAGE;
+        if (step == n - 1 && last < 128) {  // the row's end: what is behind it is read from before it, and counts as zero below
+            const uint32_t back = max((int)ch + 16 - last, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vw[i] -= back;
+#pragma unroll
+            for (int i = 0; i < 2 * TF; ++i) vx[i] -= back;
+        }
+        hp_dma16_nt<0>(wb, vw[0], sb); hp_dma16_nt<1024>(wb, vw[1], sb); hp_dma16_nt<2048>(wb, vw[2], sb); hp_dma16_nt<3072>(wb, vw[3], sb);
+        hp_dma16_nt<4096>(wb, vw[4], sb); hp_dma16_nt<5120>(wb, vw[5], sb); hp_dma16_nt<6144>(wb, vw[6], sb); hp_dma16_nt<7168>(wb, vw[7], sb);
+        hp_dma16<8192>(xb, vx[0], sb); hp_dma16<9216>(xb, vx[1], sb);
+        if constexpr (TF > 1) { hp_dma16<10240>(xb, vx[2], sb); hp_dma16<11264>(xb, vx[3], sb); }
+        if constexpr (TF > 2) { hp_dma16<12288>(xb, vx[4], sb); hp_dma16<13312>(xb, vx[5], sb); hp_dma16<14336>(xb, vx[6], sb); hp_dma16<15360>(xb, vx[7], sb); }
+        wb += 128;
+        xb += 128;
+    };
+    f32x4_t acc[TF][4];
+#pragma unroll
+    for (int q = 0; q < TF; ++q)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[q][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < HS_STAGES - 1 && i < n; ++i) ask(i, i);
+    int stage = 0;
+    for (int i = 0; i < n; ++i) {
+        // this step's loads have landed (the next steps' may be in flight), and what was read from the stage that is filled next is here
+        if (i + HS_STAGES - 1 <= n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((HS_STAGES - 2) * HS_LOADS(TF)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (i + HS_STAGES - 1 < n) ask(i + HS_STAGES - 1, stage == 0 ? HS_STAGES - 1 : stage - 1);
+        const unsigned char *p = mine + stage * STAGE + (l16 >> 3) * 1024 + (l16 & 7) * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = ((4 * h + lq) ^ (l16 & 7)) * 16;
+            const bool none = i == n - 1 && (4 * h + lq) * 16 >= last;
+            const u32x4_t zero = {0u, 0u, 0u, 0u};
+            u32x4_t xv[TF];
+#pragma unroll
+            for (int q = 0; q < TF; ++q) {
+                xv[q] = *(const u32x4_t *)(p + 8192 + q * 2048 + at);
+                if (none) xv[q] = zero;
+            }
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                u32x4_t wv = *(const u32x4_t *)(p + f * 2048 + at);
+                if (none) wv = zero;
+#pragma unroll
+                for (int q = 0; q < TF; ++q) head_few_mfma<BF>(wv, xv[q], acc[q][f]);
+            }
+        }
+        stage = stage + 1 == HS_STAGES ? 0 : stage + 1;
+    }
+    __syncthreads();  // (the rings are done with: the sums take their place)
+    head_few_end<BF, 4, TF>(acc, (f32x4_t(*)[TF][4][64])smem, t0, T, V, v0, targets, part, tlogit);
 }
 
 // ---- joins ----
@@ -836,14 +975,16 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float *loss, cons
 // dx: the slabs added in slice order, rounded once; rows without a target are zero
 template <bool BF>
 __global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ targets, int T, int V,
-                                                      int d, void *__restrict__ dx)
+                                                      int d, const float *__restrict__ mean, const float *dloss, void *__restrict__ dx)
 {
+    const float g = head_scale(mean, dloss);
     const int t = blockIdx.x, y = targets[t];
     const bool held = y >= 0 && y < V;
     for (int c = blockIdx.y * 256 + threadIdx.x; c < d; c += gridDim.y * 256) {
         float s = 0.0f;
         if (held)
             for (int k = 0; k < slices; ++k) s += slabs[(size_t)k * slab + (size_t)t * ld + c];
+        s = held ? s * g : 0.0f;
         if (BF) ((bf16_t *)dx)[(size_t)t * d + c] = f32_to_bf16(s);
         else ((float *)dx)[(size_t)t * d + c] = s;
     }
@@ -871,7 +1012,7 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
 {
     head_plan h = {};
     h.planes = a.dtype == OMEGA_DTYPE_BF16 ? 1 : 3;
-    h.few = !backward && a.T <= HEAD_FEW;
+    h.few = !backward && a.T <= HEAD_FEW(a.dtype);
     h.dp = k_pad(a.d);
     h.Tp = k_pad(a.T);
     // W in place: bf16 rows of whole pairs of k steps, 16-byte aligned (tile offsets within 32 bits)
@@ -948,6 +1089,11 @@ static hipError_t head_init_of()
 }
 hipError_t head_init(void)
 {
+    for (const void *f : {(const void *)head_stream_kernel<true, 1>, (const void *)head_stream_kernel<true, 2>, (const void *)head_stream_kernel<true, 4>,
+                          (const void *)head_stream_kernel<false, 1>, (const void *)head_stream_kernel<false, 2>, (const void *)head_stream_kernel<false, 4>}) {
+        const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, HP_SMEM);
+        if (e != hipSuccess) return e;
+    }
     hipError_t e = head_init_of<HEAD_LSE>();
     if (e == hipSuccess) e = head_init_of<HEAD_P>();
     if (e == hipSuccess) e = head_init_of<HEAD_ACC>();
@@ -1014,16 +1160,35 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
     const size_t es = bf ? 2 : 4;
     int nb = h.nb;
     if (h.few) {
-        const bool vec = a.d % (bf ? 8 : 4) == 0 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
         // 64 rows of W a workgroup read x a quarter as often as 16; vocabularies that would leave compute units idle take 16
-        const int nf = a.V >= 64 * 2 * ctx->num_cus ? 4 : 1;
+        const int nf = a.V >= 64 * ctx->num_cus ? 4 : 1;
         nb = ceil_div(a.V, 16 * nf);
-#define HEAD_FEW_K(B, VV, F) hipLaunchKernelGGL((head_few_kernel<B, VV, F>), dim3(nb), dim3(256), 0, s, a.x, a.w, a.T, a.V, a.d, a.targets, part, tlogit)
-#define HEAD_FEW_F(B, VV) do { if (nf == 4) HEAD_FEW_K(B, VV, 4); else HEAD_FEW_K(B, VV, 1); } while (0)
-        if (bf) { if (vec) HEAD_FEW_F(true, true); else HEAD_FEW_F(true, false); }
-        else { if (vec) HEAD_FEW_F(false, true); else HEAD_FEW_F(false, false); }
-#undef HEAD_FEW_F
+        const int row_bytes = a.d * (int)es, tf = a.T <= 16 ? 1 : a.T <= 32 ? 2 : 4;
+        const dim3 grid(nb, ceil_div(a.T, 16 * tf));
+        const unsigned char *x = (const unsigned char *)a.x, *w = (const unsigned char *)a.w;
+#define HEAD_STREAM_K(B, TF)                                                                                                                             \
+    hipLaunchKernelGGL((head_stream_kernel<B, TF>), grid, dim3(256), 4 * HS_STAGES * HS_LOADS(TF) * 1024, s, x, w, a.T, a.V, row_bytes, a.targets, part, \
+                       tlogit)
+#define HEAD_FEW_K(B, F, TF) hipLaunchKernelGGL((head_few_kernel<B, F, TF>), grid, dim3(256), 0, s, a.x, a.w, a.T, a.V, a.d, a.targets, part, tlogit)
+#define HEAD_FEW_T(K, ...)                  \
+    do {                                    \
+        if (tf == 1) K(__VA_ARGS__, 1);     \
+        else if (tf == 2) K(__VA_ARGS__, 2); \
+        else K(__VA_ARGS__, 4);             \
+    } while (0)
+        if (nf == 4 && row_bytes % 16 == 0 && row_bytes >= 128 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0) {
+            if (bf) HEAD_FEW_T(HEAD_STREAM_K, true);
+            else HEAD_FEW_T(HEAD_STREAM_K, false);
+        } else if (bf) {
+            if (nf == 4) HEAD_FEW_T(HEAD_FEW_K, true, 4);
+            else HEAD_FEW_T(HEAD_FEW_K, true, 1);
+        } else {
+            if (nf == 4) HEAD_FEW_T(HEAD_FEW_K, false, 4);
+            else HEAD_FEW_T(HEAD_FEW_K, false, 1);
+        }
+#undef HEAD_FEW_T
 #undef HEAD_FEW_K
+#undef HEAD_STREAM_K
     } else {
         head_images(a, a.x, a.T, a.d, (int)up_to(a.T, 64), h.dp, a.targets, base + h.x_img, h.x_plane, nullptr, 0, 0, s);
         for (int v0 = 0; v0 < a.V; v0 += h.piece) {
@@ -1084,8 +1249,6 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
         p.slices = 1;
         p.targets = a.targets;
         p.row_stats = a.row_stats;
-        p.mean = a.mean;
-        p.dloss = a.dloss;
         p.T = a.T;
         p.V = a.V;
         p.v0 = v0;
@@ -1122,6 +1285,8 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.slices = 1;
             q.out = (unsigned char *)a.dw + (size_t)v0 * a.d * es;
             q.out_bf = bf;
+            q.mean = a.mean;
+            q.dloss = a.dloss;
             q.out_vec = a.d % (bf ? 8 : 4) == 0 && (uintptr_t)q.out % 16 == 0;
             HEAD_TRY(head_product<HEAD_OUT>(ctx, q, h.planes, s));
         }
@@ -1129,8 +1294,8 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     if (a.dx) {
         const int vp0 = (int)up_to(std::min(h.piece, a.V), 256), slices = std::max(1, std::min(h.slices, vp0 / 32 / 8));
         const dim3 grid(a.T, std::min(ceil_div(a.d, 256), 1024));
-        if (bf) hipLaunchKernelGGL(head_dx_kernel<true>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.dx);
-        else hipLaunchKernelGGL(head_dx_kernel<false>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.dx);
+        if (bf) hipLaunchKernelGGL(head_dx_kernel<true>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);
+        else hipLaunchKernelGGL(head_dx_kernel<false>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);
     }
     return hipGetLastError();
 }

@@ -132,6 +132,19 @@ def test_rows_without_a_target_hold_anything(T, dtype):
     assert not got["dx"][(y < 0) | (y >= V)].any() and not got["loss"][(y < 0) | (y >= V)].any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,d", [(1, 256), (16, 64), (17, 72), (32, 200), (33, 136), (64, 1000), (65, 40), (100, 68), (128, 132), (129, 72), (5, 63), (40, 33)])
+def test_few_tokens_and_a_large_vocabulary(T, d, dtype):
+    """Forward passes that stream the head's weights: rows of whole lines, of whole 16-byte pieces and of neither."""
+    V = 16384 + 77
+    rng = np.random.default_rng(T + d)
+    w, y = normal(rng, V, d, std=d ** -0.5, dtype=dtype), targets_of(rng, T, V)
+    y[0] = V - 1
+    x = rounded(normal(rng, T, d) + np.float32(5) * w[np.clip(y, 0, V - 1)], dtype)
+    for shift in (0, 1):
+        check(run(x, w, y, dtype, shift, stats=False), reference(x, w, y, dtype), shift)
+
+
 def test_no_target_at_all_and_no_rows():
     rng = np.random.default_rng(0)
     for T in (4, 40):
