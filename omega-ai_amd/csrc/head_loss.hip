@@ -8,7 +8,7 @@
 //
 // All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], both operands contiguous in k, bf16 on
 // v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
-// to LDS in a ring of five steps of 32 k; persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that
+// to LDS in a ring of five or more steps of 32 k; persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that
 // head_images_kernel writes, transposed where the product sums over rows, zero where k goes beyond the matrix; W itself is read in
 // place where its rows are whole and aligned.
 // fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
@@ -25,10 +25,14 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 #define HP_BK 32
 #define HP_TILE 256
-#define HP_TILE_BYTES (HP_TILE * HP_BK * 2)     // one operand's step: 16 KiB
-#define HP_STAGE_BYTES (2 * HP_TILE_BYTES)
-#define HP_STAGES 5
-#define HP_SMEM (HP_STAGES * HP_STAGE_BYTES)    // 160 KiB
+#define HP_SMEM (160 * 1024)                    // all of a compute unit's LDS
+// A tile of 32 NU rows: bytes of its A operand's step and of a stage of the ring, stages (lower tiles are through with a step
+// sooner and need more of them to cover the same latency: fp32 1611 x 1760, vocabulary 1689, 64-row tiles, five stages 114 us, seven 93),
+// direct loads of a wave and step
+#define HP_A_BYTES(NU) ((NU) * 2048)
+#define HP_STAGE_BYTES(NU) (HP_A_BYTES(NU) + HP_TILE * HP_BK * 2)
+#define HP_STAGES(NU) ((NU) == 2 ? 7 : (NU) == 4 ? 6 : 5)
+#define HP_LOADS(NU) ((NU) / 2 + 4)
 // Tokens up to which the streaming kernels take a forward pass: W once for up to 64; fp32 twice for up to 128, whose other way is three
 // images of W
 #define HEAD_FEW(dtype) ((dtype) == OMEGA_DTYPE_BF16 ? 64 : 128)
@@ -169,17 +173,17 @@ struct hp_state {
     uint32_t va[4], vb[4];
 };
 
-// Loads and fragments of the ring, the MFMAs of a step.  The first 8 groups of 4 MFMAs carry the 16 fragment reads of the
-// next step, every other group one of the 8 direct loads of the step five ahead.
-#define HP_READ(FA, FB, r)                                                                            \
-    do {                                                                                              \
-        if ((r) < 8) FB[(r) & 7] = *(const bf16x8_t *)(((r) & 1 ? rb1 : rb0) + (((r) & 7) >> 1) * 2048u); \
-        else FA[((r) - 8) & 7] = *(const bf16x8_t *)(ra + (((r) - 8) & 7) * 2048u);                   \
+// Loads and fragments of the ring, the MFMAs of a step.  The first 8 groups of 4 MFMAs carry the fragment reads of the
+// next step, every other group one of the direct loads of the step that the ring is ahead.
+#define HP_READ(FA, FB, r)                                                                                                     \
+    do {                                                                                                                       \
+        if ((r) < 8) FB[(r) & 7] = *(const bf16x8_t *)(((r) & 1 ? rb1 : rb0) + (((r) & 7) >> 1) * 2048u);                      \
+        else if ((r) - 8 < NU) FA[((r) - 8) & 7] = *(const bf16x8_t *)(ra + (((r) - 8) & 7) * 2048u);                          \
     } while (0)
-#define HP_LOAD(l, sb)                                                                     \
-    do {                                                                                   \
-        if ((l) < 4) hp_dma16<((l) & 3) * 4096>(lA, st.va[(l) & 3], sb);                   \
-        else hp_dma16<HP_TILE_BYTES + ((l) & 3) * 4096>(lB, st.vb[(l) & 3], sb);           \
+#define HP_LOAD(l, sb)                                                                                                         \
+    do {                                                                                                                       \
+        if ((l) < NU / 2) hp_dma16<((l) & 3) * 4096>(lA, st.va[(l) & 3], sb);                                                  \
+        else if ((l) < HP_LOADS(NU)) hp_dma16<HP_A_BYTES(NU) + (((l) - NU / 2) & 3) * 4096>(lB, st.vb[((l) - NU / 2) & 3], sb); \
     } while (0)
 #define HP_MFMA(PA, PB, iu, c)                                                                                                    \
     do {                                                                                                                             \
@@ -215,20 +219,20 @@ struct hp_state {
         HP_LOAD(7, sb);                                                                                     \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
         HP_MFMA(PA, PB, 7, 6);                                                                           \
-        cur = cur + 1 == HP_STAGES ? 0 : cur + 1;                                                           \
-        sb = lds_wave + cur * HP_STAGE_BYTES;                                                               \
+        cur = cur + 1 == ST ? 0 : cur + 1;                                                                \
+        sb = lds_wave + cur * HP_STAGE_BYTES(NU);                                                           \
         lA += 8192;                                                                                         \
         lB += stepB;                                                                                        \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
         HP_MFMA(PA, PB, 7, 7);                                                                           \
         {                                                                                                   \
-            const unsigned char *sn = smem + (cur + 1 == HP_STAGES ? 0 : cur + 1) * HP_STAGE_BYTES;         \
+            const unsigned char *sn = smem + (cur + 1 == ST ? 0 : cur + 1) * HP_STAGE_BYTES(NU);            \
             ra = sn + pa;                                                                                   \
             rb0 = sn + pb0;                                                                                 \
             rb1 = sn + pb1;                                                                                 \
         }                                                                                                   \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
-        asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)" ::: "memory");                                        \
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * HP_LOADS(NU)) : "memory");           \
         __syncthreads();                                                                                    \
     } while (0)
 
@@ -389,6 +393,7 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
 template <int NU, int EPI, int NSEG>
 __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane0)
 {
+    constexpr int ST = HP_STAGES(NU);
     const int wm = wave >> 1, wn = wave & 1;
     int lane = hp_fresh(lane0), l16 = lane & 15, lq = lane >> 4;
     const int kt = __builtin_amdgcn_readfirstlane(it.kt);
@@ -396,23 +401,23 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     const uint32_t lds_wave = lds0 + wave * 1024;
     const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
-    const uint32_t pb0 = HP_TILE_BYTES + (uint32_t)(wn * 128 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16)) << 4);
-    const uint32_t pb1 = HP_TILE_BYTES + (uint32_t)(wn * 128 + 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | 16)) << 4);
+    const uint32_t pb0 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16)) << 4);
+    const uint32_t pb1 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | 16)) << 4);
     int cur = __builtin_amdgcn_readfirstlane(st.cur);
     const unsigned char *lA = hp_uniform(st.lA), *lB = hp_uniform(st.lB);
     nxt = hp_make_item(p, next_idx);
-    uint32_t sb = lds_wave + cur * HP_STAGE_BYTES;
+    uint32_t sb = lds_wave + cur * HP_STAGE_BYTES(NU);
     const unsigned char *ra, *rb0, *rb1;
     {
-        const unsigned char *sn = smem + (cur + 1 == HP_STAGES ? 0 : cur + 1) * HP_STAGE_BYTES;
+        const unsigned char *sn = smem + (cur + 1 == ST ? 0 : cur + 1) * HP_STAGE_BYTES(NU);
         ra = sn + pa;
         rb0 = sn + pb0;
         rb1 = sn + pb1;
     }
     f32x4_t acc[NU][8];
     const f32x4_t zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
-    // The steps of a pair of parts two at a time (their number is even, at least 8).  The loads of the last five are the next pair's
-    // or the next item's first (behind the last item: this one's once more, which nobody reads).
+    // The steps of a pair of parts two at a time (their number is even, at least 8).  The loads of the last ST are the next pair's or the
+    // next item's first (behind the last item: this one's once more, which nobody reads).
     // (zeros in the registers: a first step that starts from zero operands instead costs as many moves of registers)
 #pragma unroll
     for (int i = 0; i < NU; ++i)
@@ -425,12 +430,14 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     HP_PIN();
 #pragma unroll 1
     for (int seg = 0; seg < NSEG; ++seg) {
-        int k = kt - 6;
-        do {
-            HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
-            HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
-        } while ((k -= 2) > 0);
-        HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
+        int k = kt - ST - (ST & 1);
+        if (NU > 2 || k > 0) {  // (eight steps, seven stages: nothing yet)
+            do {
+                HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
+                HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
+            } while ((k -= 2) > 0);
+        }
+        if (ST & 1) HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
         {
             const int ns = seg + 1 < NSEG ? seg + 1 : 0;
             const hp_item &li = ns == 0 ? nxt : it;  // the item of the loads from here on
@@ -439,8 +446,8 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             lB = hp_uniform(li.B + b0);
             hp_lane_offsets(p, li, wave, hp_fresh(lane0), st.va, st.vb);
         }
-        HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
-        for (int k = 0; k < 2; ++k) {
+        if (ST & 1) HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
+        for (k = 0; k < ST / 2; ++k) {
             HP_STEP(st.fa0, st.fb0, st.fa1, st.fb1);
             HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         }
@@ -545,8 +552,9 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
     hp_lane_offsets(p, it, wave, lane, st.va, st.vb);
     const size_t stepB = p.b_ld == 0 ? 8192 : 64;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
-    for (int s5 = 0; s5 < HP_STAGES; ++s5) {  // the first item's steps 0 .. 4 (of 8 or more of its first part)
-        const uint32_t sb = lds0 + wave * 1024 + s5 * HP_STAGE_BYTES;
+    constexpr int ST = HP_STAGES(NU);
+    for (int i = 0; i < ST; ++i) {  // the first item's first steps (of 8 or more of its first part)
+        const uint32_t sb = lds0 + wave * 1024 + i * HP_STAGE_BYTES(NU);
         HP_LOAD(0, sb); HP_LOAD(1, sb); HP_LOAD(2, sb); HP_LOAD(3, sb);
         HP_LOAD(4, sb); HP_LOAD(5, sb); HP_LOAD(6, sb); HP_LOAD(7, sb);
         lA += 8192;
@@ -554,18 +562,18 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
     }
     st.lA = lA;
     st.lB = lB;
-    asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * HP_LOADS(NU)) : "memory");
     __syncthreads();
     {
         const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const uint32_t pb = HP_TILE_BYTES + (uint32_t)(wn * 128 + 16 * (r & 1) + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | ((r & 1) << 4))) << 4);
+            const uint32_t pb = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + 16 * (r & 1) + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | ((r & 1) << 4))) << 4);
             st.fb0[r] = *(const bf16x8_t *)(smem + pb + (r >> 1) * 2048u);
-            st.fa0[r] = *(const bf16x8_t *)(smem + pa + r * 2048u);
+            if (r < NU) st.fa0[r] = *(const bf16x8_t *)(smem + pa + r * 2048u);
         }
     }
-    asm volatile("s_waitcnt vmcnt(24) lgkmcnt(0)" ::: "memory");  // step 1 has landed; every wave has taken step 0 out of its stage
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * HP_LOADS(NU)) : "memory");  // step 1 has landed; every wave has taken step 0 out of its stage
     __syncthreads();
     st.cur = 0;
     for (;;) {
