@@ -6,11 +6,10 @@
 // (m_t, s_t: a row's maximum and sum.  The pair is kept instead of m + log s, whose rounding would stand in every exp.  g multiplies the
 // products' fp32 sums: within P, whose elements are rounded to bf16, the rounding of a row's -g would be the same for all rows.)
 //
-// All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], both operands contiguous in k, bf16 on
-// v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
+// All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], bf16 on v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
 // to LDS in a ring of five or more steps of 32 k; persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that
-// head_images_kernel writes, transposed where the product sums over rows, zero where k goes beyond the matrix; W itself is read in
-// place where its rows are whole and aligned.
+// head_images_kernel or the product before writes, zero where k goes beyond the matrix; W itself is read in place where its rows are whole
+// and aligned.  Where the product sums over an operand's rows (W for dx, P and x for dW), the LDS reads transpose.
 // fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
 // six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first); what is left out is below 2^-24 of a term.
 // Forward passes of up to 64 tokens (fp32: 128) stream W through a wave's LDS or registers (head_stream_kernel, head_few_kernel).
@@ -49,6 +48,9 @@ struct head_prod {
     size_t planeA, planeB;           // bytes from one part to the next (fp32)
     size_t b_ld;                     // 0: image
     int kt;                          // k steps (even, 8 or more)
+    int ktA, ktB;                    // k steps of a row group of the images (an operand read across its rows: its columns / 32)
+    int rowsA;                       // A's rows as far as the product needs them
+    int rowsB;                       // B read across its rows in place: the rows there are
     int M, N, mt, nt, slices;        // mt row tiles of `th` rows (64, 128, 192 or 256), nt column tiles of 256
     int th;
     // epilogues
@@ -65,6 +67,14 @@ struct head_prod {
     void *out;                       // OUT: row-major, ld = N
     int out_bf, out_vec;
 };
+
+// Operands that are read across their rows (the rows are k): W for dx, both for dW.  Their steps are 32 rows x 256 columns, in LDS the same blocks
+// of 16 rows x 32 columns as those of an image, two for each 32 columns; ds_read_b64_tr_b16 hands each lane 4 rows of its column.  The
+// reads are twice as many, each half as long, without bank conflicts.  Against images of the transposes, made by kernels of their own:
+// gradients of 4096 tokens, vocabulary 128000, d 4096: 9.62 -> 9.09 ms (the products 740 to 790 us each per 32000 rows of W either way);
+// 512 x 4096, 32000: 587 -> 446 us; 131 x 2072, 51750: 417 -> 361.
+#define HP_TR_A(EPI) ((EPI) == HEAD_OUT)
+#define HP_TR_B(EPI) ((EPI) >= HEAD_ACC)
 
 template <int LDS_OFF>
 __device__ __forceinline__ void hp_dma16(const void *sbase, uint32_t voff, uint32_t lds_base)
@@ -117,8 +127,10 @@ struct hp_item {
     const unsigned char *A, *B;   // first step of the tile's rows and columns
     int row0, n0, slice;          // first row and column
     int kt;                       // steps (of a part)
+    int phase, rows;              // of an operand read across its rows: first step's place in its row group, rows from there on
 };
 
+template <int EPI>
 __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
 {
     hp_item it;
@@ -130,9 +142,16 @@ __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
     it.slice = __builtin_amdgcn_readfirstlane(sl);
     const int first = ((it.slice * p.kt) / p.slices) & ~1;
     it.kt = __builtin_amdgcn_readfirstlane((it.slice + 1 == p.slices ? p.kt : (((it.slice + 1) * p.kt) / p.slices) & ~1) - first);
-    const size_t rg = (size_t)p.kt * 8192;  // bytes of a row group of an image
-    it.A = hp_uniform(p.A + (size_t)(it.row0 >> 7) * rg + (size_t)first * 8192);
-    it.B = hp_uniform(p.b_ld == 0 ? p.B + (size_t)(it.n0 >> 7) * rg + (size_t)first * 8192 : p.B + (size_t)it.n0 * p.b_ld + (size_t)first * 64);
+    it.phase = __builtin_amdgcn_readfirstlane(first & 3);
+    it.rows = __builtin_amdgcn_readfirstlane(p.b_ld == 0 ? 0x7fffffff : p.rowsB - 32 * first);
+    const size_t rgA = (size_t)p.ktA * 8192, rgB = (size_t)p.ktB * 8192;  // bytes of a row group of an image
+    const size_t across = (size_t)(first >> 2), in = (size_t)(first & 3) * 2048;
+    if (HP_TR_A(EPI)) it.A = hp_uniform(p.A + across * rgA + in + (size_t)(it.row0 >> 5) * 8192);
+    else it.A = hp_uniform(p.A + (size_t)(it.row0 >> 7) * rgA + (size_t)first * 8192);
+    if (HP_TR_B(EPI))
+        it.B = hp_uniform(p.b_ld == 0 ? p.B + across * rgB + in + (size_t)(it.n0 >> 5) * 8192 : p.B + (size_t)first * 32 * p.b_ld + (size_t)it.n0 * 2);
+    else
+        it.B = hp_uniform(p.b_ld == 0 ? p.B + (size_t)(it.n0 >> 7) * rgB + (size_t)first * 8192 : p.B + (size_t)it.n0 * p.b_ld + (size_t)first * 64);
     return it;
 }
 // The lane number as a value that the compiler cannot carry over: what follows from it is computed where it is used.  (Kept from item
@@ -142,24 +161,107 @@ __device__ __forceinline__ int hp_fresh(int lane)
     asm volatile("" : "+v"(lane));
     return lane;
 }
-// what the lane adds for the wave's loads: blocks of 16 rows wave + 4 n of the item's rows and columns
+// what the lane adds for the wave's loads, blocks wave + 4 n of the step: of 16 rows each; of an operand read across its rows, 16 rows and
+// 32 columns, the upper and the lower 16 rows in turn
+template <int EPI>
 __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_item &it, int wave, int lane, uint32_t (&va)[4], uint32_t (&vb)[4])
 {
-    const uint32_t rg = (uint32_t)p.kt * 8192u;
+    const uint32_t rgA = (uint32_t)p.ktA * 8192u, rgB = (uint32_t)p.ktB * 8192u;
     const int blk0 = (it.row0 & 127) >> 4;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int q = wave + 4 * k;
-        const bool valid = 16 * q < p.th && it.row0 + 16 * q < p.M;  // (a block without rows: every lane reads the first 16 bytes of the item's first block)
-        const int b = blk0 + (valid ? q : 0);
-        va[k] = (uint32_t)(b >> 3) * rg + (uint32_t)(b & 7) * 1024u + (valid ? (uint32_t)lane * 16u : 0u);
-        if (p.b_ld == 0) {
-            vb[k] = (uint32_t)(q >> 3) * rg + (uint32_t)(q & 7) * 1024u + (uint32_t)lane * 16u;
+        if (HP_TR_A(EPI)) {
+            const bool valid = 16 * q < p.th && it.row0 + 32 * (q >> 1) < 32 * p.ktA;
+            va[k] = valid ? (uint32_t)(q >> 1) * 8192u + (uint32_t)(q & 1) * 1024u + (uint32_t)lane * 16u : 0u;
+        } else {
+            const bool valid = 16 * q < p.th && it.row0 + 16 * q < p.rowsA;  // (a block without rows: every lane reads the first 16 bytes of the item's first block)
+            const int b = blk0 + (valid ? q : 0);
+            va[k] = (uint32_t)(b >> 3) * rgA + (uint32_t)(b & 7) * 1024u + (valid ? (uint32_t)lane * 16u : 0u);
+        }
+        if (HP_TR_B(EPI) && p.b_ld == 0) {
+            vb[k] = it.n0 + 32 * (q >> 1) < 32 * p.ktB ? (uint32_t)(q >> 1) * 8192u + (uint32_t)(q & 1) * 1024u + (uint32_t)lane * 16u : 0u;
+        } else if (HP_TR_B(EPI)) {
+            const int r = 16 * (q & 1) + (lane >> 2), c = 32 * (q >> 1) + 8 * ((lane & 3) ^ pk_swz(r));
+            vb[k] = (uint32_t)min(r, it.rows - 1) * (uint32_t)p.b_ld + (uint32_t)min(c, p.N - 8 - it.n0) * 2u;
+        } else if (p.b_ld == 0) {
+            vb[k] = (uint32_t)(q >> 3) * rgB + (uint32_t)(q & 7) * 1024u + (uint32_t)lane * 16u;
         } else {
             const int r = 16 * q + (lane >> 2);
             vb[k] = (uint32_t)min(r, p.N - 1 - it.n0) * (uint32_t)p.b_ld + (uint32_t)(((lane & 3) ^ pk_swz(r)) << 4);
         }
     }
+}
+
+// where the loads have got to
+struct hp_at {
+    const unsigned char *A, *B;
+    int phase, rows;
+};
+// ... and a step on.  Rows of W in place: where the last ones are fewer than 32, the lanes behind them read the last one, and a step that
+// has none reads the step before once more (P is zero there).
+template <int EPI>
+__device__ __forceinline__ void hp_advance(const head_prod &p, hp_at &at, uint32_t (&vb)[4], int wave, int lane)
+{
+    if (!HP_TR_B(EPI)) {
+        at.A += 8192;
+        at.B += p.b_ld == 0 ? 8192 : 64;
+        return;
+    }
+    at.phase = (at.phase + 1) & 3;
+    const bool next = at.phase == 0;  // the next row group
+    if (HP_TR_A(EPI)) at.A += next ? (size_t)p.ktA * 8192 - 6144 : 2048;
+    else at.A += 8192;
+    if (HP_TR_A(EPI) || p.b_ld == 0) {
+        at.B += next ? (size_t)p.ktB * 8192 - 6144 : 2048;
+    } else {
+        at.rows -= 32;
+        at.B += at.rows > 0 ? (size_t)32 * p.b_ld : 0;
+        if (at.rows > 0 && at.rows < 32) {
+            const int behind = max(16 * (wave & 1) + (hp_fresh(lane) >> 2) - (at.rows - 1), 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) vb[k] -= (uint32_t)behind * (uint32_t)p.b_ld;
+        }
+    }
+}
+
+// Where a lane's fragments lie in a stage.  a0, b0 / b1 (even / odd fragments of 16 columns): the 16-byte chunk lane / 16 of its row.  Read
+// across rows: rows 8 kc .. + 3 (4 more: the other address + 256) of a fragment's columns, kc = (0, 2, 1, 3)[lane / 16], which keeps the
+// lanes of a half wave in different banks; the other operand takes its chunks in the same order.
+struct hp_frag {
+    uint32_t a0, a1, b0, b1;
+};
+template <int NU, int EPI>
+__device__ __forceinline__ hp_frag hp_frag_of(int wm, int wn, int lane)
+{
+    const int l16 = lane & 15, lq = lane >> 4;
+    const int kc = HP_TR_B(EPI) ? ((lq & 1) << 1) | (lq >> 1) : lq;
+    const uint32_t across = (uint32_t)((lq & 1) * 1024 + (8 * (lq >> 1) + (l16 >> 2)) * 64 + ((((l16 >> 1) ^ (l16 >> 3) ^ (lq >> 1)) & 1) << 4) + 8 * (l16 & 1));
+    hp_frag f;
+    if (HP_TR_A(EPI)) {
+        f.a0 = across + 32u * (uint32_t)(wm ^ (lq & 1));
+        f.a1 = f.a0 ^ 32u;
+    } else {
+        f.a0 = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(kc ^ pk_swz(l16 | (wm << 4))) << 4);
+        f.a1 = 0;
+    }
+    if (HP_TR_B(EPI)) {
+        f.b0 = HP_A_BYTES(NU) + wn * 8192u + across + 32u * (uint32_t)(lq & 1);
+        f.b1 = f.b0 ^ 32u;
+    } else {
+        f.b0 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + l16) * 64 + ((uint32_t)(kc ^ pk_swz(l16)) << 4);
+        f.b1 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + 16 + l16) * 64 + ((uint32_t)(kc ^ pk_swz(l16 | 16)) << 4);
+    }
+    return f;
+}
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+__device__ __forceinline__ bf16x8_t hp_across(const unsigned char *lo, const unsigned char *hi)
+{
+    typedef __attribute__((address_space(3))) s16x4_t lds_t;
+    const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t *)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t *)hi);
+    const s16x8_t v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return *(const bf16x8_t *)&v;
 }
 
 // pairs of parts in the order they are added: (A, B) = mm, lh, hl, mh, hm, hh
@@ -169,21 +271,37 @@ __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_ite
 struct hp_state {
     int cur;                             // ring position
     bf16x8_t fa0[8], fb0[8], fa1[8], fb1[8];
-    const unsigned char *lA, *lB;        // where the loads have got to
+    hp_at at;
     uint32_t va[4], vb[4];
 };
 
-// Loads and fragments of the ring, the MFMAs of a step.  The first 8 groups of 4 MFMAs carry the fragment reads of the
-// next step, every other group one of the direct loads of the step that the ring is ahead.
+// Loads and fragments of the ring, the MFMAs of a step.  The first 8 groups of 4 MFMAs carry the fragment reads of the next step (two
+// MFMAs apart: next to each other those across rows cost 4 % of a product), every other group one of the direct loads of the step that
+// the ring is ahead.
 #define HP_READ(FA, FB, r)                                                                                                     \
     do {                                                                                                                       \
-        if ((r) < 8) FB[(r) & 7] = *(const bf16x8_t *)(((r) & 1 ? rb1 : rb0) + (((r) & 7) >> 1) * 2048u);                      \
-        else if ((r) - 8 < NU) FA[((r) - 8) & 7] = *(const bf16x8_t *)(ra + (((r) - 8) & 7) * 2048u);                          \
+        if ((r) < 8) {                                                                                                         \
+            const unsigned char *b0 = ((r) & 1 ? rb1 : rb0) + (((r) & 7) >> 1) * 2048u;                                        \
+            if (HP_TR_B(EPI)) FB[(r) & 7] = hp_across(b0, ((r) & 1 ? rb0 : rb1) + (((r) & 7) >> 1) * 2048u + 256u);            \
+            else FB[(r) & 7] = *(const bf16x8_t *)b0;                                                                          \
+        } else if ((r) - 8 < NU) {                                                                                             \
+            if (HP_TR_A(EPI)) FA[((r) - 8) & 7] = hp_across(ra + (((r) - 8) & 7) * 2048u, ra1 + (((r) - 8) & 7) * 2048u + 256u); \
+            else FA[((r) - 8) & 7] = *(const bf16x8_t *)(ra + (((r) - 8) & 7) * 2048u);                                        \
+        }                                                                                                                      \
     } while (0)
 #define HP_LOAD(l, sb)                                                                                                         \
     do {                                                                                                                       \
-        if ((l) < NU / 2) hp_dma16<((l) & 3) * 4096>(lA, st.va[(l) & 3], sb);                                                  \
-        else if ((l) < HP_LOADS(NU)) hp_dma16<HP_A_BYTES(NU) + (((l) - NU / 2) & 3) * 4096>(lB, st.vb[((l) - NU / 2) & 3], sb); \
+        if ((l) < NU / 2) hp_dma16<((l) & 3) * 4096>(at.A, st.va[(l) & 3], sb);                                                \
+        else if ((l) < HP_LOADS(NU)) hp_dma16<HP_A_BYTES(NU) + (((l) - NU / 2) & 3) * 4096>(at.B, st.vb[((l) - NU / 2) & 3], sb); \
+    } while (0)
+// fragments of the stage behind `cur`
+#define HP_STAGE_ADDR()                                                                                 \
+    do {                                                                                                \
+        const unsigned char *sn = smem + (cur + 1 == ST ? 0 : cur + 1) * HP_STAGE_BYTES(NU);            \
+        ra = sn + fr.a0;                                                                                \
+        ra1 = sn + fr.a1;                                                                               \
+        rb0 = sn + fr.b0;                                                                               \
+        rb1 = sn + fr.b1;                                                                               \
     } while (0)
 #define HP_MFMA(PA, PB, iu, c)                                                                                                    \
     do {                                                                                                                             \
@@ -193,15 +311,13 @@ struct hp_state {
 #define HP_GROUP(PA, PB, QA, QB, g)                     \
     do {                                                   \
         HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1));       \
-        if ((g) < 8) {                                     \
-            HP_READ(QA, QB, 2 * (g));                      \
-            HP_READ(QA, QB, 2 * (g) + 1);                  \
-        }                                                  \
+        if ((g) < 8) HP_READ(QA, QB, 2 * (g));             \
         __builtin_amdgcn_sched_barrier(0);                 \
         HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 1);   \
         if ((g) & 1) HP_LOAD((g) >> 1, sb);                \
         __builtin_amdgcn_sched_barrier(0);                 \
         HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 2);   \
+        if ((g) < 8) HP_READ(QA, QB, 2 * (g) + 1);         \
         __builtin_amdgcn_sched_barrier(0);                 \
         HP_MFMA(PA, PB, (g) >> 1, 4 * ((g) & 1) + 3);   \
         __builtin_amdgcn_sched_barrier(0);                 \
@@ -221,16 +337,10 @@ struct hp_state {
         HP_MFMA(PA, PB, 7, 6);                                                                           \
         cur = cur + 1 == ST ? 0 : cur + 1;                                                                \
         sb = lds_wave + cur * HP_STAGE_BYTES(NU);                                                           \
-        lA += 8192;                                                                                         \
-        lB += stepB;                                                                                        \
+        hp_advance<EPI>(p, at, st.vb, wave, lane0);                                                         \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
         HP_MFMA(PA, PB, 7, 7);                                                                           \
-        {                                                                                                   \
-            const unsigned char *sn = smem + (cur + 1 == ST ? 0 : cur + 1) * HP_STAGE_BYTES(NU);            \
-            ra = sn + pa;                                                                                   \
-            rb0 = sn + pb0;                                                                                 \
-            rb1 = sn + pb1;                                                                                 \
-        }                                                                                                   \
+        HP_STAGE_ADDR();                                                                                    \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * HP_LOADS(NU)) : "memory");           \
         __syncthreads();                                                                                    \
@@ -321,11 +431,11 @@ template <int NU, int NSEG, bool WHOLE>
 __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it, const f32x4_t (&acc)[NU][8], int wm, int wn, int l16, int lq)
 {
     const int col0 = it.n0 + wn * 128 + 4 * lq;
-    // (rows behind the last token are written with what the last one's statistics give: nothing reads them)
+    // (rows behind the last token, whose image rows are zeros, are written as zeros: they are k places of dW)
     const int KTp = p.nt * (HP_TILE / HP_BK);
     constexpr int NP = NSEG > 1 ? 3 : 1;
     // (to the image's end: rows of the tile behind it fall away)
-    const int rgs = ((p.M + 127) >> 7) - (it.row0 >> 7), kb = (it.n0 >> 5) + 4 * wn;
+    const int rgs = min(((p.rowsA + 127) >> 7) - (it.row0 >> 7), 3), kb = (it.n0 >> 5) + 4 * wn;
     __amdgpu_buffer_rsrc_t rs[NP];
 #pragma unroll
     for (int q = 0; q < NP; ++q)
@@ -344,7 +454,7 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
     for (int iu = 0; iu < NU; ++iu) {
         __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
         const int row = it.row0 + 16 * (2 * iu + wm) + l16;
-        const bool held = y[iu] >= 0 && y[iu] < p.V;
+        const bool held = row < p.M && y[iu] >= 0 && y[iu] < p.V;
         // (rows without a target: their logits here are zeros, the images' rows are; what their statistics say does not matter)
         const float fu = held ? 1.0f / f[iu] : 0.0f, mu = held ? m[iu] : 0.0f;
         const int k = y[iu] - p.v0 - col0;
@@ -397,23 +507,15 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     const int wm = wave >> 1, wn = wave & 1;
     int lane = hp_fresh(lane0), l16 = lane & 15, lq = lane >> 4;
     const int kt = __builtin_amdgcn_readfirstlane(it.kt);
-    const size_t stepB = p.b_ld == 0 ? 8192 : 64;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     const uint32_t lds_wave = lds0 + wave * 1024;
-    const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
-    const uint32_t pb0 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16)) << 4);
-    const uint32_t pb1 = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | 16)) << 4);
+    const hp_frag fr = hp_frag_of<NU, EPI>(wm, wn, lane);
     int cur = __builtin_amdgcn_readfirstlane(st.cur);
-    const unsigned char *lA = hp_uniform(st.lA), *lB = hp_uniform(st.lB);
-    nxt = hp_make_item(p, next_idx);
+    hp_at at = {hp_uniform(st.at.A), hp_uniform(st.at.B), __builtin_amdgcn_readfirstlane(st.at.phase), __builtin_amdgcn_readfirstlane(st.at.rows)};
+    nxt = hp_make_item<EPI>(p, next_idx);
     uint32_t sb = lds_wave + cur * HP_STAGE_BYTES(NU);
-    const unsigned char *ra, *rb0, *rb1;
-    {
-        const unsigned char *sn = smem + (cur + 1 == ST ? 0 : cur + 1) * HP_STAGE_BYTES(NU);
-        ra = sn + pa;
-        rb0 = sn + pb0;
-        rb1 = sn + pb1;
-    }
+    const unsigned char *ra, *ra1, *rb0, *rb1;
+    HP_STAGE_ADDR();
     f32x4_t acc[NU][8];
     const f32x4_t zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
     // The steps of a pair of parts two at a time (their number is even, at least 8).  The loads of the last ST are the next pair's or the
@@ -442,9 +544,8 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             const int ns = seg + 1 < NSEG ? seg + 1 : 0;
             const hp_item &li = ns == 0 ? nxt : it;  // the item of the loads from here on
             const size_t a0 = NSEG > 1 ? (size_t)((HP_SEG_A >> (4 * ns)) & 3) * p.planeA : 0, b0 = NSEG > 1 ? (size_t)((HP_SEG_B >> (4 * ns)) & 3) * p.planeB : 0;
-            lA = hp_uniform(li.A + a0);
-            lB = hp_uniform(li.B + b0);
-            hp_lane_offsets(p, li, wave, hp_fresh(lane0), st.va, st.vb);
+            at = {hp_uniform(li.A + a0), hp_uniform(li.B + b0), li.phase, li.rows};
+            hp_lane_offsets<EPI>(p, li, wave, hp_fresh(lane0), st.va, st.vb);
         }
         if (ST & 1) HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         for (k = 0; k < ST / 2; ++k) {
@@ -454,8 +555,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     }
     HP_PIN();
     st.cur = cur;
-    st.lA = lA;
-    st.lB = lB;
+    st.at = at;
 
     lane = hp_fresh(lane0);
     l16 = lane & 15;
@@ -539,39 +639,36 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 1, wn = wave & 1, l16 = lane & 15, lq = lane >> 4;
     const int n_wg = gridDim.x;
-    const int at = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const int at_wg = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
     const int total = p.mt * p.nt * p.slices;
-    int idx = at;
+    int idx = at_wg;
     if (idx >= total) return;
-    hp_item it = hp_make_item(p, idx);
+    hp_item it = hp_make_item<EPI>(p, idx);
     hp_state st;
-    const unsigned char *lA = hp_uniform(it.A + (NSEG > 1 ? (size_t)(HP_SEG_A & 3) * p.planeA : 0));
-    const unsigned char *lB = hp_uniform(it.B + (NSEG > 1 ? (size_t)(HP_SEG_B & 3) * p.planeB : 0));
-    hp_lane_offsets(p, it, wave, lane, st.va, st.vb);
-    const size_t stepB = p.b_ld == 0 ? 8192 : 64;
+    hp_at at = {hp_uniform(it.A + (NSEG > 1 ? (size_t)(HP_SEG_A & 3) * p.planeA : 0)), hp_uniform(it.B + (NSEG > 1 ? (size_t)(HP_SEG_B & 3) * p.planeB : 0)),
+                it.phase, it.rows};
+    hp_lane_offsets<EPI>(p, it, wave, lane, st.va, st.vb);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     constexpr int ST = HP_STAGES(NU);
     for (int i = 0; i < ST; ++i) {  // the first item's first steps (of 8 or more of its first part)
         const uint32_t sb = lds0 + wave * 1024 + i * HP_STAGE_BYTES(NU);
         HP_LOAD(0, sb); HP_LOAD(1, sb); HP_LOAD(2, sb); HP_LOAD(3, sb);
         HP_LOAD(4, sb); HP_LOAD(5, sb); HP_LOAD(6, sb); HP_LOAD(7, sb);
-        lA += 8192;
-        lB += stepB;
+        hp_advance<EPI>(p, at, st.vb, wave, lane);
     }
-    st.lA = lA;
-    st.lB = lB;
+    st.at = at;
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * HP_LOADS(NU)) : "memory");
     __syncthreads();
     {
-        const uint32_t pa = (uint32_t)(wm * 16 + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | (wm << 4))) << 4);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const uint32_t pb = HP_A_BYTES(NU) + (uint32_t)(wn * 128 + 16 * (r & 1) + l16) * 64 + ((uint32_t)(lq ^ pk_swz(l16 | ((r & 1) << 4))) << 4);
-            st.fb0[r] = *(const bf16x8_t *)(smem + pb + (r >> 1) * 2048u);
-            if (r < NU) st.fa0[r] = *(const bf16x8_t *)(smem + pa + r * 2048u);
-        }
+        const hp_frag fr = hp_frag_of<NU, EPI>(wave >> 1, wave & 1, lane);
+        const int cur = ST - 1;  // (stage 0 is the one behind it)
+        const unsigned char *ra, *ra1, *rb0, *rb1;
+        HP_STAGE_ADDR();
+        HP_READ(st.fa0, st.fb0, 0); HP_READ(st.fa0, st.fb0, 1); HP_READ(st.fa0, st.fb0, 2); HP_READ(st.fa0, st.fb0, 3);
+        HP_READ(st.fa0, st.fb0, 4); HP_READ(st.fa0, st.fb0, 5); HP_READ(st.fa0, st.fb0, 6); HP_READ(st.fa0, st.fb0, 7);
+        HP_READ(st.fa0, st.fb0, 8); HP_READ(st.fa0, st.fb0, 9); HP_READ(st.fa0, st.fb0, 10); HP_READ(st.fa0, st.fb0, 11);
+        HP_READ(st.fa0, st.fb0, 12); HP_READ(st.fa0, st.fb0, 13); HP_READ(st.fa0, st.fb0, 14); HP_READ(st.fa0, st.fb0, 15);
     }
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * HP_LOADS(NU)) : "memory");  // step 1 has landed; every wave has taken step 0 out of its stage
     __syncthreads();
@@ -588,14 +685,13 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
 }
 
 // ---- tile images ----
-// Rows 64 bx .., columns 64 by .. of a row-major matrix [R,K] as parts of a tile image (`img`, KTi k steps a row group) and of the image
-// of its transpose (`tr`, KTt k steps); zero outside the matrix and in rows whose token has no target.
+// Rows 64 bx .., columns 64 by .. of a row-major matrix [R,K] as parts of a tile image (KTi k steps a row group); zero outside the matrix and
+// in rows whose token has no target.
 template <bool BF>
 __global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict__ src, int R, int K, int vec, const int32_t *__restrict__ targets, int V,
-                                                          unsigned char *__restrict__ img, int KTi, size_t plane_i, unsigned char *__restrict__ tr, int KTt, size_t plane_t)
+                                                          unsigned char *__restrict__ img, int KTi, size_t plane_i)
 {
     constexpr int NP = BF ? 1 : 3;
-    __shared__ __attribute__((aligned(16))) uint16_t tile[NP][64][64];
     const int tid = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -638,55 +734,15 @@ __global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict
             }
         }
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            if (img) *(uint4 *)(img + q * plane_i + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = *(const uint4 *)&e[q][0];
-            if (tr) *(uint4 *)&tile[q][rr][(ch ^ (2 * (rr >> 3) & 6)) * 8] = *(const uint4 *)&e[q][0];
-        }
-    }
-    if (!tr) return;
-    __syncthreads();
-    // (column chunks swapped by row group: the chunks that a wave reads for one destination row sit in different banks)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int blk = (tid >> 6) + 4 * u, l = tid & 63;
-        const int cc = (blk & 3) * 16 + (l >> 2), kc = (blk >> 2) * 4 + (l & 3);  // destination row c0 + cc, k places 8 kc .. of the 64
-        const int col = ((cc >> 3) ^ (2 * kc & 6)) * 8 + (cc & 7);
-#pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            uint32_t v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = tile[q][kc * 8 + 2 * k][col] | (uint32_t)tile[q][kc * 8 + 2 * k + 1][col] << 16;
-            *(uint4 *)(tr + q * plane_t + pk_chunk_off(c0 + cc, (r0 >> 5) + (kc >> 2), kc & 3, KTt)) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
+        for (int q = 0; q < NP; ++q) *(uint4 *)(img + q * plane_i + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = *(const uint4 *)&e[q][0];
     }
 }
 
-// Transposes a tile image: rows 64 bx .., columns 64 by .. of `src` (KTs k steps; rows from R on count as zero), part blockIdx.z
-__global__ __launch_bounds__(256) void head_transpose_kernel(const unsigned char *__restrict__ src, int R, int KTs, size_t plane_s, unsigned char *__restrict__ dst,
-                                                             int KTd, size_t plane_d)
+// Zeros in blocks of 16 rows b0 .. b1 of an image of KT = gridDim.x k steps, part blockIdx.y
+__global__ __launch_bounds__(64) void head_zero_blocks_kernel(unsigned char *__restrict__ img, size_t plane, int b0, int b1)
 {
-    __shared__ __attribute__((aligned(16))) uint16_t tile[64][64];
-    const int tid = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-    src += blockIdx.z * plane_s;
-    dst += blockIdx.z * plane_d;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int idx = tid + u * 256, rr = idx >> 3, ch = idx & 7, c = c0 + ch * 8;
-        uint4 v = {0u, 0u, 0u, 0u};
-        if (r0 + rr < R) v = *(const uint4 *)(src + pk_chunk_off(r0 + rr, c >> 5, (c & 31) >> 3, KTs));
-        *(uint4 *)&tile[rr][(ch ^ (2 * (rr >> 3) & 6)) * 8] = v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int blk = (tid >> 6) + 4 * u, l = tid & 63;
-        const int cc = (blk & 3) * 16 + (l >> 2), kc = (blk >> 2) * 4 + (l & 3);
-        const int col = ((cc >> 3) ^ (2 * kc & 6)) * 8 + (cc & 7);
-        uint32_t v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = tile[kc * 8 + 2 * k][col] | (uint32_t)tile[kc * 8 + 2 * k + 1][col] << 16;
-        *(uint4 *)(dst + pk_chunk_off(c0 + cc, (r0 >> 5) + (kc >> 2), kc & 3, KTd)) = make_uint4(v[0], v[1], v[2], v[3]);
-    }
+    for (int b = b0; b < b1; ++b)
+        *(uint4 *)(img + blockIdx.y * plane + ((((size_t)(b >> 3) * gridDim.x + blockIdx.x) * 8 + (b & 7)) << 10) + threadIdx.x * 16) = make_uint4(0, 0, 0, 0);
 }
 
 // ---- a few tokens: W streams through registers ----
@@ -1012,8 +1068,8 @@ struct head_plan {
     int nb;                             // column blocks of the forward pass
     int slices;                         // k slices of dx
     bool direct, few;
-    size_t x_img, xT_img, w_img, wT_img, p_img, pT_img, slabs, part, tlogit, bytes;
-    size_t x_plane, xT_plane, w_plane, wT_plane, p_plane, pT_plane, slab;
+    size_t x_img, w_img, p_img, slabs, part, tlogit, bytes;
+    size_t x_plane, w_plane, p_plane, slab;
 };
 
 static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool backward)
@@ -1039,7 +1095,7 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
         return h;
     }
     // what a column of the vocabulary needs while its piece is worked on
-    const size_t per = backward ? (size_t)h.planes * 2 * (2 * (size_t)h.Tp + 2 * (size_t)h.dp) : h.direct ? 0 : (size_t)h.planes * 2 * h.dp;
+    const size_t per = (size_t)h.planes * 2 * ((backward ? h.Tp : 0) + (h.direct ? 0 : h.dp));
     const size_t budget = (size_t)1 << 30;
     const int all = (int)up_to(a.V, 256);
     h.piece = per == 0 ? all : (int)std::min<size_t>(all, std::max<size_t>(256, budget / per / 256 * 256));
@@ -1052,15 +1108,8 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
         h.w_img = take(h.w_plane * h.planes);
     }
     if (backward) {
-        const size_t dr = up_to(h.dp, 256);
-        h.xT_plane = dr * h.Tp * 2;
-        h.xT_img = take(h.xT_plane * h.planes);
-        h.wT_plane = dr * h.piece * 2;
-        h.wT_img = take(h.wT_plane * h.planes);
-        h.p_plane = up_to(a.T, 128) * (size_t)h.piece * 2;
+        h.p_plane = up_to(h.Tp, 128) * (size_t)h.piece * 2;
         h.p_img = take(h.p_plane * h.planes);
-        h.pT_plane = (size_t)h.piece * h.Tp * 2;
-        h.pT_img = take(h.pT_plane * h.planes);
         // few tiles of dx: the vocabulary is shared out to k slices, a slab of sums each
         const int tiles = ceil_div(a.T, 256) * ceil_div(a.d, 256);
         h.slices = tiles < ctx->num_cus ? std::max(1, std::min(ctx->num_cus / std::max(tiles, 1), h.piece / 32 / 16)) : 1;
@@ -1139,15 +1188,17 @@ static hipError_t head_product(const omega_ctx *ctx, head_prod p, int planes, hi
     } while (0)
 
 // Images of rows [R,K] at src: rows up to Rp (a multiple of 64), columns up to Kp
-static void head_images(const head_args &a, const void *src, int R, int K, int Rp, int Kp, const int32_t *targets, unsigned char *img, size_t plane_i,
-                        unsigned char *tr, int KTt, size_t plane_t, hipStream_t s)
+static void head_images(const head_args &a, const void *src, int R, int K, int Rp, int Kp, const int32_t *targets, unsigned char *img, size_t plane, hipStream_t s)
 {
     const bool bf = a.dtype == OMEGA_DTYPE_BF16;
     const int vec = K % 8 == 0 && (uintptr_t)src % 16 == 0;
     const dim3 grid(Rp / 64, Kp / 64);
-    if (bf) hipLaunchKernelGGL(head_images_kernel<true>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane_i, tr, KTt, plane_t);
-    else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane_i, tr, KTt, plane_t);
+    if (bf) hipLaunchKernelGGL(head_images_kernel<true>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane);
+    else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane);
 }
+
+// k steps of dx over `vc` rows of W (P has zeros up to a multiple of 256)
+static int head_dx_steps(int vc) { return std::max(8, (int)up_to(ceil_div(vc, 32), 2)); }
 
 static void head_zero(void *p, size_t bytes, hipStream_t s)
 {
@@ -1198,19 +1249,19 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
 #undef HEAD_FEW_K
 #undef HEAD_STREAM_K
     } else {
-        head_images(a, a.x, a.T, a.d, (int)up_to(a.T, 64), h.dp, a.targets, base + h.x_img, h.x_plane, nullptr, 0, 0, s);
+        head_images(a, a.x, a.T, a.d, (int)up_to(a.T, 64), h.dp, a.targets, base + h.x_img, h.x_plane, s);
         for (int v0 = 0; v0 < a.V; v0 += h.piece) {
             const int vc = std::min(h.piece, a.V - v0);
             const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
-            if (!h.direct) head_images(a, w, vc, a.d, (int)up_to(vc, 64), h.dp, nullptr, base + h.w_img, h.w_plane, nullptr, 0, 0, s);
+            if (!h.direct) head_images(a, w, vc, a.d, (int)up_to(vc, 64), h.dp, nullptr, base + h.w_img, h.w_plane, s);
             head_prod p = {};
             p.A = base + h.x_img;
             p.planeA = h.x_plane;
             p.B = h.direct ? w : base + h.w_img;
             p.planeB = h.w_plane;
             p.b_ld = h.direct ? (size_t)a.d * 2 : 0;
-            p.kt = h.dp / 32;
-            p.M = a.T;
+            p.kt = p.ktA = p.ktB = h.dp / 32;
+            p.M = p.rowsA = a.T;
             p.N = vc;
             p.slices = 1;
             p.targets = a.targets;
@@ -1239,20 +1290,22 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     }
     const head_plan h = head_plan_of(ctx, a, true);
     unsigned char *base = (unsigned char *)ws;
-    head_images(a, a.x, a.T, a.d, h.Tp, h.dp, a.targets, base + h.x_img, h.x_plane, a.dw ? base + h.xT_img : nullptr, h.Tp / 32, h.xT_plane, s);
+    head_images(a, a.x, a.T, a.d, h.Tp, h.dp, a.targets, base + h.x_img, h.x_plane, s);
     for (int v0 = 0; v0 < a.V; v0 += h.piece) {
-        const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256);
+        const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256), Tr = (int)up_to(a.T, 64);
         const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
-        if (!h.direct || a.dx)
-            head_images(a, w, vc, a.d, vp, h.dp, nullptr, h.direct ? nullptr : base + h.w_img, h.w_plane, a.dx ? base + h.wT_img : nullptr, vp / 32, h.wT_plane, s);
+        if (!h.direct) head_images(a, w, vc, a.d, vp, h.dp, nullptr, base + h.w_img, h.w_plane, s);
+        if (a.dw && Tr < h.Tp)  // (k places of dW that no tile of P reaches)
+            hipLaunchKernelGGL(head_zero_blocks_kernel, dim3(vp / 32, h.planes), dim3(64), 0, s, base + h.p_img, h.p_plane, Tr / 16, h.Tp / 16);
         head_prod p = {};
         p.A = base + h.x_img;
         p.planeA = h.x_plane;
         p.B = h.direct ? w : base + h.w_img;
         p.planeB = h.w_plane;
         p.b_ld = h.direct ? (size_t)a.d * 2 : 0;
-        p.kt = h.dp / 32;
+        p.kt = p.ktA = p.ktB = h.dp / 32;
         p.M = a.T;
+        p.rowsA = h.Tp;
         p.N = vc;
         p.slices = 1;
         p.targets = a.targets;
@@ -1267,11 +1320,15 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             head_prod q = {};
             q.A = base + h.p_img;
             q.planeA = h.p_plane;
-            q.B = base + h.wT_img;
-            q.planeB = h.wT_plane;
-            q.kt = vp / 32;
-            q.M = a.T;
+            q.B = p.B;
+            q.planeB = h.w_plane;
+            q.b_ld = p.b_ld;
+            q.kt = head_dx_steps(vc);
+            q.ktA = vp / 32;
+            q.ktB = h.dp / 32;
+            q.M = q.rowsA = a.T;
             q.N = a.d;
+            q.rowsB = vc;
             q.slices = std::max(1, std::min(h.slices, q.kt / 8));
             q.C = (float *)(base + h.slabs);
             q.slab = h.slab;
@@ -1280,14 +1337,14 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             else HEAD_TRY(head_product<HEAD_ADD>(ctx, q, h.planes, s));
         }
         if (a.dw) {
-            hipLaunchKernelGGL(head_transpose_kernel, dim3(h.Tp / 64, vp / 64, h.planes), dim3(256), 0, s, base + h.p_img, a.T, vp / 32, h.p_plane, base + h.pT_img, h.Tp / 32,
-                               h.pT_plane);
             head_prod q = {};
-            q.A = base + h.pT_img;
-            q.planeA = h.pT_plane;
-            q.B = base + h.xT_img;
-            q.planeB = h.xT_plane;
+            q.A = base + h.p_img;
+            q.planeA = h.p_plane;
+            q.B = base + h.x_img;
+            q.planeB = h.x_plane;
             q.kt = h.Tp / 32;
+            q.ktA = vp / 32;
+            q.ktB = h.dp / 32;
             q.M = vc;
             q.N = a.d;
             q.slices = 1;
@@ -1300,7 +1357,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
         }
     }
     if (a.dx) {
-        const int vp0 = (int)up_to(std::min(h.piece, a.V), 256), slices = std::max(1, std::min(h.slices, vp0 / 32 / 8));
+        const int slices = std::max(1, std::min(h.slices, head_dx_steps(std::min(h.piece, a.V)) / 8));
         const dim3 grid(a.T, std::min(ceil_div(a.d, 256), 1024));
         if (bf) hipLaunchKernelGGL(head_dx_kernel<true>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);
         else hipLaunchKernelGGL(head_dx_kernel<false>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);

@@ -57,7 +57,7 @@ def run(x, w, y, dtype, shift=0, dloss=None, stats=True):
     if stats:
         db = None if dloss is None else Buf((1,), "f32", [dloss])
         c.check(lib.omega_hip_head_loss_backward(c.handle, p["x"], p["w"], DT[dtype], T, V, d, p["y"], p["stats"], p["mean"], db.ptr if db else None, p["dx"], p["dw"]))
-        names += ["dx", "dw"]
+        names += ["dx", "dw", "stats"]
     got = {k: b[k].get() for k in names}
     for v in b.values():
         v.free()
@@ -93,7 +93,7 @@ def test_against_the_formulas(T, V, d, dtype):
         assert np.array_equal(served["loss"], got["loss"]) and np.array_equal(served["mean"], got["mean"])
 
 
-@pytest.mark.parametrize("dtype,V", [("f32", 200001), ("bf16", 600001)])
+@pytest.mark.parametrize("dtype,V", [("f32", 200001), ("bf16", 600001), ("f32", 400001), ("bf16", 1100001)])
 def test_several_pieces_of_the_vocabulary(dtype, V):
     T, d = 20, 24
     rng = np.random.default_rng(V)
@@ -101,6 +101,36 @@ def test_several_pieces_of_the_vocabulary(dtype, V):
     y[:3] = 0, V - 1, V // 2
     x = normal(rng, T, d, dtype=dtype)
     check(run(x, w, y, dtype), reference(x, w, y, dtype))
+
+
+def test_pieces_of_weights_in_place():
+    """More tokens x vocabulary than a piece holds, bf16 rows that are read where they are, a last piece that ends inside a step of 32 rows.
+    Some tokens and some rows of W against the formulas of reference(); of the rows' gradients the statistics are the call's own."""
+    T, V, d = 2100, 300017, 256
+    rng = np.random.default_rng(1)
+    w, x, y = normal(rng, V, d, std=d ** -0.5, dtype="bf16"), normal(rng, T, d, dtype="bf16"), targets_of(rng, T, V)
+    y[:3] = 0, V - 1, -1
+    got = run(x, w, y, "bf16")
+    held = (y >= 0) & (y < V)
+    n, w = int(held.sum()), w.astype(np.float64)
+    assert got["mean"][1] == n and np.isfinite(got["dw"]).all() and np.isfinite(got["dx"]).all()
+    toks = np.r_[:16, rng.integers(0, T, 16), T - 1]
+    part = reference(x[toks], w, y[toks], "bf16", dloss=float(held[toks].sum()) / n)
+    within(got["loss"][toks], *part["loss"], "loss")
+    within(got["dx"][toks], *part["dx"], "dx")
+    cols = np.r_[:4, V - 40:V, rng.integers(0, V, 60), y[held][:20]]
+    x = np.where(held[:, None], x, 0).astype(np.float64)
+    l, mag = x @ w[cols].T, np.abs(x) @ np.abs(w[cols]).T
+    m, s = (v[:, None].astype(np.float64) for v in got["stats"])
+    # (a maximum of 32 bits shifts every exp of its row, and the sum with them: only how far this column's logit is off counts)
+    e = 2 * (d / 32 + 32) * U32 * mag + 400 * U32 + 4 * U32 * np.abs(l - m)
+    P = np.where(held[:, None], np.exp(l - m) / s, 0.0)
+    eP = P * e
+    P -= held[:, None] & (y[:, None] == cols)
+    eP = (eP + (4 * U32 + U16) * np.abs(P) + 3 * 2.0 ** -126) * held[:, None] / n
+    P /= n
+    dw = P.T @ x
+    within(got["dw"][cols], dw, eP.T @ np.abs(x) + 2 * (T / 32 + 48) * U32 * (np.abs(P).T @ np.abs(x)) + U16 * np.abs(dw) * 1.01, "dw")
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
