@@ -334,7 +334,8 @@ int omega_hip_layernorm_backward(omega_ctx *ctx, const void *x, const void *dout
  * in pieces of the vocabulary: the [T,V] logits are never kept.
  *   loss[t] = log(sum_v exp(logit[t,v])) - logit[t,targets[t]], 0 for a token whose target is outside 0..V-1 (padding);
  *   mean[0] = sum of loss / n, mean[1] = n = tokens with a target (n = 0: mean[0] = 0);
- *   row_stats [2,T] = maximum of a row's logits, then the sum of exp(logit - maximum): what the backward pass needs.
+ *   row_stats [2,T] = maximum of a row's logits, then the sum of exp(logit - maximum): what the backward pass needs (of a token
+ *   without a target: not to be relied on).
  * loss and mean are required, row_stats may be NULL where no backward pass follows.  All fp32.  Products of bf16 operands are
  * summed in fp32; products of fp32 operands are formed from three bf16 parts of each factor (24 bits).
  * FullyLayer.output + the softmax and log of J/engine/gpu/SoftmaxKernel.cu:4-24. */
@@ -342,7 +343,7 @@ int omega_hip_head_loss_forward(omega_ctx *ctx, const void *x, const void *w, in
                                 const int32_t *targets, float *loss, float *row_stats, float *mean);
 /* Gradients of dloss * mean[0] (dloss: one float on the device, NULL = 1), with the same x, w and targets and what the forward
  * call returned: dx [T,d] and dw [V,d], of dtype, overwritten; either may be NULL (not computed).  Tokens without a target have
- * zero rows in dx and no part in dw, whatever their rows of x hold.  The logits are computed again; in bf16 the gradient of the
+ * zero rows in dx and no part in dw, whatever their rows of x hold, and cost no products.  The logits are computed again; in bf16 the gradient of the
  * logits is rounded to bf16 before its two products, whose sums are fp32, and dx and dw are rounded once. */
 int omega_hip_head_loss_backward(omega_ctx *ctx, const void *x, const void *w, int dtype, int T, int V, int d,
                                  const int32_t *targets, const float *row_stats, const float *mean, const float *dloss, void *dx,

@@ -6,10 +6,12 @@
 // (m_t, s_t: a row's maximum and sum.  The pair is kept instead of m + log s, whose rounding would stand in every exp.  g multiplies the
 // products' fp32 sums: within P, whose elements are rounded to bf16, the rounding of a row's -g would be the same for all rows.)
 //
-// All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], bf16 on v_mfma_f32_16x16x32_bf16 with fp32 sums.  A tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory
-// to LDS in a ring of five or more steps of 32 k; persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that
-// head_images_kernel or the product before writes, zero where k goes beyond the matrix; W itself is read in place where its rows are whole
-// and aligned.  Where the product sums over an operand's rows (W for dx, P and x for dW), the LDS reads transpose.
+// All products are one kernel (head_product_kernel): C[m,n] = sum_k A[m,k] B[n,k], bf16 on v_mfma_f32_16x16x32_bf16 with fp32 sums.  A
+// tile is 256 x 256, four waves of 128 x 128, one per SIMD; operands stream from memory to LDS in a ring of five or more steps of 32 k;
+// persistent, the ring runs on from tile to tile.  Operands are tile images (pack.h) that head_tokens_kernel, head_images_kernel or the
+// product before writes, zero where k goes beyond the matrix; W itself is read in place where its rows are whole and aligned.  Where the
+// product sums over an operand's rows (W for dx, P and x for dW), the LDS reads transpose.  Tokens without a target are in no image: the
+// products' rows are the others, whose number is read on the device.
 // fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
 // six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first); what is left out is below 2^-24 of a term.
 // Forward passes of up to 64 tokens (fp32: 128) stream W through a wave's LDS or registers (head_stream_kernel, head_few_kernel).
@@ -53,10 +55,11 @@ struct head_prod {
     int rowsB;                       // B read across its rows in place: the rows there are
     int M, N, mt, nt, slices;        // mt row tiles of `th` rows (64, 128, 192 or 256), nt column tiles of 256
     int th;
+    const int32_t *held;             // tokens with a target: M, and mt from it; of dW kt
     // epilogues
-    const int32_t *targets;
+    const int32_t *targets;          // of the tokens that have one, as their statistics
     const float *row_stats, *mean, *dloss;
-    int T, V, v0;                    // tokens, vocabulary, first column of the piece
+    int T, v0;                       // all tokens, first column of the piece
     float2 *part;                    // LSE
     float *tlogit;
     unsigned char *P;                // P
@@ -68,9 +71,9 @@ struct head_prod {
     int out_bf, out_vec;
 };
 
-// Operands that are read across their rows (the rows are k): W for dx, both for dW.  Their steps are 32 rows x 256 columns, in LDS the same blocks
-// of 16 rows x 32 columns as those of an image, two for each 32 columns; ds_read_b64_tr_b16 hands each lane 4 rows of its column.  The
-// reads are twice as many, each half as long, without bank conflicts.  Against images of the transposes, made by kernels of their own:
+// Operands that are read across their rows (the rows are k): W for dx, both for dW.  Their steps are 32 rows x 256 columns, in LDS the same
+// blocks of 16 rows x 32 columns as those of an image, two for each 32 columns; ds_read_b64_tr_b16 hands each lane 4 rows of its column.
+// The reads are twice as many, each half as long, without bank conflicts.  Against images of the transposes, made by kernels of their own:
 // gradients of 4096 tokens, vocabulary 128000, d 4096: 9.62 -> 9.09 ms (the products 740 to 790 us each per 32000 rows of W either way);
 // 512 x 4096, 32000: 587 -> 446 us; 131 x 2072, 51750: 417 -> 361.
 #define HP_TR_A(EPI) ((EPI) == HEAD_OUT)
@@ -454,8 +457,7 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
     for (int iu = 0; iu < NU; ++iu) {
         __builtin_amdgcn_sched_barrier(0);  // (a unit at a time: the registers are full)
         const int row = it.row0 + 16 * (2 * iu + wm) + l16;
-        const bool held = row < p.M && y[iu] >= 0 && y[iu] < p.V;
-        // (rows without a target: their logits here are zeros, the images' rows are; what their statistics say does not matter)
+        const bool held = row < p.M;
         const float fu = held ? 1.0f / f[iu] : 0.0f, mu = held ? m[iu] : 0.0f;
         const int k = y[iu] - p.v0 - col0;
         float v[32];
@@ -641,6 +643,22 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n_wg = gridDim.x;
     const int at_wg = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const int tokens = __builtin_amdgcn_readfirstlane(p.held[0]);
+    if (EPI == HEAD_OUT) {
+        p.kt = max(8, ((tokens + 63) >> 6) * 2);
+    } else {
+        p.M = tokens;
+        p.mt = (tokens + 32 * NU - 1) / (32 * NU);
+    }
+    if (EPI == HEAD_P && tokens <= 192) {  // (dW has eight steps at least: rows of P that no tile reaches)
+        const int KTp = p.nt * (HP_TILE / HP_BK), b0 = (tokens + 63) >> 6 << 2, per = 16 - b0;
+        for (int i = blockIdx.x * 4 + wave; i < KTp * per; i += gridDim.x * 4)
+#pragma unroll
+            for (int q = 0; q < (NSEG > 1 ? 3 : 1); ++q) {
+                const int kb = i / per, b = b0 + i - kb * per;
+                *(uint4 *)(p.P + q * p.planeP + ((((size_t)(b >> 3) * KTp + kb) * 8 + (b & 7)) << 10) + lane * 16) = make_uint4(0, 0, 0, 0);
+            }
+    }
     const int total = p.mt * p.nt * p.slices;
     int idx = at_wg;
     if (idx >= total) return;
@@ -685,64 +703,121 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
 }
 
 // ---- tile images ----
-// Rows 64 bx .., columns 64 by .. of a row-major matrix [R,K] as parts of a tile image (KTi k steps a row group); zero outside the matrix and
-// in rows whose token has no target.
+// Parts of 8 columns from c on of row `row` of a row-major matrix of K columns, zero from K on
 template <bool BF>
-__global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict__ src, int R, int K, int vec, const int32_t *__restrict__ targets, int V,
-                                                          unsigned char *__restrict__ img, int KTi, size_t plane_i)
+__device__ __forceinline__ void head_chunk(const void *__restrict__ src, size_t row, int K, int c, int vec, uint4 (&part)[BF ? 1 : 3])
+{
+    constexpr int NP = BF ? 1 : 3;
+    uint16_t e[NP][8];
+    const size_t at = row * K + c;
+    if (BF) {
+        const bf16_t *s = (const bf16_t *)src + at;
+        if (vec) {
+            *(uint4 *)&e[0][0] = *(const uint4 *)s;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[0][k] = c + k < K ? s[k] : (bf16_t)0;
+        }
+    } else {
+        const float *s = (const float *)src + at;
+        float v[8];
+        if (vec) {
+            *(float4 *)&v[0] = *(const float4 *)s;
+            *(float4 *)&v[4] = *(const float4 *)(s + 4);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = c + k < K ? s[k] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint32_t h[3];
+            hp_split(v[k], h);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) e[q][k] = (uint16_t)h[q];
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) part[q] = *(const uint4 *)&e[q][0];
+}
+
+// Rows 64 bx .., columns 64 by .. of W [R,K] as parts of a tile image (KTi k steps a row group), zero outside the matrix
+template <bool BF>
+__global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict__ src, int R, int K, int vec, unsigned char *__restrict__ img, int KTi, size_t plane)
 {
     constexpr int NP = BF ? 1 : 3;
     const int tid = threadIdx.x, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int idx = tid + u * 256, rr = idx >> 3, ch = idx & 7, row = r0 + rr, c = c0 + ch * 8;
-        uint16_t e[NP][8];
+        const int idx = tid + u * 256, row = r0 + (idx >> 3), c = c0 + (idx & 7) * 8;
+        uint4 part[NP] = {};
+        if (row < R && c < K) head_chunk<BF>(src, row, K, c, vec, part);
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[q][k] = 0;
-        bool held = row < R && c < K;
-        if (held && targets) held = targets[row] >= 0 && targets[row] < V;
-        if (held) {
-            const size_t at = (size_t)row * K + c;
-            if (BF) {
-                const bf16_t *s = (const bf16_t *)src + at;
-                if (vec) {
-                    *(uint4 *)&e[0][0] = *(const uint4 *)s;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (c + k < K) e[0][k] = s[k];
-                }
-            } else {
-                const float *s = (const float *)src + at;
-                float v[8];
-                if (vec) {
-                    *(float4 *)&v[0] = *(const float4 *)s;
-                    *(float4 *)&v[4] = *(const float4 *)(s + 4);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = c + k < K ? s[k] : 0.0f;
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    uint32_t h[3];
-                    hp_split(v[k], h);
-#pragma unroll
-                    for (int q = 0; q < NP; ++q) e[q][k] = (uint16_t)h[q];
-                }
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < NP; ++q) *(uint4 *)(img + q * plane_i + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = *(const uint4 *)&e[q][0];
+        for (int q = 0; q < NP; ++q) *(uint4 *)(img + q * plane + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = part[q];
     }
 }
 
-// Zeros in blocks of 16 rows b0 .. b1 of an image of KT = gridDim.x k steps, part blockIdx.y
-__global__ __launch_bounds__(64) void head_zero_blocks_kernel(unsigned char *__restrict__ img, size_t plane, int b0, int b1)
+// The tokens that have a target, moved together in their order: x's image, their targets and (where the backward pass wants them) statistics,
+// slot[t] = a token's place or -1, held[0] = their number n.  The products work on n rows, whatever the others hold; the image's rows from n on are
+// zeros.  A workgroup takes 64 tokens and counts for itself how many of those before have a target: a launch less than a scan of its own
+// (T / 64 workgroups read T targets each, a few us for thousands of tokens).
+template <bool BF>
+__global__ __launch_bounds__(256) void head_tokens_kernel(const void *__restrict__ x, int T, int d, int vec, const int32_t *__restrict__ targets, int V,
+                                                          const float *__restrict__ row_stats, unsigned char *__restrict__ img, int KTi, size_t plane,
+                                                          int32_t *__restrict__ held, int32_t *__restrict__ slot, int32_t *__restrict__ tok_target,
+                                                          float *__restrict__ tok_stats)
 {
-    for (int b = b0; b < b1; ++b)
-        *(uint4 *)(img + blockIdx.y * plane + ((((size_t)(b >> 3) * gridDim.x + blockIdx.x) * 8 + (b & 7)) << 10) + threadIdx.x * 16) = make_uint4(0, 0, 0, 0);
+    constexpr int NP = BF ? 1 : 3;
+    __shared__ int counts[2][4], place[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r0 = blockIdx.x * 64;
+    int before = 0, all = 0;
+#pragma unroll 4
+    for (int t = tid; t < T; t += 256) {
+        const int y = targets[t], h = y >= 0 && y < V;
+        all += h;
+        before += t < r0 ? h : 0;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        all += __shfl_xor(all, o, 64);
+        before += __shfl_xor(before, o, 64);
+    }
+    if (lane == 0) counts[0][wave] = before, counts[1][wave] = all;
+    __syncthreads();
+    before = counts[0][0] + counts[0][1] + counts[0][2] + counts[0][3];
+    const int n = counts[1][0] + counts[1][1] + counts[1][2] + counts[1][3];
+    if (wave == 0) {
+        const int t = r0 + lane, y = t < T ? targets[t] : -1;
+        const bool h = y >= 0 && y < V;
+        const uint64_t mask = __ballot(h);
+        const int at = h ? before + __popcll(mask & ((1ull << lane) - 1)) : -1;
+        place[lane] = at;
+        if (blockIdx.y == 0) {
+            if (t < T) slot[t] = at;
+            if (h) {
+                tok_target[at] = y;
+                if (tok_stats) {
+                    tok_stats[at] = row_stats[t];
+                    tok_stats[T + at] = row_stats[T + t];
+                }
+            }
+            if (t == 0) held[0] = n;
+        }
+    }
+    __syncthreads();
+    for (int c0 = blockIdx.y * 64; c0 < KTi * 32; c0 += gridDim.y * 64) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int idx = tid + u * 256, rr = idx >> 3, row = r0 + rr, c = c0 + (idx & 7) * 8, at = place[rr];
+            uint4 part[NP] = {};
+            if (row >= n)
+#pragma unroll
+                for (int q = 0; q < NP; ++q) *(uint4 *)(img + q * plane + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTi)) = part[q];
+            if (at < 0) continue;
+            if (c < d) head_chunk<BF>(x, row, d, c, vec, part);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) *(uint4 *)(img + q * plane + pk_chunk_off(at, c >> 5, (c & 31) >> 3, KTi)) = part[q];
+        }
+    }
 }
 
 // ---- a few tokens: W streams through registers ----
@@ -995,19 +1070,20 @@ __device__ void head_mean(const float *loss, const int32_t *targets, int T, int 
 // (max, sum) of a token over nb column blocks: TL tokens (a power of two) a workgroup, 1024 / TL threads each, joined in a fixed order.
 // A launch of one workgroup forms the mean too.
 __global__ __launch_bounds__(1024) void head_join_kernel(const float2 *__restrict__ part, int nb, const float *__restrict__ tlogit, const int32_t *__restrict__ targets,
-                                                         int T, int V, int TL, float *__restrict__ loss, float *__restrict__ row_stats, float *__restrict__ mean)
+                                                         const int32_t *__restrict__ slot, int T, int V, int TL, float *__restrict__ loss, float *__restrict__ row_stats, float *__restrict__ mean)
 {
     __shared__ float2 red[1024];
     const int tid = threadIdx.x, sub = tid / TL, n_sub = 1024 / TL, t = blockIdx.x * TL + (tid & (TL - 1));
     // the maximum first: one exp a block instead of two
     float m = -INFINITY, s = 0.0f;
-    if (t < T) {
+    const int at = t < T ? (slot ? slot[t] : t) : -1;  // (a token without a target has no place)
+    if (at >= 0) {
 #pragma unroll 8
-        for (int b = sub; b < nb; b += n_sub) m = fmaxf(m, part[(size_t)b * T + t].x);
+        for (int b = sub; b < nb; b += n_sub) m = fmaxf(m, part[(size_t)b * T + at].x);
         const float m0 = m == -INFINITY ? 0.0f : m;
 #pragma unroll 8
         for (int b = sub; b < nb; b += n_sub) {
-            const float2 v = part[(size_t)b * T + t];
+            const float2 v = part[(size_t)b * T + at];
             s += v.y * expf(v.x - m0);
         }
     }
@@ -1020,10 +1096,10 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const float2 *__restric
     if (tid < TL && t < T) {
         const float2 v = red[tid];
         const int y = targets[t];
-        loss[t] = y >= 0 && y < V ? (v.x - tlogit[t]) + logf(v.y) : 0.0f;
+        loss[t] = y >= 0 && y < V ? (v.x - tlogit[at]) + logf(v.y) : 0.0f;
         if (row_stats) {
-            row_stats[t] = v.x;
-            row_stats[T + t] = v.y;
+            row_stats[t] = at >= 0 ? v.x : 0.0f;
+            row_stats[T + t] = at >= 0 ? v.y : 1.0f;
         }
     }
     if (gridDim.x == 1) {
@@ -1038,19 +1114,30 @@ __global__ __launch_bounds__(1024) void head_mean_kernel(const float *loss, cons
 
 // dx: the slabs added in slice order, rounded once; rows without a target are zero
 template <bool BF>
-__global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ targets, int T, int V,
-                                                      int d, const float *__restrict__ mean, const float *dloss, void *__restrict__ dx)
+__global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ slot, int d,
+                                                      int vec, const float *__restrict__ mean, const float *dloss, void *__restrict__ dx)
 {
     const float g = head_scale(mean, dloss);
-    const int t = blockIdx.x, y = targets[t];
-    const bool held = y >= 0 && y < V;
-    for (int c = blockIdx.y * 256 + threadIdx.x; c < d; c += gridDim.y * 256) {
-        float s = 0.0f;
-        if (held)
-            for (int k = 0; k < slices; ++k) s += slabs[(size_t)k * slab + (size_t)t * ld + c];
-        s = held ? s * g : 0.0f;
-        if (BF) ((bf16_t *)dx)[(size_t)t * d + c] = f32_to_bf16(s);
-        else ((float *)dx)[(size_t)t * d + c] = s;
+    const int t = blockIdx.x, at = slot[t];
+    for (int c = 4 * (blockIdx.y * 256 + threadIdx.x); c < d; c += 4 * gridDim.y * 256) {
+        f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0) {
+#pragma unroll 4
+            for (int k = 0; k < slices; ++k) s += *(const f32x4_t *)(slabs + (size_t)k * slab + (size_t)at * ld + c);
+            s *= g;
+        }
+        const size_t o = (size_t)t * d + c;
+        if (vec) {
+            if (BF) *(uint2 *)((bf16_t *)dx + o) = make_uint2(hp_pack2(s[0], s[1]), hp_pack2(s[2], s[3]));
+            else *(f32x4_t *)((float *)dx + o) = s;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k < d) {
+                    if (BF) ((bf16_t *)dx)[o + k] = f32_to_bf16(s[k]);
+                    else ((float *)dx)[o + k] = s[k];
+                }
+        }
     }
 }
 __global__ __launch_bounds__(256) void head_zero_kernel(void *p, size_t bytes)  // (memset nodes are not for captured graphs)
@@ -1068,7 +1155,7 @@ struct head_plan {
     int nb;                             // column blocks of the forward pass
     int slices;                         // k slices of dx
     bool direct, few;
-    size_t x_img, w_img, p_img, slabs, part, tlogit, bytes;
+    size_t x_img, w_img, p_img, slabs, part, tlogit, held, slot, tok_target, tok_stats, bytes;
     size_t x_plane, w_plane, p_plane, slab;
 };
 
@@ -1103,6 +1190,10 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
     h.piece = (int)up_to(ceil_div(a.V, h.pieces), 256);
     h.x_plane = up_to(backward ? h.Tp : a.T, 128) * (size_t)h.dp * 2;
     h.x_img = take(h.x_plane * h.planes);
+    h.held = take(4);
+    h.slot = take((size_t)a.T * 4);
+    h.tok_target = take((size_t)a.T * 4);
+    if (backward) h.tok_stats = take((size_t)a.T * 8);
     if (!h.direct) {
         h.w_plane = (size_t)h.piece * h.dp * 2;
         h.w_img = take(h.w_plane * h.planes);
@@ -1188,13 +1279,22 @@ static hipError_t head_product(const omega_ctx *ctx, head_prod p, int planes, hi
     } while (0)
 
 // Images of rows [R,K] at src: rows up to Rp (a multiple of 64), columns up to Kp
-static void head_images(const head_args &a, const void *src, int R, int K, int Rp, int Kp, const int32_t *targets, unsigned char *img, size_t plane, hipStream_t s)
+static void head_images(const head_args &a, const void *w, int R, int Rp, int Kp, unsigned char *img, size_t plane, hipStream_t s)
 {
-    const bool bf = a.dtype == OMEGA_DTYPE_BF16;
-    const int vec = K % 8 == 0 && (uintptr_t)src % 16 == 0;
+    const int vec = a.d % 8 == 0 && (uintptr_t)w % 16 == 0;
     const dim3 grid(Rp / 64, Kp / 64);
-    if (bf) hipLaunchKernelGGL(head_images_kernel<true>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane);
-    else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, src, R, K, vec, targets, a.V, img, Kp / 32, plane);
+    if (a.dtype == OMEGA_DTYPE_BF16) hipLaunchKernelGGL(head_images_kernel<true>, grid, dim3(256), 0, s, w, R, a.d, vec, img, Kp / 32, plane);
+    else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, w, R, a.d, vec, img, Kp / 32, plane);
+}
+
+static void head_tokens(const head_args &a, const head_plan &h, unsigned char *base, int Rp, const float *row_stats, hipStream_t s)
+{
+    const int vec = a.d % 8 == 0 && (uintptr_t)a.x % 16 == 0;
+    // (as many workgroups a row of tiles as fill the machine; more would only count again)
+    const dim3 grid(Rp / 64, std::min(h.dp / 64, std::max(1, 4096 / (Rp / 64))));
+    const auto k = a.dtype == OMEGA_DTYPE_BF16 ? head_tokens_kernel<true> : head_tokens_kernel<false>;
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a.x, a.T, a.d, vec, a.targets, a.V, row_stats, base + h.x_img, h.dp / 32, h.x_plane, (int32_t *)(base + h.held),
+                       (int32_t *)(base + h.slot), (int32_t *)(base + h.tok_target), row_stats ? (float *)(base + h.tok_stats) : nullptr);
 }
 
 // k steps of dx over `vc` rows of W (P has zeros up to a multiple of 256)
@@ -1249,11 +1349,11 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
 #undef HEAD_FEW_K
 #undef HEAD_STREAM_K
     } else {
-        head_images(a, a.x, a.T, a.d, (int)up_to(a.T, 64), h.dp, a.targets, base + h.x_img, h.x_plane, s);
+        head_tokens(a, h, base, (int)up_to(a.T, 64), nullptr, s);
         for (int v0 = 0; v0 < a.V; v0 += h.piece) {
             const int vc = std::min(h.piece, a.V - v0);
             const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
-            if (!h.direct) head_images(a, w, vc, a.d, (int)up_to(vc, 64), h.dp, nullptr, base + h.w_img, h.w_plane, s);
+            if (!h.direct) head_images(a, w, vc, (int)up_to(vc, 64), h.dp, base + h.w_img, h.w_plane, s);
             head_prod p = {};
             p.A = base + h.x_img;
             p.planeA = h.x_plane;
@@ -1264,9 +1364,9 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
             p.M = p.rowsA = a.T;
             p.N = vc;
             p.slices = 1;
-            p.targets = a.targets;
+            p.held = (const int32_t *)(base + h.held);
+            p.targets = (const int32_t *)(base + h.tok_target);
             p.T = a.T;
-            p.V = a.V;
             p.v0 = v0;
             p.part = part;
             p.tlogit = tlogit;
@@ -1275,7 +1375,7 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
     }
     int TL = 1;
     while (TL < 64 && TL < a.T) TL *= 2;
-    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(a.T, TL)), dim3(1024), 0, s, part, nb, tlogit, a.targets, a.T, a.V, TL, a.loss, a.row_stats, a.mean);
+    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(a.T, TL)), dim3(1024), 0, s, part, nb, tlogit, a.targets, h.few ? (const int32_t *)nullptr : (const int32_t *)(base + h.slot), a.T, a.V, TL, a.loss, a.row_stats, a.mean);
     if (a.T > TL) hipLaunchKernelGGL(head_mean_kernel, dim3(1), dim3(1024), 0, s, a.loss, a.targets, a.T, a.V, a.mean);
     return hipGetLastError();
 }
@@ -1290,13 +1390,12 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     }
     const head_plan h = head_plan_of(ctx, a, true);
     unsigned char *base = (unsigned char *)ws;
-    head_images(a, a.x, a.T, a.d, h.Tp, h.dp, a.targets, base + h.x_img, h.x_plane, s);
+    head_tokens(a, h, base, h.Tp, a.row_stats, s);
+    const int32_t *held = (const int32_t *)(base + h.held);
     for (int v0 = 0; v0 < a.V; v0 += h.piece) {
-        const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256), Tr = (int)up_to(a.T, 64);
+        const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256);
         const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
-        if (!h.direct) head_images(a, w, vc, a.d, vp, h.dp, nullptr, base + h.w_img, h.w_plane, s);
-        if (a.dw && Tr < h.Tp)  // (k places of dW that no tile of P reaches)
-            hipLaunchKernelGGL(head_zero_blocks_kernel, dim3(vp / 32, h.planes), dim3(64), 0, s, base + h.p_img, h.p_plane, Tr / 16, h.Tp / 16);
+        if (!h.direct) head_images(a, w, vc, vp, h.dp, base + h.w_img, h.w_plane, s);
         head_prod p = {};
         p.A = base + h.x_img;
         p.planeA = h.x_plane;
@@ -1308,10 +1407,10 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
         p.rowsA = h.Tp;
         p.N = vc;
         p.slices = 1;
-        p.targets = a.targets;
-        p.row_stats = a.row_stats;
+        p.held = held;
+        p.targets = (const int32_t *)(base + h.tok_target);
+        p.row_stats = (const float *)(base + h.tok_stats);
         p.T = a.T;
-        p.V = a.V;
         p.v0 = v0;
         p.P = base + h.p_img;
         p.planeP = h.p_plane;
@@ -1326,6 +1425,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.kt = head_dx_steps(vc);
             q.ktA = vp / 32;
             q.ktB = h.dp / 32;
+            q.held = held;
             q.M = q.rowsA = a.T;
             q.N = a.d;
             q.rowsB = vc;
@@ -1342,6 +1442,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.planeA = h.p_plane;
             q.B = base + h.x_img;
             q.planeB = h.x_plane;
+            q.held = held;
             q.kt = h.Tp / 32;
             q.ktA = vp / 32;
             q.ktB = h.dp / 32;
@@ -1358,9 +1459,10 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     }
     if (a.dx) {
         const int slices = std::max(1, std::min(h.slices, head_dx_steps(std::min(h.piece, a.V)) / 8));
-        const dim3 grid(a.T, std::min(ceil_div(a.d, 256), 1024));
-        if (bf) hipLaunchKernelGGL(head_dx_kernel<true>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);
-        else hipLaunchKernelGGL(head_dx_kernel<false>, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), a.targets, a.T, a.V, a.d, a.mean, a.dloss, a.dx);
+        const dim3 grid(a.T, std::min(ceil_div(a.d, 1024), 1024));
+        const int vec = a.d % 4 == 0 && (uintptr_t)a.dx % (bf ? 8 : 16) == 0;
+        const auto k = bf ? head_dx_kernel<true> : head_dx_kernel<false>;
+        hipLaunchKernelGGL(k, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), (const int32_t *)(base + h.slot), a.d, vec, a.mean, a.dloss, a.dx);
     }
     return hipGetLastError();
 }

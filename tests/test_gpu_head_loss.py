@@ -175,6 +175,21 @@ def test_few_tokens_and_a_large_vocabulary(T, d, dtype):
         check(run(x, w, y, dtype, shift, stats=False), reference(x, w, y, dtype), shift)
 
 
+@pytest.mark.parametrize("dtype,d", [("f32", 260), ("bf16", 260), ("bf16", 256)])
+@pytest.mark.parametrize("T,pad", [(600, 0.97), (600, 0.6), (1000, 0.75), (300, 0.997), (300, 1.0), (70, 0.9)])
+def test_most_tokens_have_no_target(T, pad, d, dtype):
+    """The products work on the others, moved together: fewer rows than tiles, steps and statistics were laid out for."""
+    rng = np.random.default_rng(T + d)
+    V = 700
+    w, y = normal(rng, V, d, std=d ** -0.5, dtype=dtype), targets_of(rng, T, V, pad)
+    if pad < 1.0:
+        y[-1] = V - 1
+    x = normal(rng, T, d, dtype=dtype)
+    ref = reference(x, w, y, dtype)
+    x[(y < 0) | (y >= V)] = np.nan
+    check(run(x, w, y, dtype), ref)
+
+
 def test_no_target_at_all_and_no_rows():
     rng = np.random.default_rng(0)
     for T in (4, 40):
