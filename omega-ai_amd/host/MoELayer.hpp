@@ -300,6 +300,7 @@ public:
         return h;
     }
     const char *getLayerType() const override { return "feed_forward"; }
+    omega_moe *handle() const { return moe_; }
 
     void getRouting(std::vector<int32_t> &ids, std::vector<float> &w, std::vector<int32_t> &counts)
     {

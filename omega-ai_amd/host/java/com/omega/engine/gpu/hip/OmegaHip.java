@@ -61,6 +61,18 @@ public final class OmegaHip {
     private static final MethodHandle SCALE_GRAD = h("omega_moe_scale_grad", FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_FLOAT));
     private static final MethodHandle GET_ROUTING = h("omega_moe_get_routing", FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
 
+    private static final MethodHandle EMBEDDING_FORWARD = h("omega_hip_embedding_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, JAVA_INT, JAVA_FLOAT, ADDRESS));
+    private static final MethodHandle EMBEDDING_BACKWARD = h("omega_hip_embedding_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, ADDRESS, JAVA_INT));
+    private static final MethodHandle LAYERNORM_FORWARD = h("omega_hip_layernorm_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, JAVA_FLOAT, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle LAYERNORM_BACKWARD = h("omega_hip_layernorm_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle HEAD_LOSS_FORWARD = h("omega_hip_head_loss_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle HEAD_LOSS_BACKWARD = h("omega_hip_head_loss_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle CLIP_GRAD_NORM = h("omega_hip_clip_grad_norm", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_INT, JAVA_FLOAT, ADDRESS));
+
+    /** struct omega_grad_tensor: src, dst, n (uint64), dtype, reserved. */
+    private static final MemoryLayout GRAD_TENSOR = MemoryLayout.structLayout(
+            ADDRESS.withName("src"), ADDRESS.withName("dst"), JAVA_LONG.withName("n"), JAVA_INT.withName("dtype"), JAVA_INT.withName("reserved"));
+
     /** struct omega_moe_config: ten int32 in declaration order. */
     private static final MemoryLayout MOE_CONFIG = MemoryLayout.structLayout(
             JAVA_INT.withName("T_max"), JAVA_INT.withName("d"), JAVA_INT.withName("E"), JAVA_INT.withName("K"),
@@ -357,6 +369,84 @@ public final class OmegaHip {
             }
         } catch (Throwable t2) {
             throw wrap(t2);
+        }
+    }
+
+    // ---- the model around the layer (device addresses; 0 = NULL where the C call allows it) ----
+
+    private static MemorySegment at(long dptr) {
+        return dptr == 0L ? MemorySegment.NULL : MemorySegment.ofAddress(dptr);
+    }
+
+    public static void embeddingForward(MemorySegment ctx, long table, int dtype, int v, int d, long ids, int t, float scale, long out) {
+        try {
+            check(ctx, (int) EMBEDDING_FORWARD.invokeExact(ctx, at(table), dtype, v, d, at(ids), t, scale, at(out)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    /** accumulate: the sums are added to what dTable holds (a table tied to the head). */
+    public static void embeddingBackward(MemorySegment ctx, long ids, int t, long dout, int dtype, int v, int d, float scale, boolean accumulate, long dTable, int gradDtype) {
+        try {
+            check(ctx, (int) EMBEDDING_BACKWARD.invokeExact(ctx, at(ids), t, at(dout), dtype, v, d, scale, accumulate ? 1 : 0, at(dTable), gradDtype));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void layernormForward(MemorySegment ctx, long x, int dtype, int t, int d, long gamma, long beta, float eps, long out, long mean, long rstd) {
+        try {
+            check(ctx, (int) LAYERNORM_FORWARD.invokeExact(ctx, at(x), dtype, t, d, at(gamma), at(beta), eps, at(out), at(mean), at(rstd)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void layernormBackward(MemorySegment ctx, long x, long dout, int dtype, int t, int d, long gamma, long mean, long rstd, long dx, long dgamma, long dbeta) {
+        try {
+            check(ctx, (int) LAYERNORM_BACKWARD.invokeExact(ctx, at(x), at(dout), dtype, t, d, at(gamma), at(mean), at(rstd), at(dx), at(dgamma), at(dbeta)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    /** Loss of every token, mean[2] = mean loss and number of tokens with a target; rowStats [2,t] for the backward call (or 0). */
+    public static void headLossForward(MemorySegment ctx, long x, long w, int dtype, int t, int v, int d, long targets, long loss, long rowStats, long mean) {
+        try {
+            check(ctx, (int) HEAD_LOSS_FORWARD.invokeExact(ctx, at(x), at(w), dtype, t, v, d, at(targets), at(loss), at(rowStats), at(mean)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void headLossBackward(MemorySegment ctx, long x, long w, int dtype, int t, int v, int d, long targets, long rowStats, long mean, long dloss, long dx, long dw) {
+        try {
+            check(ctx, (int) HEAD_LOSS_BACKWARD.invokeExact(ctx, at(x), at(w), dtype, t, v, d, at(targets), at(rowStats), at(mean), at(dloss), at(dx), at(dw)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    /** Gradients grads[i] of n[i] elements, in place, and those of the layers (handles of moeCreate) times min(1, maxNorm / (norm + 1e-6)). */
+    public static void clipGradNorm(MemorySegment ctx, long[] grads, long[] n, int[] dtypes, MemorySegment[] layers, float maxNorm, long normOut) {
+        try (Arena a = Arena.ofConfined()) {
+            MemorySegment list = a.allocate(MemoryLayout.sequenceLayout(Math.max(grads.length, 1), GRAD_TENSOR));
+            for (int i = 0; i < grads.length; i++) {
+                MemorySegment e = list.asSlice(i * GRAD_TENSOR.byteSize(), GRAD_TENSOR.byteSize());
+                e.set(ADDRESS, 0, at(grads[i]));
+                e.set(ADDRESS, 8, at(grads[i]));
+                e.set(JAVA_LONG, 16, n[i]);
+                e.set(JAVA_INT, 24, dtypes[i]);
+                e.set(JAVA_INT, 28, 0);
+            }
+            MemorySegment handles = a.allocate(MemoryLayout.sequenceLayout(Math.max(layers.length, 1), ADDRESS));
+            for (int i = 0; i < layers.length; i++) {
+                handles.setAtIndex(ADDRESS, i, layers[i]);
+            }
+            check(ctx, (int) CLIP_GRAD_NORM.invokeExact(ctx, list, grads.length, handles, layers.length, maxNorm, at(normOut)));
+        } catch (Throwable e) {
+            throw wrap(e);
         }
     }
 }
