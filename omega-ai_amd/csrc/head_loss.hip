@@ -53,9 +53,8 @@ struct head_prod {
     int ktA, ktB;                    // k steps of a row group of the images (an operand read across its rows: its columns / 32)
     int rowsA;                       // A's rows as far as the product needs them
     int rowsB;                       // B read across its rows in place: the rows there are
-    int M, N, mt, nt, slices;        // mt row tiles of `th` rows (64, 128, 192 or 256), nt column tiles of 256
-    int th;
-    const int32_t *held;             // tokens with a target: M, and mt from it; of dW kt
+    int M, N, mt, nt, slices;        // mt row tiles of 32 NU rows, nt column tiles of 256
+    const int32_t *held;             // tokens with a target (M; of dW kt), tile heights (head_rows) of LSE / P and of ACC / ADD
     // epilogues
     const int32_t *targets;          // of the tokens that have one, as their statistics
     const float *row_stats, *mean, *dloss;
@@ -133,14 +132,14 @@ struct hp_item {
     int phase, rows;              // of an operand read across its rows: first step's place in its row group, rows from there on
 };
 
-template <int EPI>
+template <int NU, int EPI>
 __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
 {
     hp_item it;
     const int per = p.mt * p.nt;
     // column tiles outside, up to 8 row tiles inside: the 32 neighbours that an XCD works on share operand tiles in its L2
     const int sl = idx / per, rem = idx - sl * per, g = rem / (8 * p.nt), gm = min(8, p.mt - 8 * g), r2 = rem - g * 8 * p.nt, n = r2 / gm;
-    it.row0 = __builtin_amdgcn_readfirstlane((8 * g + (r2 - n * gm)) * p.th);
+    it.row0 = __builtin_amdgcn_readfirstlane((8 * g + (r2 - n * gm)) * 32 * NU);
     it.n0 = __builtin_amdgcn_readfirstlane(n * HP_TILE);
     it.slice = __builtin_amdgcn_readfirstlane(sl);
     const int first = ((it.slice * p.kt) / p.slices) & ~1;
@@ -157,16 +156,18 @@ __device__ __forceinline__ hp_item hp_make_item(const head_prod &p, int idx)
         it.B = hp_uniform(p.b_ld == 0 ? p.B + (size_t)(it.n0 >> 7) * rgB + (size_t)first * 8192 : p.B + (size_t)it.n0 * p.b_ld + (size_t)first * 64);
     return it;
 }
-// The lane number as a value that the compiler cannot carry over: what follows from it is computed where it is used.  (Kept from item
-// to item it is spilled, and the wait for a reload in the middle of a k loop drains the ring: 49 % of the matrix rate instead of 80.)
-__device__ __forceinline__ int hp_fresh(int lane)
+// The lane number, counted anew wherever it is needed, as a value that the compiler cannot carry over: nor can it what follows from it.
+// (Kept from item to item these are spilled, and the wait for a reload in the middle of a k loop drains the ring: 49 % of the matrix rate
+// instead of 80.)
+__device__ __forceinline__ int hp_lane()
 {
-    asm volatile("" : "+v"(lane));
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
     return lane;
 }
 // what the lane adds for the wave's loads, blocks wave + 4 n of the step: of 16 rows each; of an operand read across its rows, 16 rows and
 // 32 columns, the upper and the lower 16 rows in turn
-template <int EPI>
+template <int NU, int EPI>
 __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_item &it, int wave, int lane, uint32_t (&va)[4], uint32_t (&vb)[4])
 {
     const uint32_t rgA = (uint32_t)p.ktA * 8192u, rgB = (uint32_t)p.ktB * 8192u;
@@ -175,10 +176,10 @@ __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_ite
     for (int k = 0; k < 4; ++k) {
         const int q = wave + 4 * k;
         if (HP_TR_A(EPI)) {
-            const bool valid = 16 * q < p.th && it.row0 + 32 * (q >> 1) < 32 * p.ktA;
+            const bool valid = q < 2 * NU && it.row0 + 32 * (q >> 1) < 32 * p.ktA;
             va[k] = valid ? (uint32_t)(q >> 1) * 8192u + (uint32_t)(q & 1) * 1024u + (uint32_t)lane * 16u : 0u;
         } else {
-            const bool valid = 16 * q < p.th && it.row0 + 16 * q < p.rowsA;  // (a block without rows: every lane reads the first 16 bytes of the item's first block)
+            const bool valid = q < 2 * NU && it.row0 + 16 * q < p.rowsA;  // (a block without rows: every lane reads the first 16 bytes of the item's first block)
             const int b = blk0 + (valid ? q : 0);
             va[k] = (uint32_t)(b >> 3) * rgA + (uint32_t)(b & 7) * 1024u + (valid ? (uint32_t)lane * 16u : 0u);
         }
@@ -187,11 +188,13 @@ __device__ __forceinline__ void hp_lane_offsets(const head_prod &p, const hp_ite
         } else if (HP_TR_B(EPI)) {
             const int r = 16 * (q & 1) + (lane >> 2), c = 32 * (q >> 1) + 8 * ((lane & 3) ^ pk_swz(r));
             vb[k] = (uint32_t)min(r, it.rows - 1) * (uint32_t)p.b_ld + (uint32_t)min(c, p.N - 8 - it.n0) * 2u;
-        } else if (p.b_ld == 0) {
-            vb[k] = (uint32_t)(q >> 3) * rgB + (uint32_t)(q & 7) * 1024u + (uint32_t)lane * 16u;
         } else {
+            // (both forms and a choice: a branch here costs registers that the product has not got)
             const int r = 16 * q + (lane >> 2);
-            vb[k] = (uint32_t)min(r, p.N - 1 - it.n0) * (uint32_t)p.b_ld + (uint32_t)(((lane & 3) ^ pk_swz(r)) << 4);
+            const uint32_t image = (uint32_t)(q >> 3) * rgB + (uint32_t)(q & 7) * 1024u + (uint32_t)lane * 16u;
+            uint32_t rows = (uint32_t)min(r, p.N - 1 - it.n0) * (uint32_t)p.b_ld + (uint32_t)(((lane & 3) ^ pk_swz(r)) << 4);
+            asm volatile("" : "+v"(rows));
+            vb[k] = p.b_ld == 0 ? image : rows;
         }
     }
 }
@@ -204,7 +207,7 @@ struct hp_at {
 // ... and a step on.  Rows of W in place: where the last ones are fewer than 32, the lanes behind them read the last one, and a step that
 // has none reads the step before once more (P is zero there).
 template <int EPI>
-__device__ __forceinline__ void hp_advance(const head_prod &p, hp_at &at, uint32_t (&vb)[4], int wave, int lane)
+__device__ __forceinline__ void hp_advance(const head_prod &p, hp_at &at, uint32_t (&vb)[4], int wave)
 {
     if (!HP_TR_B(EPI)) {
         at.A += 8192;
@@ -221,7 +224,7 @@ __device__ __forceinline__ void hp_advance(const head_prod &p, hp_at &at, uint32
         at.rows -= 32;
         at.B += at.rows > 0 ? (size_t)32 * p.b_ld : 0;
         if (at.rows > 0 && at.rows < 32) {
-            const int behind = max(16 * (wave & 1) + (hp_fresh(lane) >> 2) - (at.rows - 1), 0);
+            const int behind = max(16 * (wave & 1) + (hp_lane() >> 2) - (at.rows - 1), 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k) vb[k] -= (uint32_t)behind * (uint32_t)p.b_ld;
         }
@@ -340,7 +343,7 @@ struct hp_state {
         HP_MFMA(PA, PB, 7, 6);                                                                           \
         cur = cur + 1 == ST ? 0 : cur + 1;                                                                \
         sb = lds_wave + cur * HP_STAGE_BYTES(NU);                                                           \
-        hp_advance<EPI>(p, at, st.vb, wave, lane0);                                                         \
+        hp_advance<EPI>(p, at, st.vb, wave);                                                                \
         __builtin_amdgcn_sched_barrier(0);                                                                  \
         HP_MFMA(PA, PB, 7, 7);                                                                           \
         HP_STAGE_ADDR();                                                                                    \
@@ -503,18 +506,18 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
 
 // A tile of 32 NU rows by 256 columns.  acc[iu][c][r]: row 16 (2 iu + wm) + lane % 16, column 128 wn + 16 c + 4 (lane / 16) + r.
 template <int NU, int EPI, int NSEG>
-__device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave, int lane0)
+__device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, const head_prod &p, const hp_item &it, hp_item &nxt, int next_idx, int wave)
 {
     constexpr int ST = HP_STAGES(NU);
     const int wm = wave >> 1, wn = wave & 1;
-    int lane = hp_fresh(lane0), l16 = lane & 15, lq = lane >> 4;
+    int lane = hp_lane(), l16 = lane & 15, lq = lane >> 4;
     const int kt = __builtin_amdgcn_readfirstlane(it.kt);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     const uint32_t lds_wave = lds0 + wave * 1024;
     const hp_frag fr = hp_frag_of<NU, EPI>(wm, wn, lane);
     int cur = __builtin_amdgcn_readfirstlane(st.cur);
     hp_at at = {hp_uniform(st.at.A), hp_uniform(st.at.B), __builtin_amdgcn_readfirstlane(st.at.phase), __builtin_amdgcn_readfirstlane(st.at.rows)};
-    nxt = hp_make_item<EPI>(p, next_idx);
+    nxt = hp_make_item<NU, EPI>(p, next_idx);
     uint32_t sb = lds_wave + cur * HP_STAGE_BYTES(NU);
     const unsigned char *ra, *ra1, *rb0, *rb1;
     HP_STAGE_ADDR();
@@ -547,7 +550,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
             const hp_item &li = ns == 0 ? nxt : it;  // the item of the loads from here on
             const size_t a0 = NSEG > 1 ? (size_t)((HP_SEG_A >> (4 * ns)) & 3) * p.planeA : 0, b0 = NSEG > 1 ? (size_t)((HP_SEG_B >> (4 * ns)) & 3) * p.planeB : 0;
             at = {hp_uniform(li.A + a0), hp_uniform(li.B + b0), li.phase, li.rows};
-            hp_lane_offsets<EPI>(p, li, wave, hp_fresh(lane0), st.va, st.vb);
+            hp_lane_offsets<NU, EPI>(p, li, wave, hp_lane(), st.va, st.vb);
         }
         if (ST & 1) HP_STEP(st.fa1, st.fb1, st.fa0, st.fb0);
         for (k = 0; k < ST / 2; ++k) {
@@ -559,7 +562,7 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
     st.cur = cur;
     st.at = at;
 
-    lane = hp_fresh(lane0);
+    lane = hp_lane();
     l16 = lane & 15;
     lq = lane >> 4;
     const int col0 = it.n0 + wn * 128 + 4 * lq;  // column of acc[.][0][0]
@@ -637,49 +640,31 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
 
 // Persistent: workgroup w takes items w, w + n, ... in rounds of n = gridDim.x; within a round XCD x (w % 8) takes neighbouring items.
 template <int NU, int EPI, int NSEG>
-__global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
+__device__ __forceinline__ void hp_run(unsigned char *smem, const head_prod &p, int wave)
 {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n_wg = gridDim.x;
     const int at_wg = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-    const int tokens = __builtin_amdgcn_readfirstlane(p.held[0]);
-    if (EPI == HEAD_OUT) {
-        p.kt = max(8, ((tokens + 63) >> 6) * 2);
-    } else {
-        p.M = tokens;
-        p.mt = (tokens + 32 * NU - 1) / (32 * NU);
-    }
-    if (EPI == HEAD_P && tokens <= 192) {  // (dW has eight steps at least: rows of P that no tile reaches)
-        const int KTp = p.nt * (HP_TILE / HP_BK), b0 = (tokens + 63) >> 6 << 2, per = 16 - b0;
-        for (int i = blockIdx.x * 4 + wave; i < KTp * per; i += gridDim.x * 4)
-#pragma unroll
-            for (int q = 0; q < (NSEG > 1 ? 3 : 1); ++q) {
-                const int kb = i / per, b = b0 + i - kb * per;
-                *(uint4 *)(p.P + q * p.planeP + ((((size_t)(b >> 3) * KTp + kb) * 8 + (b & 7)) << 10) + lane * 16) = make_uint4(0, 0, 0, 0);
-            }
-    }
     const int total = p.mt * p.nt * p.slices;
     int idx = at_wg;
     if (idx >= total) return;
-    hp_item it = hp_make_item<EPI>(p, idx);
+    hp_item it = hp_make_item<NU, EPI>(p, idx);
     hp_state st;
     hp_at at = {hp_uniform(it.A + (NSEG > 1 ? (size_t)(HP_SEG_A & 3) * p.planeA : 0)), hp_uniform(it.B + (NSEG > 1 ? (size_t)(HP_SEG_B & 3) * p.planeB : 0)),
                 it.phase, it.rows};
-    hp_lane_offsets<EPI>(p, it, wave, lane, st.va, st.vb);
+    hp_lane_offsets<NU, EPI>(p, it, wave, hp_lane(), st.va, st.vb);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
     constexpr int ST = HP_STAGES(NU);
     for (int i = 0; i < ST; ++i) {  // the first item's first steps (of 8 or more of its first part)
         const uint32_t sb = lds0 + wave * 1024 + i * HP_STAGE_BYTES(NU);
         HP_LOAD(0, sb); HP_LOAD(1, sb); HP_LOAD(2, sb); HP_LOAD(3, sb);
         HP_LOAD(4, sb); HP_LOAD(5, sb); HP_LOAD(6, sb); HP_LOAD(7, sb);
-        hp_advance<EPI>(p, at, st.vb, wave, lane);
+        hp_advance<EPI>(p, at, st.vb, wave);
     }
     st.at = at;
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * HP_LOADS(NU)) : "memory");
     __syncthreads();
     {
-        const hp_frag fr = hp_frag_of<NU, EPI>(wave >> 1, wave & 1, lane);
+        const hp_frag fr = hp_frag_of<NU, EPI>(wave >> 1, wave & 1, hp_lane());
         const int cur = ST - 1;  // (stage 0 is the one behind it)
         const unsigned char *ra, *ra1, *rb0, *rb1;
         HP_STAGE_ADDR();
@@ -695,11 +680,63 @@ __global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
         const bool more = idx + n_wg < total;
         if (more) idx += n_wg;
         hp_item nxt;  // (behind the last item: this one's loads once more, which nobody reads)
-        hp_run_item<NU, EPI, NSEG>(smem, st, p, it, nxt, idx, wave, lane);
+        hp_run_item<NU, EPI, NSEG>(smem, st, p, it, nxt, idx, wave);
         if (!more) break;
         it = nxt;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads behind the last item land in LDS that nobody reads)
+}
+
+// Height of a row tile, 64 times the result: the one that takes the least time by rounds of one tile per compute unit, a tile of n x 64 rows
+// counted as n + 1/2 (its columns' loads).
+__host__ __device__ static inline int head_rows(int M, int nt, int slices, int cus)
+{
+    uint32_t n = 0, best = 0;
+    for (uint32_t k = 4; k >= 1; --k) {
+        const uint32_t cost = (((uint32_t)M + 64 * k - 1) / (64 * k) * (uint32_t)(nt * slices) + (uint32_t)cus - 1) / (uint32_t)cus * (2 * k + 1);
+        if (n == 0 || cost < best) n = k, best = cost;
+    }
+    return (int)n;
+}
+
+// Fixed: the height is the host's (dW, whose rows are the vocabulary).  Otherwise the rows are the tokens with a target, whose number is known
+// on the device alone, and the height is what head_tokens_kernel found for them: as against the height for all T, fp32 274 x 1120,
+// vocabulary 59721, 10 % masked: 1505 -> 1235 us; nothing masked, 700 x 1024, 9000: 1 us a product more.
+template <int NU, int EPI, int NSEG>
+__global__ __launch_bounds__(256) void head_product_kernel(head_prod p)
+{
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tokens = __builtin_amdgcn_readfirstlane(p.held[0]);
+    if (NU > 0) {
+        p.kt = max(8, ((tokens + 63) >> 6) * 2);
+        hp_run<NU ? NU : 2, EPI, NSEG>(smem, p, wave);
+        return;
+    }
+    const int n = __builtin_amdgcn_readfirstlane(p.held[EPI == HEAD_LSE || EPI == HEAD_P ? 1 : 2]);
+    p.M = tokens;
+    if (EPI == HEAD_P && tokens <= 192) {  // (dW has eight steps at least: rows of P that no tile reaches)
+        const int KTp = p.nt * (HP_TILE / HP_BK), b0 = (tokens + 63) >> 6 << 2, per = 16 - b0;
+        for (int i = blockIdx.x * 4 + wave; i < KTp * per; i += gridDim.x * 4)
+#pragma unroll
+            for (int q = 0; q < (NSEG > 1 ? 3 : 1); ++q) {
+                const int kb = i / per, b = b0 + i - kb * per;
+                *(uint4 *)(p.P + q * p.planeP + ((((size_t)(b >> 3) * KTp + kb) * 8 + (b & 7)) << 10) + hp_lane() * 16) = make_uint4(0, 0, 0, 0);
+            }
+    }
+    if (n == 4) {
+        p.mt = (tokens + 255) >> 8;
+        hp_run<8, EPI, NSEG>(smem, p, wave);
+    } else if (n == 3) {
+        p.mt = (tokens + 191) / 192;
+        hp_run<6, EPI, NSEG>(smem, p, wave);
+    } else if (n == 2) {
+        p.mt = (tokens + 127) >> 7;
+        hp_run<4, EPI, NSEG>(smem, p, wave);
+    } else {
+        p.mt = (tokens + 63) >> 6;
+        hp_run<2, EPI, NSEG>(smem, p, wave);
+    }
 }
 
 // ---- tile images ----
@@ -757,14 +794,14 @@ __global__ __launch_bounds__(256) void head_images_kernel(const void *__restrict
 }
 
 // The tokens that have a target, moved together in their order: x's image, their targets and (where the backward pass wants them) statistics,
-// slot[t] = a token's place or -1, held[0] = their number n.  The products work on n rows, whatever the others hold; the image's rows from n on are
+// slot[t] = a token's place or -1, held = their number n, the tile heights of the products over them.  The products work on n rows, whatever the others hold; the image's rows from n on are
 // zeros.  A workgroup takes 64 tokens and counts for itself how many of those before have a target: a launch less than a scan of its own
 // (T / 64 workgroups read T targets each, a few us for thousands of tokens).
 template <bool BF>
 __global__ __launch_bounds__(256) void head_tokens_kernel(const void *__restrict__ x, int T, int d, int vec, const int32_t *__restrict__ targets, int V,
                                                           const float *__restrict__ row_stats, unsigned char *__restrict__ img, int KTi, size_t plane,
                                                           int32_t *__restrict__ held, int32_t *__restrict__ slot, int32_t *__restrict__ tok_target,
-                                                          float *__restrict__ tok_stats)
+                                                          float *__restrict__ tok_stats, int nt_v, int nt_d, int slices, int cus)
 {
     constexpr int NP = BF ? 1 : 3;
     __shared__ int counts[2][4], place[64];
@@ -800,7 +837,11 @@ __global__ __launch_bounds__(256) void head_tokens_kernel(const void *__restrict
                     tok_stats[T + at] = row_stats[T + t];
                 }
             }
-            if (t == 0) held[0] = n;
+            if (t == 0) {
+                held[0] = n;
+                held[1] = head_rows(n, nt_v, 1, cus);
+                held[2] = head_rows(n, nt_d, slices, cus);
+            }
         }
     }
     __syncthreads();
@@ -1068,7 +1109,8 @@ __device__ void head_mean(const float *loss, const int32_t *targets, int T, int 
     }
 }
 // (max, sum) of a token over nb column blocks: TL tokens (a power of two) a workgroup, 1024 / TL threads each, joined in a fixed order.
-// A launch of one workgroup forms the mean too.
+// A launch of one workgroup forms the mean too.  (By the last of several, behind a counter and the fences that takes: 5 us more than none,
+// a launch of its own 3 to 4.)
 __global__ __launch_bounds__(1024) void head_join_kernel(const float2 *__restrict__ part, int nb, const float *__restrict__ tlogit, const int32_t *__restrict__ targets,
                                                          const int32_t *__restrict__ slot, int T, int V, int TL, float *__restrict__ loss, float *__restrict__ row_stats, float *__restrict__ mean)
 {
@@ -1190,7 +1232,7 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
     h.piece = (int)up_to(ceil_div(a.V, h.pieces), 256);
     h.x_plane = up_to(backward ? h.Tp : a.T, 128) * (size_t)h.dp * 2;
     h.x_img = take(h.x_plane * h.planes);
-    h.held = take(4);
+    h.held = take(12);
     h.slot = take((size_t)a.T * 4);
     h.tok_target = take((size_t)a.T * 4);
     if (backward) h.tok_stats = take((size_t)a.T * 8);
@@ -1217,23 +1259,18 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
 
 size_t head_workspace(const omega_ctx *ctx, const head_args &a, bool backward) { return a.T > 0 ? head_plan_of(ctx, a, backward).bytes : 0; }
 
-template <int EPI, int NSEG>
-static const void *head_kernel_of(int th)
+static const void *head_kernel_of(int epi, int planes, int rows)
 {
-    return th == 256   ? (const void *)head_product_kernel<8, EPI, NSEG>
-           : th == 192 ? (const void *)head_product_kernel<6, EPI, NSEG>
-           : th == 128 ? (const void *)head_product_kernel<4, EPI, NSEG>
-                       : (const void *)head_product_kernel<2, EPI, NSEG>;
-}
-template <int EPI>
-static hipError_t head_init_of()
-{
-    for (int th = 64; th <= 256; th += 64)
-        for (const void *f : {head_kernel_of<EPI, 1>(th), head_kernel_of<EPI, 6>(th)}) {
-            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, HP_SMEM);
-            if (e != hipSuccess) return e;
-        }
-    return hipSuccess;
+#define HEAD_K(NU, E) (planes == 1 ? (const void *)head_product_kernel<NU, E, 1> : (const void *)head_product_kernel<NU, E, 6>)
+    return epi == HEAD_LSE   ? HEAD_K(0, HEAD_LSE)
+           : epi == HEAD_P   ? HEAD_K(0, HEAD_P)
+           : epi == HEAD_ACC ? HEAD_K(0, HEAD_ACC)
+           : epi == HEAD_ADD ? HEAD_K(0, HEAD_ADD)
+           : rows == 4       ? HEAD_K(8, HEAD_OUT)
+           : rows == 3       ? HEAD_K(6, HEAD_OUT)
+           : rows == 2       ? HEAD_K(4, HEAD_OUT)
+                             : HEAD_K(2, HEAD_OUT);
+#undef HEAD_K
 }
 hipError_t head_init(void)
 {
@@ -1242,35 +1279,25 @@ hipError_t head_init(void)
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, HP_SMEM);
         if (e != hipSuccess) return e;
     }
-    hipError_t e = head_init_of<HEAD_LSE>();
-    if (e == hipSuccess) e = head_init_of<HEAD_P>();
-    if (e == hipSuccess) e = head_init_of<HEAD_ACC>();
-    if (e == hipSuccess) e = head_init_of<HEAD_ADD>();
-    if (e == hipSuccess) e = head_init_of<HEAD_OUT>();
-    return e;
+    for (int epi = HEAD_LSE; epi <= HEAD_OUT; ++epi)
+        for (int rows = 1; rows <= (epi == HEAD_OUT ? 4 : 1); ++rows)
+            for (int planes = 1; planes <= 3; planes += 2) {
+                const hipError_t e = hipFuncSetAttribute(head_kernel_of(epi, planes, rows), hipFuncAttributeMaxDynamicSharedMemorySize, HP_SMEM);
+                if (e != hipSuccess) return e;
+            }
+    return hipSuccess;
 }
 
-template <int EPI>
-static hipError_t head_product(const omega_ctx *ctx, head_prod p, int planes, hipStream_t s)
+static hipError_t head_product(const omega_ctx *ctx, int epi, head_prod p, int planes, hipStream_t s)
 {
-    // height of a row tile: the one that takes the least time by rounds of one tile per compute unit, a tile of n x 64 rows
-    // counted as n + 1/2 (its columns' loads)
     p.nt = ceil_div(p.N, HP_TILE);
-    long long best = 0;
-    for (int n = 4; n >= 1; --n) {
-        const int mt = ceil_div(p.M, 64 * n);
-        const long long cost = ((long long)mt * p.nt * p.slices + ctx->num_cus - 1) / ctx->num_cus * (2 * n + 1);
-        if (best == 0 || cost < best) {
-            best = cost;
-            p.th = 64 * n;
-            p.mt = mt;
-        }
-    }
+    const int rows = epi == HEAD_OUT ? head_rows(p.M, p.nt, p.slices, ctx->num_cus) : 1;  // (1: the lowest, which makes the most items)
+    p.mt = ceil_div(p.M, 64 * rows);
     const long long items = (long long)p.mt * p.nt * p.slices;
     if (items > 0x3fffffff) return hipErrorInvalidValue;
     const int grid = (int)std::min<long long>(items, ctx->num_cus);
     void *args[] = {&p};
-    return hipLaunchKernel(planes == 1 ? head_kernel_of<EPI, 1>(p.th) : head_kernel_of<EPI, 6>(p.th), dim3(grid), dim3(256), args, HP_SMEM, s);
+    return hipLaunchKernel(head_kernel_of(epi, planes, rows), dim3(grid), dim3(256), args, HP_SMEM, s);
 }
 #define HEAD_TRY(expr)                          \
     do {                                        \
@@ -1287,18 +1314,22 @@ static void head_images(const head_args &a, const void *w, int R, int Rp, int Kp
     else hipLaunchKernelGGL(head_images_kernel<false>, grid, dim3(256), 0, s, w, R, a.d, vec, img, Kp / 32, plane);
 }
 
-static void head_tokens(const head_args &a, const head_plan &h, unsigned char *base, int Rp, const float *row_stats, hipStream_t s)
+// k steps of dx over `vc` rows of W (P has zeros up to a multiple of 256)
+static int head_dx_steps(int vc) { return std::max(8, (int)up_to(ceil_div(vc, 32), 2)); }
+// ... and k slices over a piece
+static int head_dx_slices(const head_args &a, const head_plan &h) { return std::max(1, std::min(h.slices, head_dx_steps(std::min(h.piece, a.V)) / 8)); }
+
+static void head_tokens(const omega_ctx *ctx, const head_args &a, const head_plan &h, unsigned char *base, int Rp, const float *row_stats, hipStream_t s)
 {
     const int vec = a.d % 8 == 0 && (uintptr_t)a.x % 16 == 0;
     // (as many workgroups a row of tiles as fill the machine; more would only count again)
     const dim3 grid(Rp / 64, std::min(h.dp / 64, std::max(1, 4096 / (Rp / 64))));
     const auto k = a.dtype == OMEGA_DTYPE_BF16 ? head_tokens_kernel<true> : head_tokens_kernel<false>;
     hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a.x, a.T, a.d, vec, a.targets, a.V, row_stats, base + h.x_img, h.dp / 32, h.x_plane, (int32_t *)(base + h.held),
-                       (int32_t *)(base + h.slot), (int32_t *)(base + h.tok_target), row_stats ? (float *)(base + h.tok_stats) : nullptr);
+                       (int32_t *)(base + h.slot), (int32_t *)(base + h.tok_target), row_stats ? (float *)(base + h.tok_stats) : nullptr, ceil_div(std::min(h.piece, a.V), HP_TILE), ceil_div(a.d, HP_TILE),
+                       head_dx_slices(a, h), ctx->num_cus);
 }
 
-// k steps of dx over `vc` rows of W (P has zeros up to a multiple of 256)
-static int head_dx_steps(int vc) { return std::max(8, (int)up_to(ceil_div(vc, 32), 2)); }
 
 static void head_zero(void *p, size_t bytes, hipStream_t s)
 {
@@ -1349,7 +1380,7 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
 #undef HEAD_FEW_K
 #undef HEAD_STREAM_K
     } else {
-        head_tokens(a, h, base, (int)up_to(a.T, 64), nullptr, s);
+        head_tokens(ctx, a, h, base, (int)up_to(a.T, 64), nullptr, s);
         for (int v0 = 0; v0 < a.V; v0 += h.piece) {
             const int vc = std::min(h.piece, a.V - v0);
             const unsigned char *w = (const unsigned char *)a.w + (size_t)v0 * a.d * es;
@@ -1370,12 +1401,13 @@ hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *w
             p.v0 = v0;
             p.part = part;
             p.tlogit = tlogit;
-            HEAD_TRY(head_product<HEAD_LSE>(ctx, p, h.planes, s));
+            HEAD_TRY(head_product(ctx, HEAD_LSE, p, h.planes, s));
         }
     }
     int TL = 1;
     while (TL < 64 && TL < a.T) TL *= 2;
-    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(a.T, TL)), dim3(1024), 0, s, part, nb, tlogit, a.targets, h.few ? (const int32_t *)nullptr : (const int32_t *)(base + h.slot), a.T, a.V, TL, a.loss, a.row_stats, a.mean);
+    const int32_t *slot = h.few ? nullptr : (const int32_t *)(base + h.slot);
+    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(a.T, TL)), dim3(1024), 0, s, part, nb, tlogit, a.targets, slot, a.T, a.V, TL, a.loss, a.row_stats, a.mean);
     if (a.T > TL) hipLaunchKernelGGL(head_mean_kernel, dim3(1), dim3(1024), 0, s, a.loss, a.targets, a.T, a.V, a.mean);
     return hipGetLastError();
 }
@@ -1390,7 +1422,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     }
     const head_plan h = head_plan_of(ctx, a, true);
     unsigned char *base = (unsigned char *)ws;
-    head_tokens(a, h, base, h.Tp, a.row_stats, s);
+    head_tokens(ctx, a, h, base, h.Tp, a.row_stats, s);
     const int32_t *held = (const int32_t *)(base + h.held);
     for (int v0 = 0; v0 < a.V; v0 += h.piece) {
         const int vc = std::min(h.piece, a.V - v0), vp = (int)up_to(vc, 256);
@@ -1414,7 +1446,7 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
         p.v0 = v0;
         p.P = base + h.p_img;
         p.planeP = h.p_plane;
-        HEAD_TRY(head_product<HEAD_P>(ctx, p, h.planes, s));
+        HEAD_TRY(head_product(ctx, HEAD_P, p, h.planes, s));
         if (a.dx) {
             head_prod q = {};
             q.A = base + h.p_img;
@@ -1433,8 +1465,8 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.C = (float *)(base + h.slabs);
             q.slab = h.slab;
             q.ld = (int)up_to(h.dp, 256);
-            if (v0 == 0) HEAD_TRY(head_product<HEAD_ACC>(ctx, q, h.planes, s));
-            else HEAD_TRY(head_product<HEAD_ADD>(ctx, q, h.planes, s));
+            if (v0 == 0) HEAD_TRY(head_product(ctx, HEAD_ACC, q, h.planes, s));
+            else HEAD_TRY(head_product(ctx, HEAD_ADD, q, h.planes, s));
         }
         if (a.dw) {
             head_prod q = {};
@@ -1454,11 +1486,11 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
             q.mean = a.mean;
             q.dloss = a.dloss;
             q.out_vec = a.d % (bf ? 8 : 4) == 0 && (uintptr_t)q.out % 16 == 0;
-            HEAD_TRY(head_product<HEAD_OUT>(ctx, q, h.planes, s));
+            HEAD_TRY(head_product(ctx, HEAD_OUT, q, h.planes, s));
         }
     }
     if (a.dx) {
-        const int slices = std::max(1, std::min(h.slices, head_dx_steps(std::min(h.piece, a.V)) / 8));
+        const int slices = head_dx_slices(a, h);
         const dim3 grid(a.T, std::min(ceil_div(a.d, 1024), 1024));
         const int vec = a.d % 4 == 0 && (uintptr_t)a.dx % (bf ? 8 : 16) == 0;
         const auto k = bf ? head_dx_kernel<true> : head_dx_kernel<false>;
