@@ -642,10 +642,15 @@ __device__ __forceinline__ void hp_run_item(unsigned char *smem, hp_state &st, c
 template <int NU, int EPI, int NSEG>
 __device__ __forceinline__ void hp_run(unsigned char *smem, const head_prod &p, int wave)
 {
-    const int n_wg = gridDim.x;
-    const int at_wg = n_wg % 8 == 0 ? (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    // (fewer items than workgroups: as many of each XCD.  Were the first XCDs filled first, or neighbours dealt out over all of them, the
+    // operands would come through fewer L2s, or through each of them: fp32 400 x 1024, vocabulary 9000: 157 us instead of 88)
     const int total = p.mt * p.nt * p.slices;
-    int idx = at_wg;
+    const int n_wg = gridDim.x % 8 == 0 ? min((int)gridDim.x, (total + 7) & ~7) : (int)gridDim.x;
+    int idx = blockIdx.x;
+    if (gridDim.x % 8 == 0) {
+        if ((int)(blockIdx.x >> 3) >= n_wg >> 3) return;
+        idx = (blockIdx.x & 7) * (n_wg >> 3) + (blockIdx.x >> 3);
+    }
     if (idx >= total) return;
     hp_item it = hp_make_item<NU, EPI>(p, idx);
     hp_state st;
@@ -687,13 +692,15 @@ __device__ __forceinline__ void hp_run(unsigned char *smem, const head_prod &p, 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads behind the last item land in LDS that nobody reads)
 }
 
-// Height of a row tile, 64 times the result: the one that takes the least time by rounds of one tile per compute unit, a tile of n x 64 rows
-// counted as n + 1/2 (its columns' loads).
-__host__ __device__ static inline int head_rows(int M, int nt, int slices, int cus)
+// Height of a row tile, 64 times the result: the one that takes the least time by rounds of one tile per compute unit.  A step of a tile of
+// k x 64 rows takes k + 7/4 parts, of fp32's products k + 3/4 (its columns' loads count most where they are W's rows in place): measured
+// with all compute units at work, 512 x 4096, vocabulary 32000, bf16 0.39, 0.52, 0.62 and 0.82 us for k = 1 to 4, fp32 1500 x 1024, 32000
+// 0.27, 0.43, 0.61 and 0.73.
+__host__ __device__ static inline int head_rows(int M, int nt, int slices, int cus, int planes)
 {
     uint32_t n = 0, best = 0;
     for (uint32_t k = 4; k >= 1; --k) {
-        const uint32_t cost = (((uint32_t)M + 64 * k - 1) / (64 * k) * (uint32_t)(nt * slices) + (uint32_t)cus - 1) / (uint32_t)cus * (2 * k + 1);
+        const uint32_t cost = (((uint32_t)M + 64 * k - 1) / (64 * k) * (uint32_t)(nt * slices) + (uint32_t)cus - 1) / (uint32_t)cus * (4 * k + (planes == 1 ? 7 : 3));
         if (n == 0 || cost < best) n = k, best = cost;
     }
     return (int)n;
@@ -839,8 +846,8 @@ __global__ __launch_bounds__(256) void head_tokens_kernel(const void *__restrict
             }
             if (t == 0) {
                 held[0] = n;
-                held[1] = head_rows(n, nt_v, 1, cus);
-                held[2] = head_rows(n, nt_d, slices, cus);
+                held[1] = head_rows(n, nt_v, 1, cus, NP);
+                held[2] = head_rows(n, nt_d, slices, cus, NP);
             }
         }
     }
@@ -1291,11 +1298,11 @@ hipError_t head_init(void)
 static hipError_t head_product(const omega_ctx *ctx, int epi, head_prod p, int planes, hipStream_t s)
 {
     p.nt = ceil_div(p.N, HP_TILE);
-    const int rows = epi == HEAD_OUT ? head_rows(p.M, p.nt, p.slices, ctx->num_cus) : 1;  // (1: the lowest, which makes the most items)
+    const int rows = epi == HEAD_OUT ? head_rows(p.M, p.nt, p.slices, ctx->num_cus, planes) : 1;  // (1: the lowest, which makes the most items)
     p.mt = ceil_div(p.M, 64 * rows);
     const long long items = (long long)p.mt * p.nt * p.slices;
     if (items > 0x3fffffff) return hipErrorInvalidValue;
-    const int grid = (int)std::min<long long>(items, ctx->num_cus);
+    const int grid = (int)std::min<long long>(up_to(items, 8), ctx->num_cus);
     void *args[] = {&p};
     return hipLaunchKernel(head_kernel_of(epi, planes, rows), dim3(grid), dim3(256), args, HP_SMEM, s);
 }
