@@ -3,7 +3,7 @@
 // (Network.clipGradNorm, J/engine/nn/network/Network.java:379-432; vectorL2NormKernel, J/engine/gpu/GlobalNormKernel.cu:3-30, adds its
 // block sums with atomicAdd, here the order is fixed).  The tensors are cut into chunks; a workgroup takes a chunk, finds its tensor in
 // a table that travels with the launch's arguments, and leaves one double; one workgroup adds these and forms coef; a second pass over
-// the chunks scales.  Squares and sums are doubles: no sum overflows or loses the small gradients beside the large ones.
+// the chunks scales.  A thread adds up to 64 squares in fp32, all else is in double: no sum overflows or loses the small gradients beside the large.
 // Bound: bytes - every element is read twice and written once.
 #include <algorithm>
 

@@ -7,7 +7,7 @@ from tests.lm_util import DT, U16, U32, Buf, ctx, normal, rounded, unit, within
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1, 1), (1, 1000, 64), (2, 33, 7), (3, 257, 40), (16, 1000, 256), (16, 40000, 64), (17, 300, 256), (64, 512, 320), (65, 513, 333), (130, 700, 64),
-          (193, 769, 260), (257, 1025, 512), (300, 256, 1000), (450, 3, 72)]
+          (193, 769, 260), (257, 1025, 512), (300, 256, 1000), (450, 3, 72), (300, 9000, 256), (330, 7001, 130), (70, 2500, 2100), (129, 300, 1280)]
 
 
 def reference(x, w, y, dtype, dloss=1.0):
