@@ -56,9 +56,10 @@ public:
     }
     Tensor &forward(const Ids &ids)
     {
-        ids_ = &ids;
+        ids_ = nullptr;  // (until the call has succeeded)
         Tensor &out = detail::sized(out_, ids.n, d_, w_.ctx);
         check(w_.ctx->get(), omega_hip_embedding_forward(w_.ctx->get(), w_.gpuData, OMEGA_DTYPE_F32, V_, d_, ids.gpuData(), ids.n, scale_, out.gpuData));
+        ids_ = &ids;
         return out;
     }
     // gradient of the weight for the ids of the last forward: into the layer's own tensor, or added to `tied` (a head's gradient)
@@ -97,10 +98,11 @@ public:
     Tensor &forward(Tensor &x)
     {
         detail::rows_of(x, d_, "input shape");
-        x_ = &x;
+        x_ = nullptr;
         Tensor &out = detail::sized(out_, x.number, d_, gamma_.ctx), &st = detail::sized(stats_, 2, x.number, gamma_.ctx);  // mean, rstd
         check(gamma_.ctx->get(), omega_hip_layernorm_forward(gamma_.ctx->get(), x.gpuData, OMEGA_DTYPE_F32, x.number, d_, (const float *)gamma_.gpuData,
                                                              (const float *)beta_.gpuData, eps_, out.gpuData, (float *)st.gpuData, (float *)st.gpuData + x.number));
+        x_ = &x;
         return out;
     }
     Tensor &back(Tensor &delta)
@@ -137,11 +139,12 @@ public:
     {
         detail::rows_of(x, d_, "input shape");
         detail::want(targets.n == x.number, "targets are one a row");
-        x_ = &x;
-        y_ = &targets;
+        x_ = nullptr;
         Tensor &loss = detail::sized(loss_, 1, x.number, w_.ctx), &st = detail::sized(stats_, 2, x.number, w_.ctx), &mean = detail::sized(mean_, 1, 2, w_.ctx);
         check(w_.ctx->get(), omega_hip_head_loss_forward(w_.ctx->get(), x.gpuData, w_.gpuData, OMEGA_DTYPE_F32, x.number, V_, d_, targets.gpuData(), (float *)loss.gpuData,
                                                          (float *)st.gpuData, (float *)mean.gpuData));
+        x_ = &x;
+        y_ = &targets;
         return loss;
     }
     // gradients of the mean loss: the input's is returned, getDiffW() the weight's

@@ -40,6 +40,9 @@ class _Layer:
             if buf is not None:
                 buf.free()
         self._owned = {}
+        for view in (getattr(self, "diffGamma", None), getattr(self, "diffBeta", None)):
+            if view is not None:
+                view.free()   # (into a buffer that has gone)
         self.input = self.diffW = self.diffGamma = self.diffBeta = None
 
 
@@ -59,10 +62,11 @@ class EmbeddingLayer(_Layer):
     def forward(self, ids):
         _want(ids.dtype == "i32" and len(ids.shape) == 1, "ids are a vector of i32")
         _want(self.weight is not None, "the layer has no weight")
-        self.input, T = ids, ids.shape[0]
+        self.input, T = None, ids.shape[0]   # (until the call has succeeded)
         out = self._buffer("out", (T, self.embedDim), self.dtype)
         self.ctx.check(self.lib.omega_hip_embedding_forward(self.ctx.handle, self.weight.ptr, _DT[self.dtype], self.nVocab, self.embedDim, ids.ptr, T,
                                                             self.scale, out.ptr))
+        self.input = ids
         return out
 
     def back(self, delta, ids=None, diffW=None):
@@ -96,11 +100,12 @@ class LNLayer(_Layer):
     def forward(self, x):
         _want(len(x.shape) == 2 and x.shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
         _want(self.gamma is not None and self.beta is not None, "the layer has no gamma or beta")
-        self.input, T = x, x.shape[0]
+        self.input, T = None, x.shape[0]
         out = self._buffer("out", x.shape, self.dtype)
         stats = self._buffer("stats", (2, T), "f32")   # mean, then rstd
         self.ctx.check(self.lib.omega_hip_layernorm_forward(self.ctx.handle, x.ptr, _DT[self.dtype], T, self.embedDim, self.gamma.ptr, self.beta.ptr, self.eps,
                                                             out.ptr, stats.ptr, stats.ptr.value + 4 * T))
+        self.input = x
         return out
 
     def back(self, delta):
@@ -134,11 +139,12 @@ class HeadLossLayer(_Layer):
         _want(len(x.shape) == 2 and x.shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
         _want(targets.shape == (x.shape[0],) and targets.dtype == "i32", "targets are one i32 a row")
         _want(self.weight is not None, "the layer has no weight")
-        self.input, self.targets, T = x, targets, x.shape[0]
+        self.input, self.targets, T = None, targets, x.shape[0]
         loss, stats = self._buffer("loss", (T,), "f32"), self._buffer("stats", (2, T), "f32")
         self.mean = self._buffer("mean", (2,), "f32")
         self.ctx.check(self.lib.omega_hip_head_loss_forward(self.ctx.handle, x.ptr, self.weight.ptr, _DT[self.dtype], T, self.nVocab, self.embedDim, targets.ptr,
                                                             loss.ptr, stats.ptr, self.mean.ptr))
+        self.input = x
         return loss
 
     def back(self, dloss=None, input_gradient=True, weight_gradient=True):

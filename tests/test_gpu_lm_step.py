@@ -265,5 +265,18 @@ def test_layers_refuse():
         with pytest.raises(RuntimeError, match="Error code 1"):
             call()
     c.close()
+    c = P.GradClip(ctx, [m.ln.diffGamma, m.ln.diffBeta])
+    m.ln.close()
+    with pytest.raises(RuntimeError, match="Error code 1"):       # views into a buffer that has gone
+        c.clip(1.0)
+    c.close()
+    # a forward pass that is refused leaves nothing to go back from (its output lies over the table)
+    out = m.emb.forward(idb)
+    own, out.ptr = out.ptr, m.weight.ptr
+    with pytest.raises(RuntimeError, match="Error code 1"):
+        m.emb.forward(idb)
+    out.ptr = own
+    with pytest.raises(RuntimeError, match="without a forward"):
+        m.emb.back(x)
     m.close()
     ctx.close()
