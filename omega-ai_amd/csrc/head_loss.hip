@@ -1040,7 +1040,7 @@ __global__ __launch_bounds__(256) void head_stream_kernel(const unsigned char *_
 #pragma unroll
             for (int i = 0; i < 2 * TF; ++i) vx[i] -= back;
         }
-        hp_dma16_nt<0>(wb, vw[0], sb); hp_dma16_nt<1024>(wb, vw[1], sb); hp_dma16_nt<2048>(wb, vw[2], sb); hp_dma16_nt<3072>(wb, vw[3], sb);
+        hp_dma16_nt<0>(wb, vw[0], sb); hp_dma16_nt<1 * 1024>(wb, vw[1], sb); hp_dma16_nt<2 * 1024>(wb, vw[2], sb); hp_dma16_nt<3 * 1024>(wb, vw[3], sb);
         hp_dma16_nt<4096>(wb, vw[4], sb); hp_dma16_nt<5120>(wb, vw[5], sb); hp_dma16_nt<6144>(wb, vw[6], sb); hp_dma16_nt<7168>(wb, vw[7], sb);
         hp_dma16<8192>(xb, vx[0], sb); hp_dma16<9216>(xb, vx[1], sb);
         if constexpr (TF > 1) { hp_dma16<10240>(xb, vx[2], sb); hp_dma16<11264>(xb, vx[3], sb); }
