@@ -264,8 +264,8 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const void *__restr
     for (int p = __builtin_amdgcn_readlane(mine, 0); p < end;) {
         const int n = min(end - p, B1 - p % B1), tok = perm[p + min(lane, n - 1)], id = sid[p + min(lane, n - 1)];
         const int id0 = __builtin_amdgcn_readlane(id, 0);
-        if (n == B1 && id0 == __builtin_amdgcn_readlane(id, B1 - 1)) {
-            // a block of one id, and what follows it of the same
+        if (part1 != nullptr && n == B1 && id0 == __builtin_amdgcn_readlane(id, B1 - 1)) {
+            // a block of one id, and what follows it of the same (a batch of fewer than two blocks has no sums: its rows are added one by one)
             if (id0 != row) {
                 write();
                 row = id0;
