@@ -350,7 +350,7 @@ int omega_hip_head_loss_backward(omega_ctx *ctx, const void *x, const void *w, i
                                  void *dw);
 
 /* Clipping by the global norm over many tensors (Network.clipGradNorm, J/engine/nn/network/Network.java:379-432) without a copy
- * to the host: norm = sqrt(sum of squares of all elements) (sums in double, of up to 64 squares in fp32 where its range holds them), coef = min(1, max_norm / (norm + 1e-6)), and every
+ * to the host: norm = sqrt(sum of squares of all elements) (sums in double, of up to 33 squares in fp32 where its range holds them), coef = min(1, max_norm / (norm + 1e-6)), and every
  * tensor times coef, rounded once per element.  Tensor i: n elements of dtype from src to dst; dst = src (in place) or a buffer
  * that overlaps no other tensor.  The gradients of `layers` (the accumulators where accGrad has run, as omega_moe_scale_grad)
  * are clipped with them, in place; the layers must belong to ctx.  norm_out: two floats on the device, norm and coef; may
