@@ -337,7 +337,8 @@ int omega_hip_layernorm_backward(omega_ctx *ctx, const void *x, const void *dout
  *   row_stats [2,T] = maximum of a row's logits, then the sum of exp(logit - maximum): what the backward pass needs (of a token
  *   without a target: not to be relied on).
  * loss and mean are required, row_stats may be NULL where no backward pass follows.  All fp32.  Products of bf16 operands are
- * summed in fp32; products of fp32 operands are formed from three bf16 parts of each factor (24 bits).
+ * summed in fp32; products of fp32 operands are formed from three bf16 parts of each factor (24 bits; a factor below 2^-110 loses up to
+ * 2^-134, and the sums that an infinite one enters are no numbers, where for up to 128 tokens of a forward pass they are infinite).
  * FullyLayer.output + the softmax and log of J/engine/gpu/SoftmaxKernel.cu:4-24. */
 int omega_hip_head_loss_forward(omega_ctx *ctx, const void *x, const void *w, int dtype, int T, int V, int d,
                                 const int32_t *targets, float *loss, float *row_stats, float *mean);

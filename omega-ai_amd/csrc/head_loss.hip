@@ -12,8 +12,9 @@
 // product before writes, zero where k goes beyond the matrix; W itself is read in place where its rows are whole and aligned.  Where the
 // product sums over an operand's rows (W for dx, P and x for dW), the LDS reads transpose.  Tokens without a target are in no image: the
 // products' rows are the others, whose number is read on the device.
-// fp32 operands are split into three bf16 parts by truncation (8 + 8 + 8 bits: exact), an image each, and the product runs over
-// six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first); what is left out is below 2^-24 of a term.
+// fp32 operands are split into three bf16 parts, each the rounding of what those before it leave (24 bits: exact from 2^-110 on; a smaller
+// number loses up to 2^-134), an image each, and the product runs over six pairs of parts (hh, hm, mh, mm, hl, lh, the small ones first);
+// what is left out, ml, lm and ll, is at most 2^-24 of a term, of either sign (|m| <= 2^-8, |l| <= 2^-17 of the number).
 // Forward passes of up to 64 tokens (fp32: 128) stream W through a wave's LDS or registers (head_stream_kernel, head_few_kernel).
 // A small vocabulary's logits make too few tiles: they are formed in k slices, whose sums stay in memory until they are joined.
 // Bound: the matrix cores (2 T V d for the loss, 8 T V d with gradients, logits formed twice); few tokens: the bytes of W.
@@ -110,20 +111,16 @@ __device__ __forceinline__ uint32_t hp_pack2(float lo, float hi)
     return *(const uint32_t *)&r;
 }
 
-// part q (0 leading) of an fp32 number: 8 bits each, by truncation.  A number that is infinite or none has it all in the leading part.
-__device__ __forceinline__ void hp_split(float v, uint32_t (&h)[3])
+// Three bf16 parts of two fp32 numbers (w[0] the leading ones, a's in the low halves).  ANY: also numbers that would round to infinity, whose
+// leading part is cut instead; without, |a| and |b| are 1 at most.  What is no number, or infinite, has parts that are none.
+template <bool ANY>
+__device__ __forceinline__ void hp_split2(float a, float b, uint32_t (&w)[3])
 {
-    const uint32_t u = __float_as_uint(v);
-    h[0] = u >> 16;
-    h[1] = h[2] = 0;
-    if ((u & 0x7f800000u) == 0x7f800000u) {
-        if (u & 0xffffu) h[0] |= 0x40u;  // no number stays none
-        return;
-    }
-    const float r1 = v - __uint_as_float(u & 0xffff0000u);
-    const uint32_t u1 = __float_as_uint(r1);
-    h[1] = u1 >> 16;
-    h[2] = __float_as_uint(r1 - __uint_as_float(u1 & 0xffff0000u)) >> 16;
+    w[0] = hp_pack2(a, b);
+    if (ANY && fmaxf(fabsf(a), fabsf(b)) >= 0x1.ffp127f) w[0] = __float_as_uint(a) >> 16 | (__float_as_uint(b) & 0xffff0000u);
+    const float ra = a - __uint_as_float(w[0] << 16), rb = b - __uint_as_float(w[0] & 0xffff0000u);
+    w[1] = hp_pack2(ra, rb);
+    w[2] = hp_pack2(ra - __uint_as_float(w[1] << 16), rb - __uint_as_float(w[1] & 0xffff0000u));
 }
 
 // One tile of a product, or a k slice of one
@@ -489,11 +486,10 @@ __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it
             } else {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    uint32_t lo[3], hi[3];
-                    hp_split(v[4 * c + 2 * w], lo);
-                    hp_split(v[4 * c + 2 * w + 1], hi);
+                    uint32_t two[3];
+                    hp_split2<false>(v[4 * c + 2 * w], v[4 * c + 2 * w + 1], two);
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) h[q][w] = lo[q] | hi[q] << 16;
+                    for (int q = 0; q < NP; ++q) h[q][w] = two[q];
                 }
             }
 #pragma unroll
@@ -754,16 +750,16 @@ template <bool BF>
 __device__ __forceinline__ void head_chunk(const void *__restrict__ src, size_t row, int K, int c, int vec, uint4 (&part)[BF ? 1 : 3])
 {
     constexpr int NP = BF ? 1 : 3;
-    uint16_t e[NP][8];
+    uint32_t w[NP][4];
     const size_t at = row * K + c;
     if (BF) {
         const bf16_t *s = (const bf16_t *)src + at;
         if (vec) {
-            *(uint4 *)&e[0][0] = *(const uint4 *)s;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[0][k] = c + k < K ? s[k] : (bf16_t)0;
+            part[0] = *(const uint4 *)s;
+            return;
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[0][k] = (c + 2 * k < K ? (uint32_t)s[2 * k] : 0u) | (c + 2 * k + 1 < K ? (uint32_t)s[2 * k + 1] : 0u) << 16;
     } else {
         const float *s = (const float *)src + at;
         float v[8];
@@ -775,15 +771,15 @@ __device__ __forceinline__ void head_chunk(const void *__restrict__ src, size_t 
             for (int k = 0; k < 8; ++k) v[k] = c + k < K ? s[k] : 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            uint32_t h[3];
-            hp_split(v[k], h);
+        for (int k = 0; k < 4; ++k) {
+            uint32_t two[3];
+            hp_split2<true>(v[2 * k], v[2 * k + 1], two);
 #pragma unroll
-            for (int q = 0; q < NP; ++q) e[q][k] = (uint16_t)h[q];
+            for (int q = 0; q < NP; ++q) w[q][k] = two[q];
         }
     }
 #pragma unroll
-    for (int q = 0; q < NP; ++q) part[q] = *(const uint4 *)&e[q][0];
+    for (int q = 0; q < NP; ++q) part[q] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
 }
 
 // Rows 64 bx .., columns 64 by .. of W [R,K] as parts of a tile image (KTi k steps a row group), zero outside the matrix
@@ -1237,11 +1233,10 @@ __global__ __launch_bounds__(256) void head_slab_p_kernel(const float *__restric
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            uint32_t lo[3], hi[3];
-            hp_split(v[2 * k], lo);
-            hp_split(v[2 * k + 1], hi);
+            uint32_t two[3];
+            hp_split2<false>(v[2 * k], v[2 * k + 1], two);
 #pragma unroll
-            for (int q = 0; q < NP; ++q) w[q][k] = lo[q] | hi[q] << 16;
+            for (int q = 0; q < NP; ++q) w[q][k] = two[q];
         }
     }
 #pragma unroll
