@@ -17,6 +17,7 @@
 #define IDX_WAVES 16
 #define IDX_NOTES 1024    // tokens a wave of the index kernel can note
 #define EMB_BLOCK 64     // sorted places of a partial sum
+#define EMB_LAUNCH_ROWS (1 << 22)  // rows of a launch (whose lanes in x are counted in 32 bits), a multiple of EMB_ROWS
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 // four elements at the alignment of one
@@ -77,12 +78,12 @@ __device__ __forceinline__ void st4(void *p, size_t row, int d, const emb_cols &
         if (x.w + k >= x.c && x.w + k < d) st1<BF>(p, row * d + x.w + k, v[k]);
 }
 
-// ---- forward: a workgroup per 4 rows x 1024 columns, 4 columns a thread (any alignment of an element serves) ----
+// ---- forward: a workgroup per 4 rows x 1024 columns, 4 columns a thread (any alignment of an element serves), rows `first` .. T - 1 ----
 template <bool BF, bool TINY>
-__global__ __launch_bounds__(256) void embedding_forward_kernel(const void *__restrict__ table, int V, int d, const int32_t *__restrict__ ids, int T,
+__global__ __launch_bounds__(256) void embedding_forward_kernel(const void *__restrict__ table, int V, int d, const int32_t *__restrict__ ids, int first, int T,
                                                                 float scale, void *__restrict__ out)
 {
-    const int t0 = blockIdx.x * 4;
+    const int t0 = first + blockIdx.x * 4;
     int id[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) id[r] = t0 + r < T ? ids[t0 + r] : -1;
@@ -102,11 +103,14 @@ __global__ __launch_bounds__(256) void embedding_forward_kernel(const void *__re
 
 hipError_t launch_embedding_forward(const void *table, int dtype, int V, int d, const int32_t *ids, int T, float scale, void *out, hipStream_t s)
 {
-    const dim3 grid(ceil_div(T, 4), std::min(ceil_div(d, 1024), 64));
-#define EMB_FWD(B, TY) hipLaunchKernelGGL((embedding_forward_kernel<B, TY>), grid, dim3(256), 0, s, table, V, d, ids, T, scale, out)
-    if (dtype == OMEGA_DTYPE_BF16) { if (d < 4) EMB_FWD(true, true); else EMB_FWD(true, false); }
-    else { if (d < 4) EMB_FWD(false, true); else EMB_FWD(false, false); }
+    for (int first = 0; first < T; first += EMB_LAUNCH_ROWS) {
+        const int end = std::min(T, first + EMB_LAUNCH_ROWS);
+        const dim3 grid(ceil_div(end - first, 4), std::min(ceil_div(d, 1024), 64));
+#define EMB_FWD(B, TY) hipLaunchKernelGGL((embedding_forward_kernel<B, TY>), grid, dim3(256), 0, s, table, V, d, ids, first, end, scale, out)
+        if (dtype == OMEGA_DTYPE_BF16) { if (d < 4) EMB_FWD(true, true); else EMB_FWD(true, false); }
+        else { if (d < 4) EMB_FWD(false, true); else EMB_FWD(false, false); }
 #undef EMB_FWD
+    }
     return hipGetLastError();
 }
 
@@ -232,18 +236,18 @@ __global__ __launch_bounds__(64) void embedding_block_kernel(const void *__restr
     if (x.c < d) st4<false>(part, b, d, x, a);
 }
 
-// The rows of the table, EMB_ROWS a workgroup: first those without a token (most of them: zeros go out without waiting for anything),
+// Rows `first` .. V - 1 of the table, EMB_ROWS a workgroup: first those without a token (most of them: zeros go out without waiting for anything),
 // then the others, each the sum of its run of sorted places.  The places of all rows are walked as one list, 64 to an aligned block and
 // eight rows of dout asked for together, so that short runs do not wait one after the other; blocks that a long run fills are
 // taken from their sums.  NT: a gradient larger than the caches goes past them (16384 tokens x 2048, vocabulary 128000, 1.05 GB: 266 -> 224 us).
 #define EMB_ROWS 16
 template <bool BF, bool GBF, bool TINY, bool NT>
-__global__ __launch_bounds__(256) void embedding_rows_kernel(const void *__restrict__ dout, int V, int d, float scale, int accumulate,
+__global__ __launch_bounds__(256) void embedding_rows_kernel(const void *__restrict__ dout, int first, int V, int d, float scale, int accumulate,
                                                              const int32_t *__restrict__ off, const int32_t *__restrict__ perm, const int32_t *__restrict__ sid,
                                                              const float *__restrict__ part1, const float *__restrict__ part2, void *__restrict__ dtable)
 {
     constexpr int B1 = EMB_BLOCK, B2 = EMB_BLOCK * EMB_BLOCK;
-    const int v0 = blockIdx.x * EMB_ROWS, lane = threadIdx.x & 63, rows = min(EMB_ROWS, V - v0);
+    const int v0 = first + blockIdx.x * EMB_ROWS, lane = threadIdx.x & 63, rows = min(EMB_ROWS, V - v0);
     const emb_cols x((blockIdx.y * 256 + threadIdx.x) * 4, d);
     const int mine = off[v0 + min(lane, rows)];  // lane r: where row r's run begins
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -346,20 +350,23 @@ hipError_t launch_embedding_backward(const int32_t *ids, int T, const void *dout
         if (l.n2 > 0) hipLaunchKernelGGL((embedding_block_kernel<B, TY, 2>), dim3(l.n2, gy), dim3(64), 0, s, (const void *)part1, d, V, off, perm, sid, part2); \
     } while (0)
 #define EMB_ROWS_N(B, G, TY, NT) \
-    hipLaunchKernelGGL((embedding_rows_kernel<B, G, TY, NT>), grid, dim3(256), 0, s, dout, V, d, scale, accumulate ? 1 : 0, off, perm, sid, part1, part2, dtable)
+    hipLaunchKernelGGL((embedding_rows_kernel<B, G, TY, NT>), grid, dim3(256), 0, s, dout, first, end, d, scale, accumulate ? 1 : 0, off, perm, sid, part1, part2, dtable)
 #define EMB_ROWS_K(B, G, TY) do { if (past) EMB_ROWS_N(B, G, TY, true); else EMB_ROWS_N(B, G, TY, false); } while (0)
 #define EMB_RUN(TY)                                                                       \
     do {                                                                                  \
-        if (bf) EMB_BLOCKS(true, TY);                                                     \
-        else EMB_BLOCKS(false, TY);                                                       \
         if (bf) { if (gbf) EMB_ROWS_K(true, true, TY); else EMB_ROWS_K(true, false, TY); } \
         else { if (gbf) EMB_ROWS_K(false, true, TY); else EMB_ROWS_K(false, false, TY); }  \
     } while (0)
-    const dim3 grid(ceil_div(V, EMB_ROWS), ceil_div(d, 1024));
+    if (bf) { if (d < 4) EMB_BLOCKS(true, true); else EMB_BLOCKS(true, false); }
+    else { if (d < 4) EMB_BLOCKS(false, true); else EMB_BLOCKS(false, false); }
     // (67 MB stay in the caches: 33 us, 35 past them; 131 MB: 91 and 70)
     const bool past = !accumulate && (size_t)V * d * (gbf ? 2 : 4) >= OMEGA_LLC_BYTES / 8 * 3;
-    if (d < 4) EMB_RUN(true);
-    else EMB_RUN(false);
+    for (int first = 0; first < V; first += EMB_LAUNCH_ROWS) {
+        const int end = std::min(V, first + EMB_LAUNCH_ROWS);
+        const dim3 grid(ceil_div(end - first, EMB_ROWS), ceil_div(d, 1024));
+        if (d < 4) EMB_RUN(true);
+        else EMB_RUN(false);
+    }
 #undef EMB_RUN
 #undef EMB_ROWS_K
 #undef EMB_ROWS_N

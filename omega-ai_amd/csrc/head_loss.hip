@@ -1243,13 +1243,13 @@ __global__ __launch_bounds__(256) void head_slab_p_kernel(const float *__restric
     for (int q = 0; q < NP; ++q) *(uint4 *)(P + q * plane + pk_chunk_off(row, c >> 5, (c & 31) >> 3, KTp)) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
 }
 
-// dx: the slabs added in slice order, rounded once; rows without a target are zero
+// dx: the slabs added in slice order, rounded once; rows without a target are zero.  Rows from `first` on
 template <bool BF>
-__global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ slot, int d,
-                                                      int vec, const float *__restrict__ mean, const float *dloss, void *__restrict__ dx)
+__global__ __launch_bounds__(256) void head_dx_kernel(const float *__restrict__ slabs, int slices, size_t slab, int ld, const int32_t *__restrict__ slot, int first,
+                                                      int d, int vec, const float *__restrict__ mean, const float *dloss, void *__restrict__ dx)
 {
     const float g = head_scale(mean, dloss);
-    const int t = blockIdx.x, at = slot[t];
+    const int t = first + blockIdx.x, at = slot[t];
     for (int c = 4 * (blockIdx.y * 256 + threadIdx.x); c < d; c += 4 * gridDim.y * 256) {
         f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
         if (at >= 0) {
@@ -1278,6 +1278,7 @@ __global__ __launch_bounds__(256) void head_zero_kernel(void *p, size_t bytes)  
 
 // ---- host side ----
 static size_t up_to(size_t x, size_t m) { return (x + m - 1) / m * m; }
+#define HEAD_DX_ROWS (1 << 18)  // rows of a launch of head_dx_kernel (lanes in x are counted in 32 bits)
 static int k_pad(int n) { return std::max(256, (int)up_to(n, 64)); }  // k of a product: whole pairs of steps, eight steps or more
 
 // Sizes of a call and where its parts lie in the workspace
@@ -1294,7 +1295,7 @@ static head_plan head_plan_of(const omega_ctx *ctx, const head_args &a, bool bac
 {
     head_plan h = {};
     h.planes = a.dtype == OMEGA_DTYPE_BF16 ? 1 : 3;
-    h.few = !backward && a.T <= HEAD_FEW(a.dtype);
+    h.few = !backward && a.T <= HEAD_FEW(a.dtype) && a.V <= 1 << 29;  // (256 lanes for 64 rows of W: counted in 32 bits)
     h.dp = k_pad(a.d);
     h.Tp = k_pad(a.T);
     // W in place: bf16 rows of whole pairs of k steps, 16-byte aligned (tile offsets within 32 bits)
@@ -1617,10 +1618,13 @@ hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *
     }
     if (a.dx) {
         const int slices = head_dx_slices(a, h);
-        const dim3 grid(a.T, std::min(ceil_div(a.d, 1024), 1024));
         const int vec = a.d % 4 == 0 && (uintptr_t)a.dx % (bf ? 8 : 16) == 0;
         const auto k = bf ? head_dx_kernel<true> : head_dx_kernel<false>;
-        hipLaunchKernelGGL(k, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), (const int32_t *)(base + h.slot), a.d, vec, a.mean, a.dloss, a.dx);
+        for (int first = 0; first < a.T; first += HEAD_DX_ROWS) {
+            const dim3 grid(std::min(a.T - first, HEAD_DX_ROWS), std::min(ceil_div(a.d, 1024), 1024));
+            hipLaunchKernelGGL(k, grid, dim3(256), 0, s, (const float *)(base + h.slabs), slices, h.slab, (int)up_to(h.dp, 256), (const int32_t *)(base + h.slot), first, a.d, vec,
+                               a.mean, a.dloss, a.dx);
+        }
     }
     return hipGetLastError();
 }

@@ -9,7 +9,7 @@
 
 static bool dtype_ok(int dt) { return dt == OMEGA_DTYPE_F32 || dt == OMEGA_DTYPE_BF16; }
 static size_t dtype_size(int dt) { return dt == OMEGA_DTYPE_BF16 ? 2 : 4; }
-#define SIZE_MAX_ROWS (1 << 30)  // sums of sizes stay within 32 bits, grids within theirs
+#define SIZE_MAX_ROWS (1 << 30)  // sums of sizes stay within 32 bits; launches whose lanes would not are cut by the launchers
 #define SIZE_MAX_COLS (1 << 20)
 static bool sizes_ok(int T, int V, int d) { return T >= 0 && V >= 1 && d >= 1 && T <= SIZE_MAX_ROWS && V <= SIZE_MAX_ROWS && d <= SIZE_MAX_COLS; }
 
