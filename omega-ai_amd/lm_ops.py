@@ -18,6 +18,26 @@ def _want(cond, what):
         raise RuntimeError("Error code 1:" + what)
 
 
+class _Param:
+    """A parameter of a layer, a buffer of the caller: looked at whenever it is set, since the kernels read it with the layer's sizes.  (One
+    that is freed later has no address, which the calls refuse.)"""
+
+    def __init__(self, shape, dtype):
+        self.shape, self.dtype = shape, dtype   # functions of the layer
+
+    def __set_name__(self, owner, name):
+        self.name = name
+
+    def __get__(self, layer, owner=None):
+        return self if layer is None else layer.__dict__.get(self.name)
+
+    def __set__(self, layer, buf):
+        if buf is not None:
+            _want(buf.shape == self.shape(layer) and buf.dtype == self.dtype(layer), self.name + " shape or dtype")
+            _want(buf.ptr, self.name + " has been freed")
+        layer.__dict__[self.name] = buf
+
+
 class _Layer:
     """Buffers of a layer: made when a batch of another size comes (Layer.init), given back by close()."""
 
@@ -50,13 +70,13 @@ class EmbeddingLayer(_Layer):
     """out[t] = scale * weight[ids[t]] (an id outside 0..nVocab-1: zeros) and its gradient by sorted tokens
     (EmbeddingFW / EmbeddingGrad, J/engine/nn/layer/gpu/EmbeddingKernel.cu:13-56)."""
 
+    weight = _Param(lambda layer: (layer.nVocab, layer.embedDim), lambda layer: layer.dtype)
+
     def __init__(self, nVocab, embedDim, scale=1.0, ctx=None, dtype="f32", weight=None, gradDtype="f32"):
         super().__init__(ctx, dtype)
         _want(gradDtype in _DT, "gradDtype is f32 or bf16")
         self.nVocab, self.embedDim, self.scale, self.gradDtype = nVocab, embedDim, float(scale), gradDtype
         self.weight = weight
-        if weight is not None:
-            _want(weight.shape == (nVocab, embedDim) and weight.dtype == dtype, "weight shape or dtype")
         self.input = self.diffW = None
 
     def forward(self, ids):
@@ -90,11 +110,13 @@ class EmbeddingLayer(_Layer):
 class LNLayer(_Layer):
     """Layer norm over the last dimension (J/engine/nn/layer/normalization): gamma and beta fp32, as the RMSNorm's gamma of the MoE layer."""
 
+    gamma = _Param(lambda layer: (layer.embedDim,), lambda layer: "f32")
+    beta = _Param(lambda layer: (layer.embedDim,), lambda layer: "f32")
+
     def __init__(self, embedDim, eps=1e-5, ctx=None, dtype="f32", gamma=None, beta=None):
         super().__init__(ctx, dtype)
-        self.embedDim, self.eps, self.gamma, self.beta = embedDim, float(eps), gamma, beta
-        for p in (gamma, beta):
-            _want(p is None or (p.shape == (embedDim,) and p.dtype == "f32"), "gamma and beta are vectors of embedDim f32")
+        self.embedDim, self.eps = embedDim, float(eps)
+        self.gamma, self.beta = gamma, beta
         self.input = self.diffGamma = self.diffBeta = None
 
     def forward(self, x):
@@ -127,11 +149,12 @@ class HeadLossLayer(_Layer):
     """logits = x weight^T, softmax cross entropy against targets and its gradients, in pieces of the vocabulary: no logits are kept
     (FullyLayer.output and the softmax of J/engine/gpu/SoftmaxKernel.cu:4-24 in one)."""
 
+    weight = _Param(lambda layer: (layer.nVocab, layer.embedDim), lambda layer: layer.dtype)
+
     def __init__(self, nVocab, embedDim, ctx=None, dtype="f32", weight=None):
         super().__init__(ctx, dtype)
-        self.nVocab, self.embedDim, self.weight = nVocab, embedDim, weight
-        if weight is not None:
-            _want(weight.shape == (nVocab, embedDim) and weight.dtype == dtype, "weight shape or dtype")
+        self.nVocab, self.embedDim = nVocab, embedDim
+        self.weight = weight
         self.input = self.targets = self.mean = self.diffW = None
 
     def forward(self, x, targets):
