@@ -175,7 +175,7 @@ class HeadLossLayer(_Layer):
         weight's (both of the layer's dtype)."""
         x = self.input
         _want(x is not None, "back without a forward")
-        _want(dloss is None or (dloss.shape == (1,) and dloss.dtype == "f32"), "dloss is one f32")
+        _want(dloss is None or (dloss.shape == (1,) and dloss.dtype == "f32" and dloss.ptr), "dloss is one f32")   # (no address would mean 1)
         dx = self._buffer("diff", x.shape, self.dtype) if input_gradient else None
         self.diffW = self._buffer("diffW", (self.nVocab, self.embedDim), self.dtype) if weight_gradient else None
         self.ctx.check(self.lib.omega_hip_head_loss_backward(self.ctx.handle, x.ptr, self.weight.ptr, _DT[self.dtype], x.shape[0], self.nVocab, self.embedDim,

@@ -77,3 +77,17 @@ def test_parameters_that_are_set_later(ctx):
         b.free()
     for layer in (emb, head, ln):
         layer.close()
+
+
+def test_a_freed_factor_of_the_loss(ctx):
+    """No address stands for a factor of 1: a buffer that has been freed has none either."""
+    x, y, w, factor = buf(ctx, T, D), buf(ctx, T, dtype="i32"), buf(ctx, V, D), buf(ctx, 1)
+    head = P.HeadLossLayer(V, D, ctx=ctx, weight=w)
+    head.forward(x, y)
+    head.back(factor)
+    head.back()
+    factor.free()
+    refused(ctx, lambda: head.back(factor), "dloss")
+    head.close()
+    for b in (x, y, w):
+        b.free()
