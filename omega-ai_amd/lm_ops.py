@@ -203,6 +203,7 @@ class GradClip:
     def clip(self, maxNorm):
         """Scales by min(1, maxNorm / (norm + 1e-6)); returns the buffer of norm and coefficient."""
         tensors, out, layers = self._kept
+        _want(self.norm.ptr, "the clip has been closed")
         _want(all(b.ptr for b in tensors) and all(b.ptr for b in out), "a gradient buffer has been freed")
         for i, layer in enumerate(layers):
             self._layers[i] = layer.handle   # (None once it is closed: refused)

@@ -91,3 +91,13 @@ def test_a_freed_factor_of_the_loss(ctx):
     head.close()
     for b in (x, y, w):
         b.free()
+
+
+def test_a_closed_clip(ctx):
+    """It has no norm to return: nothing is scaled either."""
+    g = buf(ctx, 100)
+    clip = P.GradClip(ctx, [g])
+    clip.clip(1.0)
+    clip.close()
+    refused(ctx, lambda: clip.clip(1.0), "closed")
+    g.free()
