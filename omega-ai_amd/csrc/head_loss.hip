@@ -432,6 +432,10 @@ __device__ __forceinline__ void hp_write_lse(const head_prod &p, const hp_item &
         if (lq == 0 && t < p.M) part[t] = make_float2(m[iu], s[iu]);
     }
 }
+// P of a bf16 head is rounded to bf16, an element by 2^-8 of itself at most, as x and W were when they became bf16, and each for itself: dx
+// and dw, which have 0.0017 (2-norm, against 64 bits) from their own rounding, have 0.0019 with it (4096 tokens x 4096, vocabulary 128000;
+// rows of dw without a target 0.0022).  A second part of P would take away the 0.0009 between these (in squares), for two more
+// products of 3 ms each on top of 12, and another piece of P.  fp32 heads carry all of P in three parts.
 template <int NU, int NSEG, bool WHOLE>
 __device__ __forceinline__ void hp_write_p(const head_prod &p, const hp_item &it, const f32x4_t (&acc)[NU][8], int wm, int wn, int l16, int lq)
 {
@@ -1037,10 +1041,10 @@ __global__ __launch_bounds__(256) void head_stream_kernel(const unsigned char *_
             for (int i = 0; i < 2 * TF; ++i) vx[i] -= back;
         }
         hp_dma16_nt<0>(wb, vw[0], sb); hp_dma16_nt<1 * 1024>(wb, vw[1], sb); hp_dma16_nt<2 * 1024>(wb, vw[2], sb); hp_dma16_nt<3 * 1024>(wb, vw[3], sb);
-        hp_dma16_nt<4096>(wb, vw[4], sb); hp_dma16_nt<5120>(wb, vw[5], sb); hp_dma16_nt<6144>(wb, vw[6], sb); hp_dma16_nt<7168>(wb, vw[7], sb);
-        hp_dma16<8192>(xb, vx[0], sb); hp_dma16<9216>(xb, vx[1], sb);
-        if constexpr (TF > 1) { hp_dma16<10240>(xb, vx[2], sb); hp_dma16<11264>(xb, vx[3], sb); }
-        if constexpr (TF > 2) { hp_dma16<12288>(xb, vx[4], sb); hp_dma16<13312>(xb, vx[5], sb); hp_dma16<14336>(xb, vx[6], sb); hp_dma16<15360>(xb, vx[7], sb); }
+        hp_dma16_nt<4 * 1024>(wb, vw[4], sb); hp_dma16_nt<5 * 1024>(wb, vw[5], sb); hp_dma16_nt<6 * 1024>(wb, vw[6], sb); hp_dma16_nt<7 * 1024>(wb, vw[7], sb);
+        hp_dma16<8 * 1024>(xb, vx[0], sb); hp_dma16<9 * 1024>(xb, vx[1], sb);
+        if constexpr (TF > 1) { hp_dma16<10 * 1024>(xb, vx[2], sb); hp_dma16<11 * 1024>(xb, vx[3], sb); }
+        if constexpr (TF > 2) { hp_dma16<12 * 1024>(xb, vx[4], sb); hp_dma16<13 * 1024>(xb, vx[5], sb); hp_dma16<14 * 1024>(xb, vx[6], sb); hp_dma16<15 * 1024>(xb, vx[7], sb); }
         wb += 128;
         xb += 128;
     };
