@@ -13,7 +13,7 @@
 // partial sums meet in LDS, added in wave order.  Rows come from x through the row -> token table, or from the packed copy.
 // Forward pass, us, tile kernels -> here: 1 / 16 / 64 tokens, d = 4096, H = 14336, 8 experts, top 2: 144 -> 132, 482 -> 452, 470 -> 458
 // (up product 6.6 TB/s of weights, 6.4 at 64 tokens); 16 / 48 tokens, d = 2048, H = 1408, 64 experts, top 6, 2 shared: 193 -> 163,
-// 226 -> 209; 2 tokens, d = 3072, H = 768, 4 experts, 2 shared: 86 -> 48; 4 tokens, d = 1024, H = 1024, 64 experts, top 4: 53 -> 37.
+// 226 -> 209; 4 tokens, d = 1024, H = 1024, 64 experts, top 4: 53 -> 37.
 #include "index_small.h"
 #include "pack.h"
 #include <algorithm>

@@ -639,7 +639,7 @@ __global__ __launch_bounds__(64 * NW) void router_units_kernel(const bf16_t *__r
 // SPLIT (more than 16 experts): `groups` workgroups per token tile take 16 experts each and leave the logits in logits_out, for
 // router_select_kernel: where those find a compute unit each, a chain of the vector units' and a launch more are shorter than one
 // of the matrix cores' in a workgroup that fetches the whole gate.  Router, us, matrix cores -> here: 1 token x 3328, 86 experts
-// 38.6 -> 19.5; 2 x 3072, 26 experts 22.2 -> 16.3; 48 x 2048, 64 experts 18.2 -> 15.7; 109 x 3328, 83 experts 39 -> 21.5; 500 x 2048, 128 experts 27.7 ->
+// 38.6 -> 19.5; 48 x 2048, 64 experts 18.2 -> 15.7; 109 x 3328, 83 experts 39 -> 21.5; 500 x 2048, 128 experts 27.7 ->
 // 21.0; 1 x 2048, 250 experts 44 -> 17.7.
 #define RP_STAGERS 128
 template <int EP, bool SPLIT>
