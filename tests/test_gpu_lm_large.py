@@ -215,3 +215,26 @@ def test_few_tokens_and_more_rows_than_a_launch_streams(ctx):
     head.close()
     for b in (w.buf, xb, yb):
         b.free()
+
+
+def test_clip_of_a_tensor_that_takes_several_launches(ctx):
+    """A tensor of 2^33 elements and more, whose chunks (2^20 a launch) are in two tables, and one behind it: zeros but for a few elements."""
+    d = 4096
+    n = (1 << 33) // d + 3
+    g, h = Big(ctx, n, d, "bf16", 0.0), Big(ctx, 2, d, "bf16", 0.0)
+    at = [0, 1, (1 << 31) // d, (1 << 32) // d - 1, (1 << 32) // d, n - 5, n - 4, n - 3, n - 2, n - 1]
+    for k, r in enumerate(at):
+        g.put(r, np.full(d, k + 1.0))
+    h.put(1, np.full(d, 16.0))
+    clip = P.GradClip(ctx, [g.buf, h.buf])
+    norm = np.sqrt(d * (sum((k + 1.0) ** 2 for k in range(len(at))) + 256.0))
+    got = clip.clip(0.5 * norm).to_numpy()
+    coef = float(np.float32(0.5 * norm)) / (norm + 1e-6)
+    assert abs(got[0] - norm) <= 2 * U32 * norm and abs(got[1] - coef) <= 2 * U32 * coef
+    for k, r in enumerate(at):
+        within(g.get(r)[0], np.full(d, (k + 1.0) * coef), (3 * U32 + U16) * (k + 1.0) * coef, r)
+    within(h.get(1)[0], np.full(d, 16.0 * coef), (3 * U32 + U16) * 16.0 * coef)
+    assert not g.get(2)[0].any() and not g.get(n - 6)[0].any() and not h.get(0)[0].any()
+    clip.close()
+    g.buf.free()
+    h.buf.free()
