@@ -367,6 +367,39 @@ typedef struct {
 int omega_hip_clip_grad_norm(omega_ctx *ctx, const omega_grad_tensor *tensors, int n_tensors, omega_moe *const *layers,
                              int n_layers, float max_norm, float *norm_out);
 
+/* ---- Operators around the experts of a block, on caller-owned buffers under the same terms ---- */
+
+/* RMS norm with the addition of a residual in front of it: h = x + residual rounded once to dtype (residual NULL: h = x),
+ * q = 1 / sqrt(mean(h^2) + eps), y = h q gamma.  x, residual, sum, out [T,d] of dtype, gamma [d] fp32.  Written, each may be NULL:
+ *   sum        h, what the next residual addition takes (only with a residual; may be x or residual itself);
+ *   out        y in dtype;
+ *   out8, out8_scales   y in 8 bits, the form OMEGA_KEEP8_MX (both or neither);
+ *   keep8, keep8_scales h in 8 bits, the form OMEGA_KEEP8_INT8, for the backward pass (both or neither);
+ *   rstd       q [T], what the backward pass needs.
+ * out or out8 must be there.  The addition and RMSLayer of LlamaTransformerBlock (J/engine/nn/layer/llama/LlamaTransformerBlock.java:129-136,
+ * rmsnorm_forward_kernel2, J/engine/nn/layer/normalization/gpu/RMSKernel.cu:185-223) in one pass; the sum of squares is formed in double. */
+int omega_hip_rmsnorm_forward(omega_ctx *ctx, const void *x, const void *residual, int dtype, int T, int d, const float *gamma, float eps,
+                              void *sum, void *out, uint8_t *out8, uint8_t *out8_scales, uint8_t *keep8, float *keep8_scales, float *rstd);
+/* Backward: dx [T,d] = gradient of h (of x and of the residual alike) = q (g - xh mean(g xh)) + dsum with g = dout gamma, xh = h q;
+ * dgamma [d] = sum over the rows of dout xh (fp32, overwritten, summed in a fixed order).  h as rows (h: x, or sum) or as the 8-bit copy of the
+ * forward pass (keep8, keep8_scales), not both; dsum [T,d] (NULL: none) is the gradient that reaches h past the norm, dx may be dsum
+ * itself.  rmsnorm_backward_kernel2, J/engine/nn/layer/normalization/gpu/RMSKernel.cu:226-277. */
+int omega_hip_rmsnorm_backward(omega_ctx *ctx, const void *h, const uint8_t *keep8, const float *keep8_scales, const void *dout, const void *dsum,
+                               int dtype, int T, int d, const float *gamma, const float *rstd, void *dx, float *dgamma);
+
+/* Rows kept in 8 bits, and brought back.  codes [T,d]; a scale for every group of a row (its last one may be shorter):
+ *   OMEGA_KEEP8_INT8  groups of 128, scales [T,ceil(d/128)] float: s = max(largest magnitude / 127, 2^-126), code = x / s rounded to the nearest
+ *                     whole number (halves to even), value = code s;
+ *   OMEGA_KEEP8_MX    groups of 32, scales [T,ceil(d/32)] bytes k + 127: s = 2^k is the smallest (k >= -127) with largest magnitude <= 448 s,
+ *                     code = x / s in e4m3 (1 sign, 4 exponent, 3 mantissa bits, nearest even), value = code s: the block format of
+ *                     the matrix cores' scaled products.
+ * A group with an infinity or no number in it comes back as no numbers (scale: no number; byte 255).  The reference keeps activations
+ * whole (Layer.output). */
+#define OMEGA_KEEP8_INT8 0
+#define OMEGA_KEEP8_MX 1
+int omega_hip_keep8_save(omega_ctx *ctx, const void *x, int dtype, int T, int d, int form, uint8_t *codes, void *scales);
+int omega_hip_keep8_load(omega_ctx *ctx, const uint8_t *codes, const void *scales, int form, int T, int d, void *out, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

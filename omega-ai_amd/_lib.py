@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libomega_hip.so")
 OK, ERR_INVALID_ARG, ERR_OOM, ERR_HIP, ERR_UNSUPPORTED = range(5)
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ROUTER_EXACT, ROUTER_FAST = 0, 1
+KEEP8_INT8, KEEP8_MX = 0, 1
 W_GATE, W_GATE_BIAS, W_W1, W_W3, W_W2, W_NORM = range(6)
 (STAGE_ROUTER, STAGE_DISPATCH, STAGE_UP, STAGE_DOWN, STAGE_COMBINE, STAGE_FORWARD, STAGE_INDEX, STAGE_GATHER,
  STAGE_FORWARD_BLOCK, STAGE_RMS) = range(10)
@@ -90,6 +91,10 @@ SIGNATURES = {
     "omega_hip_head_loss_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 4),
     "omega_hip_head_loss_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 6),
     "omega_hip_clip_grad_norm": (C.c_int, [C.c_void_p, C.POINTER(GradTensorStruct), C.c_int, C.POINTER(C.c_void_p), C.c_int, C.c_float, C.c_void_p]),
+    "omega_hip_rmsnorm_forward": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_void_p, C.c_float] + [C.c_void_p] * 7),
+    "omega_hip_rmsnorm_backward": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_void_p] * 4),
+    "omega_hip_keep8_save": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
+    "omega_hip_keep8_load": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int]),
 }
 
 _lib = None

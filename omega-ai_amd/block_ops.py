@@ -1,0 +1,123 @@
+"""What stands around the experts of a transformer block, over the C ABI: RMS norm with the residual's addition, rows kept in 8 bits.
+
+Classes in the manner of lm_ops.py: forward(input) returns the layer's own output buffer, back(delta) the input gradient, parameter
+gradients lie beside the parameters.
+"""
+from . import _lib as L
+from .lm_ops import _DT, _Layer, _Param, _want
+from .moe_layer import DeviceBuffer
+
+_FORMS = {"int8": L.KEEP8_INT8, "mx": L.KEEP8_MX}
+_GROUP = {"int8": 128, "mx": 32}
+
+
+class Rows8:
+    """Rows held in 8 bits: codes [T,d] and a scale for every group of a row (form "int8": of 128 elements, fp32; "mx": of 32, a byte)."""
+
+    def __init__(self, form, shape, codes, scales):
+        self.form, self.shape, self.codes, self.scales = form, shape, codes, scales
+
+
+def _rows8(layer, name, form, shape):
+    """The layer's own buffers of that name for rows of `shape`."""
+    codes = layer._buffer(name, shape, "u8")
+    scales = layer._buffer(name + "_scales", (shape[0], -(-shape[1] // _GROUP[form])), "f32" if form == "int8" else "u8")
+    return Rows8(form, shape, codes, scales)
+
+
+def _load8(layer, name, rows, dtype):
+    """`rows` as elements of dtype, in the layer's own buffer of that name."""
+    out = layer._buffer(name, rows.shape, dtype)
+    layer.ctx.check(layer.lib.omega_hip_keep8_load(layer.ctx.handle, rows.codes.ptr, rows.scales.ptr, _FORMS[rows.form], rows.shape[0], rows.shape[1], out.ptr,
+                                                   _DT[dtype]))
+    return out
+
+
+class RMSLayer(_Layer):
+    """RMS norm over the last dimension (RMSLayer, J/engine/nn/layer/normalization/RMSLayer.java), with the addition in front of it
+    (LlamaTransformerBlock.output, J/engine/nn/layer/llama/LlamaTransformerBlock.java:129-136): sum = x + residual, out = norm(sum).
+
+    out8: the output is Rows8 of the form "mx" (read8 brings them back); keep8: the forward pass keeps what was normed in 8 bits and the
+    backward pass reads those, so that neither x nor sum has to stay."""
+
+    gamma = _Param(lambda layer: (layer.embedDim,), lambda layer: "f32")
+
+    def __init__(self, embedDim, eps=1e-6, ctx=None, dtype="f32", gamma=None, out8=False, keep8=False):
+        super().__init__(ctx, dtype)
+        self.embedDim, self.eps, self.out8, self.keep8 = embedDim, float(eps), bool(out8), bool(keep8)
+        self.gamma = gamma
+        self.input = self.sum = self.kept = self.diffGamma = None
+
+    def forward(self, x, residual=None):
+        """norm(x + residual); the sum is self.sum (None without a residual)."""
+        shape = x.shape
+        _want(len(shape) == 2 and shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
+        _want(residual is None or (residual.shape == shape and residual.dtype == x.dtype and residual.ptr), "residual shape or dtype")   # (no address would mean none)
+        _want(self.gamma is not None, "the layer has no gamma")
+        self.input = None   # (until the call has succeeded)
+        self.sum = h = None if residual is None else self._buffer("sum", shape, self.dtype)
+        rstd = self._buffer("rstd", (shape[0],), "f32")
+        out = o8 = kept = None
+        if self.out8:
+            o8 = _rows8(self, "out8", "mx", shape)
+        else:
+            out = self._buffer("out", shape, self.dtype)
+        if self.keep8:
+            kept = _rows8(self, "keep8", "int8", shape)
+        self.ctx.check(self.lib.omega_hip_rmsnorm_forward(
+            self.ctx.handle, x.ptr, residual.ptr if residual else None, _DT[self.dtype], shape[0], shape[1], self.gamma.ptr, self.eps, h.ptr if h else None,
+            out.ptr if out else None, o8.codes.ptr if o8 else None, o8.scales.ptr if o8 else None, kept.codes.ptr if kept else None,
+            kept.scales.ptr if kept else None, rstd.ptr))
+        self.input, self.kept = x if h is None else h, kept
+        return out or o8
+
+    def read8(self, rows, dtype="bf16"):
+        """Rows8 as elements of dtype (bf16 holds every value of the form "mx")."""
+        _want(dtype in _DT, "dtype is f32 or bf16")
+        return _load8(self, "read8", rows, dtype)
+
+    def back(self, delta, dsum=None):
+        """Gradient of x and of the residual alike, for the last forward(); dsum: the gradient that reaches the sum past the norm.  gamma's is diffGamma."""
+        h = self.input
+        _want(h is not None, "back without a forward")
+        _want(delta.shape == h.shape and delta.dtype == self.dtype, "delta shape or dtype does not match the output")
+        _want(dsum is None or (dsum.shape == h.shape and dsum.dtype == self.dtype and dsum.ptr), "dsum shape or dtype does not match the sum")
+        kept, T = self.kept, h.shape[0]
+        dx = self._buffer("diff", h.shape, self.dtype)
+        self.diffGamma = dg = self._buffer("diffGamma", (self.embedDim,), "f32")
+        self.ctx.check(self.lib.omega_hip_rmsnorm_backward(
+            self.ctx.handle, None if kept else h.ptr, kept.codes.ptr if kept else None, kept.scales.ptr if kept else None, delta.ptr,
+            dsum.ptr if dsum else None, _DT[self.dtype], T, self.embedDim, self.gamma.ptr, self._owned["rstd"].ptr, dx.ptr, dg.ptr))
+        return dx
+
+    def close(self):
+        super().close()
+        self.sum = self.kept = None
+
+
+class Keep8Layer(_Layer):
+    """Rows kept in 8 bits between a forward pass and its backward pass: save(x) keeps them, load() brings them back (the reference keeps
+    activations whole)."""
+
+    def __init__(self, embedDim, form="int8", ctx=None, dtype="f32"):
+        super().__init__(ctx, dtype)
+        _want(form in _FORMS, "form is int8 or mx")
+        self.embedDim, self.form, self.kept = embedDim, form, None
+
+    def save(self, x):
+        _want(len(x.shape) == 2 and x.shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
+        self.kept = None
+        rows = _rows8(self, "codes", self.form, x.shape)
+        self.ctx.check(self.lib.omega_hip_keep8_save(self.ctx.handle, x.ptr, _DT[self.dtype], x.shape[0], x.shape[1], _FORMS[self.form], rows.codes.ptr,
+                                                     rows.scales.ptr))
+        self.kept = rows
+        return rows
+
+    def load(self):
+        """The rows of the last save()."""
+        _want(self.kept is not None, "load without a save")
+        return _load8(self, "out", self.kept, self.dtype)
+
+    def close(self):
+        super().close()
+        self.kept = None

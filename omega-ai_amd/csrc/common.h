@@ -380,6 +380,31 @@ struct head_args {
 size_t head_workspace(const omega_ctx *ctx, const head_args &a, bool backward);
 hipError_t launch_head_forward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s);
 hipError_t launch_head_backward(const omega_ctx *ctx, const head_args &a, void *ws, hipStream_t s);
+// omega_hip_rmsnorm_forward / _backward
+struct rmsnorm_forward {
+    const void *x, *residual;
+    int dtype, T, d;
+    const float *gamma;
+    float eps;
+    void *sum, *out;
+    uint8_t *out8, *scale8, *keep8;
+    float *keep_scale, *rstd;
+};
+struct rmsnorm_backward {
+    const void *h;
+    const uint8_t *keep8;
+    const float *keep_scale;
+    const void *dout, *dsum;
+    int dtype, T, d;
+    const float *gamma, *rstd;
+    void *dx;
+    float *dgamma;
+};
+hipError_t launch_rmsnorm_forward(const omega_ctx *ctx, const rmsnorm_forward &p, hipStream_t s);
+size_t rmsnorm_backward_workspace(const omega_ctx *ctx, int T, int d);
+hipError_t launch_rmsnorm_backward(const omega_ctx *ctx, const rmsnorm_backward &p, void *ws, hipStream_t s);
+hipError_t launch_keep8_save(const void *x, int dtype, int T, int d, int form, uint8_t *codes, void *scales, hipStream_t s);
+hipError_t launch_keep8_load(const uint8_t *codes, const void *scales, int form, int T, int d, void *out, int dtype, hipStream_t s);
 hipError_t head_init(void);  // kernel attributes (LDS beyond 64 KiB), once per device
 
 #define F32_TILE_M 128       // row-tile heights of fp32 layers: experts_f32_tile_m chooses one per batch

@@ -62,6 +62,10 @@ class Context:
             self.handle = None
 
 
+_ESIZE = {"bf16": 2, "u8": 1}
+_HOST = {"bf16": np.uint16, "i32": np.int32, "u8": np.uint8}
+
+
 class DeviceBuffer:
     """Caller-owned device memory (the role of Tensor.gpuData, J/engine/tensor/Tensor.java:23-47)."""
 
@@ -73,8 +77,8 @@ class DeviceBuffer:
         self.ptr = p
 
     def _describe(self, ctx, shape, dtype):
-        self.ctx, self.shape, self.dtype = ctx, tuple(shape), dtype   # dtype: "f32", "bf16" or "i32"
-        self.esize = 2 if dtype == "bf16" else 4
+        self.ctx, self.shape, self.dtype = ctx, tuple(shape), dtype   # dtype: "f32", "bf16", "i32" or "u8"
+        self.esize = _ESIZE.get(dtype, 4)
         self.size = math.prod(self.shape)
         self.nbytes = self.size * self.esize
 
@@ -89,19 +93,19 @@ class DeviceBuffer:
 
     @classmethod
     def from_numpy(cls, ctx, a, dtype):
-        """a: fp32 values, stored as fp32 or as bf16 (round to nearest even), or whole numbers stored as i32."""
+        """a: fp32 values, stored as fp32 or as bf16 (round to nearest even), or whole numbers stored as i32 or u8."""
         b = cls(ctx, a.shape, dtype)
         b.upload(a)
         return b
 
     def upload(self, a):
-        h = f32_to_bf16_bits(a) if self.dtype == "bf16" else np.ascontiguousarray(a, np.int32 if self.dtype == "i32" else np.float32)
+        h = f32_to_bf16_bits(a) if self.dtype == "bf16" else np.ascontiguousarray(a, _HOST.get(self.dtype, np.float32))
         assert h.nbytes == self.nbytes
         self.ctx.check(self.ctx.lib.omega_hip_memcpy_h2d(self.ctx.handle, self.ptr, h.ctypes.data, h.nbytes))
 
     def to_numpy(self):
         """Blocking copy to host (Tensor.syncHost); bf16 buffers come back widened to fp32."""
-        h = np.empty(self.shape, np.uint16 if self.dtype == "bf16" else np.int32 if self.dtype == "i32" else np.float32)
+        h = np.empty(self.shape, _HOST.get(self.dtype, np.float32))
         self.ctx.check(self.ctx.lib.omega_hip_memcpy_d2h(self.ctx.handle, h.ctypes.data, self.ptr, h.nbytes))
         return bf16_bits_to_f32(h) if self.dtype == "bf16" else h
 
