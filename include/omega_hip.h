@@ -42,8 +42,10 @@ typedef enum {
     OMEGA_W_W1 = 2,        /* [H,d] per expert */
     OMEGA_W_W3 = 3,        /* [H,d] per expert */
     OMEGA_W_W2 = 4,        /* [d,H] per expert */
-    OMEGA_W_NORM = 5       /* [d] always fp32: weight (gamma) of the RMSNorm in front of the layer, block form only
+    OMEGA_W_NORM = 5,      /* [d] always fp32: weight (gamma) of the RMSNorm in front of the layer, block form only
                               (RMSLayer.gamma, J/engine/nn/layer/normalization/RMSLayer.java) */
+    OMEGA_W_BALANCE = 6    /* [E] always fp32: bias for balance of a layer whose routing has one (omega_moe_set_routing); no
+                              gradient, no optimiser step */
 } omega_weight_kind;
 
 /* Constructor arguments of the layer, in the house style of
@@ -367,6 +369,49 @@ typedef struct {
 int omega_hip_clip_grad_norm(omega_ctx *ctx, const omega_grad_tensor *tensors, int n_tensors, omega_moe *const *layers,
                              int n_layers, float max_norm, float *norm_out);
 
+/* ---- Routing to experts other than the softmax top-k of omega_moe_config (the reference has no router) ----
+ * For logits z [T,E] (fp32) and, where there is one, a bias b [E]:
+ *   score s = softmax(z) over the experts that are open to the token, or 1 / (1 + e^-z); an expert whose logit is -infinity or no number is
+ *   closed (+infinity counts as the largest number); worth = s + b, and an expert whose worth is -infinity or no number is closed too;
+ *   groups of E / groups consecutive experts: a group's worth is the sum of the worths of its group_best (1 or 2) best open experts, the
+ *   top_groups best groups stay;
+ *   chosen are the K best experts of the groups that stay, in descending order of worth, without a bias of z; equal experts and groups in the
+ *   order of their numbers.  Worths are compared as their 64-bit values;
+ *   weight w_j = scale s_j; with renorm divided by the sum of s over the chosen.  Where fewer than K are open: id -1, weight 0.
+ * The bias takes part in the choice only and has no gradient: omega_hip_route_balance moves it against what the experts got. */
+#define OMEGA_ROUTE_SOFTMAX 0
+#define OMEGA_ROUTE_SIGMOID 1
+typedef struct {
+    int32_t E;          /* experts, 1..512                                              */
+    int32_t K;          /* chosen, 1..64, at most top_groups * (E / groups)             */
+    int32_t score;      /* OMEGA_ROUTE_SOFTMAX or OMEGA_ROUTE_SIGMOID                   */
+    int32_t renorm;     /* 1: weights divided by their sum                              */
+    int32_t groups;     /* 1..64, divides E; 1: no groups                               */
+    int32_t top_groups; /* 1..groups                                                    */
+    int32_t group_best; /* 1 or 2                                                       */
+    float scale;        /* positive                                                     */
+} omega_route_config;
+/* ids and w [T,K], counts [E] (may be NULL) = tokens that chose an expert; bias NULL: none.  Same terms for buffers as the operators above. */
+int omega_hip_route_forward(omega_ctx *ctx, const omega_route_config *cfg, const float *logits, int T, const float *bias, int32_t *ids, float *w,
+                            int32_t *counts);
+/* dlogits [T,E] (overwritten) = gradient through the weights of the chosen, the choice held: with u = w / scale
+ *   renorm        dz_j = w_j g_j, g_j = sum_k u_k (dw_j - dw_k), times 1 - s_j for sigmoid scores; zero for experts that were not chosen
+ *   else sigmoid  dz_j = w_j dw_j (1 - s_j);   else softmax   dz_e = [chosen] w_e dw_e - s_e sum_k w_k dw_k
+ * with the forward pass's ids and w.  An id outside 0..E-1 and a weight of 0 have no part.  logits may be NULL for softmax with renorm. */
+int omega_hip_route_backward(omega_ctx *ctx, const omega_route_config *cfg, const float *logits, int T, const int32_t *ids, const float *w, const float *dw,
+                             float *dlogits);
+/* bias[e] += rate where counts[e] is below the mean of counts [E], -= rate where above. */
+int omega_hip_route_balance(omega_ctx *ctx, const int32_t *counts, int E, float rate, float *bias);
+/* The routing of a MoE layer: its gate logits (with the gate bias) take this way instead of the softmax top-k, in the forward pass, the block form, the
+ * stages and the backward pass.  E and K are the layer's; cfg->renorm and scale replace its renorm.  Every token gets K experts: where fewer
+ * are open, the first others, with weight 0.  with_bias: the layer has a bias for balance (OMEGA_W_BALANCE, zeros at first).  cfg NULL: the
+ * softmax top-k again.  A forward pass must run again before the next backward pass.  The select arithmetic is the same in both router modes;
+ * omega_moe_get_router_probs returns the softmax of the logits whatever the routing. */
+int omega_moe_set_routing(omega_moe *moe, const omega_route_config *cfg, int with_bias);
+/* One step of the layer's bias for balance from the counts of its last dispatch (omega_hip_route_balance).  Where a backward pass follows, it is
+ * that of the choice that was made. */
+int omega_moe_balance(omega_moe *moe, float rate);
+
 /* ---- Operators around the experts of a block, on caller-owned buffers under the same terms ---- */
 
 /* RMS norm with the addition of a residual in front of it: h = x + residual rounded once to dtype (residual NULL: h = x),
@@ -388,8 +433,8 @@ int omega_hip_rmsnorm_backward(omega_ctx *ctx, const void *h, const uint8_t *kee
                                int dtype, int T, int d, const float *gamma, const float *rstd, void *dx, float *dgamma);
 
 /* Rows kept in 8 bits, and brought back.  codes [T,d]; a scale for every group of a row (its last one may be shorter):
- *   OMEGA_KEEP8_INT8  groups of 128, scales [T,ceil(d/128)] float: s = max(largest magnitude / 127, 2^-126), code = x / s rounded to the nearest
- *                     whole number (halves to even), value = code s;
+ *   OMEGA_KEEP8_INT8  groups of 128, scales [T,ceil(d/128)] float: s = max(largest magnitude r, 2^-126) with r = 1 / 127 rounded to float,
+ *                     code = x / s rounded to the nearest whole number (halves to even), value = code s;
  *   OMEGA_KEEP8_MX    groups of 32, scales [T,ceil(d/32)] bytes k + 127: s = 2^k is the smallest (k >= -127) with largest magnitude <= 448 s,
  *                     code = x / s in e4m3 (1 sign, 4 exponent, 3 mantissa bits, nearest even), value = code s: the block format of
  *                     the matrix cores' scaled products.

@@ -12,7 +12,8 @@ OK, ERR_INVALID_ARG, ERR_OOM, ERR_HIP, ERR_UNSUPPORTED = range(5)
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ROUTER_EXACT, ROUTER_FAST = 0, 1
 KEEP8_INT8, KEEP8_MX = 0, 1
-W_GATE, W_GATE_BIAS, W_W1, W_W3, W_W2, W_NORM = range(6)
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+W_GATE, W_GATE_BIAS, W_W1, W_W3, W_W2, W_NORM, W_BALANCE = range(7)
 (STAGE_ROUTER, STAGE_DISPATCH, STAGE_UP, STAGE_DOWN, STAGE_COMBINE, STAGE_FORWARD, STAGE_INDEX, STAGE_GATHER,
  STAGE_FORWARD_BLOCK, STAGE_RMS) = range(10)
 
@@ -20,6 +21,10 @@ W_GATE, W_GATE_BIAS, W_W1, W_W3, W_W2, W_NORM = range(6)
 class MoEConfigStruct(C.Structure):
     _fields_ = [(n, C.c_int32) for n in
                 ("T_max", "d", "E", "K", "H", "Es", "renorm", "has_gate_bias", "dtype", "router_mode")]
+
+
+class RouteConfigStruct(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("E", "K", "score", "renorm", "groups", "top_groups", "group_best")] + [("scale", C.c_float)]
 
 
 class GradTensorStruct(C.Structure):
@@ -91,6 +96,11 @@ SIGNATURES = {
     "omega_hip_head_loss_forward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 4),
     "omega_hip_head_loss_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int] + [C.c_void_p] * 6),
     "omega_hip_clip_grad_norm": (C.c_int, [C.c_void_p, C.POINTER(GradTensorStruct), C.c_int, C.POINTER(C.c_void_p), C.c_int, C.c_float, C.c_void_p]),
+    "omega_hip_route_forward": (C.c_int, [C.c_void_p, C.POINTER(RouteConfigStruct), C.c_void_p, C.c_int] + [C.c_void_p] * 4),
+    "omega_hip_route_backward": (C.c_int, [C.c_void_p, C.POINTER(RouteConfigStruct), C.c_void_p, C.c_int] + [C.c_void_p] * 4),
+    "omega_hip_route_balance": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_void_p]),
+    "omega_moe_set_routing": (C.c_int, [C.c_void_p, C.POINTER(RouteConfigStruct), C.c_int]),
+    "omega_moe_balance": (C.c_int, [C.c_void_p, C.c_float]),
     "omega_hip_rmsnorm_forward": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 3 + [C.c_void_p, C.c_float] + [C.c_void_p] * 7),
     "omega_hip_rmsnorm_backward": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 3 + [C.c_void_p] * 4),
     "omega_hip_keep8_save": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),

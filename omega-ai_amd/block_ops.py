@@ -1,11 +1,70 @@
-"""What stands around the experts of a transformer block, over the C ABI: RMS norm with the residual's addition, rows kept in 8 bits.
+"""What stands around the experts of a transformer block, over the C ABI: routing to experts, RMS norm with the residual's addition, rows
+kept in 8 bits.
 
 Classes in the manner of lm_ops.py: forward(input) returns the layer's own output buffer, back(delta) the input gradient, parameter
 gradients lie beside the parameters.
 """
+import ctypes as C
+
 from . import _lib as L
 from .lm_ops import _DT, _Layer, _Param, _want
-from .moe_layer import DeviceBuffer
+
+_SCORES = {"softmax": L.ROUTE_SOFTMAX, "sigmoid": L.ROUTE_SIGMOID}
+
+
+def route_config(nExperts, topK, score="softmax", renorm=True, scale=1.0, nGroups=1, topGroups=None, groupBest=2):
+    """omega_route_config: scores (softmax or sigmoid) of nExperts in nGroups groups, of which the topGroups (None: all) with the best sum of their
+    groupBest best stay; topK chosen, their weights times scale, divided by their sum with renorm."""
+    _want(score in _SCORES, "score is softmax or sigmoid")
+    return L.RouteConfigStruct(nExperts, topK, _SCORES[score], int(bool(renorm)), nGroups, nGroups if topGroups is None else topGroups, groupBest, float(scale))
+
+
+class RoutingLayer(_Layer):
+    """Routing of tokens to experts from the logits of a gate (fp32; the reference has no router): forward(logits) returns the weights of the chosen
+    experts [T,topK], ids [T,topK] are their numbers (-1 where none was open) and counts [nExperts] the tokens of each.
+
+    bias: the caller's buffer for balance; it takes part in the choice only, and balance(rate) moves it by the last counts."""
+
+    bias = _Param(lambda layer: (layer.nExperts,), lambda layer: "f32")
+
+    def __init__(self, nExperts, topK, score="softmax", renorm=True, scale=1.0, nGroups=1, topGroups=None, groupBest=2, ctx=None, bias=None):
+        super().__init__(ctx, "f32")
+        self.nExperts, self.topK = nExperts, topK
+        self._config = route_config(nExperts, topK, score, renorm, scale, nGroups, topGroups, groupBest)
+        self._by = C.byref(self._config)
+        self.bias = bias
+        self.input = self.w = self.ids = self.counts = None
+
+    def forward(self, logits):
+        shape = logits.shape
+        _want(len(shape) == 2 and shape[1] == self.nExperts and logits.dtype == "f32", "logits shape or dtype")
+        bias = self.bias
+        _want(bias is None or bias.ptr, "bias has been freed")   # (no address would mean none)
+        self.input, T = None, shape[0]   # (until the call has succeeded)
+        w, ids = self._buffer("w", (T, self.topK), "f32"), self._buffer("ids", (T, self.topK), "i32")
+        counts = self._buffer("counts", (self.nExperts,), "i32")
+        self.ctx.check(self.lib.omega_hip_route_forward(self.ctx.handle, self._by, logits.ptr, T, bias.ptr if bias else None, ids.ptr, w.ptr, counts.ptr))
+        self.input, self.w, self.ids, self.counts = logits, w, ids, counts
+        return w
+
+    def back(self, delta):
+        """Gradient of the logits of the last forward() from that of its weights."""
+        x = self.input
+        _want(x is not None, "back without a forward")
+        _want(delta.shape == self.w.shape and delta.dtype == "f32", "delta shape or dtype does not match the weights")
+        dx = self._buffer("diff", x.shape, "f32")
+        self.ctx.check(self.lib.omega_hip_route_backward(self.ctx.handle, self._by, x.ptr, x.shape[0], self.ids.ptr, self.w.ptr, delta.ptr, dx.ptr))
+        return dx
+
+    def balance(self, rate):
+        """bias -+= rate for the experts that the last forward() gave more or fewer tokens than the mean."""
+        _want(self.bias is not None and self.counts is not None, "balance without a bias or a forward")
+        self.ctx.check(self.lib.omega_hip_route_balance(self.ctx.handle, self.counts.ptr, self.nExperts, float(rate), self.bias.ptr))
+
+    def close(self):
+        super().close()
+        self.w = self.ids = self.counts = None
+
 
 _FORMS = {"int8": L.KEEP8_INT8, "mx": L.KEEP8_MX}
 _GROUP = {"int8": 128, "mx": 32}

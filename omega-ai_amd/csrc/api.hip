@@ -191,11 +191,11 @@ static void moe_free_backward_workspace(omega_moe *m)
 static void moe_free_workspace(omega_moe *m)
 {
     void *ptrs[] = {m->ids, m->w, m->tile_counts, m->dst, m->dstp, m->src_row, m->tiles, m->xg, m->xs, m->a, m->y,
-                    m->desc_up, m->desc_down, m->wq_up, m->wq_down, m->rms, m->hbuf, m->tokp, m->slab_tab, m->gate_logits};
+                    m->desc_up, m->desc_down, m->wq_up, m->wq_down, m->rms, m->hbuf, m->tokp, m->slab_tab, m->gate_logits, m->route_logits};
     for (void *p : ptrs)
         if (p) hipFree(p);
     m->ids = nullptr; m->w = nullptr; m->tile_counts = nullptr; m->dst = nullptr; m->dstp = nullptr; m->src_row = nullptr; m->xs = nullptr; m->desc_up = nullptr; m->desc_down = nullptr; m->wq_up = nullptr; m->wq_down = nullptr; m->rms = nullptr; m->hbuf = nullptr;
-    m->tiles = nullptr; m->xg = nullptr; m->a = nullptr; m->y = nullptr; m->tokp = nullptr; m->slab_tab = nullptr; m->gate_logits = nullptr;
+    m->tiles = nullptr; m->xg = nullptr; m->a = nullptr; m->y = nullptr; m->tokp = nullptr; m->slab_tab = nullptr; m->gate_logits = nullptr; m->route_logits = nullptr;
     m->xg_valid = m->y_partial = false;
     m->T_cap = 0;
     moe_free_backward_workspace(m);
@@ -388,6 +388,7 @@ static int moe_reserve(omega_moe *m, int T)
     }
     if (c.dtype == OMEGA_DTYPE_BF16 && c.E > 16)  // (as many tokens as such a batch can have: router.hip)
         OMEGA_HIP_CHECK(ctx, hipMalloc((void **)&m->gate_logits, (size_t)std::min(T, 16 * ctx->num_cus) * c.E * 4));
+    if (m->own_routing) OMEGA_HIP_CHECK(ctx, hipMalloc((void **)&m->route_logits, (size_t)T * c.E * 4));
     if (c.dtype == OMEGA_DTYPE_BF16 && c.Es > 0) {
         const size_t xs_rows = (size_t)ceil_div(T, bm) * bm;
         OMEGA_HIP_CHECK(ctx, hipMalloc(&m->xs, xs_rows * c.d * m->esize));
@@ -492,6 +493,7 @@ int omega_moe_destroy(omega_moe *m)
     if (m->master) hipFree(m->master);
     if (m->W2T) hipFree(m->W2T);
     if (m->W13T) hipFree(m->W13T);
+    if (m->route_bias) hipFree(m->route_bias);
     hipEventDestroy(m->ev0);
     hipEventDestroy(m->ev1);
     for (hipEvent_t ev : m->prof_events) hipEventDestroy(ev);
@@ -507,6 +509,9 @@ static int weight_slot(omega_moe *m, int which, int expert, void **ptr, size_t *
         case OMEGA_W_GATE: *ptr = m->Wg; *bytes = (size_t)c.E * c.d * m->esize; return OMEGA_OK;
         case OMEGA_W_GATE_BIAS: *ptr = m->bg; *bytes = (size_t)c.E * 4; return OMEGA_OK;
         case OMEGA_W_NORM: *ptr = m->gamma; *bytes = (size_t)c.d * 4; return OMEGA_OK;
+        case OMEGA_W_BALANCE:
+            if (!m->route_bias) return OMEGA_ERR_INVALID_ARG;
+            *ptr = m->route_bias; *bytes = (size_t)c.E * 4; return OMEGA_OK;
         case OMEGA_W_W1: case OMEGA_W_W3: case OMEGA_W_W2: {
             if (expert < 0 || expert >= m->G) return OMEGA_ERR_INVALID_ARG;
             unsigned char *base = (unsigned char *)(which == OMEGA_W_W1 ? m->W1 : which == OMEGA_W_W3 ? m->W3 : m->W2);
@@ -534,7 +539,7 @@ int omega_moe_set_weights(omega_moe *m, int which, int expert, const void *src, 
     if (!src || weight_slot(m, which, expert, &p, &bytes) != OMEGA_OK)
         OMEGA_FAIL(ctx, OMEGA_ERR_INVALID_ARG, "set_weights: bad kind, expert index or source");
     if (which == OMEGA_W_GATE) m->gate_img_valid = false;
-    m->master_valid = false;  // fp32 master copies of a bf16 layer are remade from the weights at the next update
+    if (which != OMEGA_W_BALANCE) m->master_valid = false;  // fp32 master copies of a bf16 layer are remade from the weights at the next update
     // the activations (and, in training mode, the h1 / h3 records) of the last forward belong to the old weights: a
     // backward pass needs a new forward first
     m->fwd_T = -1;
@@ -650,7 +655,8 @@ static void stage_invalidates(omega_moe *m)
 static int stage_router(omega_moe *m, const void *x, int T)
 {
     // training mode (backward workspace in place): the probabilities are kept for the backward pass
-    float *probs = keeps_for_backward(m, T) ? m->bw_probs : nullptr;
+    // (a routing of the layer's own goes back from its logits)
+    float *probs = !m->own_routing && keeps_for_backward(m, T) ? m->bw_probs : nullptr;
     m->routed_T = m->dispatched_T = -1;
     OMEGA_HIP_CHECK(m->ctx, launch_router(m, x, T, nullptr, probs, m->ctx->stream));
     m->routed_T = T;
@@ -951,7 +957,7 @@ int omega_moe_time_backward(omega_moe *m, const void *x, const void *dout, int T
     float total = 0.0f;
     for (int i = 0; i < warmup + iters; ++i) {
         if (put_back && !m->rec_valid) {
-            OMEGA_HIP_CHECK(ctx, launch_router(m, x, T, nullptr, m->bw_probs, ctx->stream));
+            if (!m->own_routing) OMEGA_HIP_CHECK(ctx, launch_router(m, x, T, nullptr, m->bw_probs, ctx->stream));
             OMEGA_HIP_CHECK(ctx, launch_product_f32(m, F32_RAW, (const float *)x, (const float *)dout, T, ctx->stream));
             m->rec_valid = true;
         }

@@ -90,6 +90,16 @@ __global__ __launch_bounds__(256) void bw_router_kernel(const float *__restrict_
     }
 }
 
+// gradient of the logits from that of the combine weights, by the softmax top-k above or by the layer's own routing (route.hip)
+static hipError_t launch_bw_router(const omega_moe *m, int T, hipStream_t s)
+{
+    const omega_moe_config &c = m->cfg;
+    if (m->own_routing) return launch_route_backward(m->route, m->route_logits, T, m->ids, m->w, m->bw_dw, m->bw_dlogits, s);
+    hipLaunchKernelGGL(bw_router_kernel, dim3(ceil_div(T, 16)), dim3(256), 0, s, (const float *)m->bw_probs, m->ids, m->w, (const float *)m->bw_dw, T, c.E, c.K,
+                       c.renorm, m->bw_dlogits);
+    return hipGetLastError();
+}
+
 // Gate weight gradient dWg[e,k] = sum_t dlogits[t,e] * x[t,k] (diffW = delta^T . input) in two steps, both with a fixed
 // order of additions: partial sums over slices of the tokens, then their sum.  A wave takes a slice of the tokens, 256
 // columns and 32 experts on the fp32 matrix cores (v_mfma_f32_32x32x2: two tokens per instruction): lane l supplies
@@ -610,7 +620,7 @@ hipError_t launch_backward_f32(omega_moe *m, const void *xv, const void *doutv, 
     const bool kept = m->rec_valid;
     m->rec_valid = false;
     if (!kept) {
-        if ((e = launch_router(m, x, T, nullptr, m->bw_probs, s)) != hipSuccess) return e;
+        if (!m->own_routing && (e = launch_router(m, x, T, nullptr, m->bw_probs, s)) != hipSuccess) return e;
         if ((e = launch_product_f32(m, F32_RAW, x, dout, T, s)) != hipSuccess) return e;
     }
     hipLaunchKernelGGL(bw_combine_kernel, dim3(T), dim3(256), 0, s, dout, m->y, m->dstp, m->w, c.K, c.d, m->bw_dy, m->bw_dw);
@@ -619,8 +629,7 @@ hipError_t launch_backward_f32(omega_moe *m, const void *xv, const void *doutv, 
     for (int op : {F32_DA, F32_DXG, F32_WG2, F32_WG13})
         if ((e = launch_product_f32(m, op, x, dout, T, s)) != hipSuccess) return e;
     // router and gate
-    hipLaunchKernelGGL(bw_router_kernel, dim3(ceil_div(T, 16)), dim3(256), 0, s, (const float *)m->bw_probs, m->ids, m->w,
-                       (const float *)m->bw_dw, T, c.E, c.K, c.renorm, m->bw_dlogits);
+    if ((e = launch_bw_router(m, T, s)) != hipSuccess) return e;
     if ((e = launch_gate_wgrad(m, x, T, s)) != hipSuccess) return e;
     if (c.has_gate_bias)
         hipLaunchKernelGGL(bw_gate_bias_kernel, dim3(c.E), dim3(256), 0, s, (const float *)m->bw_dlogits, T, c.E, m->dbg);
@@ -704,7 +713,7 @@ hipError_t launch_backward_bf16(const omega_moe *m, const void *x, const void *d
     const size_t HD = (size_t)c.H * c.d;
     hipError_t e;
 #define STEP(expr) if ((e = (expr)) != hipSuccess) return e
-    if (!m->rec_valid) STEP(launch_router(m, x, T, nullptr, m->bw_probs, s));  // a training forward kept the probabilities
+    if (!m->rec_valid && !m->own_routing) STEP(launch_router(m, x, T, nullptr, m->bw_probs, s));  // a training forward kept the probabilities
     STEP(launch_backward_tables(m, T, s));
     hipLaunchKernelGGL(bw_combine_bf16_kernel, dim3(T), dim3(256), 0, s, (const uint4 *)dout, (const float *)m->y, m->dstp, m->w,
                        c.K, c.d, (unsigned char *)m->bw_dy16, (unsigned char *)m->bw_dys16, m->bw_dw);
@@ -722,8 +731,7 @@ hipError_t launch_backward_bf16(const omega_moe *m, const void *x, const void *d
     if (sliced) STEP(launch_down_slab_reduce(m, m->bw_dxg, s));
     // router and gate, and the input gradient while the rows of dxg are in the last-level cache (behind the weight
     // gradients, which write 5.6 GB at the Mixtral shape, the launch took 60 us there)
-    hipLaunchKernelGGL(bw_router_kernel, dim3(ceil_div(T, 16)), dim3(256), 0, s, (const float *)m->bw_probs, m->ids, m->w,
-                       (const float *)m->bw_dw, T, c.E, c.K, c.renorm, m->bw_dlogits);
+    STEP(launch_bw_router(m, T, s));
     STEP(launch_gate_wgrad(m, x, T, s));
     if (c.has_gate_bias)
         hipLaunchKernelGGL(bw_gate_bias_kernel, dim3(c.E), dim3(256), 0, s, (const float *)m->bw_dlogits, T, c.E, m->dbg);

@@ -65,6 +65,11 @@ struct omega_moe {
     float *gate_img = nullptr;            // bf16 layers with more than 16 experts: fp32 image of Wg for the router (router.hip) ...
     mutable bool gate_img_valid = false;  // ... made by the next router launch after Wg has changed
     float *gate_logits = nullptr;         // ... and the logits of a batch whose tiles the router splits by experts
+    // routing other than the softmax top-k of the configuration (omega_moe_set_routing): the router leaves logits, route.hip chooses
+    bool own_routing = false;
+    omega_route_config route = {};
+    float *route_bias = nullptr;    // [E] fp32, where the routing has a bias for balance
+    float *route_logits = nullptr;  // [T,E] of the last batch; the backward pass reads them
     void *W1 = nullptr;   // [G,H,d]
     void *W3 = nullptr;   // [G,H,d]
     void *W2 = nullptr;   // [G,d,H]
@@ -405,6 +410,15 @@ size_t rmsnorm_backward_workspace(const omega_ctx *ctx, int T, int d);
 hipError_t launch_rmsnorm_backward(const omega_ctx *ctx, const rmsnorm_backward &p, void *ws, hipStream_t s);
 hipError_t launch_keep8_save(const void *x, int dtype, int T, int d, int form, uint8_t *codes, void *scales, hipStream_t s);
 hipError_t launch_keep8_load(const uint8_t *codes, const void *scales, int form, int T, int d, void *out, int dtype, hipStream_t s);
+size_t route_workspace(const omega_ctx *ctx, const omega_route_config &c, int T);
+hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &c, const float *logits, int T, const float *bias, int32_t *ids, float *w,
+                                int32_t *counts, void *ws, hipStream_t s);
+// a layer's selection: histogram rows of `tokens` tokens each, and K experts for every token (weight 0 where fewer are open)
+hipError_t launch_route_layer(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, int32_t *ids, float *w, int32_t *tile_counts,
+                              hipStream_t s);
+hipError_t launch_route_backward(const omega_route_config &c, const float *logits, int T, const int32_t *ids, const float *w, const float *dw, float *dlogits,
+                                 hipStream_t s);
+hipError_t launch_route_balance(const int32_t *counts, int E, float rate, float *bias, hipStream_t s);
 hipError_t head_init(void);  // kernel attributes (LDS beyond 64 KiB), once per device
 
 #define F32_TILE_M 128       // row-tile heights of fp32 layers: experts_f32_tile_m chooses one per batch

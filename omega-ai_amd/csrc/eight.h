@@ -1,7 +1,7 @@
 // Eight consecutive elements of a row in a lane, and the two forms in which rows are held in 8 bits.
 //
-//   OMEGA_KEEP8_INT8  groups of 128 elements of a row: scale s = max(amax / 127, 2^-126) in fp32, code = x / s to the nearest whole number,
-//                     halves to even; value = code s
+//   OMEGA_KEEP8_INT8  groups of 128 elements of a row: scale s = max(amax r, 2^-126) in fp32, r = 1 / 127 rounded to fp32, code = x / s to
+//                     the nearest whole number, halves to even; value = code s
 //   OMEGA_KEEP8_MX    groups of 32: s = 2^k, the smallest with amax <= 448 s (k >= -127), in a byte k + 127; code = x / s in e4m3 (four
 //                     significant bits), to nearest even; value = code s
 // A row's last group may be shorter.  A group that holds an infinity or no number has a scale that is no number (the byte 255) and comes back as
@@ -113,7 +113,7 @@ __device__ __forceinline__ uint32_t magnitude(const float (&v)[8])
 __device__ __forceinline__ u32x2_by to_int8(const float (&v)[8], float *scale)
 {
     const uint32_t most = max_over_16(magnitude(v));
-    const float s = fmaxf(__uint_as_float(most) / 127.0f, 0x1p-126f), inv = __builtin_amdgcn_rcpf(s);
+    const float s = fmaxf(__uint_as_float(most) * 0x1.020408p-7f, 0x1p-126f), inv = __builtin_amdgcn_rcpf(s);
     uint32_t m[8];
     float r[8], worst = 0.0f;
 #pragma unroll

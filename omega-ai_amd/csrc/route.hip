@@ -1,0 +1,709 @@
+// Routing to experts from their logits z [T,E] (an operator of its own, and the selection of MoE layers that ask for it).
+//
+//   scores   softmax(z) over a token's open experts, or 1 / (1 + e^-z);  an expert is closed to a token where z is -infinity or no number
+//   worth    score + bias (no bias: the score; a sum that is -infinity or no number closes the expert)
+//   groups   E / groups consecutive experts each; a group's worth is the sum of its group_best best; the top_groups best stay
+//   choice   the K best of what stays, by worth, without a bias by z; equal ones, experts and groups, in the order of their numbers
+//   weights  w_j = scale s_j, with renorm divided by the sum of the chosen scores
+//   back     renorm: dz_j = w_j sum_k (w_k / scale)(dw_j - dw_k) (1 - s_j for sigmoid); else sigmoid: w_j dw_j (1 - s_j), softmax: [chosen] w_j dw_j - s_e sum_k w_k dw_k
+//
+// The choice is that of worths in 64 bits.  They are formed in fp32, a few instructions an expert, and where two that the choice tells apart are nearer
+// to each other than their errors, or equal, the token is chosen for again in double, by its whole wave (route_exact).
+// L lanes share a token, V experts a lane.  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
+// replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
+// the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
+#include <float.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "rows.h"
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+#define ROUTE_MAX_E 512
+#define ROUTE_TOKENS 1024     // of a workgroup, at most
+#define ROUTE_NONE (-1)
+#define ROUTE_FILL (1 << 16)  // chosen only because a layer's token has K experts whatever is open: weight 0
+
+// what other lanes of a row of 16 hold, then across the rows
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_of(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float lane_of(float v)
+{
+    return __uint_as_float(lane_of<CTRL>(__float_as_uint(v)));
+}
+// `meet` of a value in the lanes of a token, the same in all of them
+template <int L, class F>
+__device__ __forceinline__ uint32_t over_token(uint32_t v, F meet)
+{
+    v = meet(v, lane_of<0x128>(v));  // row_ror 8, 4, 2, 1
+    v = meet(v, lane_of<0x124>(v));
+    v = meet(v, lane_of<0x122>(v));
+    v = meet(v, lane_of<0x121>(v));
+    if (L == 64) {
+        u32x2 u = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = meet(u[0], u[1]);
+        u = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = meet(u[0], u[1]);
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float token_max(float v)
+{
+    return __uint_as_float(over_token<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int L>
+__device__ __forceinline__ float token_sum(float v)
+{
+    return __uint_as_float(over_token<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+template <int L>
+__device__ __forceinline__ uint32_t token_max(uint32_t v)
+{
+    return over_token<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
+// e^x for x <= 0 to 2 units in the last place: 2^(x log2 e), what the product's rounding cuts off added to the result; 0 below 2^-126
+__device__ __forceinline__ float exp_neg(float x)
+{
+    const float t = x * 0x1.715476p+0f, lo = fmaf(x, 0x1.715476p+0f, -t) + x * 0x1.4ae0cp-26f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t < -126.0f ? 0.0f : fmaf(e, lo * 0x1.62e43p-1f, e);
+}
+// ... with the relative error |x| 2^-24 of the product: of a score that is some 2^-26, where e^x is large enough to matter x is small
+__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 0x1.715476p+0f); }
+__device__ __forceinline__ float sigmoid_near(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_near(-z)); }
+__device__ __forceinline__ float sigmoid(float z)
+{
+    const float e = exp_neg(-fabsf(z));
+    return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
+}
+// a logit as it is compared: closed ones -infinity, infinite ones the largest number
+__device__ __forceinline__ float open_logit(float z) { return z == z ? fminf(z, FLT_MAX) : -INFINITY; }
+
+// A float as a whole number of the same order, 0 for -infinity; and back
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+    const uint32_t u = __float_as_uint(v + 0.0f);  // (both zeros the same)
+    return v == -INFINITY ? 0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// the lanes of a wave see each other's LDS writes
+__device__ __forceinline__ void wave_lds()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct route_args {
+    const float *logits, *bias;
+    int T, E, K, sigmoid, renorm, groups, top_groups, group_best;
+    int per_group, group_magic, group_shift;  // experts of a group; e / per_group = e magic >> 20; 1 << shift lanes look at a group
+    float scale;
+    int tokens;      // of a workgroup
+    int fill;        // a layer's routing: every token gets K experts
+    int vec;         // rows are 16-byte aligned and whole 16-byte pieces
+    int32_t *ids;
+    float *w;
+    int32_t *part;   // [workgroups][E]: tokens that chose an expert
+};
+
+template <int CTRL>
+__device__ __forceinline__ double lane_of(double v)
+{
+    const u32x2 u = *(const u32x2 *)&v;
+    const u32x2 o = {lane_of<CTRL>(u[0]), lane_of<CTRL>(u[1])};
+    return *(const double *)&o;
+}
+// `meet` of a double over a wave
+template <class F>
+__device__ __forceinline__ double over_wave(double v, F meet)
+{
+    v = meet(v, lane_of<0x128>(v));
+    v = meet(v, lane_of<0x124>(v));
+    v = meet(v, lane_of<0x122>(v));
+    v = meet(v, lane_of<0x121>(v));
+#define ACROSS(swap)                                                                              \
+    do {                                                                                          \
+        const u32x2 u = *(const u32x2 *)&v;                                                       \
+        const u32x2 lo = swap(u[0], u[0], false, false), hi = swap(u[1], u[1], false, false);     \
+        const u32x2 x = {lo[0], hi[0]}, y = {lo[1], hi[1]};                                       \
+        v = meet(*(const double *)&x, *(const double *)&y);                                       \
+    } while (0)
+    ACROSS(__builtin_amdgcn_permlane16_swap);
+    ACROSS(__builtin_amdgcn_permlane32_swap);
+#undef ACROSS
+    return v;
+}
+__device__ __forceinline__ double wave_max(double v) { return over_wave(v, [](double a, double b) { return fmax(a, b); }); }
+
+// The choice for one token in double, by a wave: lane j's place.  row: its logits; spare: room for E doubles in LDS; top and recip: of its softmax.
+__device__ __forceinline__ int route_exact(const route_args &a, const float *row, double *spare, float *top_out, float *recip_out)
+{
+    const int lane = threadIdx.x & 63, E = a.E;
+    double m = -INFINITY, sum = 1.0;
+    if (!a.sigmoid) {
+        for (int e = lane; e < E; e += 64) m = fmax(m, (double)open_logit(row[e]));
+        m = wave_max(m);
+        sum = 0.0;
+    }
+#pragma unroll 1
+    for (int e = lane; e < E; e += 64) {
+        const double z = (double)open_logit(row[e]);
+        const double v = a.sigmoid ? 1.0 / (1.0 + exp(-z)) : z == -INFINITY ? 0.0 : exp(z - m);
+        if (!a.sigmoid) sum += v;
+        spare[e] = v;
+    }
+    if (!a.sigmoid) sum = over_wave(sum, [](double x, double y) { return x + y; });
+    *top_out = fmaxf((float)m, -FLT_MAX);
+    *recip_out = sum > 0.0 ? (float)(1.0 / sum) : 0.0f;
+#pragma unroll 1
+    for (int e = lane; e < E; e += 64) {
+        double v = a.sigmoid ? spare[e] : spare[e] / sum;
+        if (a.bias != nullptr) v += (double)a.bias[e];
+        spare[e] = open_logit(row[e]) == -INFINITY || !(v == v) ? -INFINITY : v;
+    }
+    wave_lds();
+    unsigned long long stay = ~0ull;
+    if (a.groups > 1) {
+        double best = -INFINITY;
+        if (lane < a.groups) {
+            double second = -INFINITY;
+#pragma unroll 4
+            for (int e = lane * a.per_group; e < (lane + 1) * a.per_group; ++e) {
+                const double v = spare[e];
+                second = fmax(second, fmin(best, v));
+                best = fmax(best, v);
+            }
+            if (a.group_best == 2 && second > -INFINITY) best += second;
+        }
+        int ahead = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const double v = __shfl(best, g);
+            ahead += v > best || (v == best && g < lane) ? 1 : 0;
+        }
+        stay = __ballot(lane < a.groups && ahead < a.top_groups);
+        wave_lds();
+    }
+    // what is compared, a lane's own; bit i of left: expert lane + 64 i has not been chosen
+    uint32_t left = 0;
+    for (int i = 0, e = lane; e < E; ++i, e += 64) {
+        left |= 1u << i;
+        if (!((stay >> (a.groups > 1 ? (uint32_t)e * (uint32_t)a.group_magic >> 20 : 0)) & 1)) spare[e] = -INFINITY;
+        else if (a.bias == nullptr && spare[e] > -INFINITY) spare[e] = (double)open_logit(row[e]);
+    }
+    int place = ROUTE_NONE;
+    for (int j = 0; j < a.K; ++j) {
+        double bv = -INFINITY;
+        int be = INT_MAX;
+        for (int i = 0, e = lane; e < E; ++i, e += 64) {
+            const double v = spare[e];
+            if (((left >> i) & 1) && (be == INT_MAX || v > bv)) bv = v, be = e;
+        }
+        const double top = wave_max(bv);
+        const bool none = top == -INFINITY;  // (a layer's token then takes the first of the others)
+        if (none && !a.fill) break;
+        int e = bv == top ? be : INT_MAX;
+        const unsigned long long have = __ballot(e != INT_MAX);
+        if (have & (have - 1)) {  // equal ones: the first
+            for (int s = 32; s > 0; s >>= 1) e = min(e, __shfl_xor(e, s));
+        } else e = __shfl(e, __ffsll((long long)have) - 1);
+        if ((e & 63) == lane) left &= ~(1u << (e >> 6));
+        if (lane == j) place = none ? e | ROUTE_FILL : e;
+    }
+    wave_lds();
+    return place;
+}
+
+// Weights of a token's chosen experts, and what is written of them: lane sub of L has the places sub, sub + L, ...
+template <int L>
+__device__ __forceinline__ void route_write(const route_args &a, const float *row, int t, bool live, int sub, const int (&at)[64 / L], float top, float recip, int *hist)
+{
+    constexpr int KL = 64 / L;
+    float c[KL], zt = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+        c[i] = at[i] >= 0 && at[i] < ROUTE_FILL ? open_logit(row[at[i]]) : -INFINITY;
+        zt = fmaxf(zt, c[i]);
+    }
+    zt = a.renorm ? token_max<L>(zt) : 0.0f;
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+        if (i * L >= a.K) {
+            c[i] = 0.0f;
+            continue;
+        }
+        const float zc = c[i];
+        float v;
+        if (!a.sigmoid) v = a.renorm ? exp_neg(zc - zt) : exp_neg(zc - top) * recip;
+        else {
+            // all multiplied by e^-zt where every chosen logit is negative: their ratios stay where the scores themselves vanish
+            const float e = exp_neg(-fabsf(zc));
+            v = (zc >= 0.0f ? 1.0f : a.renorm && zt < 0.0f ? exp_neg(zc - zt) : e) / (1.0f + e);
+        }
+        c[i] = zc > -INFINITY ? v : 0.0f;
+        total += c[i];
+    }
+    float by = a.scale;
+    if (a.renorm) {
+        total = token_sum<L>(total);
+        by = total > 0.0f ? a.scale / total : 0.0f;
+    }
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+        const int j = sub + i * L;
+        if (j < a.K) {
+            const int e = at[i] < 0 ? ROUTE_NONE : at[i] & (ROUTE_FILL - 1);
+            a.ids[(size_t)t * a.K + j] = e;
+            a.w[(size_t)t * a.K + j] = c[i] * by;
+            if (e >= 0) atomicAdd(&hist[e], 1);
+        }
+    }
+}
+
+// Words of LDS that a wave needs: the worths of its tokens for their groups, then the lanes' lists and one more word each; one token's worths in double
+static constexpr int route_lds(int L, int V) { return 64 * (V + 1) > 2 * L * V ? 64 * (V + 1) : 2 * L * V; }
+
+// WORTH: there is a bias or there are groups
+template <int L, int V, bool WORTH>
+__global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args a)
+{
+    constexpr int TW = 64 / L, EW = L * V, KL = 64 / L;  // tokens of a wave, experts, chosen ones of a lane
+    constexpr int C = V < 4 ? V : 4;                     // a lane's experts lie in pieces of C: k is expert (k / C) L C + sub C + k % C
+    constexpr uint32_t LOW = V - 1;                      // bits of a word that say which of a lane's experts it is
+    static_assert((V & (V - 1)) == 0 && V * L <= ROUTE_MAX_E, "places of a lane's experts in whole bits");
+    extern __shared__ __attribute__((aligned(16))) uint32_t spare_all[];
+    __shared__ u32x2 picks_all[8][TW][64 + 1];           // the chosen words and their lanes
+    __shared__ int again[ROUTE_TOKENS], n_again;         // tokens that are chosen for in double
+    __shared__ int hist[EW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & (L - 1), tok = lane / L;
+    const int E = a.E, K = a.K, NT = blockDim.x;
+    uint32_t *spare = spare_all + wave * route_lds(L, V), *list = spare + lane;
+    float *uw = (float *)spare + tok * EW;
+    u32x2 *picks = picks_all[wave][tok];
+    const bool softmax_row = !a.sigmoid && (WORTH || !a.renorm);
+    for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
+    if (threadIdx.x == 0) n_again = 0;
+    __syncthreads();
+    auto expert = [&](int k) { return (k / C) * (L * C) + sub * C + k % C; };
+    float bias[V], span = 0.0f;  // (span: the largest finite bias)
+#pragma unroll
+    for (int k = 0; k < V; ++k) bias[k] = 0.0f;
+    if (WORTH && a.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            bias[k] = expert(k) < E ? a.bias[expert(k)] : 0.0f;
+            if (fabsf(bias[k]) < INFINITY) span = fmaxf(span, fabsf(bias[k]));
+        }
+        span = token_max<L>(span);
+    }
+    // What two worths may differ by although they are equal, of twice the largest score and the largest bias.  Sigmoid: 4 2^-24 each (e^-z 2 + |z|, the
+    // addition one, the reciprocal two, weighed by the curve's slope) and a rounding with the bias, 8 2^-24 (1 + worth) in all.  Softmax: four
+    // each and twenty in common (the sum of up to 512 terms and its reciprocal, whose error the biases do not share), 28 2^-24.
+    const float unsure = a.sigmoid ? 0x1p-20f : 0x1p-19f;
+    const int end = min(a.T, (int)(blockIdx.x + 1) * a.tokens);
+    for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
+        const int t = t0 + tok;
+        const bool live = t < end;
+        const float *row = a.logits + (size_t)(live ? t : t0) * E;
+        float z[V];
+        if (a.vec && C == 4) {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const float4 u = *(const float4 *)(row + min(expert(k), E - 4));
+                z[k] = u.x, z[(k + 1) % V] = u.y, z[(k + 2) % V] = u.z, z[(k + 3) % V] = u.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) z[k] = row[min(expert(k), E - 1)];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[k] = expert(k) < E ? open_logit(z[k]) : -INFINITY;
+        // scores, where the choice or the weights need all of them
+        float top = 0.0f, recip = 1.0f;
+        if (softmax_row) {
+            top = z[0];
+#pragma unroll
+            for (int k = 1; k < V; ++k) top = fmaxf(top, z[k]);
+            top = fmaxf(token_max<L>(top), -FLT_MAX);  // (a token without open experts: every score 0)
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += exp_near(z[k] - top);
+            s = token_sum<L>(s);
+            recip = s > 0.0f ? 1.0f / s : 0.0f;
+        }
+        const float most = 2.0f * recip + span;  // (sigmoid: scores up to 1)
+        bool doubt = false;
+        uint32_t word[V];
+        if (!WORTH) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) word[k] = ordered(z[k]);
+        } else {
+            float u[V];
+            if (a.sigmoid) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) u[k] = sigmoid_near(z[k]) + bias[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) u[k] = fmaf(exp_near(z[k] - top), recip, bias[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) u[k] = z[k] > -INFINITY && u[k] == u[k] ? u[k] : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < V; ++k) word[k] = ordered(a.bias != nullptr ? u[k] : z[k]);
+            if (a.groups > 1) {
+                wave_lds();  // (what the wave's last tokens left there has been read)
+#pragma unroll
+                for (int k = 0; k < V; ++k) uw[expert(k)] = u[k];
+                wave_lds();
+                const int q = 1 << a.group_shift, g = sub >> a.group_shift, i = sub & (q - 1);
+                float best = -INFINITY, second = -INFINITY;
+                auto meet = [&](float b, float s) {
+                    second = fmaxf(fmaxf(second, s), fminf(best, b));
+                    best = fmaxf(best, b);
+                };
+                if (g < a.groups) {
+#pragma unroll 4
+                    for (int e = g * a.per_group + i; e < (g + 1) * a.per_group; e += q) meet(uw[e], -INFINITY);
+                }
+                // (after each step its lanes hold the same, so that a mirror is a neighbour)
+                if (q > 1) meet(lane_of<0xB1>(best), lane_of<0xB1>(second));
+                if (q > 2) meet(lane_of<0x4E>(best), lane_of<0x4E>(second));
+                if (q > 4) meet(lane_of<0x141>(best), lane_of<0x141>(second));
+                if (q > 8) meet(lane_of<0x140>(best), lane_of<0x140>(second));
+                if (q > 16) meet(__shfl_xor(best, 16), __shfl_xor(second, 16));
+                const float mine = a.group_best == 2 && second > -INFINITY ? best + second : best;
+                wave_lds();
+                if (i == 0) uw[g] = mine;
+                wave_lds();
+                const float tell = 2.0f * unsure * most;  // (four worths and two additions)
+                int ahead = 0;
+                bool near = false;
+                for (int o0 = 0; o0 < a.groups; o0 += 4) {
+                    const float4 o4 = *(const float4 *)(uw + o0);
+                    const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool there = o0 + k < a.groups, in_front = there && (o[k] > mine || (o[k] == mine && o0 + k < g));
+                        ahead += in_front ? 1 : 0;
+                        near |= there && !in_front && o0 + k != g && o[k] > -INFINITY && !(mine - o[k] > tell);
+                    }
+                }
+                doubt = g < a.groups && near && ahead == a.top_groups - 1;  // (the last group that stays, and one behind it)
+                const unsigned long long stays = __ballot(i == 0 && g < a.groups && ahead < a.top_groups);
+                const unsigned long long stay = L == 64 ? stays : stays >> (lane & 48);
+                if ((a.per_group & (C - 1)) == 0) {  // (a piece is one group's)
+#pragma unroll
+                    for (int k = 0; k < V; k += C) {
+                        const bool in = (stay >> ((((uint32_t)expert(k) * (uint32_t)a.group_magic >> 20) << a.group_shift) & (L - 1))) & 1;
+#pragma unroll
+                        for (int n = 0; n < C; ++n) word[k + n] = in ? word[k + n] : 0u;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; ++k)
+                        word[k] = (stay >> ((((uint32_t)expert(k) * (uint32_t)a.group_magic >> 20) << a.group_shift) & (L - 1))) & 1 ? word[k] : 0u;
+                }
+            }
+        }
+        int held = 0;  // words of the lane
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            held += word[k] ? 1 : 0;
+            word[k] = word[k] ? (word[k] & ~LOW) | (LOW - k) : 0u;
+        }
+        // descending (Batcher's odd-even merges)
+#pragma unroll
+        for (int p = 1; p < V; p *= 2)
+#pragma unroll
+            for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+                for (int j = k % p; j <= V - 1 - k; j += 2 * k)
+#pragma unroll
+                    for (int i = 0; i < k; ++i)
+                        if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                            const uint32_t x = word[i + j], y = word[i + j + k];
+                            word[i + j] = max(x, y);
+                            word[i + j + k] = min(x, y);
+                        }
+        wave_lds();
+        uint32_t first = word[0], next = V > 1 ? word[1 % V] : 0u;
+#pragma unroll
+        for (int k = 2; k < V; ++k) list[64 * k] = word[k];
+        list[64 * V] = 0u;
+        int taken = 0;
+        for (int j = 0; j < K; ++j) {
+            const uint32_t b = token_max<L>(first);
+            if (first == b) {  // (two lanes: told by what they have taken, and chosen for again; none left: all of them, nothing)
+                picks[j] = u32x2{b, (uint32_t)sub};
+                taken = min(taken + 1, held);
+                first = next;
+                next = list[64 * min(taken + 1, V)];
+            }
+        }
+        const uint32_t behind = token_max<L>(first);
+        if (sub == 0) picks[K] = u32x2{behind, 0u};
+        wave_lds();
+        // The chosen and, next to each, the one behind it: lane sub has the places sub, sub + L, ...
+        int at[KL], all = -taken;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+            const int j = sub + i * L;
+            at[i] = ROUTE_NONE;
+            if (j < K) {
+                const u32x2 p = picks[j];
+                const uint32_t b = p[0], o = picks[j + 1][0];
+                const int k = (int)(LOW - (b & LOW));
+                if (b) {
+                    at[i] = (k / C) * (L * C) + (int)p[1] * C + k % C;
+                    ++all;
+                    if (WORTH && a.bias != nullptr) doubt |= o && !(of_ordered(b & ~LOW) - of_ordered(o & ~LOW) > (unsure + (float)V * 0x1p-23f) * most);  // (the words' last bits besides)
+                    else doubt |= (b & ~LOW) == (o & ~LOW);
+                } else if (a.fill) doubt = true;
+            }
+        }
+        doubt |= token_sum<L>((float)all) != 0.0f;  // (as many taken as chosen: no two lanes held the same word)
+        const unsigned long long doubts = L == 64 ? __ballot(doubt) : __ballot(doubt) >> (lane & 48) & 0xffffull;
+        if (doubts && live && sub == 0) again[atomicAdd(&n_again, 1)] = t;
+        route_write<L>(a, row, t, live && !doubts, sub, at, top, recip, hist);
+        wave_lds();
+    }
+    __syncthreads();
+    // in double, a wave each
+    for (int i = wave; i < n_again; i += NT / 64) {
+        const int t = again[i];
+        const float *row = a.logits + (size_t)t * E;
+        float top, recip;
+        const int at[1] = {route_exact(a, row, (double *)spare, &top, &recip)};
+        route_write<64>(a, row, t, true, lane, at, top, recip, hist);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += NT) a.part[(size_t)blockIdx.x * E + e] = hist[e];
+}
+
+// counts = sums of n rows of part [n][E]: a workgroup takes 16 experts, 64 rows at a time
+__global__ __launch_bounds__(1024) void route_counts_kernel(const int32_t *__restrict__ part, int n, int E, int32_t *__restrict__ counts)
+{
+    __shared__ int red[16][16];
+    const int cc = threadIdx.x & 15, k = threadIdx.x >> 4, e = blockIdx.x * 16 + cc;
+    int s = 0;
+    for (int i0 = k; i0 < n && e < E; i0 += 64 * 8) {  // eight rows asked for together
+        int v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i0 + 64 * j < n ? part[(size_t)(i0 + 64 * j) * E + e] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if ((threadIdx.x & 48) == 0) red[threadIdx.x >> 6][cc] = s;
+    __syncthreads();
+    if (threadIdx.x >= 16 || e >= E) return;
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += red[w][cc];
+    counts[e] = s;
+}
+
+struct route_back_args {
+    const float *logits;
+    int T, E, K, sigmoid, renorm;
+    float scale;
+    const int32_t *ids;
+    const float *w, *dw;
+    float *dlogits;
+};
+// L lanes a token; a lane takes the chosen j = sub, sub + L, ... and the experts sub V .. of each stretch of L V.
+template <int L, int V>
+__global__ __launch_bounds__(256) void route_backward_kernel(const route_back_args a)
+{
+    constexpr int TW = 64 / L, KL = 64 / L;
+    __shared__ float dzs[4][TW][L * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & (L - 1), tok = lane / L;
+    const int E = a.E, K = a.K, t = (blockIdx.x * 4 + wave) * TW + tok, e0 = sub * V;
+    const bool live = t < a.T;
+    float *dz = dzs[wave][tok];
+    const size_t row = (size_t)t * E, pick = (size_t)t * K;
+    int id[KL];
+    float w[KL], g[KL], z[V];
+    const bool all = !a.sigmoid && !a.renorm;  // every score has a part in the gradient
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = all && live && e0 + k < E ? open_logit(a.logits[row + e0 + k]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+        const int j = sub + i * L;
+        id[i] = live && j < K ? a.ids[pick + j] : ROUTE_NONE;
+        if (id[i] >= E) id[i] = ROUTE_NONE;
+        w[i] = id[i] >= 0 ? a.w[pick + j] : 0.0f;
+        g[i] = id[i] >= 0 && w[i] != 0.0f ? a.dw[pick + j] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) dz[e0 + k] = 0.0f;
+    wave_lds();
+    float dot = 0.0f;
+    if (a.renorm) {
+        // by differences: what all chosen have in common has no part in the gradient
+        float d[KL];
+#pragma unroll
+        for (int i = 0; i < KL; ++i) d[i] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < KL; ++p)
+            for (int k = 0; k < min(L, K - p * L); ++k) {
+                const float wk = __shfl(w[p], k, L), gk = __shfl(g[p], k, L);
+#pragma unroll
+                for (int i = 0; i < KL; ++i) d[i] = fmaf(wk, g[i] - gk, d[i]);
+            }
+#pragma unroll
+        for (int i = 0; i < KL; ++i) g[i] = d[i] / a.scale;
+    } else if (all) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) dot = fmaf(w[i], g[i], dot);
+        dot = token_sum<L>(dot);
+    }
+#pragma unroll
+    for (int i = 0; i < KL; ++i)
+        if (w[i] != 0.0f) {
+            float v = w[i] * g[i];
+            if (a.sigmoid) v *= sigmoid(-open_logit(a.logits[row + id[i]]));  // 1 - s
+            atomicAdd(&dz[id[i]], v);
+        }
+    wave_lds();
+    float top = 0.0f, recip = 0.0f;
+    if (all) {
+        top = z[0];
+#pragma unroll
+        for (int k = 1; k < V; ++k) top = fmaxf(top, z[k]);
+        top = fmaxf(token_max<L>(top), -FLT_MAX);
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) s += exp_neg(z[k] - top);
+        s = token_sum<L>(s);
+        recip = s > 0.0f ? 1.0f / s : 0.0f;
+    }
+    if (!live) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (e0 + k < E) a.dlogits[row + e0 + k] = all ? fmaf(-exp_neg(z[k] - top) * recip, dot, dz[e0 + k]) : dz[e0 + k];
+}
+
+// bias[e] += rate where an expert was chosen less often than the mean, -= rate where more often
+__global__ __launch_bounds__(256) void route_balance_kernel(const int32_t *__restrict__ counts, int E, float rate, float *__restrict__ bias)
+{
+    __shared__ long long red[256];
+    long long s = 0;
+    for (int e = threadIdx.x; e < E; e += 256) s += counts[e];
+    red[threadIdx.x] = s;
+    for (int n = 128; n > 0; n >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < n) red[threadIdx.x] += red[threadIdx.x + n];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += 256) {
+        const long long over = (long long)counts[e] * E - red[0];
+        if (over != 0) bias[e] += over < 0 ? rate : -rate;
+    }
+}
+
+// Sixteen lanes a token do the least work for it, a wave ends soonest.  (Groups: one lane for each at least.)
+static bool route_by_waves(const omega_ctx *ctx, const omega_route_config &c, int T) { return c.E > 256 || c.groups > 16 || (c.E > 64 && T <= 16 * ctx->num_cus); }
+#define ROUTE_THREADS 512
+
+static hipError_t route_launch(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, bool waves, int threads, int fill, int32_t *ids,
+                               float *w, int32_t *part, hipStream_t s)
+{
+    const int E = c.E, L = waves ? 64 : 16, vec = E % 4 == 0 && (uintptr_t)logits % 16 == 0;
+    const bool worth = bias != nullptr || c.groups > 1;
+    int shift = 0;  // lanes of a group: as many as the next power of two of groups leaves
+    while (c.groups > 1 && (2 << shift) * c.groups <= L) ++shift;
+    const route_args a = {logits, bias, T, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.groups, c.top_groups, c.group_best, E / c.groups, (1 << 20) / (E / c.groups) + 1,
+                          shift, c.scale, tokens, fill, vec, ids, w, part};
+#define ROUTE_FORWARD(LL, V)                                                                                                                     \
+    do {                                                                                                                                         \
+        const dim3 grid(ceil_div(T, tokens));                                                                                                    \
+        const size_t lds = threads / 64 * route_lds(LL, V) * sizeof(float);                                                                      \
+        if (worth) hipLaunchKernelGGL((route_forward_kernel<LL, V, true>), grid, dim3(threads), lds, s, a);                                      \
+        else hipLaunchKernelGGL((route_forward_kernel<LL, V, false>), grid, dim3(threads), lds, s, a);                                           \
+    } while (0)
+    if (waves) {
+        if (E <= 64) ROUTE_FORWARD(64, 1);
+        else if (E <= 128) ROUTE_FORWARD(64, 2);
+        else if (E <= 256) ROUTE_FORWARD(64, 4);
+        else ROUTE_FORWARD(64, 8);
+    } else {
+        if (E <= 16) ROUTE_FORWARD(16, 1);
+        else if (E <= 64) ROUTE_FORWARD(16, 4);
+        else if (E <= 128) ROUTE_FORWARD(16, 8);
+        else ROUTE_FORWARD(16, 16);
+    }
+#undef ROUTE_FORWARD
+    return hipGetLastError();
+}
+
+// Tokens of a workgroup of the operator: whole rounds of its waves, two workgroups for a compute unit; one workgroup's up to four rounds need no
+// second launch for the counts
+static int route_tokens(const omega_ctx *ctx, const omega_route_config &c, int T)
+{
+    const int round = ROUTE_THREADS / 64 * (route_by_waves(ctx, c, T) ? 1 : 4);
+    if (T <= 4 * round) return 4 * round;
+    return std::min(std::max(1, ceil_div(ceil_div(T, 2 * ctx->num_cus), round)) * round, ROUTE_TOKENS);
+}
+size_t route_workspace(const omega_ctx *ctx, const omega_route_config &c, int T) { return (size_t)ceil_div(T, route_tokens(ctx, c, T)) * c.E * sizeof(int32_t); }
+
+hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &c, const float *logits, int T, const float *bias, int32_t *ids, float *w,
+                                int32_t *counts, void *ws, hipStream_t s)
+{
+    int n = 0;
+    if (T > 0) {
+        const int tokens = route_tokens(ctx, c, T);
+        n = ceil_div(T, tokens);
+        const hipError_t e = route_launch(c, logits, T, bias, tokens, route_by_waves(ctx, c, T), ROUTE_THREADS, 0, ids, w, n == 1 && counts ? counts : (int32_t *)ws, s);
+        if (e != hipSuccess || n == 1 || !counts) return e;
+    }
+    hipLaunchKernelGGL(route_counts_kernel, dim3(ceil_div(c.E, 16)), dim3(1024), 0, s, (const int32_t *)ws, n, c.E, counts);
+    return hipGetLastError();
+}
+
+// (workgroups of as many tokens as a row of the layer's histogram has: sixteen lanes a token are one round of four waves)
+hipError_t launch_route_layer(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, int32_t *ids, float *w, int32_t *tile_counts,
+                              hipStream_t s)
+{
+    return route_launch(c, logits, T, bias, tokens, c.E > 256 || c.groups > 16, 256, 1, ids, w, tile_counts, s);
+}
+
+#define ROUTE_RUN(K, grid, s, ...)                                                                       \
+    do {                                                                                                 \
+        if (E <= 16) hipLaunchKernelGGL((K<16, 1>), dim3(grid), dim3(256), 0, s, __VA_ARGS__);            \
+        else if (E <= 64) hipLaunchKernelGGL((K<16, 4>), dim3(grid), dim3(256), 0, s, __VA_ARGS__);       \
+        else if (E <= 128) hipLaunchKernelGGL((K<16, 8>), dim3(grid), dim3(256), 0, s, __VA_ARGS__);      \
+        else if (E <= 256) hipLaunchKernelGGL((K<16, 16>), dim3(grid), dim3(256), 0, s, __VA_ARGS__);     \
+        else hipLaunchKernelGGL((K<64, 8>), dim3(grid), dim3(256), 0, s, __VA_ARGS__);                    \
+    } while (0)
+
+hipError_t launch_route_backward(const omega_route_config &c, const float *logits, int T, const int32_t *ids, const float *w, const float *dw, float *dlogits,
+                                 hipStream_t s)
+{
+    const int E = c.E, round = E <= 256 ? 16 : 4, most = round << 22;  // (a launch holds fewer than 2^32 lanes: tokens in several)
+    for (int t = 0; t < T; t += most) {
+        const int n = std::min(most, T - t);
+        const size_t row = (size_t)t * E, pick = (size_t)t * c.K;
+        const route_back_args a = {logits ? logits + row : nullptr, n, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.scale, ids + pick, w + pick, dw + pick, dlogits + row};
+        ROUTE_RUN(route_backward_kernel, ceil_div(n, round), s, a);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_route_balance(const int32_t *counts, int E, float rate, float *bias, hipStream_t s)
+{
+    hipLaunchKernelGGL(route_balance_kernel, dim3(1), dim3(256), 0, s, counts, E, rate, bias);
+    return hipGetLastError();
+}

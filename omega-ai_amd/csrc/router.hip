@@ -795,7 +795,8 @@ hipError_t router_init(void)
     return hipSuccess;
 }
 
-hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits_out, float *probs_out, hipStream_t s)
+// K = 0: logits (and probabilities) only
+static hipError_t launch_softmax_router(const omega_moe *m, const void *x, int T, int K, float *logits_out, float *probs_out, hipStream_t s)
 {
     const omega_moe_config &c = m->cfg;
     const int tiles = ceil_div(T, router_tok_tile(m, T));
@@ -804,7 +805,7 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
     if (!exact && router_on_mfma(m) && ((uintptr_t)x % 16) == 0) {
 #define ROUTER_MFMA_LAUNCH(EPV)                                                                                          \
     hipLaunchKernelGGL(router_mfma_kernel<EPV>, dim3(tiles), dim3(256), 0, s, (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, \
-                       c.d, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out)
+                       c.d, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out)
         if (c.E <= 32) ROUTER_MFMA_LAUNCH(32);
         else if (c.E <= 64) ROUTER_MFMA_LAUNCH(64);
         else if (c.E <= 128) ROUTER_MFMA_LAUNCH(128);
@@ -825,12 +826,12 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
         ceil_div(T, tpw) * groups <= m->ctx->num_cus && c.d >= split_d && (((uintptr_t)x | (uintptr_t)m->Wg) % 16) == 0) {
         float *lg = logits_out != nullptr ? logits_out : m->gate_logits;
         hipLaunchKernelGGL((router_pipe_kernel<16, true>), dim3(ceil_div(T, tpw) * groups), dim3(16 * 16 + RP_STAGERS), router_pipe_smem_bytes(16),
-                           s, (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, lg,
+                           s, (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, lg,
                            (float *)nullptr, groups, tpw);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
 #define ROUTER_SELECT(EPV) \
-    hipLaunchKernelGGL(router_select_kernel<EPV>, dim3(tiles), dim3(256), 0, s, (const float *)lg, T, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, probs_out)
+    hipLaunchKernelGGL(router_select_kernel<EPV>, dim3(tiles), dim3(256), 0, s, (const float *)lg, T, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, probs_out)
         if (c.E <= 32) ROUTER_SELECT(32);
         else if (c.E <= 64) ROUTER_SELECT(64);
         else if (c.E <= 128) ROUTER_SELECT(128);
@@ -850,7 +851,7 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
         }
 #define ROUTER_UNITS(EPV, TTV, NWV, CEV, CTV)                                                                            \
     hipLaunchKernelGGL((router_units_kernel<EPV, TTV, NWV, CEV, CTV>), dim3(tiles), dim3(64 * NWV), 0, s, (const bf16_t *)x, \
-                       (const float4 *)m->gate_img, bg, T, c.d, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out)
+                       (const float4 *)m->gate_img, bg, T, c.d, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out)
         if (c.E <= 32) { if (tt == 16) ROUTER_UNITS(32, 16, 2, 1, 1); else ROUTER_UNITS(32, 32, 4, 1, 1); }
         else if (c.E <= 64) { if (tt == 16) ROUTER_UNITS(64, 16, 4, 1, 1); else ROUTER_UNITS(64, 32, 4, 1, 2); }
         else if (c.E <= 128) { if (tt == 16) ROUTER_UNITS(128, 16, 4, 2, 1); else ROUTER_UNITS(128, 32, 8, 1, 2); }
@@ -863,11 +864,11 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
         (((uintptr_t)x | (uintptr_t)m->Wg) % 16) == 0) {
         if (c.E <= 8)
             hipLaunchKernelGGL((router_pipe_kernel<8, false>), dim3(tiles), dim3(16 * 8 + RP_STAGERS), router_pipe_smem_bytes(8), s,
-                               (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, c.K, c.renorm, m->ids, m->w,
+                               (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, K, c.renorm, m->ids, m->w,
                                m->tile_counts, logits_out, probs_out, 1, 16);
         else
             hipLaunchKernelGGL((router_pipe_kernel<16, false>), dim3(tiles), dim3(16 * 16 + RP_STAGERS), router_pipe_smem_bytes(16), s,
-                               (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, c.K, c.renorm, m->ids, m->w,
+                               (const bf16_t *)x, (const bf16_t *)m->Wg, bg, T, c.d, c.E, K, c.renorm, m->ids, m->w,
                                m->tile_counts, logits_out, probs_out, 1, 16);
         return hipGetLastError();
     }
@@ -875,10 +876,10 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
     do {                                                                                                           \
         if (exact)                                                                                                 \
             hipLaunchKernelGGL((router_kernel<EPV, KCV, true>), dim3(tiles), dim3(ROUTER_NTHR(EPV)), 0, s, x, c.dtype, m->Wg, bg, \
-                               T, c.d, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out);   \
+                               T, c.d, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, logits_out, probs_out);   \
         else                                                                                                       \
             hipLaunchKernelGGL((router_kernel<EPV, KCV, false>), dim3(tiles), dim3(ROUTER_NTHR(EPV)), 0, s, x, c.dtype, m->Wg,    \
-                               bg, T, c.d, c.E, c.K, c.renorm, m->ids, m->w, m->tile_counts, logits_out,           \
+                               bg, T, c.d, c.E, K, c.renorm, m->ids, m->w, m->tile_counts, logits_out,           \
                                probs_out);                                                                         \
     } while (0)
     if (c.E <= 8) ROUTER_LAUNCH(8, ROUTER_KC_SMALL);
@@ -889,4 +890,12 @@ hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits
     else ROUTER_LAUNCH(256, 64);
 #undef ROUTER_LAUNCH
     return hipGetLastError();
+}
+
+hipError_t launch_router(const omega_moe *m, const void *x, int T, float *logits_out, float *probs_out, hipStream_t s)
+{
+    if (!m->own_routing) return launch_softmax_router(m, x, T, m->cfg.K, logits_out, probs_out, s);
+    float *lg = logits_out != nullptr ? logits_out : m->route_logits;
+    const hipError_t e = launch_softmax_router(m, x, T, 0, lg, probs_out, s);
+    return e != hipSuccess ? e : launch_route_layer(m->route, lg, T, m->route_bias, router_tok_tile(m, T), m->ids, m->w, m->tile_counts, s);
 }

@@ -130,6 +130,7 @@ class MoELayer:
         self.lib = self.ctx.lib
         self.embedDim, self.hidden, self.nExperts, self.topK = embedDim, hidden, nExperts, topK
         self.renorm, self.nShared, self.hasBias, self.dtype = bool(renorm), nShared, bool(bias), dtype
+        self.hasBalance = False
         self.oChannel, self.oHeight, self.oWidth = 1, 1, embedDim
         self.number = 0
         self.input = None
@@ -146,7 +147,7 @@ class MoELayer:
 
     # ---- parameters
     def _upload(self, which, expert, a):
-        if which in (L.W_GATE_BIAS, L.W_NORM) or self.dtype == "f32":
+        if which in (L.W_GATE_BIAS, L.W_NORM, L.W_BALANCE) or self.dtype == "f32":
             h = np.ascontiguousarray(a, np.float32)
         else:
             h = f32_to_bf16_bits(a)
@@ -251,6 +252,24 @@ class MoELayer:
 
     def initCache(self):
         pass
+
+    def set_routing(self, config, bias=False):
+        """Routing of the layer by a route_config (block_ops.py; its nExperts and topK are the layer's) instead of the softmax top-k; bias: with a bias for
+        balance (set_balance, balance).  None: the softmax top-k again."""
+        self.ctx.check(self.lib.omega_moe_set_routing(self.handle, C.byref(config) if config is not None else None, int(bool(bias))))
+        self.hasBalance = config is not None and bool(bias)
+
+    def set_balance(self, b):
+        """The routing's bias for balance, [nExperts] fp32."""
+        assert b.shape == (self.nExperts,)
+        self._upload(L.W_BALANCE, 0, b)
+
+    def balance(self, rate):
+        """One step of the bias for balance by what the last forward gave each expert."""
+        self.ctx.check(self.lib.omega_moe_balance(self.handle, float(rate)))
+
+    def balance_bias(self):
+        return self._download_weight(L.W_BALANCE, 0, (self.nExperts,))
 
     def set_training(self, on=True):
         """Forward keeps h1 / h3 for back(), as the reference's layers keep their outputs."""
@@ -425,9 +444,9 @@ class MoELayer:
         """Every byte of the 'a' or 'y' buffer (padding rows included) set to byte_value; 0xFF reads as NaN."""
         self.ctx.check(self.lib.omega_moe_fill_workspace(self.handle, {"a": 1, "y": 2}[which], int(byte_value)))
 
-    # ---- checkpoint: raw LE float32, order gate, (gate bias), then w1,w3,w2 per expert, routed then shared
+    # ---- checkpoint: raw LE float32, order gate, (gate bias), (bias for balance), then w1,w3,w2 per expert, routed then shared
     def _download_weight(self, which, expert, shape):
-        raw_bf16 = self.dtype == "bf16" and which not in (L.W_GATE_BIAS, L.W_NORM)   # those two are fp32 in every layer
+        raw_bf16 = self.dtype == "bf16" and which not in (L.W_GATE_BIAS, L.W_NORM, L.W_BALANCE)   # those are fp32 in every layer
         h = np.empty(shape, np.uint16 if raw_bf16 else np.float32)
         self.ctx.check(self.lib.omega_moe_get_weights(self.handle, which, expert, h.ctypes.data, 0))
         return bf16_bits_to_f32(h) if raw_bf16 else h
@@ -436,6 +455,8 @@ class MoELayer:
         items = [(L.W_GATE, 0, (self.nExperts, self.embedDim))]
         if self.hasBias:
             items.append((L.W_GATE_BIAS, 0, (self.nExperts,)))
+        if self.hasBalance:
+            items.append((L.W_BALANCE, 0, (self.nExperts,)))
         for g in range(self.nExperts + self.nShared):
             items += [(L.W_W1, g, (self.hidden, self.embedDim)), (L.W_W3, g, (self.hidden, self.embedDim)),
                       (L.W_W2, g, (self.embedDim, self.hidden))]

@@ -72,7 +72,7 @@ def test_against_the_definition(T, d, dtype, form):
 def test_quotients_on_and_next_to_a_half(dtype):
     """Whole and half multiples of a scale, and their neighbours in fp32: every code and border."""
     for most in (127.0, 127.0 * 2.0 ** -20, 254.0 * 3.0, 1.0, 3.3e38, 2.0 ** -118):
-        s = np.float32(np.float32(most) / np.float32(127.0))
+        s = np.float32(np.float32(most) * np.float32(1.0 / 127.0))
         near = (np.arange(-253, 254) * 0.5 * np.float64(s)).astype(np.float32)
         x = np.concatenate([near, np.nextafter(near, np.float32(np.inf)), np.nextafter(near, np.float32(-np.inf))])
         x = x[np.abs(x) < most]
