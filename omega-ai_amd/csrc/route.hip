@@ -8,7 +8,8 @@
 //   back     renorm: dz_j = w_j sum_k (w_k / scale)(dw_j - dw_k) (1 - s_j for sigmoid); else sigmoid: w_j dw_j (1 - s_j), softmax: [chosen] w_j dw_j - s_e sum_k w_k dw_k
 //
 // The choice is that of worths in 64 bits.  They are formed in fp32, a few instructions an expert, and where two that the choice tells apart are nearer
-// to each other than their errors, or equal, the token is chosen for again in double, by its whole wave (route_exact).
+// to each other than their errors, or equal, those few are formed in double and put in order; where they are not few, or it is groups, the whole token is
+// chosen for again in double, by a wave of its workgroup at the end (route_exact).
 // L lanes share a token, V experts a lane.  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
 // replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
 // the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
@@ -53,6 +54,12 @@ __device__ __forceinline__ uint32_t over_token(uint32_t v, F meet)
     }
     return v;
 }
+// the bits of a ballot that a token's lanes have
+template <int L>
+__device__ __forceinline__ unsigned long long token_bits(unsigned long long lanes)
+{
+    return L == 64 ? lanes : (lanes >> (threadIdx.x & 48)) & 0xffffull;
+}
 template <int L>
 __device__ __forceinline__ float token_max(float v)
 {
@@ -84,16 +91,27 @@ __device__ __forceinline__ float sigmoid(float z)
     const float e = exp_neg(-fabsf(z));
     return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
+// the larger of v and -infinity: no number becomes -infinity (written out: a comparison and a choice are two instructions)
+__device__ __forceinline__ float or_closed(float v)
+{
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(v), "s"(0xff800000u));
+    return r;
+}
 // a logit as it is compared: closed ones -infinity, infinite ones the largest number
-__device__ __forceinline__ float open_logit(float z) { return z == z ? fminf(z, FLT_MAX) : -INFINITY; }
+__device__ __forceinline__ float open_logit(float z) { return fminf(or_closed(z), FLT_MAX); }
 
-// A float as a whole number of the same order, 0 for -infinity; and back
+// A float as a whole number of the same order; and back
+#define ROUTE_OPEN 0x00800000u  // that of the lowest number: -infinity's is below, and so is 0
 __device__ __forceinline__ uint32_t ordered(float v)
 {
     const uint32_t u = __float_as_uint(v + 0.0f);  // (both zeros the same)
-    return v == -INFINITY ? 0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float of_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// element i of p, the same p in a wave
+__device__ __forceinline__ float ld_at(const float *p, uint32_t i) { return *(const float *)((const char *)p + (i << 2)); }
 
 // the lanes of a wave see each other's LDS writes
 __device__ __forceinline__ void wave_lds()
@@ -146,38 +164,51 @@ __device__ __forceinline__ double over_wave(double v, F meet)
 __device__ __forceinline__ double wave_max(double v) { return over_wave(v, [](double a, double b) { return fmax(a, b); }); }
 
 // The choice for one token in double, by a wave: lane j's place.  row: its logits; spare: room for E doubles in LDS; top and recip: of its softmax.
+template <int N>
 __device__ __forceinline__ int route_exact(const route_args &a, const float *row, double *spare, float *top_out, float *recip_out)
 {
     const int lane = threadIdx.x & 63, E = a.E;
-    double m = -INFINITY, sum = 1.0;
+    float z[N], bias[N];  // of experts lane + 64 i
+    double key[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = row[min(lane + 64 * i, E - 1)];
+#pragma unroll
+    for (int i = 0; i < N; ++i) bias[i] = a.bias != nullptr ? a.bias[min(lane + 64 * i, E - 1)] : 0.0f;
+    double m = 0.0, sum = 1.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = lane + 64 * i < E ? open_logit(z[i]) : -INFINITY;
     if (!a.sigmoid) {
-        for (int e = lane; e < E; e += 64) m = fmax(m, (double)open_logit(row[e]));
-        m = wave_max(m);
+        float top = z[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+        m = (double)fmaxf(token_max<64>(top), -FLT_MAX);
         sum = 0.0;
     }
-#pragma unroll 1
-    for (int e = lane; e < E; e += 64) {
-        const double z = (double)open_logit(row[e]);
-        const double v = a.sigmoid ? 1.0 / (1.0 + exp(-z)) : z == -INFINITY ? 0.0 : exp(z - m);
-        if (!a.sigmoid) sum += v;
-        spare[e] = v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {  // (closed ones: e^-inf = 0)
+        key[i] = exp(a.sigmoid ? -(double)z[i] : (double)z[i] - m);
+        if (!a.sigmoid) sum += key[i];
+        if (N > 2 && i & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time: registers)
     }
     if (!a.sigmoid) sum = over_wave(sum, [](double x, double y) { return x + y; });
-    *top_out = fmaxf((float)m, -FLT_MAX);
+    *top_out = (float)m;
     *recip_out = sum > 0.0 ? (float)(1.0 / sum) : 0.0f;
-#pragma unroll 1
-    for (int e = lane; e < E; e += 64) {
-        double v = a.sigmoid ? spare[e] : spare[e] / sum;
-        if (a.bias != nullptr) v += (double)a.bias[e];
-        spare[e] = open_logit(row[e]) == -INFINITY || !(v == v) ? -INFINITY : v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const double v = (a.sigmoid ? 1.0 / (1.0 + key[i]) : key[i] / sum) + (double)bias[i];
+        key[i] = z[i] == -INFINITY || !(v == v) ? -INFINITY : v;
+        if (N > 2 && i & 1) __builtin_amdgcn_sched_barrier(0);
     }
-    wave_lds();
-    unsigned long long stay = ~0ull;
     if (a.groups > 1) {
+        wave_lds();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (lane + 64 * i < E) spare[lane + 64 * i] = key[i];
+        wave_lds();
         double best = -INFINITY;
         if (lane < a.groups) {
             double second = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
             for (int e = lane * a.per_group; e < (lane + 1) * a.per_group; ++e) {
                 const double v = spare[e];
                 second = fmax(second, fmin(best, v));
@@ -190,24 +221,25 @@ __device__ __forceinline__ int route_exact(const route_args &a, const float *row
             const double v = __shfl(best, g);
             ahead += v > best || (v == best && g < lane) ? 1 : 0;
         }
-        stay = __ballot(lane < a.groups && ahead < a.top_groups);
+        const unsigned long long stay = __ballot(lane < a.groups && ahead < a.top_groups);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!((stay >> (((uint32_t)(lane + 64 * i) * (uint32_t)a.group_magic >> 20) & 63)) & 1)) key[i] = -INFINITY;
         wave_lds();
     }
-    // what is compared, a lane's own; bit i of left: expert lane + 64 i has not been chosen
-    uint32_t left = 0;
-    for (int i = 0, e = lane; e < E; ++i, e += 64) {
-        left |= 1u << i;
-        if (!((stay >> (a.groups > 1 ? (uint32_t)e * (uint32_t)a.group_magic >> 20 : 0)) & 1)) spare[e] = -INFINITY;
-        else if (a.bias == nullptr && spare[e] > -INFINITY) spare[e] = (double)open_logit(row[e]);
-    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (a.bias == nullptr && key[i] > -INFINITY) key[i] = (double)z[i];
+    uint32_t left = 0;  // bit i: expert lane + 64 i has not been chosen
+#pragma unroll
+    for (int i = 0; i < N; ++i) left |= lane + 64 * i < E ? 1u << i : 0u;
     int place = ROUTE_NONE;
     for (int j = 0; j < a.K; ++j) {
         double bv = -INFINITY;
         int be = INT_MAX;
-        for (int i = 0, e = lane; e < E; ++i, e += 64) {
-            const double v = spare[e];
-            if (((left >> i) & 1) && (be == INT_MAX || v > bv)) bv = v, be = e;
-        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (((left >> i) & 1) && (be == INT_MAX || key[i] > bv)) bv = key[i], be = lane + 64 * i;
         const double top = wave_max(bv);
         const bool none = top == -INFINITY;  // (a layer's token then takes the first of the others)
         if (none && !a.fill) break;
@@ -215,11 +247,10 @@ __device__ __forceinline__ int route_exact(const route_args &a, const float *row
         const unsigned long long have = __ballot(e != INT_MAX);
         if (have & (have - 1)) {  // equal ones: the first
             for (int s = 32; s > 0; s >>= 1) e = min(e, __shfl_xor(e, s));
-        } else e = __shfl(e, __ffsll((long long)have) - 1);
+        } else e = __builtin_amdgcn_readlane(e, __ffsll((long long)have) - 1);
         if ((e & 63) == lane) left &= ~(1u << (e >> 6));
         if (lane == j) place = none ? e | ROUTE_FILL : e;
     }
-    wave_lds();
     return place;
 }
 
@@ -271,41 +302,55 @@ __device__ __forceinline__ void route_write(const route_args &a, const float *ro
     }
 }
 
-// Words of LDS that a wave needs: the worths of its tokens for their groups, then the lanes' lists and one more word each; one token's worths in double
-static constexpr int route_lds(int L, int V) { return 64 * (V + 1) > 2 * L * V ? 64 * (V + 1) : 2 * L * V; }
+// A token in doubt, by a wave
+template <int N>
+__device__ __forceinline__ void route_again(const route_args &a, int t, double *spare, int *hist)
+{
+    const float *row = a.logits + (size_t)t * a.E;
+    float top, recip;
+    const int at[1] = {route_exact<N>(a, row, spare, &top, &recip)};
+    route_write<64>(a, row, t, true, threadIdx.x & 63, at, top, recip, hist);
+}
+
+// Words of LDS that a wave needs: the worths of its tokens for their groups (four words of padding behind 32: groups of 32 in different banks), then the
+// lanes' lists and one more word each; one token's worths in double
+static constexpr int route_worths(int E) { return E + E / 8; }
+__device__ __forceinline__ int route_padded(int e) { return e + (e >> 5) * 4; }
+static constexpr int route_lds(int L, int V) { return std::max(std::max(64 * (V + 1), 2 * L * V), 64 / L * route_worths(L * V)); }
 
 // WORTH: there is a bias or there are groups
 template <int L, int V, bool WORTH>
-__global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args a)
+__global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
 {
     constexpr int TW = 64 / L, EW = L * V, KL = 64 / L;  // tokens of a wave, experts, chosen ones of a lane
     constexpr int C = V < 4 ? V : 4;                     // a lane's experts lie in pieces of C: k is expert (k / C) L C + sub C + k % C
     constexpr uint32_t LOW = V - 1;                      // bits of a word that say which of a lane's experts it is
     static_assert((V & (V - 1)) == 0 && V * L <= ROUTE_MAX_E, "places of a lane's experts in whole bits");
     extern __shared__ __attribute__((aligned(16))) uint32_t spare_all[];
-    __shared__ u32x2 picks_all[8][TW][64 + 1];           // the chosen words and their lanes
+    __shared__ u32x2 picks_all[8][TW][64 + 2];           // the chosen words and their lanes
     __shared__ int again[ROUTE_TOKENS], n_again;         // tokens that are chosen for in double
     __shared__ int hist[EW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & (L - 1), tok = lane / L;
+    __shared__ __attribute__((aligned(16))) float bias[WORTH ? EW : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane & (L - 1), tok = lane / L;
     const int E = a.E, K = a.K, NT = blockDim.x;
-    uint32_t *spare = spare_all + wave * route_lds(L, V), *list = spare + lane;
-    float *uw = (float *)spare + tok * EW;
-    u32x2 *picks = picks_all[wave][tok];
+    uint32_t *spare = spare_all + wave * (route_lds(L, V) + TW * 2 * (K + 2)), *list = spare + lane;
+    float *uw = (float *)spare + tok * route_worths(EW);
+    u32x2 *picks = (u32x2 *)(spare + route_lds(L, V)) + tok * (K + 2);  // the chosen words and the lanes that held them, and two behind them
     const bool softmax_row = !a.sigmoid && (WORTH || !a.renorm);
-    for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
+    for (int e = threadIdx.x; e < EW; e += NT) {
+        hist[e] = 0;
+        if (WORTH) bias[e] = a.bias != nullptr && e < E ? a.bias[e] : 0.0f;
+    }
     if (threadIdx.x == 0) n_again = 0;
     __syncthreads();
-    auto expert = [&](int k) { return (k / C) * (L * C) + sub * C + k % C; };
-    float bias[V], span = 0.0f;  // (span: the largest finite bias)
-#pragma unroll
-    for (int k = 0; k < V; ++k) bias[k] = 0.0f;
+    float span = 0.0f;  // the largest finite bias
     if (WORTH && a.bias != nullptr) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            bias[k] = expert(k) < E ? a.bias[expert(k)] : 0.0f;
-            if (fabsf(bias[k]) < INFINITY) span = fmaxf(span, fabsf(bias[k]));
+        for (int k = 0; k < (EW + 63) / 64; ++k) {
+            const float b = fabsf(bias[min(lane + 64 * k, EW - 1)]);
+            span = b < INFINITY ? fmaxf(span, b) : span;
         }
-        span = token_max<L>(span);
+        span = token_max<64>(span);
     }
     // What two worths may differ by although they are equal, of twice the largest score and the largest bias.  Sigmoid: 4 2^-24 each (e^-z 2 + |z|, the
     // addition one, the reciprocal two, weighed by the curve's slope) and a rounding with the bias, 8 2^-24 (1 + worth) in all.  Softmax: four
@@ -315,20 +360,25 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
     for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
         const int t = t0 + tok;
         const bool live = t < end;
-        const float *row = a.logits + (size_t)(live ? t : t0) * E;
+        const float *rows = a.logits + (size_t)t0 * E;  // (the same for the wave: lanes' offsets are of 32 bits)
+        const int at0 = live ? tok * E : 0;
+        // (few rounds of this loop: what depends on the lane alone is not worth registers across them)
+        int lane_first = sub * C;
+        asm("" : "+v"(lane_first));
+        auto expert = [&](int k) { return (k / C) * (L * C) + lane_first + k % C; };
         float z[V];
         if (a.vec && C == 4) {
 #pragma unroll
             for (int k = 0; k < V; k += 4) {
-                const float4 u = *(const float4 *)(row + min(expert(k), E - 4));
+                const float4 u = *(const float4 *)((const char *)rows + ((uint32_t)(at0 + min(expert(k), E - 4)) << 2));
                 z[k] = u.x, z[(k + 1) % V] = u.y, z[(k + 2) % V] = u.z, z[(k + 3) % V] = u.w;
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < V; ++k) z[k] = row[min(expert(k), E - 1)];
+            for (int k = 0; k < V; ++k) z[k] = ld_at(rows, (uint32_t)(at0 + min(expert(k), E - 1)));
         }
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] = expert(k) < E ? open_logit(z[k]) : -INFINITY;
+        for (int k = 0; k < V; ++k) z[k] = open_logit(expert(k) < E ? z[k] : -INFINITY);
         // scores, where the choice or the weights need all of them
         float top = 0.0f, recip = 1.0f;
         if (softmax_row) {
@@ -350,21 +400,27 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
             for (int k = 0; k < V; ++k) word[k] = ordered(z[k]);
         } else {
             float u[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) u[k] = 0.0f;
+            if (a.bias != nullptr) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) u[k] = bias[expert(k)];
+            }
             if (a.sigmoid) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) u[k] = sigmoid_near(z[k]) + bias[k];
+                for (int k = 0; k < V; ++k) u[k] += sigmoid_near(z[k]);
             } else {
 #pragma unroll
-                for (int k = 0; k < V; ++k) u[k] = fmaf(exp_near(z[k] - top), recip, bias[k]);
+                for (int k = 0; k < V; ++k) u[k] = fmaf(exp_near(z[k] - top), recip, u[k]);
             }
 #pragma unroll
-            for (int k = 0; k < V; ++k) u[k] = z[k] > -INFINITY && u[k] == u[k] ? u[k] : -INFINITY;
+            for (int k = 0; k < V; ++k) u[k] = or_closed(fmaf(z[k], 0.0f, u[k]));  // (-infinity times 0 is no number, others' nothing)
 #pragma unroll
             for (int k = 0; k < V; ++k) word[k] = ordered(a.bias != nullptr ? u[k] : z[k]);
             if (a.groups > 1) {
                 wave_lds();  // (what the wave's last tokens left there has been read)
 #pragma unroll
-                for (int k = 0; k < V; ++k) uw[expert(k)] = u[k];
+                for (int k = 0; k < V; ++k) uw[route_padded(expert(k))] = u[k];
                 wave_lds();
                 const int q = 1 << a.group_shift, g = sub >> a.group_shift, i = sub & (q - 1);
                 float best = -INFINITY, second = -INFINITY;
@@ -373,8 +429,7 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
                     best = fmaxf(best, b);
                 };
                 if (g < a.groups) {
-#pragma unroll 4
-                    for (int e = g * a.per_group + i; e < (g + 1) * a.per_group; e += q) meet(uw[e], -INFINITY);
+                    for (int e = g * a.per_group + i; e < (g + 1) * a.per_group; e += q) meet(uw[route_padded(e)], -INFINITY);
                 }
                 // (after each step its lanes hold the same, so that a mirror is a neighbour)
                 if (q > 1) meet(lane_of<0xB1>(best), lane_of<0xB1>(second));
@@ -394,14 +449,13 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
                     const float o[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const bool there = o0 + k < a.groups, in_front = there && (o[k] > mine || (o[k] == mine && o0 + k < g));
+                        const bool there = o0 + k < a.groups, in_front = there & ((o[k] > mine) | ((o[k] == mine) & (o0 + k < g)));
                         ahead += in_front ? 1 : 0;
-                        near |= there && !in_front && o0 + k != g && o[k] > -INFINITY && !(mine - o[k] > tell);
+                        near |= there & !in_front & (o0 + k != g) & (o[k] > -INFINITY) & !(mine - o[k] > tell);
                     }
                 }
                 doubt = g < a.groups && near && ahead == a.top_groups - 1;  // (the last group that stays, and one behind it)
-                const unsigned long long stays = __ballot(i == 0 && g < a.groups && ahead < a.top_groups);
-                const unsigned long long stay = L == 64 ? stays : stays >> (lane & 48);
+                const unsigned long long stay = token_bits<L>(__ballot(i == 0 && g < a.groups && ahead < a.top_groups));
                 if ((a.per_group & (C - 1)) == 0) {  // (a piece is one group's)
 #pragma unroll
                     for (int k = 0; k < V; k += C) {
@@ -416,12 +470,8 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
                 }
             }
         }
-        int held = 0;  // words of the lane
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            held += word[k] ? 1 : 0;
-            word[k] = word[k] ? (word[k] & ~LOW) | (LOW - k) : 0u;
-        }
+        for (int k = 0; k < V; ++k) word[k] = (word[k] & ~LOW) | (LOW - k);
         // descending (Batcher's odd-even merges)
 #pragma unroll
         for (int p = 1; p < V; p *= 2)
@@ -442,51 +492,96 @@ __global__ __launch_bounds__(512, 4) void route_forward_kernel(const route_args 
         for (int k = 2; k < V; ++k) list[64 * k] = word[k];
         list[64 * V] = 0u;
         int taken = 0;
-        for (int j = 0; j < K; ++j) {
+        for (int j = 0; j < K + 2; ++j) {  // (two more: what is left has to be told from what is chosen)
             const uint32_t b = token_max<L>(first);
-            if (first == b) {  // (two lanes: told by what they have taken, and chosen for again; none left: all of them, nothing)
+            if (first == b) {  // (two lanes: told by what they have taken, and chosen for again; none open left: any of them)
                 picks[j] = u32x2{b, (uint32_t)sub};
-                taken = min(taken + 1, held);
-                first = next;
+                const bool open = b >= ROUTE_OPEN;
+                taken += open ? 1 : 0;
+                first = open ? next : b;
                 next = list[64 * min(taken + 1, V)];
             }
         }
-        const uint32_t behind = token_max<L>(first);
-        if (sub == 0) picks[K] = u32x2{behind, 0u};
         wave_lds();
         // The chosen and, next to each, the one behind it: lane sub has the places sub, sub + L, ...
         int at[KL], all = -taken;
+        bool near = false;
+        auto apart = [&](uint32_t b, uint32_t o) {  // b >= o
+            return o < ROUTE_OPEN || (WORTH && a.bias != nullptr ? of_ordered(b & ~LOW) - of_ordered(o & ~LOW) > (unsure + (float)V * 0x1p-23f) * most  // (the words' last bits besides)
+                                                                 : (b & ~LOW) != (o & ~LOW));
+        };
+        auto expert_of = [&](u32x2 p) {
+            const int k = (int)(LOW - (p[0] & LOW));
+            return p[0] >= ROUTE_OPEN ? (k / C) * (L * C) + (int)p[1] * C + k % C : ROUTE_NONE;
+        };
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int j = sub + i * L;
             at[i] = ROUTE_NONE;
             if (j < K) {
                 const u32x2 p = picks[j];
-                const uint32_t b = p[0], o = picks[j + 1][0];
-                const int k = (int)(LOW - (b & LOW));
-                if (b) {
-                    at[i] = (k / C) * (L * C) + (int)p[1] * C + k % C;
-                    ++all;
-                    if (WORTH && a.bias != nullptr) doubt |= o && !(of_ordered(b & ~LOW) - of_ordered(o & ~LOW) > (unsure + (float)V * 0x1p-23f) * most);  // (the words' last bits besides)
-                    else doubt |= (b & ~LOW) == (o & ~LOW);
-                } else if (a.fill) doubt = true;
+                at[i] = expert_of(p);
+                near |= at[i] >= 0 && !apart(p[0], picks[j + 1][0]);
+                if (at[i] < 0 && a.fill) doubt = true;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i <= KL; ++i)
+            if (sub + i * L < K + 2) all += picks[sub + i * L][0] >= ROUTE_OPEN ? 1 : 0;
+        if (__ballot(near)) {
+            // They and the two behind them once more, a lane each, without a bias as they are, else in double.  Where the last of these is near to the last
+            // chosen there may be more.
+            if (K + 2 > L) doubt |= near;
+            else {
+                const u32x2 last = picks[K - 1];
+                doubt |= last[0] >= ROUTE_OPEN && !apart(last[0], picks[K + 1][0]);
+                const int e = sub < K + 2 ? expert_of(picks[sub]) : ROUTE_NONE;
+                const float ze = e >= 0 ? open_logit(ld_at(rows, (uint32_t)(at0 + e))) : -INFINITY;
+                int ahead = 0;
+                if (WORTH && a.bias != nullptr) {
+                    double v = -INFINITY, sum = 0.0;
+                    if (!a.sigmoid) {
+                        float zo[V];
+#pragma unroll
+                        for (int k = 0; k < V; ++k) zo[k] = ld_at(rows, (uint32_t)(at0 + min(expert(k), E - 1)));
+#pragma unroll
+                        for (int k = 0; k < V; ++k) {
+                            zo[k] = open_logit(expert(k) < E ? zo[k] : -INFINITY);
+                            sum += zo[k] == -INFINITY ? 0.0 : exp((double)zo[k] - (double)top);
+                            __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
+                        }
+                        for (int n = L / 2; n > 0; n >>= 1) sum += __shfl_xor(sum, n);
+                    }
+                    v = exp(a.sigmoid ? -(double)ze : (double)ze - (double)top);
+                    v = (a.sigmoid ? 1.0 / (1.0 + v) : v / sum) + (e >= 0 ? (double)bias[e] : 0.0);
+                    if (e < 0 || !(v == v)) v = -INFINITY;
+                    for (int o = 0; o < K + 2; ++o) {
+                        const double x = __shfl(v, o, L);
+                        const int y = __shfl(e, o, L);
+                        ahead += (x > v) | ((x == v) & (y < e)) ? 1 : 0;
+                    }
+                } else {
+                    for (int o = 0; o < K + 2; ++o) {
+                        const float x = __shfl(ze, o, L);
+                        const int y = __shfl(e, o, L);
+                        ahead += (x > ze) | ((x == ze) & (y < e)) ? 1 : 0;
+                    }
+                }
+                wave_lds();
+                if (e >= 0) picks[ahead] = u32x2{(uint32_t)e, 0u};
+                wave_lds();
+                if (at[0] >= 0) at[0] = (int)picks[sub][0];
             }
         }
         doubt |= token_sum<L>((float)all) != 0.0f;  // (as many taken as chosen: no two lanes held the same word)
-        const unsigned long long doubts = L == 64 ? __ballot(doubt) : __ballot(doubt) >> (lane & 48) & 0xffffull;
+        const unsigned long long doubts = token_bits<L>(__ballot(doubt));
         if (doubts && live && sub == 0) again[atomicAdd(&n_again, 1)] = t;
-        route_write<L>(a, row, t, live && !doubts, sub, at, top, recip, hist);
+        route_write<L>(a, rows + at0, t, live && !doubts, sub, at, top, recip, hist);
         wave_lds();
     }
     __syncthreads();
     // in double, a wave each
-    for (int i = wave; i < n_again; i += NT / 64) {
-        const int t = again[i];
-        const float *row = a.logits + (size_t)t * E;
-        float top, recip;
-        const int at[1] = {route_exact(a, row, (double *)spare, &top, &recip)};
-        route_write<64>(a, row, t, true, lane, at, top, recip, hist);
-    }
+    for (int i = wave; i < n_again; i += NT / 64) route_again<(L * V + 63) / 64>(a, again[i], (double *)spare, hist);
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += NT) a.part[(size_t)blockIdx.x * E + e] = hist[e];
 }
@@ -517,38 +612,50 @@ __global__ __launch_bounds__(1024) void route_counts_kernel(const int32_t *__res
 
 struct route_back_args {
     const float *logits;
-    int T, E, K, sigmoid, renorm;
+    int T, E, K, sigmoid, renorm, vec;
     float scale;
     const int32_t *ids;
     const float *w, *dw;
     float *dlogits;
 };
-// L lanes a token; a lane takes the chosen j = sub, sub + L, ... and the experts sub V .. of each stretch of L V.
+// L lanes a token; a lane takes the chosen j = sub, sub + L, ... and, as in the forward pass, V experts in pieces of C
 template <int L, int V>
 __global__ __launch_bounds__(256) void route_backward_kernel(const route_back_args a)
 {
-    constexpr int TW = 64 / L, KL = 64 / L;
-    __shared__ float dzs[4][TW][L * V];
+    constexpr int TW = 64 / L, KL = 64 / L, C = V < 4 ? V : 4;
+    __shared__ __attribute__((aligned(16))) float dzs[4][TW][L * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & (L - 1), tok = lane / L;
-    const int E = a.E, K = a.K, t = (blockIdx.x * 4 + wave) * TW + tok, e0 = sub * V;
+    const int E = a.E, K = a.K, t = (blockIdx.x * 4 + wave) * TW + tok;
     const bool live = t < a.T;
     float *dz = dzs[wave][tok];
     const size_t row = (size_t)t * E, pick = (size_t)t * K;
+    auto expert = [&](int k) { return (k / C) * (L * C) + sub * C + k % C; };
     int id[KL];
     float w[KL], g[KL], z[V];
     const bool all = !a.sigmoid && !a.renorm;  // every score has a part in the gradient
 #pragma unroll
-    for (int k = 0; k < V; ++k) z[k] = all && live && e0 + k < E ? open_logit(a.logits[row + e0 + k]) : -INFINITY;
-#pragma unroll
     for (int i = 0; i < KL; ++i) {
         const int j = sub + i * L;
-        id[i] = live && j < K ? a.ids[pick + j] : ROUTE_NONE;
-        if (id[i] >= E) id[i] = ROUTE_NONE;
-        w[i] = id[i] >= 0 ? a.w[pick + j] : 0.0f;
-        g[i] = id[i] >= 0 && w[i] != 0.0f ? a.dw[pick + j] : 0.0f;
+        id[i] = ROUTE_NONE;
+        w[i] = g[i] = 0.0f;
+        if (live && j < K) {
+            id[i] = a.ids[pick + j];
+            w[i] = a.w[pick + j];
+            g[i] = a.dw[pick + j];
+        }
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) dz[e0 + k] = 0.0f;
+    for (int k = 0; k < V; ++k) z[k] = all && live && expert(k) < E ? open_logit(a.logits[row + expert(k)]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+        if (id[i] < 0 || id[i] >= E) w[i] = 0.0f;
+        if (w[i] == 0.0f) id[i] = ROUTE_NONE, g[i] = 0.0f;
+    }
+    float rest[KL];  // 1 - s
+#pragma unroll
+    for (int i = 0; i < KL; ++i) rest[i] = a.sigmoid && id[i] >= 0 ? sigmoid(-open_logit(a.logits[row + id[i]])) : 1.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) dz[expert(k)] = 0.0f;
     wave_lds();
     float dot = 0.0f;
     if (a.renorm) {
@@ -572,11 +679,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const route_back_ar
     }
 #pragma unroll
     for (int i = 0; i < KL; ++i)
-        if (w[i] != 0.0f) {
-            float v = w[i] * g[i];
-            if (a.sigmoid) v *= sigmoid(-open_logit(a.logits[row + id[i]]));  // 1 - s
-            atomicAdd(&dz[id[i]], v);
-        }
+        if (id[i] >= 0) atomicAdd(&dz[id[i]], w[i] * g[i] * rest[i]);
     wave_lds();
     float top = 0.0f, recip = 0.0f;
     if (all) {
@@ -591,9 +694,24 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const route_back_ar
         recip = s > 0.0f ? 1.0f / s : 0.0f;
     }
     if (!live) return;
+    float o[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-        if (e0 + k < E) a.dlogits[row + e0 + k] = all ? fmaf(-exp_neg(z[k] - top) * recip, dot, dz[e0 + k]) : dz[e0 + k];
+    for (int k = 0; k < V; ++k) o[k] = dz[expert(k)];
+    if (all) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = fmaf(-exp_neg(z[k] - top) * recip, dot, o[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < V; k += C) {
+        float *p = a.dlogits + row + expert(k);
+        if (C == 4 && a.vec) {
+            if (expert(k) < E) *(float4 *)p = make_float4(o[k], o[(k + 1) % V], o[(k + 2) % V], o[(k + 3) % V]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < C; ++n)
+                if (expert(k) + n < E) p[n] = o[k + n];
+        }
+    }
 }
 
 // bias[e] += rate where an expert was chosen less often than the mean, -= rate where more often
@@ -614,23 +732,44 @@ __global__ __launch_bounds__(256) void route_balance_kernel(const int32_t *__res
     }
 }
 
-// Sixteen lanes a token do the least work for it, a wave ends soonest.  (Groups: one lane for each at least.)
-static bool route_by_waves(const omega_ctx *ctx, const omega_route_config &c, int T) { return c.E > 256 || c.groups > 16 || (c.E > 64 && T <= 16 * ctx->num_cus); }
-#define ROUTE_THREADS 512
+// How a batch is cut.  Sixteen lanes a token do the least work for it, a wave ends soonest (64 experts and fewer leave half of it idle); a few tokens are
+// one workgroup's, which needs no second launch for the counts.  (Groups: one lane for each at least.)
+struct route_cut {
+    bool waves;           // a wave a token
+    int threads, tokens;  // of a workgroup
+};
+// words of LDS of a wave
+static int route_wave_words(int E, int K, bool waves)
+{
+    const int L = waves ? 64 : 16, V = waves ? (E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : 8) : E <= 16 ? 1 : E <= 64 ? 4 : E <= 128 ? 8 : 16;
+    return route_lds(L, V) + 64 / L * 2 * (K + 2);
+}
+static route_cut route_cut_of(const omega_ctx *ctx, const omega_route_config &c, int T)
+{
+    const bool must = c.groups > 16 || c.E > 256;
+    // (sixteen waves where their LDS is within 64 KB, beside the workgroup's own)
+    if (!must && T <= 64) return {T <= 16, 16 * 4 * route_wave_words(c.E, c.K, T <= 16) <= 56 << 10 ? 1024 : 512, 64};
+    const bool waves = must || (c.E > 64 && T <= 16 * ctx->num_cus);
+    const int round = waves ? 8 : 32;  // tokens that the waves of a workgroup take at once
+    return {waves, 512, std::min(std::max(1, ceil_div(ceil_div(T, 2 * ctx->num_cus), round)) * round, ROUTE_TOKENS)};
+}
 
-static hipError_t route_launch(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, bool waves, int threads, int fill, int32_t *ids,
-                               float *w, int32_t *part, hipStream_t s)
+static route_args route_arguments(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, bool waves, int32_t *ids, float *w)
 {
     const int E = c.E, L = waves ? 64 : 16, vec = E % 4 == 0 && (uintptr_t)logits % 16 == 0;
-    const bool worth = bias != nullptr || c.groups > 1;
     int shift = 0;  // lanes of a group: as many as the next power of two of groups leaves
     while (c.groups > 1 && (2 << shift) * c.groups <= L) ++shift;
-    const route_args a = {logits, bias, T, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.groups, c.top_groups, c.group_best, E / c.groups, (1 << 20) / (E / c.groups) + 1,
-                          shift, c.scale, tokens, fill, vec, ids, w, part};
+    return {logits, bias, T, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.groups, c.top_groups, c.group_best, E / c.groups, (1 << 20) / (E / c.groups) + 1,
+            shift, c.scale, tokens, 0, vec, ids, w, nullptr};
+}
+static hipError_t route_launch(const route_args &a, bool waves, int threads, hipStream_t s)
+{
+    const int E = a.E, T = a.T, tokens = a.tokens;
+    const bool worth = a.bias != nullptr || a.groups > 1;
 #define ROUTE_FORWARD(LL, V)                                                                                                                     \
     do {                                                                                                                                         \
         const dim3 grid(ceil_div(T, tokens));                                                                                                    \
-        const size_t lds = threads / 64 * route_lds(LL, V) * sizeof(float);                                                                      \
+        const size_t lds = (size_t)threads / 64 * route_wave_words(E, a.K, waves) * sizeof(float);                                                \
         if (worth) hipLaunchKernelGGL((route_forward_kernel<LL, V, true>), grid, dim3(threads), lds, s, a);                                      \
         else hipLaunchKernelGGL((route_forward_kernel<LL, V, false>), grid, dim3(threads), lds, s, a);                                           \
     } while (0)
@@ -649,24 +788,18 @@ static hipError_t route_launch(const omega_route_config &c, const float *logits,
     return hipGetLastError();
 }
 
-// Tokens of a workgroup of the operator: whole rounds of its waves, two workgroups for a compute unit; one workgroup's up to four rounds need no
-// second launch for the counts
-static int route_tokens(const omega_ctx *ctx, const omega_route_config &c, int T)
-{
-    const int round = ROUTE_THREADS / 64 * (route_by_waves(ctx, c, T) ? 1 : 4);
-    if (T <= 4 * round) return 4 * round;
-    return std::min(std::max(1, ceil_div(ceil_div(T, 2 * ctx->num_cus), round)) * round, ROUTE_TOKENS);
-}
-size_t route_workspace(const omega_ctx *ctx, const omega_route_config &c, int T) { return (size_t)ceil_div(T, route_tokens(ctx, c, T)) * c.E * sizeof(int32_t); }
+size_t route_workspace(const omega_ctx *ctx, const omega_route_config &c, int T) { return (size_t)std::max(1, ceil_div(T, route_cut_of(ctx, c, T).tokens)) * c.E * sizeof(int32_t); }
 
 hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &c, const float *logits, int T, const float *bias, int32_t *ids, float *w,
                                 int32_t *counts, void *ws, hipStream_t s)
 {
     int n = 0;
     if (T > 0) {
-        const int tokens = route_tokens(ctx, c, T);
-        n = ceil_div(T, tokens);
-        const hipError_t e = route_launch(c, logits, T, bias, tokens, route_by_waves(ctx, c, T), ROUTE_THREADS, 0, ids, w, n == 1 && counts ? counts : (int32_t *)ws, s);
+        const route_cut cut = route_cut_of(ctx, c, T);
+        n = ceil_div(T, cut.tokens);
+        route_args a = route_arguments(c, logits, T, bias, cut.tokens, cut.waves, ids, w);
+        a.part = n == 1 && counts ? counts : (int32_t *)ws;
+        const hipError_t e = route_launch(a, cut.waves, cut.threads, s);
         if (e != hipSuccess || n == 1 || !counts) return e;
     }
     hipLaunchKernelGGL(route_counts_kernel, dim3(ceil_div(c.E, 16)), dim3(1024), 0, s, (const int32_t *)ws, n, c.E, counts);
@@ -677,7 +810,11 @@ hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &
 hipError_t launch_route_layer(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, int32_t *ids, float *w, int32_t *tile_counts,
                               hipStream_t s)
 {
-    return route_launch(c, logits, T, bias, tokens, c.E > 256 || c.groups > 16, 256, 1, ids, w, tile_counts, s);
+    const bool waves = c.groups > 16 || c.E > 256;
+    route_args a = route_arguments(c, logits, T, bias, tokens, waves, ids, w);
+    a.fill = 1;
+    a.part = tile_counts;
+    return route_launch(a, waves, 256, s);
 }
 
 #define ROUTE_RUN(K, grid, s, ...)                                                                       \
@@ -696,7 +833,7 @@ hipError_t launch_route_backward(const omega_route_config &c, const float *logit
     for (int t = 0; t < T; t += most) {
         const int n = std::min(most, T - t);
         const size_t row = (size_t)t * E, pick = (size_t)t * c.K;
-        const route_back_args a = {logits ? logits + row : nullptr, n, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.scale, ids + pick, w + pick, dw + pick, dlogits + row};
+        const route_back_args a = {logits ? logits + row : nullptr, n, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, E % 4 == 0 && (uintptr_t)dlogits % 16 == 0, c.scale, ids + pick, w + pick, dw + pick, dlogits + row};
         ROUTE_RUN(route_backward_kernel, ceil_div(n, round), s, a);
     }
     return hipGetLastError();
