@@ -7,7 +7,7 @@
 //   omega::MoELayer  constructor in the house style of LlamaMLPLayer(embedDim, nChannel, multiple_of, bias, network)
 //                    (J/engine/nn/layer/llama/LlamaMLPLayer.java:47-63) with the explicit hidden size of DiTSwiGLUFFN;
 //                    forward(Tensor) = setInput -> init -> output (LlamaMLPLayer.java:200-217);
-//                    saveModel/loadModel write raw little-endian float32 in the order gate, (gate bias), then
+//                    saveModel/loadModel write raw little-endian float32 in the order gate, (gate bias), (bias for balance), then
 //                    w1,w3,w2 per expert (routed, then shared), as LlamaMLPLayer.java:273-283 does for one MLP;
 //                    a failing library call throws std::runtime_error("Error code N:msg"), the checkCUDA style
 //                    (J/engine/gpu/CUDAMemoryManager.java:179-201); back(Tensor) = initBack -> setDelta -> diff
@@ -266,6 +266,21 @@ public:
     /// OMEGA_GATHER_AUTO / _COPY / _ON_LOAD: how the rows of x reach the experts of a bf16 layer
     void setGatherMode(int mode) { check(ctx_.get(), omega_moe_set_gather_mode(moe_, mode)); }
     bool gatherOnLoad() const { return omega_moe_gather_on_load(moe_) != 0; }
+    /// a routing of the layer's own (nullptr: the softmax top-k again), with a bias for balance or without; E and K are the layer's
+    void setRouting(const omega_route_config *config, bool balance = false)
+    {
+        check(ctx_.get(), omega_moe_set_routing(moe_, config, balance ? 1 : 0));
+        balance_ = config && balance;
+    }
+    void setBalance(const float *b) { check(ctx_.get(), omega_moe_set_weights(moe_, OMEGA_W_BALANCE, 0, b, 0)); }
+    std::vector<float> getBalance()
+    {
+        std::vector<float> b(nExperts_);
+        check(ctx_.get(), omega_moe_get_weights(moe_, OMEGA_W_BALANCE, 0, b.data(), 0));
+        return b;
+    }
+    /// one step of the bias for balance by what the last forward pass gave each expert
+    void balance(float rate) { check(ctx_.get(), omega_moe_balance(moe_, rate)); }
     // update() of a layer without an updater: w -= learnRate * diffW (FullyLayer.update, FullyLayer.java:569-590)
     float learnRate = 0.0f;
     bool freeze = false;  // Layer.freeze: a frozen layer's update() does nothing (FullyLayer.java:571)
@@ -327,7 +342,7 @@ public:
         loadModel(f);
     }
     void saveModel(FILE *f) { eachParam([&](int which, int g, size_t n) { std::vector<float> h = download(which, g, n); if (fwrite(h.data(), 4, n, f) != n) throw std::runtime_error("Error code 1:short write"); }); }
-    void loadModel(FILE *f) { eachParam([&](int which, int g, size_t n) { std::vector<float> h(n); if (fread(h.data(), 4, n, f) != n) throw std::runtime_error("Error code 1:checkpoint ends early"); if (which == OMEGA_W_GATE_BIAS) check(ctx_.get(), omega_moe_set_weights(moe_, which, g, h.data(), 0)); else upload(which, g, h.data(), n); }); }
+    void loadModel(FILE *f) { eachParam([&](int which, int g, size_t n) { std::vector<float> h(n); if (fread(h.data(), 4, n, f) != n) throw std::runtime_error("Error code 1:checkpoint ends early"); if (which == OMEGA_W_GATE_BIAS || which == OMEGA_W_BALANCE) check(ctx_.get(), omega_moe_set_weights(moe_, which, g, h.data(), 0)); else upload(which, g, h.data(), n); }); }
 
 private:
     void run(bool block)
@@ -346,6 +361,7 @@ private:
     {
         f(OMEGA_W_GATE, 0, (size_t)nExperts_ * embedDim_);
         if (bias_) f(OMEGA_W_GATE_BIAS, 0, (size_t)nExperts_);
+        if (balance_) f(OMEGA_W_BALANCE, 0, (size_t)nExperts_);
         for (int g = 0; g < nExperts_ + nShared_; ++g) {
             f(OMEGA_W_W1, g, (size_t)hidden_ * embedDim_);
             f(OMEGA_W_W3, g, (size_t)hidden_ * embedDim_);
@@ -372,7 +388,7 @@ private:
     std::vector<float> download(int which, int g, size_t n)
     {
         std::vector<float> h(n);
-        if (dtype_ == OMEGA_DTYPE_F32 || which == OMEGA_W_GATE_BIAS) {
+        if (dtype_ == OMEGA_DTYPE_F32 || which == OMEGA_W_GATE_BIAS || which == OMEGA_W_BALANCE) {
             check(ctx_.get(), omega_moe_get_weights(moe_, which, g, h.data(), 0));
             return h;
         }
@@ -391,7 +407,7 @@ private:
     Context &ctx_;
     omega_moe *moe_ = nullptr;
     int embedDim_, hidden_, nExperts_, topK_, nShared_;
-    bool bias_;
+    bool bias_, balance_ = false;
     int dtype_;
     std::unique_ptr<Tensor> output_, diff_;
     Tensor *delta_ = nullptr;

@@ -68,6 +68,22 @@ public final class OmegaHip {
     private static final MethodHandle HEAD_LOSS_FORWARD = h("omega_hip_head_loss_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
     private static final MethodHandle HEAD_LOSS_BACKWARD = h("omega_hip_head_loss_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
     private static final MethodHandle CLIP_GRAD_NORM = h("omega_hip_clip_grad_norm", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_INT, JAVA_FLOAT, ADDRESS));
+    private static final MethodHandle RMSNORM_FORWARD = h("omega_hip_rmsnorm_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, JAVA_FLOAT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle RMSNORM_BACKWARD = h("omega_hip_rmsnorm_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle KEEP8_SAVE = h("omega_hip_keep8_save", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS));
+    private static final MethodHandle KEEP8_LOAD = h("omega_hip_keep8_load", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, JAVA_INT, ADDRESS, JAVA_INT));
+    private static final MethodHandle ROUTE_FORWARD = h("omega_hip_route_forward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle ROUTE_BACKWARD = h("omega_hip_route_backward", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
+    private static final MethodHandle ROUTE_BALANCE = h("omega_hip_route_balance", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, JAVA_FLOAT, ADDRESS));
+    private static final MethodHandle SET_ROUTING = h("omega_moe_set_routing", FunctionDescriptor.of(JAVA_INT, ADDRESS, ADDRESS, JAVA_INT));
+    private static final MethodHandle BALANCE = h("omega_moe_balance", FunctionDescriptor.of(JAVA_INT, ADDRESS, JAVA_FLOAT));
+
+    /** struct omega_route_config: seven int32, then the scale. */
+    private static final MemoryLayout ROUTE_CONFIG = MemoryLayout.structLayout(
+            JAVA_INT.withName("E"), JAVA_INT.withName("K"), JAVA_INT.withName("score"), JAVA_INT.withName("renorm"), JAVA_INT.withName("groups"),
+            JAVA_INT.withName("top_groups"), JAVA_INT.withName("group_best"), JAVA_FLOAT.withName("scale"));
+    public static final int ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1;
+    public static final int KEEP8_INT8 = 0, KEEP8_MX = 1;
 
     /** struct omega_grad_tensor: src, dst, n (uint64), dtype, reserved. */
     private static final MemoryLayout GRAD_TENSOR = MemoryLayout.structLayout(
@@ -81,7 +97,7 @@ public final class OmegaHip {
 
     public static final int F32 = 0, BF16 = 1;
     public static final int ROUTER_EXACT = 0, ROUTER_FAST = 1;
-    public static final int W_GATE = 0, W_GATE_BIAS = 1, W_W1 = 2, W_W3 = 3, W_W2 = 4, W_NORM = 5;
+    public static final int W_GATE = 0, W_GATE_BIAS = 1, W_W1 = 2, W_W3 = 3, W_W2 = 4, W_NORM = 5, W_BALANCE = 6;
 
     private OmegaHip() {
     }
@@ -408,6 +424,96 @@ public final class OmegaHip {
             check(ctx, (int) LAYERNORM_BACKWARD.invokeExact(ctx, at(x), at(dout), dtype, t, d, at(gamma), at(mean), at(rstd), at(dx), at(dgamma), at(dbeta)));
         } catch (Throwable e) {
             throw wrap(e);
+        }
+    }
+
+    /** sum = x + residual (residual 0: none), out = norm(sum); out8 / keep8 with their scales, sum, out and rstd may be 0. */
+    public static void rmsnormForward(MemorySegment ctx, long x, long residual, int dtype, int t, int d, long gamma, float eps, long sum, long out, long out8, long out8Scales,
+            long keep8, long keep8Scales, long rstd) {
+        try {
+            check(ctx, (int) RMSNORM_FORWARD.invokeExact(ctx, at(x), at(residual), dtype, t, d, at(gamma), eps, at(sum), at(out), at(out8), at(out8Scales), at(keep8),
+                    at(keep8Scales), at(rstd)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    /** From the rows h, or from their 8-bit copy (h = 0); dsum 0: none. */
+    public static void rmsnormBackward(MemorySegment ctx, long h, long keep8, long keep8Scales, long dout, long dsum, int dtype, int t, int d, long gamma, long rstd, long dx,
+            long dgamma) {
+        try {
+            check(ctx, (int) RMSNORM_BACKWARD.invokeExact(ctx, at(h), at(keep8), at(keep8Scales), at(dout), at(dsum), dtype, t, d, at(gamma), at(rstd), at(dx), at(dgamma)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void keep8Save(MemorySegment ctx, long x, int dtype, int t, int d, int form, long codes, long scales) {
+        try {
+            check(ctx, (int) KEEP8_SAVE.invokeExact(ctx, at(x), dtype, t, d, form, at(codes), at(scales)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void keep8Load(MemorySegment ctx, long codes, long scales, int form, int t, int d, long out, int dtype) {
+        try {
+            check(ctx, (int) KEEP8_LOAD.invokeExact(ctx, at(codes), at(scales), form, t, d, at(out), dtype));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    /** A routing to experts (omega_route_config) in the arena's memory. */
+    public static MemorySegment routeConfig(Arena a, int e, int k, int score, boolean renorm, int groups, int topGroups, int groupBest, float scale) {
+        MemorySegment c = a.allocate(ROUTE_CONFIG);
+        int[] v = {e, k, score, renorm ? 1 : 0, groups, topGroups, groupBest};
+        for (int i = 0; i < v.length; i++) {
+            c.setAtIndex(JAVA_INT, i, v[i]);
+        }
+        c.setAtIndex(JAVA_FLOAT, v.length, scale);
+        return c;
+    }
+
+    /** ids and w [t,K], counts [E] (or 0); bias 0: none. */
+    public static void routeForward(MemorySegment ctx, MemorySegment config, long logits, int t, long bias, long ids, long w, long counts) {
+        try {
+            check(ctx, (int) ROUTE_FORWARD.invokeExact(ctx, config, at(logits), t, at(bias), at(ids), at(w), at(counts)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void routeBackward(MemorySegment ctx, MemorySegment config, long logits, int t, long ids, long w, long dw, long dlogits) {
+        try {
+            check(ctx, (int) ROUTE_BACKWARD.invokeExact(ctx, config, at(logits), t, at(ids), at(w), at(dw), at(dlogits)));
+        } catch (Throwable e) {
+            throw wrap(e);
+        }
+    }
+
+    public static void routeBalance(MemorySegment ctx, long counts, int e, float rate, long bias) {
+        try {
+            check(ctx, (int) ROUTE_BALANCE.invokeExact(ctx, at(counts), e, rate, at(bias)));
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    /** The routing of a layer (MemorySegment.NULL: the softmax top-k again), with a bias for balance or without. */
+    public static void setRouting(MemorySegment ctx, MemorySegment moe, MemorySegment config, boolean balance) {
+        try {
+            check(ctx, (int) SET_ROUTING.invokeExact(moe, config, balance ? 1 : 0));
+        } catch (Throwable t) {
+            throw wrap(t);
+        }
+    }
+
+    public static void balance(MemorySegment ctx, MemorySegment moe, float rate) {
+        try {
+            check(ctx, (int) BALANCE.invokeExact(moe, rate));
+        } catch (Throwable t) {
+            throw wrap(t);
         }
     }
 

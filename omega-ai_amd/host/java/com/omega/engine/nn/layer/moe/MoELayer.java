@@ -7,6 +7,7 @@ package com.omega.engine.nn.layer.moe;
 
 import java.io.IOException;
 import java.io.RandomAccessFile;
+import java.lang.foreign.Arena;
 import java.lang.foreign.MemorySegment;
 import java.nio.ByteBuffer;
 import java.nio.ByteOrder;
@@ -32,6 +33,7 @@ import com.omega.engine.updater.UpdaterFactory;
 public class MoELayer extends Layer {
     private final int embedDim, hidden, nExperts, topK, nShared;
     private final boolean renorm, gateBias;
+    private boolean balance;
     private final int dtype;                       // OmegaHip.F32 or OmegaHip.BF16: storage type inside the layer
     private final MemorySegment ctx, moe;
     // fp32 device copies of the host tensors (input, output, delta, diff) and, for bf16 layers, their bf16 twins
@@ -83,7 +85,7 @@ public class MoELayer extends Layer {
     // ---- parameters: fp32 host arrays in the reference's [out,in] layout (FullyLayer.java:181) ----
 
     private void upload(int which, int g, float[] h) {
-        if (dtype == OmegaHip.F32 || which == OmegaHip.W_GATE_BIAS || which == OmegaHip.W_NORM) {
+        if (dtype == OmegaHip.F32 || which == OmegaHip.W_GATE_BIAS || which == OmegaHip.W_NORM || which == OmegaHip.W_BALANCE) {
             OmegaHip.setWeightsHost(ctx, moe, which, g, h);
             return;
         }
@@ -100,7 +102,7 @@ public class MoELayer extends Layer {
 
     private float[] download(int which, int g, int n) {
         float[] h = new float[n];
-        if (dtype == OmegaHip.F32 || which == OmegaHip.W_GATE_BIAS || which == OmegaHip.W_NORM) {
+        if (dtype == OmegaHip.F32 || which == OmegaHip.W_GATE_BIAS || which == OmegaHip.W_NORM || which == OmegaHip.W_BALANCE) {
             OmegaHip.getWeightsHost(ctx, moe, which, g, h);
             return h;
         }
@@ -337,6 +339,34 @@ public class MoELayer extends Layer {
         OmegaHip.setGatherMode(ctx, moe, mode);
     }
 
+    /** A routing of the layer's own instead of the softmax top-k (its experts and their number per token are the layer's), with a bias for balance
+     *  or without. */
+    public void setRouting(int score, boolean renorm, int groups, int topGroups, int groupBest, float scale, boolean balance) {
+        try (Arena a = Arena.ofConfined()) {
+            OmegaHip.setRouting(ctx, moe, OmegaHip.routeConfig(a, nExperts, topK, score, renorm, groups, topGroups, groupBest, scale), balance);
+        }
+        this.balance = balance;
+    }
+
+    /** The softmax top-k again. */
+    public void clearRouting() {
+        OmegaHip.setRouting(ctx, moe, MemorySegment.NULL, false);
+        this.balance = false;
+    }
+
+    public void setBalance(float[] b) {
+        upload(OmegaHip.W_BALANCE, 0, b);
+    }
+
+    public float[] getBalance() {
+        return download(OmegaHip.W_BALANCE, 0, nExperts);
+    }
+
+    /** One step of the bias for balance by what the last forward pass gave each expert. */
+    public void balance(float rate) {
+        OmegaHip.balance(ctx, moe, rate);
+    }
+
     /** One parameter gradient (fp32, layout of its weight): W_GATE, W_GATE_BIAS, W_NORM, W_W1 / W_W3 / W_W2 of expert g. */
     public float[] grad(int which, int g) {
         int n = which == OmegaHip.W_GATE ? nExperts * embedDim
@@ -394,6 +424,9 @@ public class MoELayer extends Layer {
         f.visit(OmegaHip.W_GATE, 0, nExperts * embedDim);
         if (gateBias) {
             f.visit(OmegaHip.W_GATE_BIAS, 0, nExperts);
+        }
+        if (balance) {
+            f.visit(OmegaHip.W_BALANCE, 0, nExperts);
         }
         for (int g = 0; g < nExperts + nShared; g++) {
             f.visit(OmegaHip.W_W1, g, hidden * embedDim);
