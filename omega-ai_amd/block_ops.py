@@ -74,14 +74,25 @@ class Rows8:
     """Rows held in 8 bits: codes [T,d] and a scale for every group of a row (form "int8": of 128 elements, fp32; "mx": of 32, a byte)."""
 
     def __init__(self, form, shape, codes, scales):
-        self.form, self.shape, self.codes, self.scales = form, shape, codes, scales
+        _want(form in _FORMS, "form is int8 or mx")
+        _want(len(shape) == 2 and codes.shape == tuple(shape) and codes.dtype == "u8", "codes shape or dtype")
+        _want((scales.shape, scales.dtype) == _scales(form, shape), "scales shape or dtype")
+        self.form, self.shape, self.codes, self.scales = form, codes.shape, codes, scales
+
+
+def _scales(form, shape):
+    """Shape and dtype of the scales of rows of `shape`."""
+    return (shape[0], -(-shape[1] // _GROUP[form])), "f32" if form == "int8" else "u8"
 
 
 def _rows8(layer, name, form, shape):
     """The layer's own buffers of that name for rows of `shape`."""
-    codes = layer._buffer(name, shape, "u8")
-    scales = layer._buffer(name + "_scales", (shape[0], -(-shape[1] // _GROUP[form])), "f32" if form == "int8" else "u8")
-    return Rows8(form, shape, codes, scales)
+    rows = layer.__dict__.get(name)
+    if rows is None or rows.shape != shape or not rows.codes.ptr:
+        layer.__dict__[name] = None
+        codes = layer._buffer(name, shape, "u8")
+        rows = layer.__dict__[name] = Rows8(form, shape, codes, layer._buffer(name + "_scales", *_scales(form, shape)))
+    return rows
 
 
 def _load8(layer, name, rows, dtype):
@@ -105,7 +116,18 @@ class RMSLayer(_Layer):
         super().__init__(ctx, dtype)
         self.embedDim, self.eps, self.out8, self.keep8 = embedDim, float(eps), bool(out8), bool(keep8)
         self.gamma = gamma
-        self.input = self.sum = self.kept = self.diffGamma = None
+        self.input = self.sum = self.kept = self.diffGamma = self._for = None
+
+    def _ready(self, shape, summed):
+        """What a batch of that shape is written to: sum, rstd, out, out8, kept.  (Looked up together: one by one costs a decode step's call 1 of 6 us.)"""
+        batch = (shape, summed, self.out8, self.keep8)
+        if batch != self._for:
+            self._for = None
+            self._held = (self._buffer("sum", shape, self.dtype) if summed else None, self._buffer("rstd", (shape[0],), "f32"),
+                          None if self.out8 else self._buffer("out", shape, self.dtype), _rows8(self, "rows8_out", "mx", shape) if self.out8 else None,
+                          _rows8(self, "rows8_kept", "int8", shape) if self.keep8 else None)
+            self._for = batch
+        return self._held
 
     def forward(self, x, residual=None):
         """norm(x + residual); the sum is self.sum (None without a residual)."""
@@ -114,17 +136,11 @@ class RMSLayer(_Layer):
         _want(residual is None or (residual.shape == shape and residual.dtype == x.dtype and residual.ptr), "residual shape or dtype")   # (no address would mean none)
         _want(self.gamma is not None, "the layer has no gamma")
         self.input = None   # (until the call has succeeded)
-        self.sum = h = None if residual is None else self._buffer("sum", shape, self.dtype)
-        rstd = self._buffer("rstd", (shape[0],), "f32")
-        out = o8 = kept = None
-        if self.out8:
-            o8 = _rows8(self, "out8", "mx", shape)
-        else:
-            out = self._buffer("out", shape, self.dtype)
-        if self.keep8:
-            kept = _rows8(self, "keep8", "int8", shape)
+        self.sum, rstd, out, o8, kept = self._ready(shape, residual is not None)
+        h = self.sum
+        _want(h is None or h.ptr, "sum has been freed")
         self.ctx.check(self.lib.omega_hip_rmsnorm_forward(
-            self.ctx.handle, x.ptr, residual.ptr if residual else None, _DT[self.dtype], shape[0], shape[1], self.gamma.ptr, self.eps, h.ptr if h else None,
+            self.ctx.handle, x.ptr, residual.ptr if h else None, _DT[self.dtype], shape[0], shape[1], self.gamma.ptr, self.eps, h.ptr if h else None,
             out.ptr if out else None, o8.codes.ptr if o8 else None, o8.scales.ptr if o8 else None, kept.codes.ptr if kept else None,
             kept.scales.ptr if kept else None, rstd.ptr))
         self.input, self.kept = x if h is None else h, kept
@@ -141,6 +157,7 @@ class RMSLayer(_Layer):
         _want(h is not None, "back without a forward")
         _want(delta.shape == h.shape and delta.dtype == self.dtype, "delta shape or dtype does not match the output")
         _want(dsum is None or (dsum.shape == h.shape and dsum.dtype == self.dtype and dsum.ptr), "dsum shape or dtype does not match the sum")
+        _want(self.gamma is not None, "the layer has no gamma")
         kept, T = self.kept, h.shape[0]
         dx = self._buffer("diff", h.shape, self.dtype)
         self.diffGamma = dg = self._buffer("diffGamma", (self.embedDim,), "f32")
@@ -151,7 +168,7 @@ class RMSLayer(_Layer):
 
     def close(self):
         super().close()
-        self.sum = self.kept = None
+        self.sum = self.kept = self._for = self._held = None
 
 
 class Keep8Layer(_Layer):
@@ -166,7 +183,7 @@ class Keep8Layer(_Layer):
     def save(self, x):
         _want(len(x.shape) == 2 and x.shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
         self.kept = None
-        rows = _rows8(self, "codes", self.form, x.shape)
+        rows = _rows8(self, "rows8", self.form, x.shape)
         self.ctx.check(self.lib.omega_hip_keep8_save(self.ctx.handle, x.ptr, _DT[self.dtype], x.shape[0], x.shape[1], _FORMS[self.form], rows.codes.ptr,
                                                      rows.scales.ptr))
         self.kept = rows

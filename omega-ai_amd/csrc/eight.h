@@ -15,13 +15,13 @@
 
 typedef uint32_t u32x2_by __attribute__((ext_vector_type(2), aligned(1)));
 
-// eight elements as they lie in memory
+// eight elements as they lie in memory; in fp32 the second four may lie H elements behind the first
 template <bool BF>
 struct oct {
     uint32_t u[BF ? 4 : 8];
 };
-// from element i of p on, n of them (the rest: zero; n <= 0: nothing is read)
-template <bool BF>
+// from element i of p on, n elements to the row's end (behind it: zero; n <= 0: nothing is read)
+template <bool BF, int H = 4>
 __device__ __forceinline__ oct<BF> ld_oct(const void *p, size_t i, int n)
 {
     oct<BF> r;
@@ -29,11 +29,21 @@ __device__ __forceinline__ oct<BF> ld_oct(const void *p, size_t i, int n)
 #pragma unroll
     for (int k = 0; k < 4; ++k) r.u[k] = a.u[k];
     if (!BF) {
-        const piece<BF> b = ld_piece<BF>(p, i + 4, n - 4);
+        const piece<BF> b = ld_piece<BF>(p, i + H, n - H);
 #pragma unroll
         for (int k = 0; k < 4; ++k) r.u[(BF ? 0 : 4) + k] = b.u[k];
     }
     return r;
+}
+// as many fp32 parameters
+template <int H>
+__device__ __forceinline__ void ld_par8(const float *p, int i, int n, float (&v)[8])
+{
+    float a[4], b[4];
+    ld_par<4>(p, i, n, a);
+    ld_par<4>(p, i + H, n - H, b);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
 }
 template <bool BF>
 __device__ __forceinline__ float el8(const oct<BF> &r, int k)
@@ -48,33 +58,41 @@ __device__ __forceinline__ oct<BF> to_oct(const float (&v)[8])
     for (int k = 0; k < (BF ? 4 : 8); ++k) r.u[k] = BF ? pack_bf16(v[2 * k & 7], v[(2 * k + 1) & 7]) : __float_as_uint(v[k]);
     return r;
 }
-template <bool BF>
+template <bool BF, int H = 4>
 __device__ __forceinline__ void st_oct(void *p, size_t i, int n, const oct<BF> &r)
 {
-    if (n >= 8) {
-        u32x4_bf a = {r.u[0], r.u[1], r.u[2], r.u[3]};
-        if (BF) *(u32x4_bf *)((bf16_t *)p + i) = a;
-        else {
-            u32x4_bf b = {r.u[BF ? 0 : 4], r.u[BF ? 0 : 5], r.u[BF ? 0 : 6], r.u[BF ? 0 : 7]};
-            *(u32x4_bf *)((float *)p + i) = a;
-            *(u32x4_bf *)((float *)p + i + 4) = b;
-        }
-    } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) {
-                if (BF) ((bf16_t *)p)[i + k] = (bf16_t)(r.u[k >> 1] >> (16 * (k & 1)));
-                else ((uint32_t *)p)[i + k] = r.u[BF ? 0 : k];
-            }
+    for (int h = 0; h < (BF ? 1 : 2); ++h, i += H, n -= H) {
+        constexpr int W = BF ? 8 : 4;
+        if (n >= W) {
+            u32x4_bf a;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = r.u[BF ? k : 4 * h + k];
+            if (BF) *(u32x4_bf *)((bf16_t *)p + i) = a;
+            else *(u32x4_bf *)((float *)p + i) = a;
+        } else {
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                if (k < n) {
+                    if (BF) ((bf16_t *)p)[i + k] = (bf16_t)(r.u[(k >> 1) & 3] >> (16 * (k & 1)));
+                    else ((uint32_t *)p)[i + k] = r.u[BF ? 0 : 4 * h + (k & 3)];
+                }
+        }
     }
 }
-// eight codes
+// eight codes, or the first four
+template <int W = 8>
 __device__ __forceinline__ u32x2_by ld_codes(const uint8_t *p, size_t i, int n)
 {
+    typedef uint32_t u32_by __attribute__((aligned(1)));
     u32x2_by r = {0u, 0u};
-    if (n >= 8) return *(const u32x2_by *)(p + i);
+    if (n >= W) {
+        if (W == 8) return *(const u32x2_by *)(p + i);
+        r[0] = *(const u32_by *)(p + i);
+        return r;
+    }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < W; ++k)
         if (k < n) r[k >> 2] |= (uint32_t)p[i + k] << (8 * (k & 3));
     return r;
 }

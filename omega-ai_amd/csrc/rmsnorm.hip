@@ -114,9 +114,12 @@ struct rms_forward_args {
 };
 
 #define RMS_THREADS(L) ((L) < 256 ? 256 : (L))
+// Where the second half of a lane's eight elements lies: in fp32 a piece of the row further, so that the lanes' 16 bytes follow each other, but for codes,
+// whose groups are neighbours' (4001 x 1023: forward 9.1 us, 9.8 with eight together; backward 12.0 and 13.4)
+#define RMS_HALF(BF, CODES, L) ((BF) || (CODES) ? 4 : 4 * (L))
 
 // h of eight elements (v), and to where it goes on
-template <bool BF>
+template <bool BF, int H>
 __device__ __forceinline__ void add_residual(const rms_forward_args &a, const oct<BF> &x, const oct<BF> &r, size_t at, int n, float (&v)[8])
 {
 #pragma unroll
@@ -129,10 +132,10 @@ __device__ __forceinline__ void add_residual(const rms_forward_args &a, const oc
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = el8<BF>(h, k);
     }
-    if (a.sum != nullptr && n > 0) st_oct<BF>(a.sum, at, n, h);
+    if (a.sum != nullptr && n > 0) st_oct<BF, H>(a.sum, at, n, h);
 }
 // what is written of eight elements of h once q is known
-template <bool BF, bool EIGHT>
+template <bool BF, bool EIGHT, int H>
 __device__ __forceinline__ void write_normed(const rms_forward_args &a, const float (&v)[8], double q, const float (&gamma)[8], int t, int c)
 {
     const int n = a.d - c;
@@ -141,7 +144,7 @@ __device__ __forceinline__ void write_normed(const rms_forward_args &a, const fl
     float y[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = v[k] * r * gamma[k];
-    if (a.out != nullptr && n > 0) st_oct<BF>(a.out, at, n, to_oct<BF>(y));
+    if (a.out != nullptr && n > 0) st_oct<BF, H>(a.out, at, n, to_oct<BF>(y));
     if (!EIGHT) return;
     if (a.out8 != nullptr) {  // (lanes behind the row's end take part in their group: zeros)
         uint32_t b;
@@ -160,7 +163,7 @@ __device__ __forceinline__ void write_normed(const rms_forward_args &a, const fl
 template <bool BF, int N, int L, bool EIGHT>
 __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_forward_kernel(const rms_forward_args a)
 {
-    constexpr int R = RMS_THREADS(L) / L;
+    constexpr int R = RMS_THREADS(L) / L, H = RMS_HALF(BF, EIGHT, L), W = H == 4 ? 8 : 4;
     __shared__ double red[2][16];
     const int l = threadIdx.x & (L - 1), step = gridDim.x * R, d = a.d;
     int t = blockIdx.x * R + threadIdx.x / L, turn = 0;
@@ -169,22 +172,22 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_forward_kernel(const r
     auto ask = [&](int row) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = (n * L + l) * 8;
-            nx[n] = ld_oct<BF>(a.x, (size_t)row * d + c, d - c);
-            if (a.res != nullptr) nr[n] = ld_oct<BF>(a.res, (size_t)row * d + c, d - c);
+            const int c = n * L * 8 + l * W;
+            nx[n] = ld_oct<BF, H>(a.x, (size_t)row * d + c, d - c);
+            if (a.res != nullptr) nr[n] = ld_oct<BF, H>(a.res, (size_t)row * d + c, d - c);
         }
     };
     ask(t);
     float g[N][8];
 #pragma unroll
-    for (int n = 0; n < N; ++n) ld_par<8>(a.gamma, (n * L + l) * 8, d - (n * L + l) * 8, g[n]);
+    for (int n = 0; n < N; ++n) ld_par8<H>(a.gamma, n * L * 8 + l * W, d - (n * L * 8 + l * W), g[n]);
     for (; t < a.T; t += step) {
         float v[N][8];
         double s = 0.0;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = (n * L + l) * 8;
-            add_residual<BF>(a, nx[n], nr[n], (size_t)t * d + c, d - c, v[n]);
+            const int c = n * L * 8 + l * W;
+            add_residual<BF, H>(a, nx[n], nr[n], (size_t)t * d + c, d - c, v[n]);
         }
         if (t + step < a.T) ask(t + step);
 #pragma unroll
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_forward_kernel(const r
         turn ^= 1;
         if (l == 0 && a.rstd != nullptr) a.rstd[t] = (float)q;
 #pragma unroll
-        for (int n = 0; n < N; ++n) write_normed<BF, EIGHT>(a, v[n], q, g[n], t, (n * L + l) * 8);
+        for (int n = 0; n < N; ++n) write_normed<BF, EIGHT, H>(a, v[n], q, g[n], t, n * L * 8 + l * W);
     }
 }
 
@@ -211,7 +214,7 @@ __global__ __launch_bounds__(256) void rmsnorm_forward_long_kernel(const rms_for
     for (int c = threadIdx.x * 8; c < whole; c += 2048) {
         float v[8];
         const oct<BF> x = ld_oct<BF>(a.x, row + c, d - c), r = a.res != nullptr ? ld_oct<BF>(a.res, row + c, d - c) : x;
-        add_residual<BF>(a, x, r, row + c, d - c, v);
+        add_residual<BF, 4>(a, x, r, row + c, d - c, v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) s = fma((double)v[k], (double)v[k], s);
     }
@@ -223,9 +226,9 @@ __global__ __launch_bounds__(256) void rmsnorm_forward_long_kernel(const rms_for
     for (int c = threadIdx.x * 8; c < whole; c += 2048) {
         float v[8], g[8];
         const oct<BF> x = ld_oct<BF>(b.x, row + c, d - c), r = b.res != nullptr ? ld_oct<BF>(b.res, row + c, d - c) : x;
-        add_residual<BF>(b, x, r, row + c, d - c, v);
+        add_residual<BF, 4>(b, x, r, row + c, d - c, v);
         ld_par<8>(a.gamma, c, d - c, g);
-        write_normed<BF, EIGHT>(b, v, q, g, t, c);
+        write_normed<BF, EIGHT, 4>(b, v, q, g, t, c);
     }
 }
 
@@ -240,7 +243,7 @@ struct rms_backward_args {
     float *part;            // [workgroups][d]: their sums of dy xh
 };
 // eight elements of what is read of a row
-template <bool BF, bool KEPT>
+template <bool BF, bool KEPT, int H>
 struct rms_back_row {
     oct<BF> h, dy, ds;
     u32x2_by codes;
@@ -252,9 +255,9 @@ struct rms_back_row {
         if (KEPT) {
             codes = ld_codes(a.keep8, at, n);
             scale = n > 0 ? a.keep_scale[(size_t)t * ceil_div(a.d, KEEP8_INT8_GROUP) + c / KEEP8_INT8_GROUP] : 0.0f;
-        } else h = ld_oct<BF>(a.h, at, n);
-        dy = ld_oct<BF>(a.dout, at, n);
-        if (a.dsum != nullptr) ds = ld_oct<BF>(a.dsum, at, n);
+        } else h = ld_oct<BF, H>(a.h, at, n);
+        dy = ld_oct<BF, H>(a.dout, at, n);
+        if (a.dsum != nullptr) ds = ld_oct<BF, H>(a.dsum, at, n);
     }
     __device__ __forceinline__ void values(float (&v)[8]) const
     {
@@ -269,16 +272,16 @@ struct rms_back_row {
 template <bool BF, int N, int L, bool KEPT>
 __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_backward_kernel(const rms_backward_args a)
 {
-    constexpr int R = RMS_THREADS(L) / L;
+    constexpr int R = RMS_THREADS(L) / L, H = RMS_HALF(BF, KEPT, L), W = H == 4 ? 8 : 4;
     __shared__ float red[2][16];
-    extern __shared__ __attribute__((aligned(16))) float cols[];  // L = 64: [3][d rounded up to a multiple of 8], the sums of waves 1 .. 3
+    extern __shared__ __attribute__((aligned(16))) float cols[];  // L = 64: [3][N][64][8], the sums of waves 1 .. 3
     const int l = threadIdx.x & (L - 1), sub = threadIdx.x / L, d = a.d;
     float g[N][8], ag[N][8];
-    rms_back_row<BF, KEPT> nx[N];  // the next row
+    rms_back_row<BF, KEPT, H> nx[N];  // the next row
     float nr = 0.0f;
     auto ask = [&](int t) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) nx[n].ask(a, t, (n * L + l) * 8);
+        for (int n = 0; n < N; ++n) nx[n].ask(a, t, n * L * 8 + l * W);
         nr = a.rstd[t];
     };
     int t = blockIdx.x * R + sub, turn = 0;
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_backward_kernel(const 
     if (t < a.T) ask(t);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        ld_par<8>(a.gamma, (n * L + l) * 8, d - (n * L + l) * 8, g[n]);
+        ld_par8<H>(a.gamma, n * L * 8 + l * W, d - (n * L * 8 + l * W), g[n]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) ag[n][k] = 0.0f;
     }
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_backward_kernel(const 
         turn ^= 1;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = (n * L + l) * 8;
+            const int c = n * L * 8 + l * W;
             if (c >= d) continue;
             float o[8];
 #pragma unroll
@@ -326,39 +329,34 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_backward_kernel(const 
 #pragma unroll
                 for (int k = 0; k < 8; ++k) o[k] += el8<BF>(ds[n], k);
             }
-            st_oct<BF>(a.dx, (size_t)t * d + c, d - c, to_oct<BF>(o));
+            st_oct<BF, H>(a.dx, (size_t)t * d + c, d - c, to_oct<BF>(o));
         }
     }
-    const int dp = ceil_div(d, 8) * 8;
     if (L == 64) {
         if (sub > 0) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int c = (n * L + l) * 8;
-                if (c >= d) continue;
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) cols[(size_t)(sub - 1) * dp + c + k] = ag[n][k];
-            }
+                for (int k = 0; k < 8; ++k) cols[(((sub - 1) * N + n) * L + l) * 8 + k] = ag[n][k];
         }
         __syncthreads();
         if (sub > 0) return;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = (n * L + l) * 8;
-            if (c >= d) continue;
+        for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int w = 0; w < 3; ++w)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) ag[n][k] += cols[(size_t)w * dp + c + k];
-        }
+                for (int k = 0; k < 8; ++k) ag[n][k] += cols[((w * N + n) * L + l) * 8 + k];
     }
     float *pg = a.part + (size_t)blockIdx.x * d;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int c = (n * L + l) * 8;
+        const int c = n * L * 8 + l * W;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (c + k < d) pg[c + k] = ag[n][k];
+        for (int k = 0; k < 8; ++k) {
+            const int at = c + k + (k < 4 ? 0 : H - 4);
+            if (at < d) pg[at] = ag[n][k];
+        }
     }
 }
 
@@ -370,7 +368,7 @@ __global__ __launch_bounds__(256) void rmsnorm_backward_long_kernel(const rms_ba
     const float r = a.rstd[t];
     float s = 0.0f;
     auto terms = [&](int c, float (&xh)[8], float (&dv)[8], oct<BF> *ds) {
-        rms_back_row<BF, KEPT> o;
+        rms_back_row<BF, KEPT, 4> o;
         float g[8];
         o.ask(a, t, c);
         o.values(xh);
@@ -406,7 +404,7 @@ __global__ __launch_bounds__(64) void rmsnorm_columns_kernel(rms_backward_args a
     float ag[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     a.dsum = nullptr;
     for (int t = blockIdx.y; t < a.T; t += gridDim.y) {
-        rms_back_row<BF, KEPT> o;
+        rms_back_row<BF, KEPT, 4> o;
         float v[8];
         o.ask(a, t, c);
         o.values(v);
@@ -419,33 +417,38 @@ __global__ __launch_bounds__(64) void rmsnorm_columns_kernel(rms_backward_args a
         if (c + k < d) a.part[(size_t)blockIdx.y * d + c + k] = ag[k];
 }
 
-// dgamma = sums of n rows of part [n][d]: a workgroup takes 64 columns, its 16 waves a sixteenth of the rows each, joined in LDS
+// dgamma = sums of n rows of part [n][d]: a workgroup takes 16 columns, 64 slices of the rows, joined across lanes and in LDS
 __global__ __launch_bounds__(1024) void rmsnorm_join_kernel(const float *__restrict__ part, int n, int d, float *__restrict__ dgamma)
 {
-    __shared__ float red[16][64];
-    const int cc = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + cc;
+    __shared__ float red[16][16];
+    const int cc = threadIdx.x & 15, k = threadIdx.x >> 4, c = blockIdx.x * 16 + cc;
     float s = 0.0f;
-    for (int i0 = k; i0 < n && c < d; i0 += 16 * 16) {  // sixteen rows asked for together
-        float v[16];
+    for (int i0 = k; i0 < n && c < d; i0 += 64 * 8) {  // eight rows asked for together
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = i0 + 16 * j < n ? part[(size_t)(i0 + 16 * j) * d + c] : 0.0f;
+        for (int j = 0; j < 8; ++j) v[j] = i0 + 64 * j < n ? part[(size_t)(i0 + 64 * j) * d + c] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s += v[j];
+        for (int j = 0; j < 8; ++j) s += v[j];
     }
-    red[k][cc] = s;
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if ((threadIdx.x & 48) == 0) red[threadIdx.x >> 6][cc] = s;
     __syncthreads();
-    if (k > 0 || c >= d) return;
+    if (threadIdx.x >= 16 || c >= d) return;
+    s = 0.0f;
 #pragma unroll
-    for (int w = 1; w < 16; ++w) s += red[w][cc];
+    for (int w = 0; w < 16; ++w) s += red[w][cc];
     dgamma[c] = s;
 }
 
-// Lanes that share a row of d elements, 8 each: a wave, or a workgroup of 4, 8 or 16 (0: too long for them)
-static int rms_lanes(int d) { return d <= 512 ? 64 : d <= 2048 ? 256 : d <= 4096 ? 512 : d <= 8192 ? 1024 : 0; }
+// Lanes that share a row of d elements, 8 each: a wave (16 each above 512: 4001 x 1023 in fp32, forward 9.0 us and backward 12.8, where four waves a row
+// took 9.5 and 13.4), or a workgroup of 4, 8 or 16 waves (0: too long for them)
+static int rms_lanes(int d) { return d <= 1024 ? 64 : d <= 2048 ? 256 : d <= 4096 ? 512 : d <= 8192 ? 1024 : 0; }
 
 #define RMS_L(B, K, X, grid, lds, s, ...)                                                                       \
     do {                                                                                                        \
-        if (lanes == 64) hipLaunchKernelGGL((K<B, 1, 64, X>), grid, dim3(256), lds, s, __VA_ARGS__);            \
+        if (lanes == 64 && a.d <= 512) hipLaunchKernelGGL((K<B, 1, 64, X>), grid, dim3(256), lds, s, __VA_ARGS__); \
+        else if (lanes == 64) hipLaunchKernelGGL((K<B, 2, 64, X>), grid, dim3(256), lds, s, __VA_ARGS__);       \
         else if (lanes == 256) hipLaunchKernelGGL((K<B, 1, 256, X>), grid, dim3(256), 0, s, __VA_ARGS__);       \
         else if (lanes == 512) hipLaunchKernelGGL((K<B, 1, 512, X>), grid, dim3(512), 0, s, __VA_ARGS__);       \
         else hipLaunchKernelGGL((K<B, 1, 1024, X>), grid, dim3(1024), 0, s, __VA_ARGS__);                       \
@@ -480,7 +483,10 @@ hipError_t launch_rmsnorm_forward(const omega_ctx *ctx, const rmsnorm_forward &p
     return hipGetLastError();
 }
 
-// Workgroups of the backward launch = rows of partial sums, which are written and read besides
+// Workgroups of the backward launch = rows of partial sums, which are written and read besides: as few as keep the memory busy.  A compute unit
+// holds 3 of d <= 1024 (16384 x 1024 in bf16: 24.2 us, 2 of them 24.6, 4 of them 28.7), 2 of d <= 2048 (4096 x 2048: 15.2 us, 4 of them 17.5), 1 of
+// longer rows (4096 x 4096: 25.6 us, 2 of them 27.2).  Small batches: two rows at least for each row of sums (2048 x 768: 7.5 us and 2.8 for the
+// sums, with half as many 6.8 and 3.3).
 static int rms_backward_groups(const omega_ctx *ctx, int T, int d)
 {
     const int lanes = rms_lanes(d), per = lanes == 64 ? 3 : lanes == 256 ? 2 : 1, rows = lanes == 64 ? 4 : 1;
@@ -501,10 +507,10 @@ hipError_t launch_rmsnorm_backward(const omega_ctx *ctx, const rmsnorm_backward 
             RMS_LONG(rmsnorm_columns_kernel, kept, dim3(ceil_div(p.d, 512), n), 64, a);
             RMS_LONG(rmsnorm_backward_long_kernel, kept, dim3(p.T), 256, a);
         } else {
-            const size_t lds = lanes == 64 ? (size_t)3 * ((p.d + 7) & ~7) * sizeof(float) : 0;
+            const size_t lds = lanes == 64 ? (size_t)3 * (p.d <= 512 ? 512 : 1024) * sizeof(float) : 0;
             RMS_RUN(rmsnorm_backward_kernel, kept, dim3(n), lds, s, a);
         }
     }
-    hipLaunchKernelGGL(rmsnorm_join_kernel, dim3(ceil_div(p.d, 64)), dim3(1024), 0, s, (const float *)ws, n, p.d, p.dgamma);
+    hipLaunchKernelGGL(rmsnorm_join_kernel, dim3(ceil_div(p.d, 16)), dim3(1024), 0, s, (const float *)ws, n, p.d, p.dgamma);
     return hipGetLastError();
 }
