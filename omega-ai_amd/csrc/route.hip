@@ -10,7 +10,8 @@
 // The choice is that of worths in 64 bits.  They are formed in fp32, a few instructions an expert, and where two that the choice tells apart are nearer
 // to each other than their errors, or equal, those few are formed in double and put in order; where they are not few, or it is groups, the whole token is
 // chosen for again in double, by a wave of its workgroup at the end (route_exact).
-// L lanes share a token, V experts a lane.  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
+// L lanes share a token, V experts a lane (vector instructions are the bound: 16384 x 256 with bias and groups 18 us, 1.0 TB/s, with neither 9 us; the bytes
+// alone would take 3).  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
 // replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
 // the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
 #include <float.h>
@@ -46,10 +47,12 @@ __device__ __forceinline__ uint32_t over_token(uint32_t v, F meet)
     v = meet(v, lane_of<0x124>(v));
     v = meet(v, lane_of<0x122>(v));
     v = meet(v, lane_of<0x121>(v));
-    if (L == 64) {
-        u32x2 u = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    if (L >= 32) {
+        const u32x2 u = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         v = meet(u[0], u[1]);
-        u = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    }
+    if (L == 64) {
+        const u32x2 u = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         v = meet(u[0], u[1]);
     }
     return v;
@@ -58,7 +61,7 @@ __device__ __forceinline__ uint32_t over_token(uint32_t v, F meet)
 template <int L>
 __device__ __forceinline__ unsigned long long token_bits(unsigned long long lanes)
 {
-    return L == 64 ? lanes : (lanes >> (threadIdx.x & 48)) & 0xffffull;
+    return L == 64 ? lanes : (lanes >> (threadIdx.x & (64 - L))) & ((1ull << (L & 63)) - 1);
 }
 template <int L>
 __device__ __forceinline__ float token_max(float v)
@@ -105,8 +108,13 @@ __device__ __forceinline__ float open_logit(float z) { return fminf(or_closed(z)
 #define ROUTE_OPEN 0x00800000u  // that of the lowest number: -infinity's is below, and so is 0
 __device__ __forceinline__ uint32_t ordered(float v)
 {
-    const uint32_t u = __float_as_uint(v + 0.0f);  // (both zeros the same)
+    const uint32_t u = __float_as_uint(v);
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long ordered(double v)
+{
+    const unsigned long long u = *(const unsigned long long *)&v;
+    return u ^ ((unsigned long long)((long long)u >> 63) | 1ull << 63);
 }
 __device__ __forceinline__ float of_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
@@ -161,49 +169,54 @@ __device__ __forceinline__ double over_wave(double v, F meet)
 #undef ACROSS
     return v;
 }
-__device__ __forceinline__ double wave_max(double v) { return over_wave(v, [](double a, double b) { return fmax(a, b); }); }
 
-// The choice for one token in double, by a wave: lane j's place.  row: its logits; spare: room for E doubles in LDS; top and recip: of its softmax.
+// The choice for one token in double, by a wave: lane j's place.  row: its logits; spare: room for 64 N doubles in LDS, where each lane keeps its experts'
+// (loops that are not unrolled: few waves come here, and wait for their instructions most of all); top and recip: of its softmax.
 template <int N>
-__device__ __forceinline__ int route_exact(const route_args &a, const float *row, double *spare, float *top_out, float *recip_out)
+__device__ __forceinline__ int route_exact(const route_args &a, const float *row, const float *bias, double *spare, float *top_out, float *recip_out)
 {
     const int lane = threadIdx.x & 63, E = a.E;
-    float z[N], bias[N];  // of experts lane + 64 i
-    double key[N];
+    float z[N];  // of experts lane + 64 i
+    double *own = spare + lane;
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] = row[min(lane + 64 * i, E - 1)];
+    float top = -FLT_MAX;
+    uint32_t left = 0, shut = 0;  // bit i: expert lane + 64 i has not been chosen; it is closed
 #pragma unroll
-    for (int i = 0; i < N; ++i) bias[i] = a.bias != nullptr ? a.bias[min(lane + 64 * i, E - 1)] : 0.0f;
+    for (int i = 0; i < N; ++i) {
+        left |= lane + 64 * i < E ? 1u << i : 0u;
+        z[i] = lane + 64 * i < E ? open_logit(z[i]) : -INFINITY;
+        shut |= z[i] == -INFINITY ? 1u << i : 0u;
+        top = fmaxf(top, z[i]);
+    }
+    wave_lds();  // (what the wave had there has been read)
+#pragma unroll
+    for (int i = 0; i < N; ++i) own[64 * i] = (double)z[i];
     double m = 0.0, sum = 1.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = lane + 64 * i < E ? open_logit(z[i]) : -INFINITY;
     if (!a.sigmoid) {
-        float top = z[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
-        m = (double)fmaxf(token_max<64>(top), -FLT_MAX);
+        m = (double)token_max<64>(top);
         sum = 0.0;
     }
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < N; ++i) {  // (closed ones: e^-inf = 0)
-        key[i] = exp(a.sigmoid ? -(double)z[i] : (double)z[i] - m);
-        if (!a.sigmoid) sum += key[i];
-        if (N > 2 && i & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time: registers)
+        const double x = exp(a.sigmoid ? -own[64 * i] : own[64 * i] - m);
+        own[64 * i] = x;
+        if (!a.sigmoid) sum += x;
     }
     if (!a.sigmoid) sum = over_wave(sum, [](double x, double y) { return x + y; });
     *top_out = (float)m;
     *recip_out = sum > 0.0 ? (float)(1.0 / sum) : 0.0f;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < N; ++i) {
-        const double v = (a.sigmoid ? 1.0 / (1.0 + key[i]) : key[i] / sum) + (double)bias[i];
-        key[i] = z[i] == -INFINITY || !(v == v) ? -INFINITY : v;
-        if (N > 2 && i & 1) __builtin_amdgcn_sched_barrier(0);
+        const double x = own[64 * i];
+        double v = (a.sigmoid ? 1.0 : x) / (a.sigmoid ? 1.0 + x : sum);
+        if (bias != nullptr) v += (double)bias[min(lane + 64 * i, E - 1)];
+        own[64 * i] = ((shut >> i) & 1) || !(v == v) ? -INFINITY : v;
     }
-    if (a.groups > 1) {
-        wave_lds();
+    double key[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (lane + 64 * i < E) spare[lane + 64 * i] = key[i];
+    for (int i = 0; i < N; ++i) key[i] = own[64 * i];
+    if (a.groups > 1) {
         wave_lds();
         double best = -INFINITY;
         if (lane < a.groups) {
@@ -217,8 +230,10 @@ __device__ __forceinline__ int route_exact(const route_args &a, const float *row
             if (a.group_best == 2 && second > -INFINITY) best += second;
         }
         int ahead = 0;
+        const u32x2 u = *(const u32x2 *)&best;
         for (int g = 0; g < a.groups; ++g) {
-            const double v = __shfl(best, g);
+            const u32x2 o = {(uint32_t)__builtin_amdgcn_readlane((int)u[0], g), (uint32_t)__builtin_amdgcn_readlane((int)u[1], g)};
+            const double v = *(const double *)&o;
             ahead += v > best || (v == best && g < lane) ? 1 : 0;
         }
         const unsigned long long stay = __ballot(lane < a.groups && ahead < a.top_groups);
@@ -229,10 +244,7 @@ __device__ __forceinline__ int route_exact(const route_args &a, const float *row
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        if (a.bias == nullptr && key[i] > -INFINITY) key[i] = (double)z[i];
-    uint32_t left = 0;  // bit i: expert lane + 64 i has not been chosen
-#pragma unroll
-    for (int i = 0; i < N; ++i) left |= lane + 64 * i < E ? 1u << i : 0u;
+        if (bias == nullptr && key[i] > -INFINITY) key[i] = (double)z[i];
     int place = ROUTE_NONE;
     for (int j = 0; j < a.K; ++j) {
         double bv = -INFINITY;
@@ -240,13 +252,17 @@ __device__ __forceinline__ int route_exact(const route_args &a, const float *row
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (((left >> i) & 1) && (be == INT_MAX || key[i] > bv)) bv = key[i], be = lane + 64 * i;
-        const double top = wave_max(bv);
-        const bool none = top == -INFINITY;  // (a layer's token then takes the first of the others)
+        // the largest of the upper halves of their orders, mostly one lane's, else of the lower ones among those
+        const unsigned long long o = be != INT_MAX ? ordered(bv + 0.0) : 0ull;
+        const uint32_t hi = (uint32_t)(o >> 32), top = token_max<64>(hi);
+        const bool none = top < 0x00100000u;  // (-infinity at best; a layer's token then takes the first of the others)
         if (none && !a.fill) break;
-        int e = bv == top ? be : INT_MAX;
-        const unsigned long long have = __ballot(e != INT_MAX);
-        if (have & (have - 1)) {  // equal ones: the first
-            for (int s = 32; s > 0; s >>= 1) e = min(e, __shfl_xor(e, s));
+        int e = be != INT_MAX && hi == top ? be : INT_MAX;
+        unsigned long long have = __ballot(e != INT_MAX);
+        if (have & (have - 1)) {
+            const uint32_t lo = e != INT_MAX ? (uint32_t)o : 0u;
+            if (lo != token_max<64>(lo)) e = INT_MAX;
+            for (int s = 32; s > 0; s >>= 1) e = min(e, __shfl_xor(e, s));  // equal ones: the first
         } else e = __builtin_amdgcn_readlane(e, __ffsll((long long)have) - 1);
         if ((e & 63) == lane) left &= ~(1u << (e >> 6));
         if (lane == j) place = none ? e | ROUTE_FILL : e;
@@ -304,11 +320,11 @@ __device__ __forceinline__ void route_write(const route_args &a, const float *ro
 
 // A token in doubt, by a wave
 template <int N>
-__device__ __forceinline__ void route_again(const route_args &a, int t, double *spare, int *hist)
+__device__ __forceinline__ void route_again(const route_args &a, int t, const float *bias, double *spare, int *hist)
 {
     const float *row = a.logits + (size_t)t * a.E;
     float top, recip;
-    const int at[1] = {route_exact<N>(a, row, spare, &top, &recip)};
+    const int at[1] = {route_exact<N>(a, row, bias, spare, &top, &recip)};
     route_write<64>(a, row, t, true, threadIdx.x & 63, at, top, recip, hist);
 }
 
@@ -327,7 +343,6 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     constexpr uint32_t LOW = V - 1;                      // bits of a word that say which of a lane's experts it is
     static_assert((V & (V - 1)) == 0 && V * L <= ROUTE_MAX_E, "places of a lane's experts in whole bits");
     extern __shared__ __attribute__((aligned(16))) uint32_t spare_all[];
-    __shared__ u32x2 picks_all[8][TW][64 + 2];           // the chosen words and their lanes
     __shared__ int again[ROUTE_TOKENS], n_again;         // tokens that are chosen for in double
     __shared__ int hist[EW];
     __shared__ __attribute__((aligned(16))) float bias[WORTH ? EW : 1];
@@ -378,7 +393,11 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
             for (int k = 0; k < V; ++k) z[k] = ld_at(rows, (uint32_t)(at0 + min(expert(k), E - 1)));
         }
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] = open_logit(expert(k) < E ? z[k] : -INFINITY);
+        for (int k = 0; k < V; ++k) z[k] = open_logit(z[k]);
+        if (E < EW) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) z[k] = expert(k) < E ? z[k] : -INFINITY;
+        }
         // scores, where the choice or the weights need all of them
         float top = 0.0f, recip = 1.0f;
         if (softmax_row) {
@@ -397,7 +416,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         uint32_t word[V];
         if (!WORTH) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) word[k] = ordered(z[k]);
+            for (int k = 0; k < V; ++k) word[k] = ordered(z[k] + 0.0f);  // (both zeros the same)
         } else {
             float u[V];
 #pragma unroll
@@ -415,12 +434,28 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
             }
 #pragma unroll
             for (int k = 0; k < V; ++k) u[k] = or_closed(fmaf(z[k], 0.0f, u[k]));  // (-infinity times 0 is no number, others' nothing)
+            if (a.bias != nullptr) {  // (no sum of a score and a bias is -0)
 #pragma unroll
-            for (int k = 0; k < V; ++k) word[k] = ordered(a.bias != nullptr ? u[k] : z[k]);
+                for (int k = 0; k < V; ++k) word[k] = ordered(u[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) word[k] = ordered(z[k] + 0.0f);
+            }
             if (a.groups > 1) {
                 wave_lds();  // (what the wave's last tokens left there has been read)
+                const bool whole = C == 4 && (a.per_group & 3) == 0;  // a piece of four experts is one group's: its two best are enough
+                float2 *ub = (float2 *)uw;
+                if (whole) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) uw[route_padded(expert(k))] = u[k];
+                    for (int k = 0; k + 3 < V; k += 4) {
+                        const float m0 = fmaxf(u[k], u[k + 1]), n0 = fminf(u[k], u[k + 1]), m1 = fmaxf(u[k + 2], u[k + 3]), n1 = fminf(u[k + 2], u[k + 3]);
+                        const int at = k / 4 * L + sub;
+                        ub[at + (at >> 3)] = make_float2(fmaxf(m0, m1), fmaxf(fmaxf(n0, n1), fminf(m0, m1)));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) uw[route_padded(expert(k))] = u[k];
+                }
                 wave_lds();
                 const int q = 1 << a.group_shift, g = sub >> a.group_shift, i = sub & (q - 1);
                 float best = -INFINITY, second = -INFINITY;
@@ -429,7 +464,15 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
                     best = fmaxf(best, b);
                 };
                 if (g < a.groups) {
-                    for (int e = g * a.per_group + i; e < (g + 1) * a.per_group; e += q) meet(uw[route_padded(e)], -INFINITY);
+                    if (whole) {
+                        const int n = a.per_group >> 2;
+                        for (int at = g * n + i; at < (g + 1) * n; at += q) {
+                            const float2 b = ub[at + (at >> 3)];
+                            meet(b.x, b.y);
+                        }
+                    } else {
+                        for (int e = g * a.per_group + i; e < (g + 1) * a.per_group; e += q) meet(uw[route_padded(e)], -INFINITY);
+                    }
                 }
                 // (after each step its lanes hold the same, so that a mirror is a neighbour)
                 if (q > 1) meet(lane_of<0xB1>(best), lane_of<0xB1>(second));
@@ -581,7 +624,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     }
     __syncthreads();
     // in double, a wave each
-    for (int i = wave; i < n_again; i += NT / 64) route_again<(L * V + 63) / 64>(a, again[i], (double *)spare, hist);
+    for (int i = wave; i < n_again; i += NT / 64) route_again<(L * V + 63) / 64>(a, again[i], WORTH && a.bias != nullptr ? bias : nullptr, (double *)spare, hist);
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += NT) a.part[(size_t)blockIdx.x * E + e] = hist[e];
 }
@@ -732,52 +775,65 @@ __global__ __launch_bounds__(256) void route_balance_kernel(const int32_t *__res
     }
 }
 
-// How a batch is cut.  Sixteen lanes a token do the least work for it, a wave ends soonest (64 experts and fewer leave half of it idle); a few tokens are
-// one workgroup's, which needs no second launch for the counts.  (Groups: one lane for each at least.)
+// How a batch is cut.  Few lanes a token do the least work for it (16; above 256 experts 32: 65536 x 512, softmax, 49 us, with a wave a token 78), a wave ends
+// soonest: sixteen tokens a compute unit and fewer have one each (E = 256, sigmoid, 8 groups: 4096 tokens 13.0 us, with 16 lanes 13.8; 8192 tokens 17.4 and
+// 14.0; at 64 experts and fewer half of it is idle).  What one workgroup takes at once it does alone, without a second launch for the counts (64
+// tokens of 128 experts 5.4 us a call, in several workgroups 6.3; 64 of 256 experts, two rounds of its waves, 7.9 and 6.4).  Groups: one lane for each at
+// least.
 struct route_cut {
-    bool waves;           // a wave a token
-    int threads, tokens;  // of a workgroup
+    int lanes, threads, tokens;  // of a token; of a workgroup
 };
-// words of LDS of a wave
-static int route_wave_words(int E, int K, bool waves)
+static int route_per_lane(int E, int lanes)
 {
-    const int L = waves ? 64 : 16, V = waves ? (E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : 8) : E <= 16 ? 1 : E <= 64 ? 4 : E <= 128 ? 8 : 16;
-    return route_lds(L, V) + 64 / L * 2 * (K + 2);
+    if (lanes == 64) return E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : 8;
+    return lanes == 32 ? 16 : E <= 16 ? 1 : E <= 64 ? 4 : E <= 128 ? 8 : 16;
+}
+// words of LDS of a wave
+static int route_wave_words(int E, int K, int lanes) { return route_lds(lanes, route_per_lane(E, lanes)) + 64 / lanes * 2 * (K + 2); }
+static int route_lanes(const omega_route_config &c, bool few)
+{
+    const int least = c.E <= 256 ? 16 : 32;
+    return c.groups > least || (few && c.E > 64) ? 64 : least;
 }
 static route_cut route_cut_of(const omega_ctx *ctx, const omega_route_config &c, int T)
 {
     const bool must = c.groups > 16 || c.E > 256;
-    // (sixteen waves where their LDS is within 64 KB, beside the workgroup's own)
-    if (!must && T <= 64) return {T <= 16, 16 * 4 * route_wave_words(c.E, c.K, T <= 16) <= 56 << 10 ? 1024 : 512, 64};
-    const bool waves = must || (c.E > 64 && T <= 16 * ctx->num_cus);
-    const int round = waves ? 8 : 32;  // tokens that the waves of a workgroup take at once
-    return {waves, 512, std::min(std::max(1, ceil_div(ceil_div(T, 2 * ctx->num_cus), round)) * round, ROUTE_TOKENS)};
+    if (!must) {
+        // one workgroup of sixteen waves, of eight where their LDS would not be within 64 KB, beside the workgroup's own: its tokens at once
+        const int lanes = T <= 16 ? 64 : 16, threads = 16 * 4 * route_wave_words(c.E, c.K, lanes) <= 56 << 10 ? 1024 : 512;
+        if (T <= threads / lanes) return {lanes, threads, 64};
+    }
+    const int lanes = route_lanes(c, T <= 16 * ctx->num_cus);
+    const int round = 8 * (64 / lanes);  // tokens that the waves of a workgroup take at once
+    return {lanes, 512, std::min(std::max(1, ceil_div(ceil_div(T, 2 * ctx->num_cus), round)) * round, ROUTE_TOKENS)};
 }
 
-static route_args route_arguments(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, bool waves, int32_t *ids, float *w)
+static route_args route_arguments(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, int L, int32_t *ids, float *w)
 {
-    const int E = c.E, L = waves ? 64 : 16, vec = E % 4 == 0 && (uintptr_t)logits % 16 == 0;
+    const int E = c.E, vec = E % 4 == 0 && (uintptr_t)logits % 16 == 0;
     int shift = 0;  // lanes of a group: as many as the next power of two of groups leaves
     while (c.groups > 1 && (2 << shift) * c.groups <= L) ++shift;
     return {logits, bias, T, E, c.K, c.score == OMEGA_ROUTE_SIGMOID, c.renorm, c.groups, c.top_groups, c.group_best, E / c.groups, (1 << 20) / (E / c.groups) + 1,
             shift, c.scale, tokens, 0, vec, ids, w, nullptr};
 }
-static hipError_t route_launch(const route_args &a, bool waves, int threads, hipStream_t s)
+static hipError_t route_launch(const route_args &a, int lanes, int threads, hipStream_t s)
 {
     const int E = a.E, T = a.T, tokens = a.tokens;
     const bool worth = a.bias != nullptr || a.groups > 1;
 #define ROUTE_FORWARD(LL, V)                                                                                                                     \
     do {                                                                                                                                         \
         const dim3 grid(ceil_div(T, tokens));                                                                                                    \
-        const size_t lds = (size_t)threads / 64 * route_wave_words(E, a.K, waves) * sizeof(float);                                                \
+        const size_t lds = (size_t)threads / 64 * route_wave_words(E, a.K, lanes) * sizeof(float);                                                \
         if (worth) hipLaunchKernelGGL((route_forward_kernel<LL, V, true>), grid, dim3(threads), lds, s, a);                                      \
         else hipLaunchKernelGGL((route_forward_kernel<LL, V, false>), grid, dim3(threads), lds, s, a);                                           \
     } while (0)
-    if (waves) {
+    if (lanes == 64) {
         if (E <= 64) ROUTE_FORWARD(64, 1);
         else if (E <= 128) ROUTE_FORWARD(64, 2);
         else if (E <= 256) ROUTE_FORWARD(64, 4);
         else ROUTE_FORWARD(64, 8);
+    } else if (lanes == 32) {
+        ROUTE_FORWARD(32, 16);
     } else {
         if (E <= 16) ROUTE_FORWARD(16, 1);
         else if (E <= 64) ROUTE_FORWARD(16, 4);
@@ -797,9 +853,9 @@ hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &
     if (T > 0) {
         const route_cut cut = route_cut_of(ctx, c, T);
         n = ceil_div(T, cut.tokens);
-        route_args a = route_arguments(c, logits, T, bias, cut.tokens, cut.waves, ids, w);
+        route_args a = route_arguments(c, logits, T, bias, cut.tokens, cut.lanes, ids, w);
         a.part = n == 1 && counts ? counts : (int32_t *)ws;
-        const hipError_t e = route_launch(a, cut.waves, cut.threads, s);
+        const hipError_t e = route_launch(a, cut.lanes, cut.threads, s);
         if (e != hipSuccess || n == 1 || !counts) return e;
     }
     hipLaunchKernelGGL(route_counts_kernel, dim3(ceil_div(c.E, 16)), dim3(1024), 0, s, (const int32_t *)ws, n, c.E, counts);
@@ -810,11 +866,11 @@ hipError_t launch_route_forward(const omega_ctx *ctx, const omega_route_config &
 hipError_t launch_route_layer(const omega_route_config &c, const float *logits, int T, const float *bias, int tokens, int32_t *ids, float *w, int32_t *tile_counts,
                               hipStream_t s)
 {
-    const bool waves = c.groups > 16 || c.E > 256;
-    route_args a = route_arguments(c, logits, T, bias, tokens, waves, ids, w);
+    const int lanes = route_lanes(c, false);
+    route_args a = route_arguments(c, logits, T, bias, tokens, lanes, ids, w);
     a.fill = 1;
     a.part = tile_counts;
-    return route_launch(a, waves, 256, s);
+    return route_launch(a, lanes, 256, s);
 }
 
 #define ROUTE_RUN(K, grid, s, ...)                                                                       \
