@@ -56,18 +56,18 @@ def _tensor(meta, shape, key):
 def _names(scheme, i):
     if scheme == "omega":
         p = f"layers.{i}.feed_forward."
-        return dict(gate=p + "gate.weight", gate_bias=p + "gate.bias", norm=f"layers.{i}.ffn_norm.weight",
+        return dict(gate=p + "gate.weight", gate_bias=p + "gate.bias", balance=p + "gate.balance", norm=f"layers.{i}.ffn_norm.weight",
                     expert=lambda e, w: f"{p}experts.{e}.{w}.weight",
                     shared=lambda s, w: f"{p}shared_experts.{s}.{w}.weight", dense=lambda w: f"{p}{w}.weight",
                     fused_shared=None)
     if scheme == "mixtral":
         p = f"model.layers.{i}.block_sparse_moe."
-        return dict(gate=p + "gate.weight", gate_bias=None, norm=f"model.layers.{i}.post_attention_layernorm.weight",
+        return dict(gate=p + "gate.weight", gate_bias=None, balance=None, norm=f"model.layers.{i}.post_attention_layernorm.weight",
                     expert=lambda e, w: f"{p}experts.{e}.{w}.weight", shared=None, dense=None, fused_shared=None)
     if scheme == "deepseek":
         p = f"model.layers.{i}.mlp."
         proj = {"w1": "gate_proj", "w3": "up_proj", "w2": "down_proj"}
-        return dict(gate=p + "gate.weight", gate_bias=p + "gate.e_score_correction_bias",
+        return dict(gate=p + "gate.weight", gate_bias=p + "gate.e_score_correction_bias", balance=p + "gate.e_score_correction_bias",
                     norm=f"model.layers.{i}.post_attention_layernorm.weight",
                     expert=lambda e, w: f"{p}experts.{e}.{proj[w]}.weight", shared=None, dense=None,
                     fused_shared=lambda w: f"{p}shared_experts.{proj[w]}.weight")
@@ -77,7 +77,7 @@ def _names(scheme, i):
 def load_moe_weights(layer, weight_map, layer_index=0, scheme="omega", strict=True):
     """Copies the entries of `weight_map` (a dict as read_weight_map returns, or a path) that belong to layer
     `layer_index` into `layer` (anything with embedDim, hidden, nExperts, nShared, hasBias, set_gate, set_expert,
-    set_norm).  Returns the list of expected names that were absent; with strict=True (default) an absent
+    set_norm; with hasBalance also set_balance: the bias of its routing, which takes the name "deepseek" has for either).  Returns the list of expected names that were absent; with strict=True (default) an absent
     expert or gate weight raises instead (the reference reports "<key> is null." and goes on; a layer with
     unset experts is never what the caller wants).  The norm weight is optional: it belongs to the block form."""
     if isinstance(weight_map, (str, bytes)):
@@ -96,10 +96,15 @@ def load_moe_weights(layer, weight_map, layer_index=0, scheme="omega", strict=Tr
         raise RuntimeError("Error code 1:sigmoid-gated shared expert (shared_expert_gate) is not supported by this layer")
     Wg = get(nm["gate"], (E, d))
     bg = None
-    if layer.hasBias and nm["gate_bias"] is not None:
+    balance = nm["balance"] if getattr(layer, "hasBalance", False) else None
+    if layer.hasBias and nm["gate_bias"] is not None and nm["gate_bias"] != balance:
         bg = get(nm["gate_bias"], (E,))
     if Wg is not None:
         layer.set_gate(Wg, bg)
+    if balance is not None:
+        b = get(balance, (E,))
+        if b is not None:
+            layer.set_balance(b)
     def one_expert(key):
         """(W1, W3, W2) of the expert whose parameter names key(w) gives, from the separate or the fused form."""
         if scheme == "omega" and key("w12") in weight_map:
@@ -143,7 +148,7 @@ def load_moe_weights(layer, weight_map, layer_index=0, scheme="omega", strict=Tr
 
 
 def export_moe_weights(arrays, layer_index=0, scheme="omega", gamma=None, fused12=False):
-    """The inverse, for tests and for exporting a layer: arrays = dict(Wg [E,d], bg [E]|None, W1,W3 [E+Es,H,d],
+    """The inverse, for tests and for exporting a layer: arrays = dict(Wg [E,d], bg [E]|None, balance [E]|None, W1,W3 [E+Es,H,d],
     W2 [E+Es,d,H]) -> {name: nested lists}.  fused12 ("omega" only): every expert in the DiTSwiGLUFFN form, w12 =
     [w1; w3] and the down projection under the name w3."""
     if fused12 and scheme != "omega":
@@ -154,6 +159,10 @@ def export_moe_weights(arrays, layer_index=0, scheme="omega", gamma=None, fused1
     out = {nm["gate"]: arrays["Wg"].tolist()}
     if arrays.get("bg") is not None and nm["gate_bias"] is not None:
         out[nm["gate_bias"]] = arrays["bg"].tolist()
+    if arrays.get("balance") is not None and nm["balance"] is not None:
+        if nm["balance"] in out:
+            raise ValueError(f"scheme {scheme!r} has one name for the gate's bias and the routing's")
+        out[nm["balance"]] = arrays["balance"].tolist()
     def put(key, g):
         if fused12:
             out[key("w12")] = np.concatenate([arrays["W1"][g], arrays["W3"][g]], axis=0).tolist()
