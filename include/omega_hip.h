@@ -397,7 +397,7 @@ int omega_hip_route_forward(omega_ctx *ctx, const omega_route_config *cfg, const
 /* dlogits [T,E] (overwritten) = gradient through the weights of the chosen, the choice held: with u = w / scale
  *   renorm        dz_j = w_j g_j, g_j = sum_k u_k (dw_j - dw_k), times 1 - s_j for sigmoid scores; zero for experts that were not chosen
  *   else sigmoid  dz_j = w_j dw_j (1 - s_j);   else softmax   dz_e = [chosen] w_e dw_e - s_e sum_k w_k dw_k
- * with the forward pass's ids and w.  An id outside 0..E-1 and a weight of 0 have no part.  logits may be NULL for softmax with renorm. */
+ * with the forward pass's ids and w, the ids of a token different ones.  An id outside 0..E-1 and a weight of 0 have no part.  logits may be NULL for softmax with renorm. */
 int omega_hip_route_backward(omega_ctx *ctx, const omega_route_config *cfg, const float *logits, int T, const int32_t *ids, const float *w, const float *dw,
                              float *dlogits);
 /* bias[e] += rate where counts[e] is below the mean of counts [E], -= rate where above. */
@@ -415,7 +415,7 @@ int omega_moe_balance(omega_moe *moe, float rate);
 /* ---- Operators around the experts of a block, on caller-owned buffers under the same terms ---- */
 
 /* RMS norm with the addition of a residual in front of it: h = x + residual rounded once to dtype (residual NULL: h = x),
- * q = 1 / sqrt(mean(h^2) + eps), y = h q gamma.  x, residual, sum, out [T,d] of dtype, gamma [d] fp32.  Written, each may be NULL:
+ * q = 1 / sqrt(mean(h^2) + eps), y = h q gamma; q is a float: infinite where eps is 0 and the mean below 2^-256.  x, residual, sum, out [T,d] of dtype, gamma [d] fp32.  Written, each may be NULL:
  *   sum        h, what the next residual addition takes (only with a residual; may be x or residual itself);
  *   out        y in dtype;
  *   out8, out8_scales   y in 8 bits, the form OMEGA_KEEP8_MX (both or neither);

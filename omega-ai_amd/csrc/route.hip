@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const route_back_ar
         dot = token_sum<L>(dot);
     }
 #pragma unroll
-    for (int i = 0; i < KL; ++i)
+    for (int i = 0; i < KL; ++i)  // (a token's ids differ: one addition a place, of which no order shows)
         if (id[i] >= 0) atomicAdd(&dz[id[i]], w[i] * g[i] * rest[i]);
     wave_lds();
     float top = 0.0f, recip = 0.0f;

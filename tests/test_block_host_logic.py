@@ -190,6 +190,7 @@ def test_a_layers_routing(lib, ctx, dtype):
     lib.host_take_block()
     assert kept(lib.omega_moe_balance, 0.1) == 0 and lib.host_take_block() == b"balance\n"
     assert lib.omega_moe_backward(m, A, D, 40, E) == 0                  # a step of the bias leaves the batch as it is
+    assert lib.omega_moe_get_grad(m, L.W_BALANCE, 0, host.ctypes.data, 0) == BAD    # it has no gradient
     assert lib.omega_moe_forward(m, A, 100, B) == 0                     # a larger batch: the logits grow with the workspace
     assert kept(lib.omega_moe_set_routing, C.byref(config(groups=1, top_groups=1)), 0) == 0
     assert weights(lib.omega_moe_get_weights) == BAD and lib.omega_moe_forward(m, A, 100, B) == 0 and kept(lib.omega_moe_balance, 0.1) == BAD
