@@ -118,31 +118,36 @@ class RMSLayer(_Layer):
         self.gamma = gamma
         self.input = self.sum = self.kept = self.diffGamma = self._for = None
 
-    def _ready(self, shape, summed):
-        """What a batch of that shape is written to: sum, rstd, out, out8, kept.  (Looked up together: one by one costs a decode step's call 1 of 6 us.)"""
-        batch = (shape, summed, self.out8, self.keep8)
-        if batch != self._for:
-            self._for = None
-            self._held = (self._buffer("sum", shape, self.dtype) if summed else None, self._buffer("rstd", (shape[0],), "f32"),
-                          None if self.out8 else self._buffer("out", shape, self.dtype), _rows8(self, "rows8_out", "mx", shape) if self.out8 else None,
-                          _rows8(self, "rows8_kept", "int8", shape) if self.keep8 else None)
-            self._for = batch
-        return self._held
+    def _ready(self, x, summed):
+        """What a batch like x is written to: sum, rstd, out, out8, kept.  (Made, and x looked at, when another batch comes: both again for every call would cost a
+        decode step's 1.5 of 5 us.)"""
+        shape = x.shape
+        _want(len(shape) == 2 and shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
+        self.input = self._for = None
+        self._held = (self._buffer("sum", shape, self.dtype) if summed else None, self._buffer("rstd", (shape[0],), "f32"),
+                      None if self.out8 else self._buffer("out", shape, self.dtype), _rows8(self, "rows8_out", "mx", shape) if self.out8 else None,
+                      _rows8(self, "rows8_kept", "int8", shape) if self.keep8 else None)
 
     def forward(self, x, residual=None):
         """norm(x + residual); the sum is self.sum (None without a residual)."""
-        shape = x.shape
-        _want(len(shape) == 2 and shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
-        _want(residual is None or (residual.shape == shape and residual.dtype == x.dtype and residual.ptr), "residual shape or dtype")   # (no address would mean none)
-        _want(self.gamma is not None, "the layer has no gamma")
-        self.input = None   # (until the call has succeeded)
-        self.sum, rstd, out, o8, kept = self._ready(shape, residual is not None)
-        h = self.sum
-        _want(h is None or h.ptr, "sum has been freed")
-        self.ctx.check(self.lib.omega_hip_rmsnorm_forward(
-            self.ctx.handle, x.ptr, residual.ptr if h else None, _DT[self.dtype], shape[0], shape[1], self.gamma.ptr, self.eps, h.ptr if h else None,
+        shape, gamma, ctx = x.shape, self.gamma, self.ctx
+        _want(gamma is not None, "the layer has no gamma")
+        if residual is not None:
+            _want(residual.shape == shape and residual.dtype == x.dtype and residual.ptr, "residual shape or dtype")   # (no address would mean none)
+        batch = (shape, x.dtype, residual is None, self.out8, self.keep8)
+        if batch != self._for:
+            self._ready(x, residual is not None)
+            self._for = batch
+        h, rstd, out, o8, kept = self._held
+        self.input, self.sum = None, h   # (no input until the call has succeeded)
+        if h is not None:
+            _want(h.ptr, "sum has been freed")
+        st = self.lib.omega_hip_rmsnorm_forward(
+            ctx.handle, x.ptr, residual.ptr if h else None, _DT[x.dtype], shape[0], shape[1], gamma.ptr, self.eps, h.ptr if h else None,
             out.ptr if out else None, o8.codes.ptr if o8 else None, o8.scales.ptr if o8 else None, kept.codes.ptr if kept else None,
-            kept.scales.ptr if kept else None, rstd.ptr))
+            kept.scales.ptr if kept else None, rstd.ptr)
+        if st:
+            ctx.check(st)
         self.input, self.kept = x if h is None else h, kept
         return out or o8
 
