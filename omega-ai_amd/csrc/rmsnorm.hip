@@ -486,11 +486,12 @@ hipError_t launch_rmsnorm_forward(const omega_ctx *ctx, const rmsnorm_forward &p
 // Workgroups of the backward launch = rows of partial sums, which are written and read besides: as few as keep the memory busy.  A compute unit
 // holds 3 of d <= 1024 (16384 x 1024 in bf16: 24.2 us, 2 of them 24.6, 4 of them 28.7), 2 of d <= 2048 (4096 x 2048: 15.2 us, 4 of them 17.5), 1 of
 // longer rows (4096 x 4096: 25.6 us, 2 of them 27.2).  Small batches: two rows at least for each row of sums (2048 x 768: 7.5 us and 2.8 for the
-// sums, with half as many 6.8 and 3.3).
+// sums, with half as many 6.8 and 3.3).  Up to sixteen rows of a wave each, four of others: one workgroup, whose sums are dgamma (360 elements: 16 rows 5.0 us a call,
+// as two launches 6.0; 32 rows 7.4 and 6.0; 4096 elements: 4 rows 6.0 and 7.0, 8 rows 8.6 and 7.0).
 static int rms_backward_groups(const omega_ctx *ctx, int T, int d)
 {
     const int lanes = rms_lanes(d), per = lanes == 64 ? 3 : lanes == 256 ? 2 : 1, rows = lanes == 64 ? 4 : 1;
-    return std::max(1, std::min(per * ctx->num_cus, ceil_div(T, 2 * rows)));
+    return T <= 4 * rows ? 1 : std::min(per * ctx->num_cus, ceil_div(T, 2 * rows));
 }
 
 size_t rmsnorm_backward_workspace(const omega_ctx *ctx, int T, int d) { return (size_t)rms_backward_groups(ctx, T, d) * d * sizeof(float); }
@@ -498,11 +499,11 @@ size_t rmsnorm_backward_workspace(const omega_ctx *ctx, int T, int d) { return (
 hipError_t launch_rmsnorm_backward(const omega_ctx *ctx, const rmsnorm_backward &p, void *ws, hipStream_t s)
 {
     const bool bf = p.dtype == OMEGA_DTYPE_BF16, kept = p.keep8 != nullptr;
-    const rms_backward_args a = {p.h, p.keep8, p.keep_scale, p.dout, p.dsum, p.T, p.d, p.gamma, p.rstd, p.dx, (float *)ws};
     int n = 0;
     if (p.T > 0) {
         const int lanes = rms_lanes(p.d);
         n = rms_backward_groups(ctx, p.T, p.d);
+        const rms_backward_args a = {p.h, p.keep8, p.keep_scale, p.dout, p.dsum, p.T, p.d, p.gamma, p.rstd, p.dx, n == 1 ? p.dgamma : (float *)ws};
         if (lanes == 0) {
             RMS_LONG(rmsnorm_columns_kernel, kept, dim3(ceil_div(p.d, 512), n), 64, a);
             RMS_LONG(rmsnorm_backward_long_kernel, kept, dim3(p.T), 256, a);
@@ -510,6 +511,7 @@ hipError_t launch_rmsnorm_backward(const omega_ctx *ctx, const rmsnorm_backward 
             const size_t lds = lanes == 64 ? (size_t)3 * (p.d <= 512 ? 512 : 1024) * sizeof(float) : 0;
             RMS_RUN(rmsnorm_backward_kernel, kept, dim3(n), lds, s, a);
         }
+        if (n == 1) return hipGetLastError();
     }
     hipLaunchKernelGGL(rmsnorm_join_kernel, dim3(ceil_div(p.d, 16)), dim3(1024), 0, s, (const float *)ws, n, p.d, p.dgamma);
     return hipGetLastError();

@@ -367,10 +367,10 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         }
         span = token_max<64>(span);
     }
-    // What two worths may differ by although they are equal, of twice the largest score and the largest bias.  Sigmoid: 4 2^-24 each (e^-z 2 + |z|, the
-    // addition one, the reciprocal two, weighed by the curve's slope) and a rounding with the bias, 8 2^-24 (1 + worth) in all.  Softmax: four
-    // each and twenty in common (the sum of up to 512 terms and its reciprocal, whose error the biases do not share), 28 2^-24.
-    const float unsure = a.sigmoid ? 0x1p-20f : 0x1p-19f;
+    // What two worths may differ by although they are equal, of twice the largest score and the largest bias, in units of 2^-24.  Sigmoid: e^-z 2 + 1.22 |z| of
+    // itself, a score by 0.8 of that at most (its slope is s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each, of 2 + |b| 8
+    // in all.  Softmax: four each and twenty in common (the sum of up to 512 terms and its reciprocal, whose error the biases do not share), 28.
+    const float unsure = a.sigmoid ? 0x1p-21f : 0x1p-19f;
     const int end = min(a.T, (int)(blockIdx.x + 1) * a.tokens);
     for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
         const int t = t0 + tok;
