@@ -56,14 +56,14 @@ public:
         }
         h_ = nullptr;  // (until the call has succeeded)
         Tensor &out = detail::sized(out_, x.number, d_, gamma_.ctx), &st = detail::sized(rstd_, 1, x.number, gamma_.ctx);
-        if (residual) detail::sized(sum_, x.number, d_, gamma_.ctx);
-        else sum_.reset();
+        Tensor *h = residual ? &detail::sized(sum_, x.number, d_, gamma_.ctx) : nullptr;  // (an older sum stays: x may be it)
+        summed_ = h != nullptr;
         uint8_t *codes = keep_ ? (uint8_t *)codes_.of((size_t)x.number * d_) : nullptr;
         float *scales = keep_ ? (float *)scales_.of((size_t)x.number * ((d_ + 127) / 128) * 4) : nullptr;
         check(gamma_.ctx->get(), omega_hip_rmsnorm_forward(gamma_.ctx->get(), x.gpuData, residual ? residual->gpuData : nullptr, OMEGA_DTYPE_F32, x.number, d_,
-                                                           (const float *)gamma_.gpuData, eps_, sum_ ? sum_->gpuData : nullptr, out.gpuData, nullptr, nullptr,
+                                                           (const float *)gamma_.gpuData, eps_, h ? h->gpuData : nullptr, out.gpuData, nullptr, nullptr,
                                                            codes, scales, (float *)st.gpuData));
-        h_ = sum_ ? sum_.get() : &x;
+        h_ = h ? h : &x;
         rows_ = x.number;
         return out;
     }
@@ -73,6 +73,10 @@ public:
         detail::want(h_, "back without a forward");
         detail::rows_of(delta, d_, "delta shape does not match the output");
         detail::want(delta.number == rows_, "delta shape does not match the output");
+        if (!keep_) {
+            detail::rows_of(*h_, d_, "the input has another shape than in the forward pass");
+            detail::want(h_->number == rows_, "the input has another shape than in the forward pass");
+        }
         if (dsum) {
             detail::rows_of(*dsum, d_, "dsum shape does not match the sum");
             detail::want(dsum->number == rows_, "dsum shape does not match the sum");
@@ -84,13 +88,13 @@ public:
                                                             (float *)dg.gpuData));
         return dx;
     }
-    Tensor *getSum() { return sum_.get(); }
+    Tensor *getSum() { return summed_ ? sum_.get() : nullptr; }
     Tensor *getDiffGamma() { return diffGamma_.get(); }
 
 private:
     int d_, rows_ = 0;
     float eps_;
-    bool keep_;
+    bool keep_, summed_ = false;
     Tensor &gamma_, *h_ = nullptr;
     detail::Memory codes_, scales_;
     std::unique_ptr<Tensor> out_, sum_, rstd_, diff_, diffGamma_;
@@ -143,15 +147,18 @@ public:
         check(ctx_.get(), omega_hip_route_forward(ctx_.get(), &c_, (const float *)logits.gpuData, logits.number, bias_ ? (const float *)bias_->gpuData : nullptr,
                                                   (int32_t *)ids_.of((size_t)logits.number * c_.K * 4), (float *)w.gpuData, (int32_t *)counts_.of((size_t)c_.E * 4)));
         x_ = &logits;
+        rows_ = logits.number;
         return w;
     }
     Tensor &back(Tensor &delta)
     {
         detail::want(x_, "back without a forward");
         detail::rows_of(delta, c_.K, "delta shape does not match the weights");
-        detail::want(delta.number == x_->number, "delta shape does not match the weights");
-        Tensor &dx = detail::sized(diff_, x_->number, c_.E, &ctx_);
-        check(ctx_.get(), omega_hip_route_backward(ctx_.get(), &c_, (const float *)x_->gpuData, x_->number, (const int32_t *)ids_.get(), (const float *)w_->gpuData,
+        detail::want(delta.number == rows_, "delta shape does not match the weights");
+        detail::rows_of(*x_, c_.E, "the logits have another shape than in the forward pass");
+        detail::want(x_->number == rows_, "the logits have another shape than in the forward pass");
+        Tensor &dx = detail::sized(diff_, rows_, c_.E, &ctx_);
+        check(ctx_.get(), omega_hip_route_backward(ctx_.get(), &c_, (const float *)x_->gpuData, rows_, (const int32_t *)ids_.get(), (const float *)w_->gpuData,
                                                    (const float *)delta.gpuData, (float *)dx.gpuData));
         return dx;
     }
@@ -160,7 +167,7 @@ public:
         detail::want(x_ && bias_, "balance without a bias or a forward");
         check(ctx_.get(), omega_hip_route_balance(ctx_.get(), (const int32_t *)counts_.get(), c_.E, rate, (float *)bias_->gpuData));
     }
-    std::vector<int32_t> getIds() const { return host(ids_, (size_t)(x_ ? x_->number : 0) * c_.K); }
+    std::vector<int32_t> getIds() const { return host(ids_, (size_t)(x_ ? rows_ : 0) * c_.K); }
     std::vector<int32_t> getCounts() const { return host(counts_, x_ ? (size_t)c_.E : 0); }
 
 private:
@@ -173,6 +180,7 @@ private:
     omega_route_config c_;
     Context &ctx_;
     Tensor *bias_, *x_ = nullptr;
+    int rows_ = 0;
     detail::Memory ids_, counts_;
     std::unique_ptr<Tensor> w_, diff_;
 };
