@@ -57,13 +57,13 @@ __device__ __forceinline__ F row_total(F s, F *red)
     for (int w = 0; w < L / 64; ++w) s += red[w];
     return s;
 }
-// 1 / sqrt(a) to a rounding or two of double: two steps of Newton's from the instruction's 2^-26
+// 1 / sqrt(a) to a rounding or two of double: two steps of Newton's from the instruction's 2^-26 (which is the answer for 0 and infinity)
 __device__ __forceinline__ double rsqrt64(double a)
 {
-    double q = __builtin_amdgcn_rsq(a);
-    const double h = 0.5 * a;
-    q = q * fma(-h * q, q, 1.5);
-    return q * fma(-h * q, q, 1.5);
+    const double q = __builtin_amdgcn_rsq(a), h = 0.5 * a;
+    double r = q * fma(-h * q, q, 1.5);
+    r = r * fma(-h * r, r, 1.5);
+    return r == r ? r : q;
 }
 
 // Codes of y = v q gamma and their group's scale, those of y in double: y in fp32 is within three roundings of it, and what lies nearer to a border
