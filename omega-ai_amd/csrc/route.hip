@@ -10,8 +10,8 @@
 // The choice is that of worths in 64 bits.  They are formed in fp32, a few instructions an expert, and where two that the choice tells apart are nearer
 // to each other than their errors, or equal, those few are formed in double and put in order; where they are not few, or it is groups, the whole token is
 // chosen for again in double, by a wave of its workgroup at the end (route_exact).
-// L lanes share a token, V experts a lane (vector instructions are the bound: 16384 x 256 with bias and groups 18 us, 1.0 TB/s, with neither 9 us; the bytes
-// alone would take 3).  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
+// L lanes share a token, V experts a lane (vector instructions are the bound: 16384 x 256 with bias and groups 13 us, and 5 more where a token
+// is chosen for again; with neither 9 us; the bytes alone would take 3).  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
 // replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
 // the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
 #include <float.h>
@@ -62,6 +62,12 @@ template <int L>
 __device__ __forceinline__ unsigned long long token_bits(unsigned long long lanes)
 {
     return L == 64 ? lanes : (lanes >> (threadIdx.x & (64 - L))) & ((1ull << (L & 63)) - 1);
+}
+// the first lane of each token's of a ballot that every token has a lane in
+template <int L>
+__device__ __forceinline__ unsigned long long first_lanes(unsigned long long lanes)
+{
+    return lanes & ((L == 64 ? 1ull : L == 32 ? 0x0000000100000001ull : 0x0001000100010001ull) + ~lanes);
 }
 template <int L>
 __device__ __forceinline__ float token_max(float v)
@@ -369,8 +375,9 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     }
     // What two worths may differ by although they are equal, of twice the largest score and the largest bias, in units of 2^-24.  Sigmoid: e^-z 2 + 1.22 |z| of
     // itself, a score by 0.8 of that at most (its slope is s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each, of 2 + |b| 8
-    // in all.  Softmax: four each and twenty in common (the sum of up to 512 terms and its reciprocal, whose error the biases do not share), 28.
-    const float unsure = a.sigmoid ? 0x1p-21f : 0x1p-19f;
+    // in all.  Softmax: e^x 2.5 (|x| e^x is 0.37 at most), the bias's rounding s + |b|, in common the sum's V + 8 and the reciprocal's 1, whose error the biases do
+    // not share: (V + 16) s + 2 |b| in all, and twice that and 4 (s + |b|) for the sums of two that groups are told by.
+    const float unsure = a.sigmoid ? 0x1p-21f : (float)(V + 24) * 0x1p-25f;
     const int end = min(a.T, (int)(blockIdx.x + 1) * a.tokens);
     for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
         const int t = t0 + tok;
@@ -537,7 +544,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         int taken = 0;
         for (int j = 0; j < K + 2; ++j) {  // (two more: what is left has to be told from what is chosen)
             const uint32_t b = token_max<L>(first);
-            if (first == b) {  // (two lanes: told by what they have taken, and chosen for again; none open left: any of them)
+            if (__builtin_amdgcn_inverse_ballot_w64(first_lanes<L>(__ballot(first == b)))) {  // (two lanes that hold it: their turn one by one)
                 picks[j] = u32x2{b, (uint32_t)sub};
                 const bool open = b >= ROUTE_OPEN;
                 taken += open ? 1 : 0;
@@ -547,7 +554,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         }
         wave_lds();
         // The chosen and, next to each, the one behind it: lane sub has the places sub, sub + L, ...
-        int at[KL], all = -taken;
+        int at[KL];
         bool near = false;
         auto apart = [&](uint32_t b, uint32_t o) {  // b >= o
             return o < ROUTE_OPEN || (WORTH && a.bias != nullptr ? of_ordered(b & ~LOW) - of_ordered(o & ~LOW) > (unsure + (float)V * 0x1p-23f) * most  // (the words' last bits besides)
@@ -568,9 +575,6 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
                 if (at[i] < 0 && a.fill) doubt = true;
             }
         }
-#pragma unroll
-        for (int i = 0; i <= KL; ++i)
-            if (sub + i * L < K + 2) all += picks[sub + i * L][0] >= ROUTE_OPEN ? 1 : 0;
         if (__ballot(near)) {
             // They and the two behind them once more, a lane each, without a bias as they are, else in double.  Where the last of these is near to the last
             // chosen there may be more.
@@ -616,7 +620,6 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
                 if (at[0] >= 0) at[0] = (int)picks[sub][0];
             }
         }
-        doubt |= token_sum<L>((float)all) != 0.0f;  // (as many taken as chosen: no two lanes held the same word)
         const unsigned long long doubts = token_bits<L>(__ballot(doubt));
         if (doubts && live && sub == 0) again[atomicAdd(&n_again, 1)] = t;
         route_write<L>(a, rows + at0, t, live && !doubts, sub, at, top, recip, hist);
@@ -775,7 +778,7 @@ __global__ __launch_bounds__(256) void route_balance_kernel(const int32_t *__res
     }
 }
 
-// How a batch is cut.  Few lanes a token do the least work for it (16; above 256 experts 32: 65536 x 512, softmax, 49 us, with a wave a token 78), a wave ends
+// How a batch is cut.  Few lanes a token do the least work for it (16; above 256 experts 32: 65536 x 512, softmax, 44 us, with a wave a token 78), a wave ends
 // soonest: sixteen tokens a compute unit and fewer have one each (E = 256, sigmoid, 8 groups: 4096 tokens 13.0 us, with 16 lanes 13.8; 8192 tokens 17.4 and
 // 14.0; at 64 experts and fewer half of it is idle).  What one workgroup takes at once it does alone, without a second launch for the counts (64
 // tokens of 128 experts 5.4 us a call, in several workgroups 6.3; 64 of 256 experts, two rounds of its waves, 7.9 and 6.4).  Groups: one lane for each at
