@@ -11,8 +11,8 @@
 // to each other than their errors, or equal, those few are formed in double and put in order; where they are not few, or it is groups, the whole token is
 // chosen for again in double, by a wave of its workgroup at the end (route_exact).
 // L lanes share a token, V experts a lane (vector instructions are the bound: 16384 x 256 with bias and groups 13 us, and 5 more where a token
-// is chosen for again; with neither 9 us; the bytes alone would take 3).  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
-// replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
+// is chosen for again; with neither 9 us; the bytes alone would take 3).  What is compared of an expert is one word: its worth as a whole number
+// of the same order, the last bits replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
 // the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
 #include <float.h>
 
@@ -632,7 +632,8 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     for (int e = threadIdx.x; e < E; e += NT) a.part[(size_t)blockIdx.x * E + e] = hist[e];
 }
 
-// counts = sums of n rows of part [n][E]: a workgroup takes 16 experts, 64 rows at a time
+// counts = sums of n rows of part [n][E]: a workgroup takes 16 experts, 64 rows at a time (512 x 256: 3.8 us, 128 x 128: 2.5; one memory latency
+// and the launch)
 __global__ __launch_bounds__(1024) void route_counts_kernel(const int32_t *__restrict__ part, int n, int E, int32_t *__restrict__ counts)
 {
     __shared__ int red[16][16];
@@ -664,7 +665,9 @@ struct route_back_args {
     const float *w, *dw;
     float *dlogits;
 };
-// L lanes a token; a lane takes the chosen j = sub, sub + L, ... and, as in the forward pass, V experts in pieces of C
+// L lanes a token; a lane takes the chosen j = sub, sub + L, ... and, as in the forward pass, V experts in pieces of C.  The gradients of the chosen meet
+// the row in LDS, so that every element of dlogits is written once, 16 bytes a lane.  Bound: bytes (65536 x 256, all scores: 33 us, 4.1 TB/s; 16384 x 128:
+// 5.6 us, a launch and 8 MB).
 template <int L, int V>
 __global__ __launch_bounds__(256) void route_backward_kernel(const route_back_args a)
 {
