@@ -336,9 +336,11 @@ __device__ __forceinline__ void route_again(const route_args &a, int t, const fl
 
 // Words of LDS that a wave needs: the worths of its tokens for their groups (four words of padding behind 32: groups of 32 in different banks), then the
 // lanes' lists and one more word each; one token's worths in double
-static constexpr int route_worths(int E) { return E + E / 8; }
+static constexpr int route_worths(int E) { return (E + E / 8 + 3) & ~3; }
 __device__ __forceinline__ int route_padded(int e) { return e + (e >> 5) * 4; }
 static constexpr int route_lds(int L, int V) { return std::max(std::max(64 * (V + 1), 2 * L * V), 64 / L * route_worths(L * V)); }
+// ... and with the picks of its tokens, all of a wave (pieces of 16 bytes)
+__host__ __device__ static constexpr int route_words(int L, int V, int K) { return (route_lds(L, V) + 64 / L * 2 * (K + 2) + 3) & ~3; }
 
 // WORTH: there is a bias or there are groups
 template <int L, int V, bool WORTH>
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     __shared__ __attribute__((aligned(16))) float bias[WORTH ? EW : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane & (L - 1), tok = lane / L;
     const int E = a.E, K = a.K, NT = blockDim.x;
-    uint32_t *spare = spare_all + wave * (route_lds(L, V) + TW * 2 * (K + 2)), *list = spare + lane;
+    uint32_t *spare = spare_all + wave * route_words(L, V, K), *list = spare + lane;
     float *uw = (float *)spare + tok * route_worths(EW);
     u32x2 *picks = (u32x2 *)(spare + route_lds(L, V)) + tok * (K + 2);  // the chosen words and the lanes that held them, and two behind them
     const bool softmax_row = !a.sigmoid && (WORTH || !a.renorm);
@@ -794,8 +796,7 @@ static int route_per_lane(int E, int lanes)
     if (lanes == 64) return E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : 8;
     return lanes == 32 ? 16 : E <= 16 ? 1 : E <= 64 ? 4 : E <= 128 ? 8 : 16;
 }
-// words of LDS of a wave
-static int route_wave_words(int E, int K, int lanes) { return route_lds(lanes, route_per_lane(E, lanes)) + 64 / lanes * 2 * (K + 2); }
+static int route_wave_words(int E, int K, int lanes) { return route_words(lanes, route_per_lane(E, lanes), K); }
 static int route_lanes(const omega_route_config &c, bool few)
 {
     const int least = c.E <= 256 ? 16 : 32;
