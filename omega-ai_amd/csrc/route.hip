@@ -100,15 +100,16 @@ __device__ __forceinline__ float sigmoid(float z)
     const float e = exp_neg(-fabsf(z));
     return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
-// the larger of v and -infinity: no number becomes -infinity (written out: a comparison and a choice are two instructions)
+// the larger of v and -infinity: no number becomes -infinity.  v is a result of arithmetic: of a signalling NaN, which only memory holds, the instruction
+// makes a quiet one (written out: the compiler would quiet v again in front of it)
 __device__ __forceinline__ float or_closed(float v)
 {
     float r;
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(v), "s"(0xff800000u));
     return r;
 }
-// a logit as it is compared: closed ones -infinity, infinite ones the largest number
-__device__ __forceinline__ float open_logit(float z) { return fminf(or_closed(z), FLT_MAX); }
+// a logit as it is compared: closed ones -infinity, infinite ones the largest number (v from memory: quieted first, as fmaxf does)
+__device__ __forceinline__ float open_logit(float z) { return fminf(fmaxf(z, -INFINITY), FLT_MAX); }
 
 // A float as a whole number of the same order; and back
 #define ROUTE_OPEN 0x00800000u  // that of the lowest number: -infinity's is below, and so is 0
