@@ -335,11 +335,11 @@ __device__ __forceinline__ void route_again(const route_args &a, int t, const fl
     route_write<64>(a, row, t, true, threadIdx.x & 63, at, top, recip, hist);
 }
 
-// Words of LDS that a wave needs: the worths of its tokens for their groups (four words of padding behind 32: groups of 32 in different banks), then the
-// lanes' lists and one more word each; one token's worths in double
-static constexpr int route_worths(int E) { return (E + E / 8 + 3) & ~3; }
+// Words of LDS that a wave needs: the worths of its tokens for their groups (four words of padding behind 32: groups of 32 in different banks) and then two
+// words for each group, of which a token has as many as lanes at most; the lanes' lists and one more word each; one token's worths in double
+static constexpr int route_worths(int L, int V) { return std::max((L * V + L * V / 8 + 3) & ~3, 2 * L); }
 __device__ __forceinline__ int route_padded(int e) { return e + (e >> 5) * 4; }
-static constexpr int route_lds(int L, int V) { return std::max(std::max(64 * (V + 1), 2 * L * V), 64 / L * route_worths(L * V)); }
+static constexpr int route_lds(int L, int V) { return std::max(std::max(64 * (V + 1), 2 * L * V), 64 / L * route_worths(L, V)); }
 // ... and with the picks of its tokens, all of a wave (pieces of 16 bytes)
 __host__ __device__ static constexpr int route_words(int L, int V, int K) { return (route_lds(L, V) + 64 / L * 2 * (K + 2) + 3) & ~3; }
 
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane & (L - 1), tok = lane / L;
     const int E = a.E, K = a.K, NT = blockDim.x;
     uint32_t *spare = spare_all + wave * route_words(L, V, K), *list = spare + lane;
-    float *uw = (float *)spare + tok * route_worths(EW);
+    float *uw = (float *)spare + tok * route_worths(L, V);
     u32x2 *picks = (u32x2 *)(spare + route_lds(L, V)) + tok * (K + 2);  // the chosen words and the lanes that held them, and two behind them
     const bool softmax_row = !a.sigmoid && (WORTH || !a.renorm);
     for (int e = threadIdx.x; e < EW; e += NT) {
@@ -367,19 +367,11 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     }
     if (threadIdx.x == 0) n_again = 0;
     __syncthreads();
-    float span = 0.0f;  // the largest finite bias
-    if (WORTH && a.bias != nullptr) {
-#pragma unroll
-        for (int k = 0; k < (EW + 63) / 64; ++k) {
-            const float b = fabsf(bias[min(lane + 64 * k, EW - 1)]);
-            span = b < INFINITY ? fmaxf(span, b) : span;
-        }
-        span = token_max<64>(span);
-    }
-    // What two worths may differ by although they are equal, of twice the largest score and the largest bias, in units of 2^-24.  Sigmoid: e^-z 2 + 1.22 |z| of
-    // itself, a score by 0.8 of that at most (its slope is s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each, of 2 + |b| 8
-    // in all.  Softmax: e^x 2.5 (|x| e^x is 0.37 at most), the bias's rounding s + |b|, in common the sum's V + 8 and the reciprocal's 1, whose error the biases do
-    // not share: (V + 16) s + 2 |b| in all, and twice that and 4 (s + |b|) for the sums of two that groups are told by.
+    // What two worths u may differ by although they are equal, of twice the largest score and the larger |u| (a bias is at most |u| + s: one that switches
+    // an expert off says nothing about others), in units of 2^-24.  Sigmoid: e^-z 2 + 1.22 |z| of itself, a score by 0.8 of that at most (its slope is
+    // s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each, 12 + 2 |u| of both, of 2 + |u| 8 in all.  Softmax: e^x 2.5
+    // (|x| e^x is 0.37 at most), the bias's rounding s + |b|, in common the sum's V + 8 and the reciprocal's 1, whose error the biases do not share:
+    // (V + 18) s + 2 |u| in all.  Sums of two, by which groups are told apart: each group twice that, 2 |u| for the addition and as much for the bound itself.
     const float unsure = a.sigmoid ? 0x1p-21f : (float)(V + 24) * 0x1p-25f;
     const int end = min(a.T, (int)(blockIdx.x + 1) * a.tokens);
     for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
@@ -421,7 +413,8 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
             s = token_sum<L>(s);
             recip = s > 0.0f ? 1.0f / s : 0.0f;
         }
-        const float most = 2.0f * recip + span;  // (sigmoid: scores up to 1)
+        // of a worth's size, and of the score's part in it (sigmoid: scores up to 1; an infinite bias is as far from the others as the largest number)
+        auto doubtful = [&](float u) { return fmaf(2.0f, recip, fminf(u, FLT_MAX)); };
         bool doubt = false;
         uint32_t word[V];
         if (!WORTH) {
@@ -490,21 +483,23 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
                 if (q > 4) meet(lane_of<0x141>(best), lane_of<0x141>(second));
                 if (q > 8) meet(lane_of<0x140>(best), lane_of<0x140>(second));
                 if (q > 16) meet(__shfl_xor(best, 16), __shfl_xor(second, 16));
-                const float mine = a.group_best == 2 && second > -INFINITY ? best + second : best;
+                const bool two = a.group_best == 2 && second > -INFINITY;
+                const float mine = two ? best + second : best;
+                // what it may be at most and at least, of which every group has its own
+                const float off = unsure * doubtful(two ? fmaxf(fabsf(best), fabsf(second)) : fabsf(best)), least = mine - off;
                 wave_lds();
-                if (i == 0) uw[g] = mine;
+                if (i == 0) ((float2 *)uw)[g] = make_float2(mine, mine + off);
                 wave_lds();
-                const float tell = 2.0f * unsure * most;  // (four worths and two additions)
                 int ahead = 0;
                 bool near = false;
                 for (int o0 = 0; o0 < a.groups; o0 += 4) {
-                    const float4 o4 = *(const float4 *)(uw + o0);
-                    const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+                    const float4 o2[2] = {((const float4 *)uw)[o0 / 2], ((const float4 *)uw)[o0 / 2 + 1]};
+                    const float o[4] = {o2[0].x, o2[0].z, o2[1].x, o2[1].z}, at_most[4] = {o2[0].y, o2[0].w, o2[1].y, o2[1].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool there = o0 + k < a.groups, in_front = there & ((o[k] > mine) | ((o[k] == mine) & (o0 + k < g)));
                         ahead += in_front ? 1 : 0;
-                        near |= there & !in_front & (o0 + k != g) & (o[k] > -INFINITY) & !(mine - o[k] > tell);
+                        near |= there & !in_front & (o0 + k != g) & (o[k] > -INFINITY) & !(least > at_most[k]);
                     }
                 }
                 doubt = g < a.groups && near && ahead == a.top_groups - 1;  // (the last group that stays, and one behind it)
@@ -560,8 +555,9 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         int at[KL];
         bool near = false;
         auto apart = [&](uint32_t b, uint32_t o) {  // b >= o
-            return o < ROUTE_OPEN || (WORTH && a.bias != nullptr ? of_ordered(b & ~LOW) - of_ordered(o & ~LOW) > (unsure + (float)V * 0x1p-23f) * most  // (the words' last bits besides)
-                                                                 : (b & ~LOW) != (o & ~LOW));
+            if (!WORTH || a.bias == nullptr) return o < ROUTE_OPEN || (b & ~LOW) != (o & ~LOW);
+            const float x = of_ordered(b & ~LOW), y = of_ordered(o & ~LOW);
+            return o < ROUTE_OPEN || x - y > (unsure + (float)V * 0x1p-23f) * doubtful(fmaxf(fabsf(x), fabsf(y)));  // (the words' last bits besides)
         };
         auto expert_of = [&](u32x2 p) {
             const int k = (int)(LOW - (p[0] & LOW));
