@@ -484,7 +484,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
                 if (q > 8) meet(lane_of<0x140>(best), lane_of<0x140>(second));
                 if (q > 16) meet(__shfl_xor(best, 16), __shfl_xor(second, 16));
                 const bool two = a.group_best == 2 && second > -INFINITY;
-                const float mine = two ? best + second : best;
+                const float mine = two ? fmaxf(best + second, -FLT_MAX) : best;  // (below the lowest number: in doubt, but not closed)
                 // what it may be at most and at least, of which every group has its own
                 const float off = unsure * doubtful(two ? fmaxf(fabsf(best), fabsf(second)) : fabsf(best)), least = mine - off;
                 wave_lds();

@@ -30,3 +30,23 @@ def test_the_value_that_switches_off_does_not_matter(T, E, K, groups, top, best,
     for ids, w, counts in got[1:]:
         assert np.array_equal(ids, got[0][0]) and np.array_equal(counts, got[0][2])
         assert np.array_equal(w, got[0][1])
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("T", [7, 200, 4200])
+@pytest.mark.parametrize("E", [8, 24, 128, 384])
+def test_groups_worth_less_than_the_lowest_number(E, T, sigmoid):
+    """The sum of two worths may lie below what fp32 holds: such a group is behind the others and in front of one that has nothing open."""
+    rng = np.random.default_rng(E + T)
+    groups, n = 4, E // 4
+    z = rng.standard_normal((T, E)).astype(np.float32)
+    b = (0.1 * rng.standard_normal(E)).astype(np.float32)
+    z[:, 3:n] = -np.inf                               # the first group: three open at most
+    z[:, n:2 * n] = -np.inf                           # the second: nothing
+    for low in (LOWEST, LOWEST / 2):                  # the third: switched off; the fourth: a little less so
+        b[2 * n:3 * n] = LOWEST
+        b[3 * n:] = low
+        for top in (2, 3):
+            R.check(z, b, 2 * n if n < 5 else 7, sigmoid=sigmoid, groups=groups, top=top, best=2)
+        b[3 * n:] = 0.05
+        R.check(z, b, 2, sigmoid=sigmoid, groups=groups, top=3, best=2)
