@@ -127,7 +127,7 @@ __device__ __forceinline__ uint32_t magnitude(const float (&v)[8])
 // Codes of eight elements of a group of 128 and the group's scale (the same in its 16 lanes).
 // m = x (1/s) + 1.5 2^23, rounded once, holds the whole number in its low bits; r = x - q s is exact (a multiple of the lower of x's and s's last
 // places, below s).  q is the nearest unless |r| reaches s / 2, which a quotient next to a half may do by the error of 1/s: then it moves on by one,
-// on a half where it is odd.
+// on a half where it is odd.  (2 |r| against s: half of a scale below 2^-125 need not be a number of fp32.)
 __device__ __forceinline__ u32x2_by to_int8(const float (&v)[8], float *scale)
 {
     const uint32_t most = max_over_16(magnitude(v));
@@ -141,11 +141,11 @@ __device__ __forceinline__ u32x2_by to_int8(const float (&v)[8], float *scale)
         r[k] = fmaf(-(t - 0x1.8p23f), s, v[k]);
         worst = fmaxf(worst, fabsf(r[k]));
     }
-    if (worst >= 0.5f * s) {
+    if (worst + worst >= s) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float a = fabsf(r[k]);
-            if (a > 0.5f * s || (a == 0.5f * s && (m[k] & 1))) m[k] += r[k] < 0.0f ? -1 : 1;
+            const float a = fabsf(r[k]) + fabsf(r[k]);
+            if (a > s || (a == s && (m[k] & 1))) m[k] += r[k] < 0.0f ? -1 : 1;
         }
     }
     const bool none = most >= 0x7f800000u;
