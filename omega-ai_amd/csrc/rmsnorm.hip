@@ -67,24 +67,29 @@ __device__ __forceinline__ double rsqrt64(double a)
     return r == r ? r : q;
 }
 
-// Codes of y = v q gamma and their group's scale, those of y in double: y in fp32 is within three roundings of it, and what lies nearer to a border
-// (of the codes, odd multiples of half a step; of the scale, 448 2^k) is formed again.
-__device__ __forceinline__ u32x2_by norm_to_mx(const float (&v)[8], double q, const float (&gamma)[8], const float (&y)[8], uint32_t *scale)
+// Codes of y = v r gamma (r: q in fp32) and their group's scale, those of v q gamma in double: y in fp32 is within three roundings of it, and what lies
+// nearer to a border (of the codes, odd multiples of half a step; of the scale, 448 2^k) is formed again.  So is everything of a wave where that is not so:
+// where an element's v r is below the least normal number, or r is.  (y itself may be: that rounding is of multiples of 2^-149, which the borders are too.)
+__device__ __forceinline__ u32x2_by norm_to_mx(const float (&v)[8], double q, float r, const float (&gamma)[8], const float (&y)[8], uint32_t *scale)
 {
-    uint32_t most = max_over_4(magnitude(y));
+    const uint32_t most = max_over_4(magnitude(y));
     uint32_t b = mx_scale(most);
-    if ((most & 0x7fffffu) - 0x5ffffcu <= 8u && most < 0x7f800000u) {  // (the same in the group's four lanes)
+    bool low = r < 0x1p-126f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) low |= (fabsf(v[k] * r) < 0x1p-126f) & (v[k] != 0.0f);
+    low = __any(low);
+    if (((most & 0x7fffffu) - 0x5ffffcu <= 8u || low) && most < 0x7f800000u) {  // (the same in the group's four lanes)
         double m = 0.0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmax(m, fabs((double)v[k] * q * (double)gamma[k]));
-        // above 448 2^k or not: a float on the same side of it
-        const float at = __uint_as_float((most & 0x7f800000u) | 0x600000u);
-        b = mx_scale(max_over_4(m > (double)at ? __float_as_uint(at) + 1u : __float_as_uint(at)));
+        // the float above it, which is on the same side of 448 2^k
+        const float f = (float)m;
+        b = mx_scale(max_over_4(min(__float_as_uint(f) + ((double)f < m ? 1u : 0u), 0x7f7fffffu)));
     }
     *scale = b;
     const float inv = b == 255u ? 0.0f : mx_inverse(b);
     float u[8];
-    bool near = false;
+    bool near = low && b != 255u;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         u[k] = b == 255u ? 0.0f : y[k] * inv;
@@ -149,7 +154,7 @@ __device__ __forceinline__ void write_normed(const rms_forward_args &a, const fl
     if (!EIGHT) return;
     if (a.out8 != nullptr) {  // (lanes behind the row's end take part in their group: zeros)
         uint32_t b;
-        const u32x2_by codes = norm_to_mx(v, q, gamma, y, &b);
+        const u32x2_by codes = norm_to_mx(v, q, r, gamma, y, &b);
         if (n > 0) st_codes(a.out8, at, n, codes);
         if (n > 0 && c % KEEP8_MX_GROUP == 0) a.scale8[(size_t)t * ceil_div(a.d, KEEP8_MX_GROUP) + c / KEEP8_MX_GROUP] = (uint8_t)b;
     }
