@@ -367,11 +367,21 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
     }
     if (threadIdx.x == 0) n_again = 0;
     __syncthreads();
-    // What two worths u may differ by although they are equal, of twice the largest score and the larger |u| (a bias is at most |u| + s: one that switches
-    // an expert off says nothing about others), in units of 2^-24.  Sigmoid: e^-z 2 + 1.22 |z| of itself, a score by 0.8 of that at most (its slope is
-    // s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each, 12 + 2 |u| of both, of 2 + |u| 8 in all.  Softmax: e^x 2.5
-    // (|x| e^x is 0.37 at most), the bias's rounding s + |b|, in common the sum's V + 8 and the reciprocal's 1, whose error the biases do not share:
-    // (V + 18) s + 2 |u| in all.  Sums of two, by which groups are told apart: each group twice that, 2 |u| for the addition and as much for the bound itself.
+    float span = 0.0f;  // the largest bias that scores, which are 1 at most, compete with: of 16 and more it switches its expert on or off
+    if (WORTH && a.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < (EW + 63) / 64; ++k) {
+            const float b = fabsf(bias[min(lane + 64 * k, EW - 1)]);
+            span = b < 16.0f ? fmaxf(span, b) : span;
+        }
+        span = token_max<64>(span);
+    }
+    // What two worths u may differ by although they are equal, of twice the largest score and the larger bias of the two, in units of 2^-24.  Sigmoid: e^-z 2 +
+    // 1.22 |z| of itself, a score by 0.8 of that at most (its slope is s (1 - s)), the addition 1, the reciprocal 2, the bias's rounding 1 + |b|: 5 + |b| each,
+    // of 2 + |b| 8 in all.  Softmax: e^x 2.5 (|x| e^x is 0.37 at most), the bias's rounding s + |b|, in common the sum's V + 8 and the reciprocal's 1, whose
+    // error the biases do not share: (V + 16) s + 2 |b| in all.  Sums of two, by which groups are told apart: twice that, and 8 (s + |b|) for the two additions
+    // and for the bounds that each group is given.  Where |u| is below 14 the bias is at most `span`, else at most |u| + s: one that switches an expert off
+    // says nothing about the others.
     const float unsure = a.sigmoid ? 0x1p-21f : (float)(V + 24) * 0x1p-25f;
     const int end = min(a.T, (int)(blockIdx.x + 1) * a.tokens);
     for (int t0 = blockIdx.x * a.tokens + wave * TW; t0 < end; t0 += NT / 64 * TW) {
@@ -413,8 +423,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
             s = token_sum<L>(s);
             recip = s > 0.0f ? 1.0f / s : 0.0f;
         }
-        // of a worth's size, and of the score's part in it (sigmoid: scores up to 1; an infinite bias is as far from the others as the largest number)
-        auto doubtful = [&](float u) { return fmaf(2.0f, recip, fminf(u, FLT_MAX)); };
+        auto doubtful = [&](float u) { return fmaf(2.0f, recip, u < 14.0f ? span : fminf(u, FLT_MAX) + recip); };  // (sigmoid: scores up to 1)
         bool doubt = false;
         uint32_t word[V];
         if (!WORTH) {
@@ -567,6 +576,7 @@ __global__ __launch_bounds__(1024) void route_forward_kernel(const route_args a)
         for (int i = 0; i < KL; ++i) {
             const int j = sub + i * L;
             at[i] = ROUTE_NONE;
+            if (i * L >= K) continue;
             if (j < K) {
                 const u32x2 p = picks[j];
                 at[i] = expert_of(p);
