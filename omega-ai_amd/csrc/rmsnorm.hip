@@ -68,28 +68,44 @@ __device__ __forceinline__ double rsqrt64(double a)
 }
 
 // Codes of y = v r gamma (r: q in fp32) and their group's scale, those of v q gamma in double: y in fp32 is within three roundings of it, and what lies
-// nearer to a border (of the codes, odd multiples of half a step; of the scale, 448 2^k) is formed again.  So is everything of a wave where that is not so:
-// where an element's v r is below the least normal number, or r is.  (y itself may be: that rounding is of multiples of 2^-149, which the borders are too.)
-__device__ __forceinline__ u32x2_by norm_to_mx(const float (&v)[8], double q, float r, const float (&gamma)[8], const float (&y)[8], uint32_t *scale)
-{
-    const uint32_t most = max_over_4(magnitude(y));
-    uint32_t b = mx_scale(most);
-    bool low = r < 0x1p-126f;
+// nearer to a border (of the codes, odd multiples of half a step; of the scale, 448 2^k) is formed again.
+// A v r below the least normal number is off by up to 2^-149, y by that times gamma; less than 2^-30 of the scale unless the group's largest y is below 2^-110
+// of its largest gamma: such groups, and rows whose r is below the least normal number, have their y from double.  (A group of zeros is one, or has codes of
+// zero, up to a gamma of 2^12.  y itself may be subnormal: it is rounded to multiples of 2^-149, which the borders are too.)
+struct norm_small {
+    uint32_t least, span;  // groups whose largest y, as a whole number, is in least .. least + span
+    __device__ __forceinline__ explicit norm_small(const float (&gamma)[8])
+    {
+        float m = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) low |= (fabsf(v[k] * r) < 0x1p-126f) & (v[k] != 0.0f);
-    low = __any(low);
-    if (((most & 0x7fffffu) - 0x5ffffcu <= 8u || low) && most < 0x7f800000u) {  // (the same in the group's four lanes)
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(gamma[k]));
+        const float g = __uint_as_float(max_over_4(__float_as_uint(m)));
+        least = g < 0x1p12f ? 1u : 0u;
+        span = max(__float_as_uint(g * 0x1p-110f), 1u) - least;
+    }
+    __device__ __forceinline__ norm_small() {}
+};
+__device__ __forceinline__ u32x2_by norm_to_mx(const float (&v)[8], double q, float r, const float (&gamma)[8], norm_small small, float (&y)[8], uint32_t *scale)
+{
+    uint32_t most = max_over_4(magnitude(y));
+    if (__builtin_expect(r < 0x1p-126f || most - small.least <= small.span, 0)) {  // (the same in the group's four lanes)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = (float)((double)v[k] * q * (double)gamma[k]);
+        most = max_over_4(magnitude(y));
+    }
+    uint32_t b = mx_scale(most);
+    if ((most & 0x7fffffu) - 0x5ffffcu <= 8u && most < 0x7f800000u) {  // (as above)
         double m = 0.0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmax(m, fabs((double)v[k] * q * (double)gamma[k]));
-        // the float above it, which is on the same side of 448 2^k
-        const float f = (float)m;
-        b = mx_scale(max_over_4(min(__float_as_uint(f) + ((double)f < m ? 1u : 0u), 0x7f7fffffu)));
+        // above 448 2^k or not: a float on the same side of it
+        const float at = __uint_as_float((most & 0x7f800000u) | 0x600000u);
+        b = mx_scale(max_over_4(m > (double)at ? __float_as_uint(at) + 1u : __float_as_uint(at)));
     }
     *scale = b;
     const float inv = b == 255u ? 0.0f : mx_inverse(b);
     float u[8];
-    bool near = low && b != 255u;
+    bool near = false;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         u[k] = b == 255u ? 0.0f : y[k] * inv;
@@ -142,7 +158,7 @@ __device__ __forceinline__ void add_residual(const rms_forward_args &a, const oc
 }
 // what is written of eight elements of h once q is known
 template <bool BF, bool EIGHT, int H>
-__device__ __forceinline__ void write_normed(const rms_forward_args &a, const float (&v)[8], double q, const float (&gamma)[8], int t, int c)
+__device__ __forceinline__ void write_normed(const rms_forward_args &a, const float (&v)[8], double q, const float (&gamma)[8], norm_small small, int t, int c)
 {
     const int n = a.d - c;
     const size_t at = (size_t)t * a.d + c;
@@ -154,7 +170,7 @@ __device__ __forceinline__ void write_normed(const rms_forward_args &a, const fl
     if (!EIGHT) return;
     if (a.out8 != nullptr) {  // (lanes behind the row's end take part in their group: zeros)
         uint32_t b;
-        const u32x2_by codes = norm_to_mx(v, q, r, gamma, y, &b);
+        const u32x2_by codes = norm_to_mx(v, q, r, gamma, small, y, &b);
         if (n > 0) st_codes(a.out8, at, n, codes);
         if (n > 0 && c % KEEP8_MX_GROUP == 0) a.scale8[(size_t)t * ceil_div(a.d, KEEP8_MX_GROUP) + c / KEEP8_MX_GROUP] = (uint8_t)b;
     }
@@ -185,8 +201,12 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_forward_kernel(const r
     };
     ask(t);
     float g[N][8];
+    norm_small small[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) ld_par8<H>(a.gamma, n * L * 8 + l * W, d - (n * L * 8 + l * W), g[n]);
+    for (int n = 0; n < N; ++n) {
+        ld_par8<H>(a.gamma, n * L * 8 + l * W, d - (n * L * 8 + l * W), g[n]);
+        if (EIGHT) small[n] = norm_small(g[n]);
+    }
     for (; t < a.T; t += step) {
         float v[N][8];
         double s = 0.0;
@@ -205,7 +225,7 @@ __global__ __launch_bounds__(RMS_THREADS(L)) void rmsnorm_forward_kernel(const r
         turn ^= 1;
         if (l == 0 && a.rstd != nullptr) a.rstd[t] = (float)q;
 #pragma unroll
-        for (int n = 0; n < N; ++n) write_normed<BF, EIGHT, H>(a, v[n], q, g[n], t, n * L * 8 + l * W);
+        for (int n = 0; n < N; ++n) write_normed<BF, EIGHT, H>(a, v[n], q, g[n], small[n], t, n * L * 8 + l * W);
     }
 }
 
@@ -235,7 +255,7 @@ __global__ __launch_bounds__(256) void rmsnorm_forward_long_kernel(const rms_for
         const oct<BF> x = ld_oct<BF>(b.x, row + c, d - c), r = b.res != nullptr ? ld_oct<BF>(b.res, row + c, d - c) : x;
         add_residual<BF, 4>(b, x, r, row + c, d - c, v);
         ld_par<8>(a.gamma, c, d - c, g);
-        write_normed<BF, EIGHT, 4>(b, v, q, g, t, c);
+        write_normed<BF, EIGHT, 4>(b, v, q, g, EIGHT ? norm_small(g) : norm_small(), t, c);
     }
 }
 
