@@ -108,7 +108,8 @@ class RMSLayer(_Layer):
     (LlamaTransformerBlock.output, J/engine/nn/layer/llama/LlamaTransformerBlock.java:129-136): sum = x + residual, out = norm(sum).
 
     out8: the output is Rows8 of the form "mx" (read8 brings them back); keep8: the forward pass keeps what was normed in 8 bits and the
-    backward pass reads those, so that neither x nor sum has to stay."""
+    backward pass reads those.  Then the layer holds neither x nor the sum after forward(); the sum takes no memory of its own where forward() is given a
+    buffer for it, which may be the residual."""
 
     gamma = _Param(lambda layer: (layer.embedDim,), lambda layer: "f32")
 
@@ -116,30 +117,36 @@ class RMSLayer(_Layer):
         super().__init__(ctx, dtype)
         self.embedDim, self.eps, self.out8, self.keep8 = embedDim, float(eps), bool(out8), bool(keep8)
         self.gamma = gamma
-        self.input = self.sum = self.kept = self.diffGamma = self._for = None
+        self.input = self.sum = self.kept = self.diffGamma = self._for = self._rows = None
 
     def _ready(self, x, summed):
-        """What a batch like x is written to: sum, rstd, out, out8, kept.  (Made, and x looked at, when another batch comes: both again for every call would cost a
+        """What a batch like x is written to: sum (the layer's own), rstd, out, out8, kept.  (Made, and x looked at, when another batch comes: both again for every call would cost a
         decode step's 1.5 of 5 us.)"""
         shape = x.shape
         _want(len(shape) == 2 and shape[1] == self.embedDim and x.dtype == self.dtype, "input shape or dtype")
-        self.input = self._for = None
+        self.input = self._rows = self._for = None
         self._held = (self._buffer("sum", shape, self.dtype) if summed else None, self._buffer("rstd", (shape[0],), "f32"),
                       None if self.out8 else self._buffer("out", shape, self.dtype), _rows8(self, "rows8_out", "mx", shape) if self.out8 else None,
                       _rows8(self, "rows8_kept", "int8", shape) if self.keep8 else None)
 
-    def forward(self, x, residual=None):
-        """norm(x + residual); the sum is self.sum (None without a residual)."""
+    def forward(self, x, residual=None, sum=None):
+        """norm(x + residual); the sum is self.sum (None without a residual), written to the buffer `sum` of the caller (x or residual themselves, say) or
+        to the layer's own."""
         shape, gamma, ctx = x.shape, self.gamma, self.ctx
         _want(gamma is not None, "the layer has no gamma")
         if residual is not None:
             _want(residual.shape == shape and residual.dtype == x.dtype and residual.ptr, "residual shape or dtype")   # (no address would mean none)
-        batch = (shape, x.dtype, residual is None, self.out8, self.keep8)
+        if sum is not None:
+            _want(residual is not None, "a sum without a residual")
+            _want(sum.shape == shape and sum.dtype == x.dtype, "sum shape or dtype")
+        batch = (shape, x.dtype, residual is None or sum is not None, self.out8, self.keep8)
         if batch != self._for:
-            self._ready(x, residual is not None)
+            self._ready(x, not batch[2])
             self._for = batch
         h, rstd, out, o8, kept = self._held
-        self.input, self.sum = None, h   # (no input until the call has succeeded)
+        if sum is not None:
+            h = sum
+        self.input, self._rows, self.sum = None, None, h   # (no rows until the call has succeeded)
         if h is not None:
             _want(h.ptr, "sum has been freed")
         st = self.lib.omega_hip_rmsnorm_forward(
@@ -148,7 +155,9 @@ class RMSLayer(_Layer):
             kept.scales.ptr if kept else None, rstd.ptr)
         if st:
             ctx.check(st)
-        self.input, self.kept = x if h is None else h, kept
+        self._rows, self.kept = shape, kept
+        if kept is None:
+            self.input = x if h is None else h
         return out or o8
 
     def read8(self, rows, dtype="bf16"):
@@ -158,22 +167,21 @@ class RMSLayer(_Layer):
 
     def back(self, delta, dsum=None):
         """Gradient of x and of the residual alike, for the last forward(); dsum: the gradient that reaches the sum past the norm.  gamma's is diffGamma."""
-        h = self.input
-        _want(h is not None, "back without a forward")
-        _want(delta.shape == h.shape and delta.dtype == self.dtype, "delta shape or dtype does not match the output")
-        _want(dsum is None or (dsum.shape == h.shape and dsum.dtype == self.dtype and dsum.ptr), "dsum shape or dtype does not match the sum")
+        h, rows, kept = self.input, self._rows, self.kept
+        _want(rows is not None, "back without a forward")
+        _want(delta.shape == rows and delta.dtype == self.dtype, "delta shape or dtype does not match the output")
+        _want(dsum is None or (dsum.shape == rows and dsum.dtype == self.dtype and dsum.ptr), "dsum shape or dtype does not match the sum")
         _want(self.gamma is not None, "the layer has no gamma")
-        kept, T = self.kept, h.shape[0]
-        dx = self._buffer("diff", h.shape, self.dtype)
+        dx = self._buffer("diff", rows, self.dtype)
         self.diffGamma = dg = self._buffer("diffGamma", (self.embedDim,), "f32")
         self.ctx.check(self.lib.omega_hip_rmsnorm_backward(
             self.ctx.handle, None if kept else h.ptr, kept.codes.ptr if kept else None, kept.scales.ptr if kept else None, delta.ptr,
-            dsum.ptr if dsum else None, _DT[self.dtype], T, self.embedDim, self.gamma.ptr, self._owned["rstd"].ptr, dx.ptr, dg.ptr))
+            dsum.ptr if dsum else None, _DT[self.dtype], rows[0], self.embedDim, self.gamma.ptr, self._owned["rstd"].ptr, dx.ptr, dg.ptr))
         return dx
 
     def close(self):
         super().close()
-        self.sum = self.kept = self._for = self._held = None
+        self.sum = self.kept = self._for = self._held = self._rows = None
 
 
 class Keep8Layer(_Layer):

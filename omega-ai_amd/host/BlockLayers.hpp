@@ -3,7 +3,7 @@
 //
 //   omega::RMSLayer      RMS norm with the addition in front of it: sum = x + residual, out = norm(sum) (RMSLayer,
 //                        J/engine/nn/layer/normalization/RMSLayer.java; the additions of LlamaTransformerBlock.java:129-136); may keep
-//                        what it normed in 8 bits and go back from those
+//                        what it normed in 8 bits and go back from those, and then holds neither x nor the sum
 //   omega::Keep8Layer    rows kept in 8 bits and brought back
 //   omega::RoutingLayer  routing to experts from a gate's logits (the reference has no router)
 #pragma once
@@ -47,30 +47,38 @@ public:
         detail::rows_of(gamma, embedDim, "gamma shape");
         detail::want(gamma.number == 1, "gamma shape");
     }
-    Tensor &forward(Tensor &x, Tensor *residual = nullptr)
+    // sum: where x + residual goes (x or residual themselves, say); nullptr: the layer's own tensor
+    Tensor &forward(Tensor &x, Tensor *residual = nullptr, Tensor *sum = nullptr)
     {
         detail::rows_of(x, d_, "input shape");
         if (residual) {
             detail::rows_of(*residual, d_, "residual shape");
             detail::want(residual->number == x.number, "residual shape");
         }
-        h_ = nullptr;  // (until the call has succeeded)
+        if (sum) {
+            detail::want(residual, "a sum without a residual");
+            detail::rows_of(*sum, d_, "sum shape");
+            detail::want(sum->number == x.number, "sum shape");
+        }
+        h_ = summed_ = nullptr;
+        ran_ = false;  // (until the call has succeeded)
         Tensor &out = detail::sized(out_, x.number, d_, gamma_.ctx), &st = detail::sized(rstd_, 1, x.number, gamma_.ctx);
-        Tensor *h = residual ? &detail::sized(sum_, x.number, d_, gamma_.ctx) : nullptr;  // (an older sum stays: x may be it)
-        summed_ = h != nullptr;
+        Tensor *h = sum ? sum : residual ? &detail::sized(sum_, x.number, d_, gamma_.ctx) : nullptr;  // (an older sum stays: x may be it)
+        summed_ = h;
         uint8_t *codes = keep_ ? (uint8_t *)codes_.of((size_t)x.number * d_) : nullptr;
         float *scales = keep_ ? (float *)scales_.of((size_t)x.number * ((d_ + 127) / 128) * 4) : nullptr;
         check(gamma_.ctx->get(), omega_hip_rmsnorm_forward(gamma_.ctx->get(), x.gpuData, residual ? residual->gpuData : nullptr, OMEGA_DTYPE_F32, x.number, d_,
                                                            (const float *)gamma_.gpuData, eps_, h ? h->gpuData : nullptr, out.gpuData, nullptr, nullptr,
                                                            codes, scales, (float *)st.gpuData));
-        h_ = h ? h : &x;
+        if (!keep_) h_ = h ? h : &x;
         rows_ = x.number;
+        ran_ = true;
         return out;
     }
     // gradient of the input and of the residual alike; dsum: the gradient that reaches the sum past the norm
     Tensor &back(Tensor &delta, Tensor *dsum = nullptr)
     {
-        detail::want(h_, "back without a forward");
+        detail::want(ran_, "back without a forward");
         detail::rows_of(delta, d_, "delta shape does not match the output");
         detail::want(delta.number == rows_, "delta shape does not match the output");
         if (!keep_) {
@@ -88,14 +96,14 @@ public:
                                                             (float *)dg.gpuData));
         return dx;
     }
-    Tensor *getSum() { return summed_ ? sum_.get() : nullptr; }
+    Tensor *getSum() { return summed_; }
     Tensor *getDiffGamma() { return diffGamma_.get(); }
 
 private:
     int d_, rows_ = 0;
     float eps_;
-    bool keep_, summed_ = false;
-    Tensor &gamma_, *h_ = nullptr;
+    bool keep_, ran_ = false;
+    Tensor &gamma_, *h_ = nullptr, *summed_ = nullptr;  // what back() reads, where that is not the kept rows; the last sum
     detail::Memory codes_, scales_;
     std::unique_ptr<Tensor> out_, sum_, rstd_, diff_, diffGamma_;
 };
