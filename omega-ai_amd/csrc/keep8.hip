@@ -1,7 +1,7 @@
 // Rows kept in 8 bits (eight.h describes the two forms) and brought back: activations between a forward pass and its backward pass.
 // A lane takes eight elements, with no loop: the groups' largest elements are found among neighbours, and loads of many waves are in flight.  Bound: bytes (x in,
 // codes and scales out, and the other way round): 16384 x 4096 bf16, whole numbers: saved in 43.4 us (4.7 TB/s), brought back in 30.7 (6.6 TB/s); 2999 x 1333 fp32 in
-// e4m3: 5.8 and 5.8 us.
+// e4m3: 5.8 and 5.7 us; 16384 x 4096 fp32, either form: 57 and 65 us (5.9 and 5.2 TB/s).
 #include "eight.h"
 
 // Row of a lane and eight times its place there, `per` lanes a row (a launch holds at most 2^30 lanes: the workgroup's division is of 32 bits)

@@ -10,10 +10,13 @@
 // The choice is that of worths in 64 bits.  They are formed in fp32, a few instructions an expert, and where two that the choice tells apart are nearer
 // to each other than their errors, or equal, those few are formed in double and put in order; where they are not few, or it is groups, the whole token is
 // chosen for again in double, by a wave of its workgroup at the end (route_exact).
-// L lanes share a token, V experts a lane (vector instructions are the bound: 16384 x 256 with bias and groups 13 us, and 5 more where a token
-// is chosen for again; with neither 9 us; the bytes alone would take 3).  What is compared of an expert is one word: its worth as a whole number
-// of the same order, the last bits replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
+// L lanes share a token, V experts a lane.  What is compared of an expert is one word: its worth as a whole number of the same order, the last bits
+// replaced by the expert's place in its lane.  A lane sorts its words by minima and maxima and leaves them in LDS; a round of the choice is the largest of
 // the lanes' first ones, found in the lanes' own pipeline, and a step in the list of the lane that holds it.
+// Bound: waiting.  16384 x 256 with bias and groups takes 13 us, and 4 to 5 more where a token is chosen for again; 1086 vector instructions a wave, four
+// waves a SIMD, are 7 of them, the bytes 3; a wave makes one round of its loop, and its fetch, its sort and its K + 2 rounds follow each other.  16384 x 128
+// with neither: 6.5 us, 377 instructions (2.5), the bytes 2.  Logits that are equal or next to each other at the edge of the choice cost what is done in
+// double: rounded to bf16 13.2 us a call in place of 8.7 (128 experts, softmax), a tenth of the rows at the lowest number 20.9, all of them equal 44.4.
 #include <float.h>
 
 #include <algorithm>
@@ -790,7 +793,7 @@ __global__ __launch_bounds__(256) void route_balance_kernel(const int32_t *__res
     }
 }
 
-// How a batch is cut.  Few lanes a token do the least work for it (16; above 256 experts 32: 65536 x 512, softmax, 44 us, with a wave a token 78), a wave ends
+// How a batch is cut.  Few lanes a token do the least work for it (16; above 256 experts 32: 65536 x 512, softmax, 41 us, with a wave a token 78), a wave ends
 // soonest: sixteen tokens a compute unit and fewer have one each (E = 256, sigmoid, 8 groups: 4096 tokens 13.0 us, with 16 lanes 13.8; 8192 tokens 17.4 and
 // 14.0; at 64 experts and fewer half of it is idle).  What one workgroup takes at once it does alone, without a second launch for the counts (64
 // tokens of 128 experts 5.4 us a call, in several workgroups 6.3; 64 of 256 experts, two rounds of its waves, 7.9 and 6.4).  Groups: one lane for each at

