@@ -378,6 +378,8 @@ int omega_hip_clip_grad_norm(omega_ctx *ctx, const omega_grad_tensor *tensors, i
  *   chosen are the K best experts of the groups that stay, in descending order of worth, without a bias of z; equal experts and groups in the
  *   order of their numbers.  Worths are compared as their 64-bit values;
  *   weight w_j = scale s_j; with renorm divided by the sum of s over the chosen.  Where fewer than K are open: id -1, weight 0.
+ *   In weights and gradients a score counts as 0 below 2^-126 of the token's largest (softmax) or of 1 (sigmoid), with renorm below 2^-126 of the
+ *   largest that is chosen (sigmoid: where all of those are below a half).
  * The bias takes part in the choice only and has no gradient: omega_hip_route_balance moves it against what the experts got. */
 #define OMEGA_ROUTE_SOFTMAX 0
 #define OMEGA_ROUTE_SIGMOID 1
